@@ -269,6 +269,94 @@ int axc_depthwise_conv2d_minmax(const axc_table *table, const axc_conv2d_desc *d
                                 float input_min, float input_max, float filter_min, float filter_max,
                                 float *output, void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- transformer layers in the same arithmetic: dense layers, the loss over a vocabulary, residual norms ----------------
+ * No counterpart in the reference, whose only table op is the convolution: here its layer call
+ * (tf2/python/keras/layers/fake_approx_convolutional.py:223-261) is made around matrix products.  Tensors are row-major and
+ * contiguous, of the types below, at addresses of a multiple of their element size; outputs overlap nothing. */
+enum { AXC_F32 = 0, AXC_BF16 = 1, AXC_F16 = 2 };
+enum { AXC_ACT_GELU = 2, AXC_ACT_GELU_TANH = 3, AXC_ACT_SILU = 4 };   /* dense layers only, beside NONE and RELU */
+
+/* A dense layer: input [rows][depth], kernel [depth][columns] as Keras has it, output [rows][columns].  Both operands are
+ * quantized to the 8-bit grid of their (smallest, largest) value, with a = code of the input and b = code of the kernel
+ *   product = s_in s_k sum over depth of (T[a][b] - z_k a - z_in b + z_in z_k),
+ * the brackets in whole numbers, what follows in float32, rounded once to the output's type.  depth below 32768.
+ * The kernel's range is its own; the input's is its own, or what a call before has reported of it (`input_range`,
+ * AXC_RANGE_BYTES, as in axc_layer_ranges), or fixed by the caller (range_known), in this order of precedence: fixed, reported,
+ * its own.  NaN in an operand counts as the upper end of its range, as in the convolutions. */
+typedef struct axc_dense_desc {
+    int64_t rows, depth, columns;
+    int32_t input_type;      /* also of residual, output, pre and their gradients */
+    int32_t kernel_type;     /* also of the gradients of kernel and bias */
+    int32_t bias_type;
+    int32_t activation;      /* AXC_ACT_* */
+    int32_t range_known;     /* 1: input_min, input_max */
+    float input_min, input_max;
+} axc_dense_desc;
+
+/* The kernel's codes, laid out once for many calls (rows of the desc does not matter): device memory of this size, 256-byte
+ * aligned, which the call fills and axc_fake_approx_dense reads in the kernel's place. */
+int axc_dense_packed_bytes(const axc_dense_desc *desc, size_t *bytes);
+int axc_dense_pack(const axc_dense_desc *desc, const void *kernel, void *packed, void *stream);
+
+/* output = residual + activation(product + bias).  Exactly one of kernel and packed is not null; bias, residual, input_range may
+ * be null.  pre: not null: what the activation is given (product + bias) is stored there too, for the gradients.
+ * `packed` in the query: 1 for calls that pass it. */
+int axc_fake_approx_dense_workspace_bytes(const axc_dense_desc *desc, int packed, size_t *bytes);
+int axc_fake_approx_dense(const axc_table *table, const axc_dense_desc *desc, const void *input, const void *input_range,
+                          const void *kernel, const void *packed, const void *bias, const void *residual, void *output, void *pre,
+                          void *workspace, size_t workspace_bytes, void *stream);
+/* Gradients, straight through the grid: a quantized product counts as the exact product of the values on their grids, and the
+ * grid as the identity where a value lies inside it (nudged range, both ends), as constant elsewhere; ranges count as constants.
+ *   dz = grad_output activation'(pre),  grad_input = dz kernel^T,  grad_kernel = input^T dz,  grad_bias = column sums of dz
+ * (the residual's gradient is grad_output itself).  pre may be null without an activation; outputs may be null, each.  Gradients
+ * are rounded to bfloat16 ahead of a product only where its result is bfloat16.  rows at most 4 194 176. */
+int axc_fake_approx_dense_gradients_workspace_bytes(const axc_dense_desc *desc, size_t *bytes);
+int axc_fake_approx_dense_gradients(const axc_dense_desc *desc, const void *grad_output, const void *input,
+                                    const void *input_range, const void *kernel, const void *pre, void *grad_input,
+                                    void *grad_kernel, void *grad_bias, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Softmax cross entropy whose logits are a dense layer's product + bias over a vocabulary (the desc's columns; no activation),
+ * made a piece of the vocabulary at a time and never kept:
+ *   loss of a row = log(sum over v of exp(logit[v])) - logit[target]
+ * targets: rows int64.  Rows whose target is ignore_index count for nothing (they do count for the input's range); one whose
+ * target is no column otherwise has the loss NaN.  loss: `rows` floats (AXC_LOSS_NONE) or one (the sum, or the sum over the number
+ * of rows that count, 0 if none does).  The gradients, of the loss times grad_loss (device memory, like loss; null = ones), are
+ * those of the dense layer; any may be null.  `gradients` in the query: 1 if one of them is not.  rows at most 4 194 176. */
+enum { AXC_LOSS_NONE = 0, AXC_LOSS_SUM = 1, AXC_LOSS_MEAN = 2 };
+int axc_fake_approx_cross_entropy_workspace_bytes(const axc_dense_desc *desc, int gradients, size_t *bytes);
+int axc_fake_approx_cross_entropy(const axc_table *table, const axc_dense_desc *desc, const void *input, const void *input_range,
+                                  const void *kernel, const void *bias, const int64_t *targets, int64_t ignore_index,
+                                  int reduction, const float *grad_loss, float *loss, void *grad_input, void *grad_kernel,
+                                  void *grad_bias, void *workspace, size_t workspace_bytes, void *stream);
+
+/* The norms before and after a block of a residual network, with the block's gate and scale:
+ *   u = norm(block) post_weight (block itself without post_weight),  h = x + scale gate u,  y = norm(h) weight + bias
+ * norm divides by sqrt(mean of squares + eps) (AXC_NORM_RMS), or subtracts the mean first (AXC_NORM_LAYER).  x, block, h, y: rows x
+ * width of `type`; gate: gate_groups x width of `type`, each for rows / gate_groups neighbouring rows; weight, bias, scale,
+ * post_weight: width of `vector_type`.  block, gate, scale, post_weight, bias may be null; without a block there is no gate, scale
+ * or post_weight, h is x and not written.  y is the norm of h as stored.  output_range: AXC_RANGE_BYTES that get the range of y, for
+ * the input_range of a dense layer, or null.  width at most 32768. */
+enum { AXC_NORM_RMS = 0, AXC_NORM_LAYER = 1 };
+typedef struct axc_residual_norm_desc {
+    int64_t rows, width, gate_groups;   /* gate_groups: 0 without a gate */
+    int32_t type, vector_type, kind;
+    float eps;
+} axc_residual_norm_desc;
+typedef struct axc_residual_norm_tensors {
+    const void *x, *block, *weight, *bias, *gate, *scale, *post_weight;
+} axc_residual_norm_tensors;
+int axc_residual_norm(const axc_residual_norm_desc *desc, const axc_residual_norm_tensors *in, void *h, void *y,
+                      void *output_range, void *stream);
+/* Gradients, from those of h and y (one of them may be null: zeros): x of `in` is not read, h is what the call above wrote (x
+ * itself without a block).  grad_x and, with a block, grad_block are always written; the others may be null, each. */
+typedef struct axc_residual_norm_gradients_out {
+    void *x, *block, *weight, *bias, *gate, *scale, *post_weight;
+} axc_residual_norm_gradients_out;
+int axc_residual_norm_gradients_workspace_bytes(const axc_residual_norm_desc *desc, size_t *bytes);
+int axc_residual_norm_gradients(const axc_residual_norm_desc *desc, const axc_residual_norm_tensors *in, const void *h,
+                                const void *grad_h, const void *grad_y, const axc_residual_norm_gradients_out *out,
+                                void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- parity entry points (stages of the op, exposed so each can be checked bit for bit) ---- */
 
 /* The quantize expression (approx_nn_conv_kernels.cpp:193,197,243,293) on n floats:

@@ -13,3 +13,11 @@ from .ops import (  # noqa: F401
     approx_conv2d_with_min_max_vars,
     approx_depthwise_conv2d_with_min_max_vars,
 )
+from .layers import (  # noqa: F401
+    DenseGradients,
+    FakeApproxCrossEntropy,
+    FakeApproxDense,
+    PackedKernel,
+    ResidualNorm,
+    ResidualNormGradients,
+)

@@ -47,10 +47,29 @@ class QuantProps(ctypes.Structure):
         "s1xs2", "m1", "m2", "m1xm2")] + [("input_zero_code", ctypes.c_int32)]
 
 
+F32, BF16, F16 = 0, 1, 2
+
+
+class DenseDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in ("rows", "depth", "columns")] + [
+        (n, ctypes.c_int32) for n in ("input_type", "kernel_type", "bias_type", "activation", "range_known")] + [
+        (n, ctypes.c_float) for n in ("input_min", "input_max")]
+
+
+class ResidualNormDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int64) for n in ("rows", "width", "gate_groups")] + [
+        (n, ctypes.c_int32) for n in ("type", "vector_type", "kind")] + [("eps", ctypes.c_float)]
+
+
+class ResidualNormTensors(ctypes.Structure):   # and their gradients
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "block", "weight", "bias", "gate", "scale", "post_weight")]
+
+
 # every symbol include/axconv.h declares: (name, restype, argtypes)
 _vp, _sz, _i64 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int64
 _f = ctypes.c_float
 _desc = ctypes.POINTER(ConvDesc)
+_dense, _norm, _norm_tensors = (ctypes.POINTER(t) for t in (DenseDesc, ResidualNormDesc, ResidualNormTensors))
 _launch_tail = [_f, _f, _f, _f, _vp, _vp, _sz, _vp]
 SYMBOLS = [
     ("axc_status_string", ctypes.c_char_p, [ctypes.c_int]),
@@ -93,6 +112,18 @@ SYMBOLS = [
     ("axc_conv2d_minmax_acc_i32", ctypes.c_int, [_vp, _desc, _vp, _vp] + _launch_tail),
     ("axc_depthwise_conv2d_minmax_acc_i32", ctypes.c_int, [_vp, _desc, _vp, _vp] + _launch_tail),
     ("axc_conv2d_codes_acc_i32", ctypes.c_int, [_vp, _desc, _vp, _vp, ctypes.c_int, _vp, _vp, _sz, _vp]),
+    ("axc_dense_packed_bytes", ctypes.c_int, [_dense, ctypes.POINTER(_sz)]),
+    ("axc_dense_pack", ctypes.c_int, [_dense, _vp, _vp, _vp]),
+    ("axc_fake_approx_dense_workspace_bytes", ctypes.c_int, [_dense, ctypes.c_int, ctypes.POINTER(_sz)]),
+    ("axc_fake_approx_dense", ctypes.c_int, [_vp, _dense] + [_vp] * 9 + [_sz, _vp]),
+    ("axc_fake_approx_dense_gradients_workspace_bytes", ctypes.c_int, [_dense, ctypes.POINTER(_sz)]),
+    ("axc_fake_approx_dense_gradients", ctypes.c_int, [_dense] + [_vp] * 9 + [_sz, _vp]),
+    ("axc_fake_approx_cross_entropy_workspace_bytes", ctypes.c_int, [_dense, ctypes.c_int, ctypes.POINTER(_sz)]),
+    ("axc_fake_approx_cross_entropy", ctypes.c_int,
+     [_vp, _dense] + [_vp] * 5 + [_i64, ctypes.c_int] + [_vp] * 6 + [_sz, _vp]),
+    ("axc_residual_norm", ctypes.c_int, [_norm, _norm_tensors, _vp, _vp, _vp, _vp]),
+    ("axc_residual_norm_gradients_workspace_bytes", ctypes.c_int, [_norm, ctypes.POINTER(_sz)]),
+    ("axc_residual_norm_gradients", ctypes.c_int, [_norm, _norm_tensors, _vp, _vp, _vp, _norm_tensors, _vp, _sz, _vp]),
     ("axc_profile_enable", ctypes.c_int, [ctypes.c_int]),
     ("axc_profile_reset", ctypes.c_int, []),
     ("axc_profile_read", ctypes.c_int, [ctypes.c_int, ctypes.c_char_p, _sz, ctypes.POINTER(ctypes.c_double),

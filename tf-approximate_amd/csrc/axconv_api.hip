@@ -1,5 +1,6 @@
 // C-ABI entry points of libaxconv_hip.so: validation, geometry, planning, workspace carving, launches.
 #include "axconv_internal.h"
+#include "layers_internal.h"
 
 #include <math.h>
 #include <stdlib.h>
@@ -18,13 +19,6 @@
 #include <vector>
 
 using namespace axc;
-
-struct axc_table {
-    uint16_t *dev_tableT; // [257 filter code][256 input code]; row 256 is zero
-    uint16_t *dev_tableF; // behind it in the same allocation: the same with the top bit of every byte flipped,
-    uint16_t *dev_tableS; // and [257 input code][256 filter code], flipped too
-    int device;
-};
 
 // Workspace of axc_conv2d_minmax_static: a fixed array in the library's device image, one copy per GPU, held until
 // the process ends.  In host code this name is only a handle for hipGetSymbolAddress; the address each device
@@ -1859,6 +1853,14 @@ int run_depthwise(const axc_table *table, const axc_conv2d_desc *desc, const flo
 
 // ---------------------------------------------------------------------------------------------
 
+namespace axc {
+int api_fail(int status, const char *msg) { return fail(status, msg); }
+int api_fail_hip(hipError_t e, const char *what) { return fail_hip(e, what); }
+int api_check_table(const axc_table *table) { return check_table_device(table); }
+ApiTimer::ApiTimer(const char *name, hipStream_t stream) : scope_(g_prof_enabled.load() ? new ProfScope(name, stream) : nullptr) {}
+ApiTimer::~ApiTimer() { delete static_cast<ProfScope *>(scope_); }
+} // namespace axc
+
 extern "C" {
 
 const char *axc_status_string(int status)
@@ -1880,10 +1882,10 @@ int axc_table_create(const uint16_t *host_table, axc_table **out)
         return fail(AXC_INVALID_ARGUMENT, "null argument");
     // weight-code major: tableT[b][a] = T[(a << 8) | b], in squares that the first-level cache holds by row and by column, and
     // the two flipped copies by whole vectors (us a table with its upload, on one machine: entry by entry 143 for the first
-    // alone, 181 for three; 42)
+    // alone, 181 for three; 42); behind them input-code major rows for dense layers of few rows
     const size_t entries = (size_t)kTableRows * 256, used = 65536;   // row 256: the null weight's, zeros
-    std::vector<uint16_t> t(3 * entries);
-    uint16_t *const T = t.data(), *const F = T + entries, *const S = F + entries;
+    std::vector<uint16_t> t(4 * entries);
+    uint16_t *const T = t.data(), *const F = T + entries, *const S = F + entries, *const I = S + entries;
     for (int a0 = 0; a0 < 256; a0 += 16)
         for (int b0 = 0; b0 < 256; b0 += 16)
             for (int b = b0; b < b0 + 16; ++b)
@@ -1895,15 +1897,20 @@ int axc_table_create(const uint16_t *host_table, axc_table **out)
         S[i] = host_table[i] ^ 0x8080u;
     for (size_t i = used; i < entries; ++i)
         S[i] = 0x8080u;
+    for (int a = 0; a < 256; ++a)   // entry 4 l + i is that of filter code l + 64 i: what a lane loads at once
+        for (int l = 0; l < 64; ++l)
+            for (int i = 0; i < 4; ++i)
+                I[a * 256 + 4 * l + i] = host_table[a * 256 + l + 64 * i];
     axc_table *tab = new axc_table;
     tab->dev_tableT = nullptr;
     hipError_t e = hipGetDevice(&tab->device);
     if (e == hipSuccess)
-        e = hipMalloc(reinterpret_cast<void **>(&tab->dev_tableT), 3 * (size_t)kTableAllocBytes);
+        e = hipMalloc(reinterpret_cast<void **>(&tab->dev_tableT), 4 * (size_t)kTableAllocBytes);
     if (e == hipSuccess)
-        e = hipMemcpy(tab->dev_tableT, t.data(), 3 * (size_t)kTableAllocBytes, hipMemcpyHostToDevice);
+        e = hipMemcpy(tab->dev_tableT, t.data(), 4 * (size_t)kTableAllocBytes, hipMemcpyHostToDevice);
     tab->dev_tableF = tab->dev_tableT + entries;
     tab->dev_tableS = tab->dev_tableF + entries;
+    tab->dev_tableI = tab->dev_tableS + entries;
     if (e != hipSuccess) {
         if (tab->dev_tableT)
             (void)hipFree(tab->dev_tableT);

@@ -1,0 +1,520 @@
+// Dense layers by table products: ranges, codes, the sums of few rows, and what is made of the sums.
+//
+//   product[m][n] = s_in s_k sum_k (T[a][b] - z_k a - z_in b + z_in z_k)
+//                 = s_in s_k (sum_k T[a][b] - z_k sum_k a - z_in sum_k b + K z_in z_k)
+//
+// a, b: codes of the input and of the kernel, s, z: scale and zero point of their grids.  Everything in the brackets is a whole
+// number and is computed as one, so a product is rounded three times: s_in s_k, the bracket, and the two multiplied.
+//
+// The sums of many rows are made by the kernels that make them for 1x1 convolutions (axc_conv2d_codes_acc_i32); those of few
+// rows, where building rows for every filter element would cost more than the lookups, by few_rows_kernel.
+#include "layers_internal.h"
+
+namespace axc {
+namespace {
+
+// ---- ranges ----
+// fminf and fmaxf pass over NaN, as the convolutions' range pass does.
+template <typename T>
+__device__ void range_of(const T *__restrict__ p, int64_t n, int64_t index, int64_t stride, float &lo, float &hi)
+{
+    constexpr int V = 16 / sizeof(T);
+    int64_t done = 0;
+    if (((uintptr_t)p & 15) == 0) {
+        const int64_t nv = n / V;
+#pragma unroll 4
+        for (int64_t i = index; i < nv; i += stride) {
+            float v[V];
+            load_values<T, V>(p + i * V, V, true, 0.0f, v);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                lo = fminf(lo, v[j]);
+                hi = fmaxf(hi, v[j]);
+            }
+        }
+        done = nv * V;
+    }
+    for (int64_t i = done + index; i < n; i += stride) {
+        lo = fminf(lo, (float)p[i]);
+        hi = fmaxf(hi, (float)p[i]);
+    }
+}
+__device__ void range_of_any(const void *p, int type, int64_t n, int64_t index, int64_t stride, float &lo, float &hi)
+{
+    if (type == AXC_F32)
+        range_of(static_cast<const float *>(p), n, index, stride, lo, hi);
+    else if (type == AXC_BF16)
+        range_of(static_cast<const bf16 *>(p), n, index, stride, lo, hi);
+    else
+        range_of(static_cast<const f16 *>(p), n, index, stride, lo, hi);
+}
+
+// One pair per workgroup; the first x_blocks take the input, the others the kernel.  All of them clear `zeros`, into which a
+// later launch adds.
+__global__ void __launch_bounds__(1024) range_kernel(const void *x, int x_type, int64_t nx, int x_blocks, const void *kernel,
+                                                     int kernel_type, int64_t nk, float *x_pairs, float *kernel_pairs,
+                                                     int32_t *zeros, int64_t n_zeros)
+{
+    __shared__ float red[32];
+    const bool second = (int)blockIdx.x >= x_blocks;
+    const int block = second ? (int)blockIdx.x - x_blocks : (int)blockIdx.x;
+    const int blocks = second ? (int)gridDim.x - x_blocks : x_blocks;
+    for (int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x; i < n_zeros; i += (int64_t)gridDim.x * 1024)
+        zeros[i] = 0;
+    float lo = INFINITY, hi = -INFINITY;
+    range_of_any(second ? kernel : x, second ? kernel_type : x_type, second ? nk : nx, (int64_t)block * 1024 + threadIdx.x,
+                 (int64_t)blocks * 1024, lo, hi);
+    block_range(lo, hi, red);
+    if (threadIdx.x == 0) {
+        float *const to = second ? kernel_pairs : x_pairs;
+        to[2 * block] = lo;
+        to[2 * block + 1] = hi;
+    }
+}
+
+__device__ void fold(const RangeSource &src, float &lo, float &hi, float *red)
+{
+    lo = src.lo;
+    hi = src.hi;
+    if (src.pairs) {
+        lo = INFINITY;
+        hi = -INFINITY;
+        for (int i = threadIdx.x; i < src.count; i += blockDim.x) {
+            const float2 p = reinterpret_cast<const float2 *>(src.pairs)[i];
+            lo = fminf(lo, p.x);
+            hi = fmaxf(hi, p.y);
+        }
+        block_range(lo, hi, red);
+    }
+}
+
+__global__ void __launch_bounds__(256) grids_kernel(RangeSource in, RangeSource kernel, int has_in, int has_kernel, Grids *grids)
+{
+    __shared__ float red[8];
+    float lo, hi;
+    if (has_in) {
+        fold(in, lo, hi, red);
+        if (threadIdx.x == 0)
+            grids->in = grid_of_range(lo, hi);
+    }
+    if (has_kernel) {
+        fold(kernel, lo, hi, red);
+        if (threadIdx.x == 0)
+            grids->kernel = grid_of_range(lo, hi);
+    }
+}
+
+// ---- codes ----
+// Codes of one row by a group of `threads` threads, and this thread's part of their sum.  Behind the depth come pad codes, 0.
+template <typename T>
+__device__ int32_t row_codes(const T *__restrict__ x, int K, int Kp, bool whole, const Grid &g, uint8_t *__restrict__ codes,
+                             int thread, int threads)
+{
+    int32_t sum = 0;
+    for (int k = 4 * thread; k < Kp; k += 4 * threads) {
+        float v[4];
+        load_values<T, 4>(x + k, K - k, whole, 0.0f, v);
+        uint32_t word = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t c = whole || k + j < K ? code_of(v[j], g) : 0u;
+            word |= c << (8 * j);
+            sum += (int32_t)c;
+        }
+        *reinterpret_cast<uint32_t *>(codes + k) = word;
+    }
+    return sum;
+}
+__device__ __forceinline__ int32_t row_codes_any(const void *x, int type, int64_t at, int K, int Kp, const Grid &g, uint8_t *codes,
+                                                 int thread, int threads)
+{
+    // (a row's first value is aligned as the tensor's is where the depth is a multiple of four)
+    const bool whole = (K & 3) == 0 && ((uintptr_t)x & (type == AXC_F32 ? 15 : 7)) == 0;
+    if (type == AXC_F32)
+        return row_codes(static_cast<const float *>(x) + at, K, Kp, whole, g, codes, thread, threads);
+    if (type == AXC_BF16)
+        return row_codes(static_cast<const bf16 *>(x) + at, K, Kp, whole, g, codes, thread, threads);
+    return row_codes(static_cast<const f16 *>(x) + at, K, Kp, whole, g, codes, thread, threads);
+}
+
+// A wavefront a row; rows up to the next multiple of four are pad rows, of code 0.
+__global__ void __launch_bounds__(256) input_codes_kernel(const void *x, int type, int64_t rows, int K, int Kp, const Grids *grids,
+                                                          uint8_t *codes, int32_t *row_sums)
+{
+    const int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
+    const int lane = threadIdx.x & 63;
+    if (r >= rows) {
+        for (int k = 4 * lane; k < Kp; k += 256)
+            *reinterpret_cast<uint32_t *>(codes + r * Kp + k) = 0u;
+        if (lane == 0)
+            row_sums[r] = 0;
+        return;
+    }
+    const Grid g = grids->in;
+    const int32_t sum = wave_sum(row_codes_any(x, type, r * K, K, Kp, g, codes + r * Kp, lane, 64));
+    if (lane == 0)
+        row_sums[r] = sum;
+}
+
+// Few rows: every workgroup finds the range itself, of all rows, and then takes its own row.
+__global__ void __launch_bounds__(512) few_codes_kernel(const void *x, int type, int rows, int K, int Kp, RangeSource src,
+                                                        const Grid *kernel_grid, Grids *grids, uint8_t *codes, int32_t *row_sums)
+{
+    __shared__ float red[16];
+    __shared__ int32_t sums[8];
+    float lo, hi;
+    if (!src.pairs && src.count < 0) {
+        lo = INFINITY;
+        hi = -INFINITY;
+        range_of_any(x, type, (int64_t)rows * K, threadIdx.x, 512, lo, hi);
+        block_range(lo, hi, red);
+    } else {
+        fold(src, lo, hi, red);
+    }
+    const Grid g = grid_of_range(lo, hi);
+    const int64_t r = blockIdx.x;
+    const int32_t part = wave_sum(row_codes_any(x, type, r * K, K, Kp, g, codes + r * Kp, (int)threadIdx.x, 512));
+    if ((threadIdx.x & 63) == 0)
+        sums[threadIdx.x / 64] = part;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int32_t sum = 0;
+        for (int i = 0; i < 8; ++i)
+            sum += sums[i];
+        row_sums[r] = sum;
+        if (r == 0) {
+            grids->in = g;
+            grids->kernel = *kernel_grid;
+        }
+    }
+}
+
+constexpr int kSlab = 64;   // depth a workgroup of kernel_codes_kernel takes
+
+template <typename T>
+__device__ void kernel_slab(const T *__restrict__ w, int K, int64_t N, const Pieces &pc, const Grid &g, uint8_t *__restrict__ codes,
+                            int64_t c, int k0, int (&sum)[4])
+{
+    const int piece = (int)(c / pc.width);
+    uint8_t *const to = codes + pc.offset(piece) + (c - pc.first(piece));
+    const int pitch = pc.width_of(piece);
+    const bool whole = c + 4 <= N && (N & 3) == 0 && ((uintptr_t)w & (4 * sizeof(T) - 1)) == 0;
+#pragma unroll 4
+    for (int i = 0; i < kSlab / 4; ++i) {
+        const int k = k0 + 4 * i;
+        if (k >= pc.Kp)
+            break;
+        float v[4];
+        uint32_t word = 0;
+        if (k < K) {
+            load_values<T, 4>(w + (int64_t)k * N + c, N - c, whole, 0.0f, v);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t q = c + j < N ? code_of(v[j], g) : 0u;
+                word |= q << (8 * j);
+                sum[j] += (int)q;
+            }
+        }
+        *reinterpret_cast<uint32_t *>(to + (size_t)k * pitch) = word;
+    }
+}
+
+// 256 columns (four a lane) by kSlab of the depth (a wavefront takes every fourth); column sums are added to what the launch
+// before cleared, as whole numbers, so in any order.
+__global__ void __launch_bounds__(256) kernel_codes_kernel(const void *w, int type, int K, int64_t N, Pieces pc, const Grids *grids,
+                                                           uint8_t *codes, int32_t *column_sums)
+{
+    __shared__ int32_t red[4][256];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+    const int64_t c = ((int64_t)blockIdx.x * 64 + lane) * 4;
+    int sum[4] = {};
+    if (c < pc.Np) {
+        const Grid g = grids->kernel;
+        const int k0 = (int)blockIdx.y * kSlab + wave;
+        if (type == AXC_F32)
+            kernel_slab(static_cast<const float *>(w), K, N, pc, g, codes, c, k0, sum);
+        else if (type == AXC_BF16)
+            kernel_slab(static_cast<const bf16 *>(w), K, N, pc, g, codes, c, k0, sum);
+        else
+            kernel_slab(static_cast<const f16 *>(w), K, N, pc, g, codes, c, k0, sum);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        red[wave][4 * lane + j] = sum[j];
+    __syncthreads();
+    const int64_t column = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (column < pc.Np)
+        atomicAdd(column_sums + column, red[0][threadIdx.x] + red[1][threadIdx.x] + red[2][threadIdx.x] + red[3][threadIdx.x]);
+}
+
+// ---- sums of few rows ----
+// A wavefront takes MT rows, 512 columns (eight a lane) and one element of the depth at a time.  It turns the MT table rows that
+// the rows' codes name into R[b] = entries of filter code b for all MT rows, in LDS of its own, and a lane then reads the entries
+// of all MT rows for one weight with one access of 2 MT bytes.  Sums of two rows share a dword as they come: one register adds
+// whole dwords modulo 2^32, another the upper halves.  Building costs 256 entries a row and element where the lookups are 512.
+template <int MT>
+__global__ void __launch_bounds__(256) few_rows_kernel(const uint16_t *__restrict__ tableI, const uint8_t *__restrict__ x_codes,
+                                                       int rows, int Kp, const uint8_t *__restrict__ kernel_codes, int width,
+                                                       int32_t *__restrict__ acc)
+{
+    constexpr int H = (MT + 1) / 2;   // dwords of an entry
+    constexpr int kRowBytes = 256 * 2 * MT;
+    __shared__ __align__(16) unsigned char lds[4 * (kRowBytes > 2048 ? kRowBytes : 2048)];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    unsigned char *const R = lds + wave * kRowBytes;
+    const int c = (int)blockIdx.x * 512 + lane * 8;
+    const int row0 = (int)blockIdx.z * MT;
+    const int quads = Kp / 4, splits = gridDim.y;
+    const int q_end = (int)((int64_t)quads * (blockIdx.y + 1) / splits);
+    const bool in0 = c < width, in1 = c + 4 < width;
+
+    uint32_t even[8][H] = {}, odd[8][H] = {};
+    for (int q = (int)((int64_t)quads * blockIdx.y / splits) + wave; q < q_end; q += 4) {
+        uint32_t a[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)   // (rows beyond the last repeat it; nobody stores them)
+            a[m] = *reinterpret_cast<const uint32_t *>(x_codes + (int64_t)min(row0 + m, rows - 1) * Kp + 4 * q);
+        uint32_t b[4][2];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint8_t *const p = kernel_codes + (size_t)(4 * q + j) * width + c;
+            b[j][0] = in0 ? *reinterpret_cast<const uint32_t *>(p) : 0u;
+            b[j][1] = in1 ? *reinterpret_cast<const uint32_t *>(p + 4) : 0u;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint2 t[MT];
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+                t[m] = *reinterpret_cast<const uint2 *>(tableI + ((a[m] >> (8 * j)) & 255u) * 256u + lane * 4);
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {   // filter code lane + 64 i
+                const uint32_t sel = i & 1 ? 0x07060302u : 0x05040100u;
+                uint32_t e[H];
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    const uint32_t lo = i < 2 ? t[2 * h].x : t[2 * h].y;
+                    const uint32_t hi = MT == 1 ? 0u : i < 2 ? t[(2 * h + 1) % MT].x : t[(2 * h + 1) % MT].y;
+                    e[h] = __builtin_amdgcn_perm(hi, lo, sel);
+                }
+                unsigned char *const to = R + (lane + 64 * i) * (2 * MT);
+                if constexpr (MT == 1)
+                    *reinterpret_cast<uint16_t *>(to) = (uint16_t)e[0];
+                else if constexpr (MT == 2)
+                    *reinterpret_cast<uint32_t *>(to) = e[0];
+                else if constexpr (MT == 4)
+                    *reinterpret_cast<uint2 *>(to) = make_uint2(e[0], e[1]);
+                else
+                    *reinterpret_cast<uint4 *>(to) = make_uint4(e[0], e[1], e[2], e[3]);
+            }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                const unsigned char *const from = R + ((b[j][n / 4] >> (8 * (n & 3))) & 255u) * (2 * MT);
+                uint32_t e[H];
+                if constexpr (MT == 1) {
+                    e[0] = *reinterpret_cast<const uint16_t *>(from);
+                } else if constexpr (MT == 2) {
+                    e[0] = *reinterpret_cast<const uint32_t *>(from);
+                } else if constexpr (MT == 4) {
+                    const uint2 v = *reinterpret_cast<const uint2 *>(from);
+                    e[0] = v.x;
+                    e[1] = v.y;
+                } else {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(from);
+                    e[0] = v.x;
+                    e[1] = v.y;
+                    e[2] = v.z;
+                    e[3] = v.w;
+                }
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    even[n][h] += e[h];
+                    if constexpr (MT > 1)
+                        odd[n][h] += e[h] >> 16;
+                }
+            }
+        }
+    }
+    // the four wavefronts' sums, a row at a time through LDS
+    int32_t *const red = reinterpret_cast<int32_t *>(lds);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            const uint32_t v = m & 1 ? odd[n][m / 2] : even[n][m / 2] - (MT > 1 ? odd[n][m / 2] << 16 : 0u);
+            red[wave * 512 + n * 64 + lane] = (int32_t)v;
+        }
+        __syncthreads();
+        if (row0 + m < rows) {
+            int32_t *const to = acc + ((int64_t)blockIdx.y * rows + row0 + m) * width;
+            for (int i = threadIdx.x; i < 512; i += 256) {   // column 8 * lane + n stands at n * 64 + lane
+                const int col = (int)blockIdx.x * 512 + i, at = (i & 7) * 64 + i / 8;
+                if (col < width)
+                    to[col] = red[at] + red[512 + at] + red[1024 + at] + red[1536 + at];
+            }
+        }
+    }
+}
+
+// ---- what is made of the sums ----
+// residual + activation(product + bias), four columns a lane, a wavefront a row at a time.  Products and everything behind them
+// are in float32, rounded once to the output's type (`pre`, what the activation is given, once more).
+template <typename T>
+__global__ void __launch_bounds__(256) dense_out_kernel(TableSums s, int64_t rows, int columns, DenseOut o)
+{
+    const int c = ((int)blockIdx.x * 64 + (threadIdx.x & 63)) * 4;
+    if (c >= columns)
+        return;
+    const float scale = __fmul_rn(s.grids->in.scale, s.grids->kernel.scale);
+    const int64_t zi = s.grids->in.zero;
+    const bool whole = c + 4 <= columns && (o.ld & 3) == 0 && ((uintptr_t)o.out & (4 * sizeof(T) - 1)) == 0 &&
+                       ((uintptr_t)o.residual & (4 * sizeof(T) - 1)) == 0 && ((uintptr_t)o.pre & (4 * sizeof(T) - 1)) == 0;
+    int64_t column[4];
+    float bias[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const bool there = c + j < columns;
+        column[j] = there ? zi * s.column_sums[c + j] : 0;
+        bias[j] = there && o.bias ? load_any(o.bias, c + j, o.bias_type) : 0.0f;
+    }
+    for (int64_t r = (int64_t)blockIdx.y * 4 + threadIdx.x / 64; r < rows; r += (int64_t)gridDim.y * 4) {
+        const int64_t at = r * s.pitch + c;
+        int32_t t[4] = {};
+#pragma unroll 8
+        for (int i = 0; i < s.splits; ++i) {
+            const i32x4 v = *reinterpret_cast<const i32x4 *>(s.acc + i * s.split_stride + at);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                t[j] += v[j];
+        }
+        const int64_t row = row_term(s, r);
+        float z[4], y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            z[j] = __fmul_rn((float)((int64_t)t[j] + row - column[j]), scale);
+            if (o.bias)
+                z[j] = __fadd_rn(z[j], bias[j]);
+            y[j] = activate(z[j], o.activation);
+        }
+        const int64_t to = r * o.ld + c;
+        if (o.pre)
+            store_values<T, 4>(static_cast<T *>(o.pre) + to, columns - c, whole, z);
+        if (o.residual) {
+            float v[4];
+            load_values<T, 4>(static_cast<const T *>(o.residual) + to, columns - c, whole, 0.0f, v);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                y[j] = __fadd_rn(y[j], v[j]);
+        }
+        store_values<T, 4>(static_cast<T *>(o.out) + to, columns - c, whole, y);
+    }
+}
+
+__global__ void __launch_bounds__(256) zero_kernel(uint16_t *p, int64_t n)   // halfwords: what elements are multiples of
+{
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
+        p[i] = 0;
+}
+
+} // namespace
+
+hipError_t launch_zero(void *p, int64_t bytes, hipStream_t stream)
+{
+    const int64_t n = bytes / 2, blocks = (n + 255) / 256;
+    if (n > 0)
+        hipLaunchKernelGGL(zero_kernel, dim3((unsigned)(blocks > 4096 ? 4096 : blocks)), dim3(256), 0, stream,
+                           static_cast<uint16_t *>(p), n);
+    return hipGetLastError();
+}
+
+hipError_t launch_range(const void *x, int x_type, int64_t nx, const void *kernel, int kernel_type, int64_t nk, float *x_pairs,
+                        float *kernel_pairs, int32_t *zeros, int64_t n_zeros, int *x_count, int *kernel_count, hipStream_t stream)
+{
+    auto blocks = [](int64_t n) {   // 16 values a thread and more
+        const int64_t b = (n + 16383) / 16384;
+        return (int)(b > kRangeBlocks ? kRangeBlocks : b);
+    };
+    const int bx = x ? blocks(nx) : 0, bk = kernel ? blocks(nk) : 0;
+    *x_count = bx;
+    *kernel_count = bk;
+    const int total = bx + bk;
+    if (total == 0)
+        return hipSuccess;
+    hipLaunchKernelGGL(range_kernel, dim3(total), dim3(1024), 0, stream, x, x_type, nx, bx, kernel, kernel_type, nk, x_pairs,
+                       kernel_pairs, zeros, n_zeros);
+    return hipGetLastError();
+}
+
+hipError_t launch_grids(const RangeSource &in, const RangeSource &kernel, bool has_in, bool has_kernel, Grids *grids,
+                        hipStream_t stream)
+{
+    hipLaunchKernelGGL(grids_kernel, dim3(1), dim3(256), 0, stream, in, kernel, (int)has_in, (int)has_kernel, grids);
+    return hipGetLastError();
+}
+
+hipError_t launch_input_codes(const void *x, int type, int64_t rows, int K, int Kp, const Grids *grids, uint8_t *codes,
+                              int32_t *row_sums, hipStream_t stream)
+{
+    hipLaunchKernelGGL(input_codes_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, x, type, rows, K, Kp, grids,
+                       codes, row_sums);
+    return hipGetLastError();
+}
+
+hipError_t launch_few_codes(const void *x, int type, int rows, int K, int Kp, const RangeSource &src, const Grid *kernel_grid,
+                            Grids *grids, uint8_t *codes, int32_t *row_sums, hipStream_t stream)
+{
+    hipLaunchKernelGGL(few_codes_kernel, dim3(rows), dim3(512), 0, stream, x, type, rows, K, Kp, src, kernel_grid, grids, codes,
+                       row_sums);
+    return hipGetLastError();
+}
+
+hipError_t launch_kernel_codes(const void *kernel, int type, int K, int64_t N, const Pieces &pieces, const Grids *grids,
+                               uint8_t *codes, int32_t *column_sums, hipStream_t stream)
+{
+    hipLaunchKernelGGL(kernel_codes_kernel, dim3((unsigned)((pieces.Np + 255) / 256), (unsigned)((pieces.Kp + kSlab - 1) / kSlab)),
+                       dim3(256), 0, stream, kernel, type, K, N, pieces, grids, codes, column_sums);
+    return hipGetLastError();
+}
+
+// Enough workgroups for the chip, four a CU, but at least two quads of the depth for every wavefront.
+int few_rows_splits(int64_t rows, int K, int width)
+{
+    const int64_t groups = (rows + kFewRows - 1) / kFewRows * ((width + 511) / 512);
+    const int64_t want = 1024 / groups, most = ((K + 3) / 4) / 8;
+    const int64_t s = want < most ? want : most;
+    return (int)(s < 1 ? 1 : s);
+}
+
+hipError_t launch_few_rows(const uint16_t *tableI, const uint8_t *x_codes, int rows, int Kp, const uint8_t *kernel_codes, int width,
+                           int splits, int32_t *acc, hipStream_t stream)
+{
+    const int mt = rows == 1 ? 1 : rows == 2 ? 2 : rows <= 4 ? 4 : 8;
+    const dim3 grid((unsigned)((width + 511) / 512), (unsigned)splits, (unsigned)((rows + mt - 1) / mt));
+    if (mt == 1)
+        hipLaunchKernelGGL(few_rows_kernel<1>, grid, dim3(256), 0, stream, tableI, x_codes, rows, Kp, kernel_codes, width, acc);
+    else if (mt == 2)
+        hipLaunchKernelGGL(few_rows_kernel<2>, grid, dim3(256), 0, stream, tableI, x_codes, rows, Kp, kernel_codes, width, acc);
+    else if (mt == 4)
+        hipLaunchKernelGGL(few_rows_kernel<4>, grid, dim3(256), 0, stream, tableI, x_codes, rows, Kp, kernel_codes, width, acc);
+    else
+        hipLaunchKernelGGL(few_rows_kernel<8>, grid, dim3(256), 0, stream, tableI, x_codes, rows, Kp, kernel_codes, width, acc);
+    return hipGetLastError();
+}
+
+hipError_t launch_dense_out(const TableSums &s, int64_t rows, int columns, const DenseOut &o, hipStream_t stream)
+{
+    const int64_t by = (rows + 3) / 4;
+    const dim3 grid((unsigned)((columns + 255) / 256), (unsigned)(by > 4096 ? 4096 : by));
+    if (o.type == AXC_F32)
+        hipLaunchKernelGGL(dense_out_kernel<float>, grid, dim3(256), 0, stream, s, rows, columns, o);
+    else if (o.type == AXC_BF16)
+        hipLaunchKernelGGL(dense_out_kernel<bf16>, grid, dim3(256), 0, stream, s, rows, columns, o);
+    else
+        hipLaunchKernelGGL(dense_out_kernel<f16>, grid, dim3(256), 0, stream, s, rows, columns, o);
+    return hipGetLastError();
+}
+
+} // namespace axc

@@ -1,0 +1,411 @@
+// Products of a layer's backward pass: gradients times codes.
+//
+//   dz = dy activation'(pre)                                  [M][N]
+//   dx[m][k]  = s_k  sum_n dz[m][n] (b[k][n] - z_k)           where x lies inside its grid, else 0
+//   dkernel[k][n] = s_in sum_m (a[m][k] - z_in) dz[m][n]      where the kernel does
+//
+// Codes minus their zero point are whole numbers of at most 8 bits: bfloat16 holds them exactly, so the matrix cores' bfloat16
+// instructions multiply them without a rounding.  The gradient is the other operand.  For a bfloat16 result it is rounded to
+// bfloat16 itself; for float16 it is the sum of two bfloat16 terms (16 bits), for float32 of three (24 bits, all that a float
+// has), and the product runs over the terms one after the other as over a longer depth.  Sums are float32 throughout.
+//
+// Both products run over the depth that is contiguous in both operands: dz is written straight and turned, the input's codes
+// turned, the kernel's straight.  All are padded with zeros to whole tiles, so the product has no edges to look at but in its
+// stores.
+#include "layers_internal.h"
+
+namespace axc {
+namespace {
+
+__device__ __forceinline__ void load4_any(const void *p, int64_t at, int64_t n, int type, float (&v)[4])
+{
+    if (type == AXC_F32) {
+        const float *const q = static_cast<const float *>(p) + at;
+        load_values<float, 4>(q, n, n >= 4 && ((uintptr_t)q & 15) == 0, 0.0f, v);
+    } else if (type == AXC_BF16) {
+        const bf16 *const q = static_cast<const bf16 *>(p) + at;
+        load_values<bf16, 4>(q, n, n >= 4 && ((uintptr_t)q & 7) == 0, 0.0f, v);
+    } else {
+        const f16 *const q = static_cast<const f16 *>(p) + at;
+        load_values<f16, 4>(q, n, n >= 4 && ((uintptr_t)q & 7) == 0, 0.0f, v);
+    }
+}
+__device__ __forceinline__ void store4_any(void *p, int64_t at, int64_t n, int type, const float (&v)[4])
+{
+    if (type == AXC_F32) {
+        float *const q = static_cast<float *>(p) + at;
+        store_values<float, 4>(q, n, n >= 4 && ((uintptr_t)q & 15) == 0, v);
+    } else if (type == AXC_BF16) {
+        bf16 *const q = static_cast<bf16 *>(p) + at;
+        store_values<bf16, 4>(q, n, n >= 4 && ((uintptr_t)q & 7) == 0, v);
+    } else {
+        f16 *const q = static_cast<f16 *>(p) + at;
+        store_values<f16, 4>(q, n, n >= 4 && ((uintptr_t)q & 7) == 0, v);
+    }
+}
+
+// Four neighbouring values as `parts` terms, `pitch` elements from one term to the next.
+__device__ __forceinline__ void store_terms(bf16 *p, int parts, int64_t pitch, float (&v)[4])
+{
+    for (int t = 0; t < parts; ++t) {
+        bf16x4 b;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            b[j] = (bf16)v[j];
+            v[j] = __fsub_rn(v[j], (float)b[j]);   // exact; of an infinity or NaN it is NaN, and so is the sum of the terms
+        }
+        *reinterpret_cast<bf16x4 *>(p + t * pitch) = b;
+    }
+}
+
+// Gradient in front of the product, 64 x 64 of it a workgroup: straight, turned through LDS, and summed by columns.
+template <bool LOSS>
+__global__ void __launch_bounds__(256) grad_terms_kernel(GradSource g, int64_t rows, int64_t cols, int64_t ld,
+                                                         int straight_parts, bf16 *__restrict__ straight, int turned_parts,
+                                                         bf16 *__restrict__ turned, float *__restrict__ column_partials)
+{
+    __shared__ float tile[64][65];
+    const int64_t r0 = (int64_t)blockIdx.y * 64, c0 = (int64_t)blockIdx.x * 64;
+    const int64_t rows_pad = (int64_t)gridDim.y * 64, cols_pad = (int64_t)gridDim.x * 64;
+    const int quad = (threadIdx.x & 15) * 4, line = threadIdx.x / 16;
+    const int64_t c = c0 + quad;
+    float scale = 0.0f, bias[4] = {};
+    int64_t column[4] = {};
+    if constexpr (LOSS) {
+        scale = __fmul_rn(g.sums.grids->in.scale, g.sums.grids->kernel.scale);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (c + j < cols) {
+                column[j] = (int64_t)g.sums.grids->in.zero * g.sums.column_sums[c + j];
+                bias[j] = g.bias ? load_any(g.bias, c + j, g.bias_type) : 0.0f;
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t r = r0 + line + 16 * i;
+        float v[4] = {};
+        if (r < rows && c < cols) {
+            if constexpr (LOSS) {
+                const float share = g.coefficient[r], lse = g.lse[r];
+                if (share != 0.0f) {   // a row that does not count has no gradient, whatever its logits are
+                    const int64_t row = row_term(g.sums, r), target = g.targets[r] - g.first_column;
+                    const int32_t *const acc = g.sums.acc + r * g.sums.pitch + c;
+                    int32_t t[4] = {};
+                    for (int k = 0; k < g.sums.splits; ++k) {
+                        const i32x4 a = *reinterpret_cast<const i32x4 *>(acc + k * g.sums.split_stride);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            t[j] += a[j];
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        float z = __fmul_rn((float)((int64_t)t[j] + row - column[j]), scale);
+                        if (g.bias)
+                            z = __fadd_rn(z, bias[j]);
+                        const float p = expf(z - lse);
+                        v[j] = c + j < cols ? share * (c + j == target ? p - 1.0f : p) : 0.0f;
+                    }
+                }
+            } else {
+                load4_any(g.grad, r * ld + c, cols - c, g.type, v);
+                if (g.pre) {
+                    float z[4];
+                    load4_any(g.pre, r * ld + c, cols - c, g.type, z);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (c + j < cols)
+                            v[j] *= activation_slope(z[j], g.activation);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            tile[line + 16 * i][quad + j] = v[j];
+        if (straight)
+            store_terms(straight + r * straight_parts * cols_pad + c, straight_parts, cols_pad, v);
+    }
+    __syncthreads();
+    if (turned)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int col = line + 16 * i;
+            float v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                v[j] = tile[quad + j][col];
+            store_terms(turned + (c0 + col) * turned_parts * rows_pad + r0 + quad, turned_parts, rows_pad, v);
+        }
+    if (column_partials && threadIdx.x < 64) {
+        float sum = 0.0f;
+        for (int i = 0; i < 64; ++i)
+            sum += tile[i][threadIdx.x];
+        column_partials[(int64_t)blockIdx.y * cols_pad + c0 + threadIdx.x] = sum;
+    }
+}
+
+// Codes minus zero point of a tensor, straight or turned, 64 x 64 a workgroup; pads are zeros.
+template <bool TURN>
+__global__ void __launch_bounds__(256) centered_kernel(const void *values, int type, int64_t rows, int64_t cols, int64_t ld,
+                                                       const Grid *grid, bf16 *__restrict__ out)
+{
+    __shared__ float tile[TURN ? 64 : 1][65];
+    const int64_t r0 = (int64_t)blockIdx.y * 64, c0 = (int64_t)blockIdx.x * 64;
+    const int quad = (threadIdx.x & 15) * 4, line = threadIdx.x / 16;
+    const Grid g = *grid;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t r = r0 + line + 16 * i, c = c0 + quad;
+        float v[4] = {};
+        if (r < rows && c < cols) {
+            load4_any(values, r * ld + c, cols - c, type, v);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                v[j] = c + j < cols ? (float)((int)code_of(v[j], g) - g.zero) : 0.0f;
+        }
+        if constexpr (TURN) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                tile[line + 16 * i][quad + j] = v[j];
+        } else {
+            bf16x4 b;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                b[j] = (bf16)v[j];
+            *reinterpret_cast<bf16x4 *>(out + r * ((int64_t)gridDim.x * 64) + c) = b;
+        }
+    }
+    if constexpr (TURN) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int col = line + 16 * i;
+            bf16x4 b;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                b[j] = (bf16)tile[quad + j][col];
+            *reinterpret_cast<bf16x4 *>(out + (c0 + col) * ((int64_t)gridDim.y * 64) + r0 + quad) = b;
+        }
+    }
+}
+
+// Four results that the product or the pass over its partial sums has at (r, c).
+__device__ __forceinline__ void store_result(const ProductOut &o, int64_t r, int64_t c, int64_t cols, float (&v)[4])
+{
+    const float scale = o.factor ? o.scale->scale * *o.factor : o.scale->scale;
+    float at[4];
+    load4_any(o.values, r * o.values_ld + c, cols - c, o.values_type, at);
+    const Grid g = *o.grid;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        v[j] = inside(at[j], g) ? v[j] * scale : 0.0f;
+    store4_any(o.out, r * o.ld + c, cols - c, o.type, v);
+}
+
+constexpr int kStep = 64;   // of the depth
+
+__device__ __forceinline__ void load_to_lds(const bf16 *from, bf16 *to)
+{
+    // 16 bytes a lane, to `to` of the wavefront plus 16 times the lane
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t *)from,
+                                     (__attribute__((address_space(3))) uint32_t *)to, 16, 0, 0);
+}
+
+// A tile of 128 x 128 by four wavefronts, 64 x 64 each; two buffers of 64 of the depth in LDS, filled straight from memory while
+// the other is multiplied.  In LDS a line of 64 elements is eight chunks of 16 bytes, chunk q of line r in place q ^ (r & 7): the
+// 16 lanes that read neighbouring lines then meet different banks.  The loads write LDS in order, so it is their addresses that
+// are exchanged.  PARTIAL: sums go to `partials` (added to what is there with `accumulate`).
+template <bool PARTIAL>
+__global__ void __launch_bounds__(256, 2) product_kernel(const bf16 *__restrict__ a, const bf16 *__restrict__ b, int64_t rows,
+                                                         int64_t cols, int row_tiles, int col_tiles, int depth, int parts,
+                                                         int split_a, int splits, float *__restrict__ partials, int accumulate,
+                                                         ProductOut o)
+{
+    __shared__ __align__(16) bf16 lds[2][2][kProductTile * kStep];
+    // Workgroups go round the eight XCDs; each XCD gets a run of neighbouring tiles, in bands of eight row tiles, so that its L2
+    // serves them.
+    const int tiles = row_tiles * col_tiles * splits;
+    int id = (int)blockIdx.x;
+    {
+        const int per = tiles / 8, more = tiles % 8, xcd = id % 8;
+        id = xcd * per + (xcd < more ? xcd : more) + id / 8;
+    }
+    const int split = id / (row_tiles * col_tiles);
+    id -= split * row_tiles * col_tiles;
+    const int band = id / (8 * col_tiles), in_band = id - band * 8 * col_tiles;
+    const int band_rows = row_tiles - band * 8 < 8 ? row_tiles - band * 8 : 8;
+    const int row_tile = band * 8 + in_band % band_rows, col_tile = in_band / band_rows;
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int per_part = depth / kStep, steps = per_part * parts;
+    const int first = (int)((int64_t)steps * split / splits), last = (int)((int64_t)steps * (split + 1) / splits);
+    const int64_t lda = split_a ? (int64_t)depth * parts : depth, ldb = split_a ? depth : (int64_t)depth * parts;
+    const int line = wave * 32 + lane / 8, chunk = ((lane & 7) ^ (lane >> 3)) * 8;
+    const bf16 *const pa = a + ((int64_t)row_tile * kProductTile + line) * lda + chunk;
+    const bf16 *const pb = b + ((int64_t)col_tile * kProductTile + line) * ldb + chunk;
+
+    auto fetch = [&](int step, int buffer) {
+        const int wrapped = step % per_part;
+        const int64_t ka = (int64_t)(split_a ? step : wrapped) * kStep, kb = (int64_t)(split_a ? wrapped : step) * kStep;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            load_to_lds(pa + ka + i * 8 * lda, &lds[buffer][0][(wave * 32 + i * 8) * kStep]);
+            load_to_lds(pb + kb + i * 8 * ldb, &lds[buffer][1][(wave * 32 + i * 8) * kStep]);
+        }
+    };
+
+    f32x4 acc[4][4] = {};
+    const int wr = (wave >> 1) * 64, wc = (wave & 1) * 64, in_line = lane & 15, group = lane >> 4;
+    if (first < last)
+        fetch(first, 0);
+    for (int step = first; step < last; ++step) {
+        const int buffer = (step - first) & 1;
+        // This buffer is full, by all wavefronts' loads (a barrier alone does not wait for loads into LDS), and the other is no
+        // longer read.
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (step + 1 < last)
+            fetch(step + 1, buffer ^ 1);
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            bf16x8 fa[4], fb[4];
+            const int place = ((kk * 4 + group) ^ (in_line & 7)) * 8;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                fa[i] = *reinterpret_cast<const bf16x8 *>(&lds[buffer][0][(wr + i * 16 + in_line) * kStep + place]);
+                fb[i] = *reinterpret_cast<const bf16x8 *>(&lds[buffer][1][(wc + i * 16 + in_line) * kStep + place]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)   // b first: a lane's four results are neighbours in a row
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j], fa[i], acc[i][j], 0, 0, 0);
+        }
+    }
+    const int64_t rows_pad = (int64_t)row_tiles * kProductTile, cols_pad = (int64_t)col_tiles * kProductTile;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t r = (int64_t)row_tile * kProductTile + wr + i * 16 + in_line;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int64_t c = (int64_t)col_tile * kProductTile + wc + j * 16 + group * 4;
+            if constexpr (PARTIAL) {
+                f32x4 *const to = reinterpret_cast<f32x4 *>(partials + ((int64_t)split * rows_pad + r) * cols_pad + c);
+                *to = accumulate ? *to + acc[i][j] : acc[i][j];
+            } else if (r < rows && c < cols) {
+                float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+                store_result(o, r, c, cols, v);
+            }
+        }
+    }
+}
+
+__global__ void __launch_bounds__(256) product_out_kernel(const float *__restrict__ partials, int splits, int64_t rows, int64_t cols,
+                                                          int64_t rows_pad, int64_t cols_pad, ProductOut o)
+{
+    const int64_t c = ((int64_t)blockIdx.x * 64 + (threadIdx.x & 63)) * 4;
+    if (c >= cols)
+        return;
+    for (int64_t r = (int64_t)blockIdx.y * 4 + threadIdx.x / 64; r < rows; r += (int64_t)gridDim.y * 4) {
+        f32x4 sum = {};
+#pragma unroll 4
+        for (int s = 0; s < splits; ++s)
+            sum += *reinterpret_cast<const f32x4 *>(partials + ((int64_t)s * rows_pad + r) * cols_pad + c);
+        float v[4] = {sum[0], sum[1], sum[2], sum[3]};
+        store_result(o, r, c, cols, v);
+    }
+}
+
+// Sums of the column partials, 64 columns a workgroup, in one order.
+__global__ void __launch_bounds__(256) column_sums_kernel(const float *__restrict__ partials, int64_t count, int64_t cols,
+                                                          int64_t pitch, const float *factor, void *out, int type)
+{
+    __shared__ float red[4][64];
+    const int64_t c = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+    float sum = 0.0f;
+    if (c < cols)
+        for (int64_t i = threadIdx.x / 64; i < count; i += 4)
+            sum += partials[i * pitch + c];
+    red[threadIdx.x / 64][threadIdx.x & 63] = sum;
+    __syncthreads();
+    if (threadIdx.x < 64 && c < cols)
+        store_any(out, c, type, ((red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x])) *
+                                    (factor ? *factor : 1.0f));
+}
+
+} // namespace
+
+hipError_t launch_grad_terms(const GradSource &g, bool loss, int64_t rows, int64_t cols, int64_t ld, int straight_parts,
+                             bf16 *straight, int turned_parts, bf16 *turned, float *column_partials, hipStream_t stream)
+{
+    const dim3 grid((unsigned)(product_pad(cols) / 64), (unsigned)(product_pad(rows) / 64));
+    if (loss)
+        hipLaunchKernelGGL(grad_terms_kernel<true>, grid, dim3(256), 0, stream, g, rows, cols, ld, straight_parts, straight,
+                           turned_parts, turned, column_partials);
+    else
+        hipLaunchKernelGGL(grad_terms_kernel<false>, grid, dim3(256), 0, stream, g, rows, cols, ld, straight_parts, straight,
+                           turned_parts, turned, column_partials);
+    return hipGetLastError();
+}
+
+hipError_t launch_centered(const void *v, int type, int64_t rows, int64_t cols, int64_t ld, const Grid *grid, bool turn, bf16 *out,
+                           hipStream_t stream)
+{
+    const dim3 blocks((unsigned)(product_pad(cols) / 64), (unsigned)(product_pad(rows) / 64));
+    if (turn)
+        hipLaunchKernelGGL(centered_kernel<true>, blocks, dim3(256), 0, stream, v, type, rows, cols, ld, grid, out);
+    else
+        hipLaunchKernelGGL(centered_kernel<false>, blocks, dim3(256), 0, stream, v, type, rows, cols, ld, grid, out);
+    return hipGetLastError();
+}
+
+ProductPlan plan_product(int64_t rows, int64_t cols, int64_t depth_pad, int parts, bool keep)
+{
+    const int64_t tiles = (product_pad(rows) / kProductTile) * (product_pad(cols) / kProductTile);
+    const int64_t steps = depth_pad / kStep * parts;
+    int64_t splits = tiles >= 256 ? 1 : 512 / tiles;
+    if (splits > steps / 4)
+        splits = steps / 4;
+    if (splits < 1)
+        splits = 1;
+    ProductPlan plan = {(int)splits, 0};
+    if (splits > 1 || keep)
+        plan.partial_bytes = (size_t)splits * product_pad(rows) * product_pad(cols) * sizeof(float);
+    return plan;
+}
+
+hipError_t launch_product(const bf16 *a, const bf16 *b, int64_t rows, int64_t cols, int64_t depth_pad, int parts, bool split_a,
+                          const ProductPlan &plan, float *partials, bool keep, bool accumulate, const ProductOut &o,
+                          hipStream_t stream)
+{
+    const int row_tiles = (int)(product_pad(rows) / kProductTile), col_tiles = (int)(product_pad(cols) / kProductTile);
+    const dim3 grid((unsigned)((int64_t)row_tiles * col_tiles * plan.splits));
+    if (plan.splits > 1 || keep) {
+        hipLaunchKernelGGL(product_kernel<true>, grid, dim3(256), 0, stream, a, b, rows, cols, row_tiles, col_tiles, (int)depth_pad,
+                           parts, (int)split_a, plan.splits, partials, (int)accumulate, o);
+        if (hipError_t e = hipGetLastError())
+            return e;
+        return keep ? hipSuccess : launch_product_out(partials, plan.splits, rows, cols, o, stream);
+    }
+    hipLaunchKernelGGL(product_kernel<false>, grid, dim3(256), 0, stream, a, b, rows, cols, row_tiles, col_tiles, (int)depth_pad,
+                       parts, (int)split_a, 1, partials, 0, o);
+    return hipGetLastError();
+}
+
+hipError_t launch_product_out(const float *partials, int splits, int64_t rows, int64_t cols, const ProductOut &o,
+                              hipStream_t stream)
+{
+    const int64_t by = (rows + 3) / 4;
+    hipLaunchKernelGGL(product_out_kernel, dim3((unsigned)((cols + 255) / 256), (unsigned)(by > 16384 ? 16384 : by)), dim3(256), 0,
+                       stream, partials, splits, rows, cols, product_pad(rows), product_pad(cols), o);
+    return hipGetLastError();
+}
+
+hipError_t launch_column_sums(const float *partials, int64_t count, int64_t cols, int64_t pitch, const float *factor, void *out,
+                              int type, hipStream_t stream)
+{
+    hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)((cols + 63) / 64)), dim3(256), 0, stream, partials, count, cols, pitch,
+                       factor, out, type);
+    return hipGetLastError();
+}
+
+} // namespace axc

@@ -1,0 +1,868 @@
+// C-ABI entry points of the transformer layers: checks, workspaces, launches.
+#include "layers_internal.h"
+
+#include <string.h>
+
+#include <algorithm>
+
+using namespace axc;
+
+namespace {
+
+#define AXC_HIP(call)                                \
+    do {                                             \
+        hipError_t e_ = (call);                      \
+        if (e_ != hipSuccess)                        \
+            return api_fail_hip(e_, #call);          \
+    } while (0)
+
+bool known_type(int type) { return type == AXC_F32 || type == AXC_BF16 || type == AXC_F16; }
+
+int check_desc(const axc_dense_desc *d)
+{
+    if (!d)
+        return api_fail(AXC_INVALID_ARGUMENT, "null argument");
+    if (d->rows < 0 || d->columns < 0 || d->depth < 0)
+        return api_fail(AXC_INVALID_ARGUMENT, "rows, depth and columns must not be negative");
+    if (d->depth < 1)
+        return api_fail(AXC_INVALID_ARGUMENT, "depth must be at least 1");
+    if (d->depth >= 32768)   // 32768 * 65535 would overflow the int32 accumulator
+        return api_fail(AXC_INVALID_ARGUMENT, "depth must be below 32768 for int32 accumulation");
+    const int64_t most = ((int64_t)1 << 31) - 256;
+    if (d->rows > most || d->columns > most || d->rows * d->columns >= ((int64_t)1 << 40) ||
+        d->columns * d->depth >= ((int64_t)1 << 40))
+        return api_fail(AXC_INVALID_ARGUMENT, "tensor too large");
+    if (!known_type(d->input_type) || !known_type(d->kernel_type) || !known_type(d->bias_type))
+        return api_fail(AXC_INVALID_ARGUMENT, "unknown element type");
+    if (d->activation < AXC_ACT_NONE || d->activation > AXC_ACT_SILU)
+        return api_fail(AXC_INVALID_ARGUMENT, "unknown activation");
+    return AXC_OK;
+}
+constexpr int64_t kMostGradientRows = (int64_t)65535 * 64 / kProductTile * kProductTile;   // 64 a workgroup, in the grid's y
+
+// Hands out parts of a workspace; without one it only counts.
+class Carver {
+public:
+    explicit Carver(void *base) : base_(static_cast<char *>(base)) {}
+    template <typename T>
+    T *take(size_t n)
+    {
+        T *const p = base_ ? reinterpret_cast<T *>(base_ + at_) : nullptr;
+        at_ += (n * sizeof(T) + 255) & ~(size_t)255;
+        return p;
+    }
+    size_t bytes() const { return at_; }
+
+private:
+    char *base_;
+    size_t at_ = 0;
+};
+
+int check_workspace(const void *workspace, size_t have, size_t need)
+{
+    if (have < need || (!workspace && need))
+        return api_fail(AXC_INVALID_ARGUMENT, "workspace too small (see the call's workspace query)");
+    if (((uintptr_t)workspace & 255) != 0)
+        return api_fail(AXC_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
+    return AXC_OK;
+}
+
+const void *element(const void *p, int64_t i, int type) { return p ? static_cast<const char *>(p) + i * type_bytes(type) : nullptr; }
+void *element(void *p, int64_t i, int type) { return p ? static_cast<char *>(p) + i * type_bytes(type) : nullptr; }
+
+int64_t fours(int64_t n) { return (n + 3) & ~(int64_t)3; }
+
+// Columns in pieces of about the same width, `most` at most.
+Pieces pieces_of(int64_t depth, int64_t columns, int64_t most)
+{
+    Pieces p = {};
+    p.Np = fours(columns);
+    p.Kp = (int32_t)fours(depth);
+    const int64_t count = std::max<int64_t>(1, (p.Np + most - 1) / most);
+    const int64_t each = (p.Np + count - 1) / count;
+    p.width = (int32_t)std::min<int64_t>(std::max<int64_t>(4, p.Np), (each + 63) / 64 * 64);
+    p.count = (int32_t)std::max<int64_t>(1, (p.Np + p.width - 1) / p.width);
+    return p;
+}
+
+// ---- sums of table entries: input codes [rows][Kp] by a piece of the kernel's ----
+constexpr int64_t kRowRun = 16384;       // rows a LUT-GEMM call takes (its rows must be below 32768)
+constexpr int64_t kSumsAtOnce = (int64_t)1 << 25;   // int32 sums in the workspace: 128 MiB, half the memory-side cache
+constexpr int64_t kFewRowsMost = 16;
+
+bool few_rows(int64_t rows) { return rows <= kFewRowsMost; }
+
+axc_conv2d_desc conv_desc(int64_t rows, int Kp, int width)
+{
+    axc_conv2d_desc c;
+    memset(&c, 0, sizeof(c));
+    c.input_shape[0] = c.input_shape[1] = 1;
+    c.input_shape[2] = rows;
+    c.input_shape[3] = Kp;
+    c.filter_shape[0] = c.filter_shape[1] = 1;
+    c.filter_shape[2] = Kp;
+    c.filter_shape[3] = width;
+    for (int i = 0; i < 4; ++i)
+        c.strides[i] = c.dilations[i] = 1;
+    c.padding = AXC_PAD_VALID;
+    c.data_format = AXC_FORMAT_NHWC;
+    c.num_bits = 8;
+    return c;
+}
+
+// What the sums of `rows` rows (of up to kRowRun at a time) and any piece need beside their own memory.
+int sums_workspace(int64_t rows, const Pieces &pc, size_t *bytes)
+{
+    *bytes = 0;
+    if (few_rows(rows))
+        return AXC_OK;
+    const int64_t runs[2] = {std::min(fours(rows), kRowRun), fours(rows) % kRowRun};
+    const int widths[2] = {pc.width_of(0), pc.width_of(pc.count - 1)};
+    for (const int64_t run : runs)
+        for (const int width : widths) {
+            if (run == 0)
+                continue;
+            const axc_conv2d_desc c = conv_desc(run, pc.Kp, width);
+            size_t need = 0;
+            if (int rc = axc_conv2d_workspace_bytes(&c, &need))
+                return rc;
+            *bytes = std::max(*bytes, need);
+        }
+    return AXC_OK;
+}
+size_t sums_count(int64_t rows, const Pieces &pc)   // int32 values
+{
+    if (!few_rows(rows))
+        return (size_t)fours(rows) * pc.width;
+    size_t most = 0;
+    for (const int width : {pc.width_of(0), pc.width_of(pc.count - 1)})
+        most = std::max(most, (size_t)few_rows_splits(rows, pc.Kp, width) * rows * width);
+    return most;
+}
+
+// Sums of `rows` rows and piece p into acc.
+int table_sums(const axc_table *table, const uint8_t *input_codes, int64_t rows, const Pieces &pc, int p, const uint8_t *kernel_codes,
+               int32_t *acc, void *ws, size_t ws_bytes, hipStream_t stream, TableSums *out)
+{
+    const int width = pc.width_of(p);
+    const uint8_t *const codes = kernel_codes + pc.offset(p);
+    out->acc = acc;
+    out->pitch = width;
+    out->splits = 1;
+    out->split_stride = 0;
+    if (few_rows(rows)) {
+        out->splits = few_rows_splits(rows, pc.Kp, width);
+        out->split_stride = rows * width;
+        ApiTimer t("few_rows", stream);
+        AXC_HIP(launch_few_rows(table->dev_tableI, input_codes, (int)rows, pc.Kp, codes, width, out->splits, acc, stream));
+        return AXC_OK;
+    }
+    for (int64_t r = 0; r < fours(rows); r += kRowRun) {
+        const axc_conv2d_desc c = conv_desc(std::min(kRowRun, fours(rows) - r), pc.Kp, width);
+        if (int rc = axc_conv2d_codes_acc_i32(table, &c, input_codes + r * pc.Kp, codes, 0, acc + r * width, ws, ws_bytes, stream))
+            return rc;
+    }
+    return AXC_OK;
+}
+
+// ---- operands ----
+struct Operands {
+    Grids *grids;
+    float *x_pairs, *kernel_pairs;
+    uint8_t *x_codes, *kernel_codes;
+    int32_t *row_sums, *column_sums;
+};
+
+Operands carve_operands(Carver &c, const axc_dense_desc *d, const Pieces &pc, bool with_kernel, bool codes)
+{
+    Operands o = {};
+    o.grids = c.take<Grids>(1);
+    o.x_pairs = c.take<float>(2 * kRangeBlocks);
+    o.kernel_pairs = c.take<float>(2 * kRangeBlocks);
+    if (codes) {
+        o.x_codes = c.take<uint8_t>((size_t)fours(d->rows) * pc.Kp);
+        o.row_sums = c.take<int32_t>((size_t)fours(d->rows));
+    }
+    if (codes && with_kernel) {
+        o.kernel_codes = c.take<uint8_t>(pc.bytes());
+        o.column_sums = c.take<int32_t>((size_t)pc.Np);
+    }
+    return o;
+}
+
+RangeSource input_source(const axc_dense_desc *d, const void *range)
+{
+    if (d->range_known)
+        return {nullptr, 0, d->input_min, d->input_max};
+    if (range)
+        return {static_cast<const float *>(range), kRangePairs, 0.0f, 0.0f};
+    return {nullptr, -1, 0.0f, 0.0f};
+}
+
+// Grids of input and kernel (kernel_grid: it is known already), and the column sums cleared.
+int find_grids(const axc_dense_desc *d, const void *input, const void *range, const void *kernel, const Operands &o, int64_t Np,
+               hipStream_t stream)
+{
+    RangeSource in = input_source(d, range), k = {o.kernel_pairs, 0, 0.0f, 0.0f};
+    const bool look = !in.pairs && in.count < 0;
+    int x_count = 0, k_count = 0;
+    {
+        ApiTimer t("layer_range", stream);
+        AXC_HIP(launch_range(look ? input : nullptr, d->input_type, d->rows * d->depth, kernel, d->kernel_type,
+                             d->depth * d->columns, o.x_pairs, o.kernel_pairs, o.column_sums, o.column_sums ? Np : 0, &x_count,
+                             &k_count, stream));
+    }
+    if (look)
+        in = {o.x_pairs, x_count, 0.0f, 0.0f};
+    k.count = k_count;
+    ApiTimer t("layer_grids", stream);
+    AXC_HIP(launch_grids(in, k, true, true, o.grids, stream));
+    return AXC_OK;
+}
+
+int make_codes(const axc_dense_desc *d, const void *input, const void *kernel, const Operands &o, const Pieces &pc, hipStream_t stream)
+{
+    ApiTimer t("layer_codes", stream);
+    AXC_HIP(launch_input_codes(input, d->input_type, d->rows, (int)d->depth, pc.Kp, o.grids, o.x_codes, o.row_sums, stream));
+    AXC_HIP(launch_kernel_codes(kernel, d->kernel_type, (int)d->depth, d->columns, pc, o.grids, o.kernel_codes, o.column_sums,
+                                stream));
+    return AXC_OK;
+}
+
+// ---- dense ----
+constexpr int64_t kDensePiece = 8192;    // columns; packed kernels are laid out by it, whatever rows they meet
+
+struct Packed {                          // a packed kernel
+    Grids *grids;
+    float *pairs;
+    int32_t *column_sums;
+    uint8_t *codes;
+    size_t bytes;
+};
+Packed packed_parts(const Pieces &pc, void *base)
+{
+    Carver c(base);
+    Packed p = {};
+    p.grids = c.take<Grids>(1);
+    p.pairs = c.take<float>(2 * kRangeBlocks);
+    p.column_sums = c.take<int32_t>((size_t)pc.Np);
+    p.codes = c.take<uint8_t>(pc.bytes());
+    p.bytes = c.bytes();
+    return p;
+}
+
+int64_t dense_run(int64_t rows, const Pieces &pc)   // rows whose sums are in the workspace at a time
+{
+    const int64_t run = std::min(kRowRun, std::max<int64_t>(1024, kSumsAtOnce / pc.width & ~(int64_t)3));
+    return std::min(fours(rows), run);
+}
+
+struct DenseScratch {
+    Operands o;
+    int32_t *acc;
+    char *lut;
+    size_t lut_bytes, bytes;
+};
+int carve_dense(const axc_dense_desc *d, bool packed, void *base, DenseScratch *s)
+{
+    const Pieces pc = pieces_of(d->depth, d->columns, kDensePiece);
+    Carver c(base);
+    s->o = carve_operands(c, d, pc, !packed, true);
+    s->lut_bytes = 0;
+    size_t count = 0;
+    const int64_t run = dense_run(d->rows, pc), rest = run ? d->rows % run : 0;
+    for (const int64_t rows : {few_rows(d->rows) ? d->rows : run, rest}) {
+        if (rows == 0)
+            continue;
+        size_t need = 0;
+        if (int rc = sums_workspace(rows, pc, &need))
+            return rc;
+        s->lut_bytes = std::max(s->lut_bytes, need);
+        count = std::max(count, sums_count(rows, pc));
+    }
+    s->acc = c.take<int32_t>(count);
+    s->lut = c.take<char>(s->lut_bytes);
+    s->bytes = c.bytes();
+    return AXC_OK;
+}
+
+// ---- gradients ----
+struct GradScratch {
+    Operands o;
+    bf16 *straight, *turned, *x_turned, *kernel;
+    float *column_partials, *partials;
+};
+
+} // namespace
+
+extern "C" {
+
+int axc_dense_packed_bytes(const axc_dense_desc *desc, size_t *bytes)
+{
+    if (int rc = check_desc(desc))
+        return rc;
+    if (!bytes)
+        return api_fail(AXC_INVALID_ARGUMENT, "null argument");
+    *bytes = packed_parts(pieces_of(desc->depth, desc->columns, kDensePiece), nullptr).bytes;
+    return AXC_OK;
+}
+
+int axc_dense_pack(const axc_dense_desc *desc, const void *kernel, void *packed, void *stream_v)
+{
+    if (int rc = check_desc(desc))
+        return rc;
+    if (desc->columns == 0)
+        return AXC_OK;
+    if (!kernel || !packed)
+        return api_fail(AXC_INVALID_ARGUMENT, "null tensor pointer");
+    if (((uintptr_t)packed & 255) != 0)
+        return api_fail(AXC_INVALID_ARGUMENT, "a packed kernel must be 256-byte aligned");
+    hipStream_t stream = static_cast<hipStream_t>(stream_v);
+    const Pieces pc = pieces_of(desc->depth, desc->columns, kDensePiece);
+    const Packed p = packed_parts(pc, packed);
+    int unused = 0, count = 0;
+    ApiTimer t("dense_pack", stream);
+    AXC_HIP(launch_range(nullptr, AXC_F32, 0, kernel, desc->kernel_type, desc->depth * desc->columns, nullptr, p.pairs,
+                         p.column_sums, pc.Np, &unused, &count, stream));
+    AXC_HIP(launch_grids({}, {p.pairs, count, 0.0f, 0.0f}, false, true, p.grids, stream));
+    AXC_HIP(launch_kernel_codes(kernel, desc->kernel_type, (int)desc->depth, desc->columns, pc, p.grids, p.codes, p.column_sums,
+                                stream));
+    return AXC_OK;
+}
+
+int axc_fake_approx_dense_workspace_bytes(const axc_dense_desc *desc, int packed, size_t *bytes)
+{
+    if (int rc = check_desc(desc))
+        return rc;
+    if (!bytes)
+        return api_fail(AXC_INVALID_ARGUMENT, "null argument");
+    *bytes = 0;
+    if (desc->rows == 0 || desc->columns == 0)
+        return AXC_OK;
+    DenseScratch s;
+    if (int rc = carve_dense(desc, packed != 0, nullptr, &s))
+        return rc;
+    *bytes = s.bytes;
+    return AXC_OK;
+}
+
+int axc_fake_approx_dense(const axc_table *table, const axc_dense_desc *desc, const void *input, const void *input_range,
+                          const void *kernel, const void *packed, const void *bias, const void *residual, void *output, void *pre,
+                          void *workspace, size_t workspace_bytes, void *stream_v)
+{
+    if (!table)
+        return api_fail(AXC_INVALID_ARGUMENT, "null argument");
+    if (int rc = check_desc(desc))
+        return rc;
+    if (int rc = api_check_table(table))
+        return rc;
+    if (desc->rows == 0 || desc->columns == 0)
+        return AXC_OK;
+    if (!input || !output || (!kernel && !packed))
+        return api_fail(AXC_INVALID_ARGUMENT, "null tensor pointer");
+    if (kernel && packed)
+        return api_fail(AXC_INVALID_ARGUMENT, "either a kernel or a packed one");
+    const Pieces pc = pieces_of(desc->depth, desc->columns, kDensePiece);
+    DenseScratch s;
+    if (int rc = carve_dense(desc, packed != nullptr, workspace, &s))
+        return rc;
+    if (int rc = check_workspace(workspace, workspace_bytes, s.bytes))
+        return rc;
+    hipStream_t stream = static_cast<hipStream_t>(stream_v);
+    const int K = (int)desc->depth;
+    Operands &o = s.o;
+    if (packed) {
+        const Packed p = packed_parts(pc, const_cast<void *>(packed));
+        o.kernel_codes = p.codes;
+        o.column_sums = p.column_sums;
+        RangeSource in = input_source(desc, input_range);
+        if (few_rows(desc->rows)) {
+            ApiTimer t("layer_codes", stream);
+            AXC_HIP(launch_few_codes(input, desc->input_type, (int)desc->rows, K, pc.Kp, in, &p.grids->kernel, o.grids, o.x_codes,
+                                     o.row_sums, stream));
+        } else {
+            if (!in.pairs && in.count < 0) {
+                int count = 0, unused = 0;
+                ApiTimer t("layer_range", stream);
+                AXC_HIP(launch_range(input, desc->input_type, desc->rows * desc->depth, nullptr, AXC_F32, 0, o.x_pairs, nullptr,
+                                     nullptr, 0, &count, &unused, stream));
+                in = {o.x_pairs, count, 0.0f, 0.0f};
+            }
+            {
+                // (the kernel's range as pairs again: what it was packed with)
+                const int64_t n = desc->depth * desc->columns;
+                const int count = (int)std::min<int64_t>((n + 16383) / 16384, kRangeBlocks);
+                ApiTimer t("layer_grids", stream);
+                AXC_HIP(launch_grids(in, {p.pairs, count, 0.0f, 0.0f}, true, true, o.grids, stream));
+            }
+            ApiTimer t("layer_codes", stream);
+            AXC_HIP(launch_input_codes(input, desc->input_type, desc->rows, K, pc.Kp, o.grids, o.x_codes, o.row_sums, stream));
+        }
+    } else {
+        if (int rc = find_grids(desc, input, input_range, kernel, o, pc.Np, stream))
+            return rc;
+        if (int rc = make_codes(desc, input, kernel, o, pc, stream))
+            return rc;
+    }
+    const int64_t run = few_rows(desc->rows) ? desc->rows : dense_run(desc->rows, pc);
+    for (int p = 0; p < pc.count; ++p)
+        for (int64_t r = 0; r < desc->rows; r += run) {
+            const int64_t rows = std::min(run, desc->rows - r), c = pc.first(p);
+            TableSums sums = {};
+            if (int rc = table_sums(table, o.x_codes + r * pc.Kp, rows, pc, p, o.kernel_codes, s.acc, s.lut, s.lut_bytes, stream,
+                                    &sums))
+                return rc;
+            sums.row_sums = o.row_sums + r;
+            sums.column_sums = o.column_sums + c;
+            sums.table = table->dev_tableT;
+            sums.grids = o.grids;
+            sums.K = K;
+            sums.pad = pc.Kp - K;
+            const int64_t at = r * desc->columns + c;
+            const DenseOut out = {element(bias, c, desc->bias_type), element(residual, at, desc->input_type),
+                                  element(output, at, desc->input_type), element(pre, at, desc->input_type), desc->bias_type,
+                                  desc->input_type, desc->activation, desc->columns};
+            ApiTimer t("dense_out", stream);
+            AXC_HIP(launch_dense_out(sums, rows, (int)std::min<int64_t>(pc.width_of(p), desc->columns - c), out, stream));
+        }
+    return AXC_OK;
+}
+
+// Operands and workspace of the gradients.
+static int carve_gradients(const axc_dense_desc *d, void *base, GradScratch *s, size_t *bytes)
+{
+    if (d->rows > kMostGradientRows)
+        return api_fail(AXC_UNIMPLEMENTED, "gradients of more than 4194176 rows");
+    const Pieces pc = pieces_of(d->depth, d->columns, kDensePiece);
+    const int64_t M = product_pad(d->rows), N = product_pad(d->columns), K = product_pad(d->depth);
+    const int px = parts_of(d->input_type), pk = parts_of(d->kernel_type);
+    Carver c(base);
+    s->o = carve_operands(c, d, pc, false, false);
+    s->straight = c.take<bf16>((size_t)M * N * px);
+    s->turned = c.take<bf16>((size_t)M * N * pk);
+    s->x_turned = c.take<bf16>((size_t)M * K);
+    s->kernel = c.take<bf16>((size_t)K * N);
+    s->column_partials = c.take<float>((size_t)(M / 64) * N);
+    s->partials = reinterpret_cast<float *>(c.take<char>(std::max(plan_product(d->rows, d->depth, N, px, false).partial_bytes,
+                                                                  plan_product(d->depth, d->columns, M, pk, false).partial_bytes)));
+    *bytes = c.bytes();
+    return AXC_OK;
+}
+
+int axc_fake_approx_dense_gradients_workspace_bytes(const axc_dense_desc *desc, size_t *bytes)
+{
+    if (int rc = check_desc(desc))
+        return rc;
+    if (!bytes)
+        return api_fail(AXC_INVALID_ARGUMENT, "null argument");
+    *bytes = 0;
+    if (desc->rows == 0 || desc->columns == 0)
+        return AXC_OK;
+    GradScratch s;
+    return carve_gradients(desc, nullptr, &s, bytes);
+}
+
+static int fill_zero(void *p, int64_t n, int type, hipStream_t stream)
+{
+    if (!p || n == 0)
+        return AXC_OK;
+    AXC_HIP(launch_zero(p, n * type_bytes(type), stream));
+    return AXC_OK;
+}
+
+int axc_fake_approx_dense_gradients(const axc_dense_desc *desc, const void *grad_output, const void *input,
+                                    const void *input_range, const void *kernel, const void *pre, void *grad_input,
+                                    void *grad_kernel, void *grad_bias, void *workspace, size_t workspace_bytes, void *stream_v)
+{
+    if (int rc = check_desc(desc))
+        return rc;
+    hipStream_t stream = static_cast<hipStream_t>(stream_v);
+    if (desc->rows == 0 || desc->columns == 0) {   // empty sums
+        if (int rc = fill_zero(grad_input, desc->rows * desc->depth, desc->input_type, stream))
+            return rc;
+        if (int rc = fill_zero(grad_kernel, desc->depth * desc->columns, desc->kernel_type, stream))
+            return rc;
+        return fill_zero(grad_bias, desc->columns, desc->kernel_type, stream);
+    }
+    if (!grad_output || !input || !kernel)
+        return api_fail(AXC_INVALID_ARGUMENT, "null tensor pointer");
+    if (!pre && desc->activation != AXC_ACT_NONE)
+        return api_fail(AXC_INVALID_ARGUMENT, "the gradient of an activation needs what the activation was given");
+    GradScratch s;
+    size_t need = 0;
+    if (int rc = carve_gradients(desc, workspace, &s, &need))
+        return rc;
+    if (int rc = check_workspace(workspace, workspace_bytes, need))
+        return rc;
+    if (!grad_input && !grad_kernel && !grad_bias)
+        return AXC_OK;
+    const int64_t rows = desc->rows, K = desc->depth, N = desc->columns;
+    const int px = parts_of(desc->input_type), pk = parts_of(desc->kernel_type);
+    if (int rc = find_grids(desc, input, input_range, kernel, s.o, 0, stream))
+        return rc;
+    {
+        GradSource g = {};
+        g.grad = grad_output;
+        g.pre = desc->activation == AXC_ACT_NONE ? nullptr : pre;
+        g.type = desc->input_type;
+        g.activation = desc->activation;
+        ApiTimer t("grad_terms", stream);
+        AXC_HIP(launch_grad_terms(g, false, rows, N, N, px, grad_input ? s.straight : nullptr, pk, grad_kernel ? s.turned : nullptr,
+                                  grad_bias ? s.column_partials : nullptr, stream));
+    }
+    if (grad_bias) {
+        ApiTimer t("column_sums", stream);
+        AXC_HIP(launch_column_sums(s.column_partials, product_pad(rows) / 64, N, product_pad(N), nullptr, grad_bias,
+                                   desc->kernel_type, stream));
+    }
+    if (grad_input) {
+        {
+            ApiTimer t("centered", stream);
+            AXC_HIP(launch_centered(kernel, desc->kernel_type, K, N, N, &s.o.grids->kernel, false, s.kernel, stream));
+        }
+        const ProductOut o = {grad_input, desc->input_type, K, input, desc->input_type, K, &s.o.grids->in, &s.o.grids->kernel,
+                              nullptr};
+        ApiTimer t("grad_product", stream);
+        AXC_HIP(launch_product(s.straight, s.kernel, rows, K, product_pad(N), px, true, plan_product(rows, K, product_pad(N), px, false),
+                               s.partials, false, false, o, stream));
+    }
+    if (grad_kernel) {
+        {
+            ApiTimer t("centered", stream);
+            AXC_HIP(launch_centered(input, desc->input_type, rows, K, K, &s.o.grids->in, true, s.x_turned, stream));
+        }
+        const ProductOut o = {grad_kernel, desc->kernel_type, N, kernel, desc->kernel_type, N, &s.o.grids->kernel, &s.o.grids->in,
+                              nullptr};
+        ApiTimer t("grad_product", stream);
+        AXC_HIP(launch_product(s.x_turned, s.turned, K, N, product_pad(rows), pk, false,
+                               plan_product(K, N, product_pad(rows), pk, false), s.partials, false, false, o, stream));
+    }
+    return AXC_OK;
+}
+
+// ---- loss ----
+static Pieces loss_pieces(const axc_dense_desc *d)
+{
+    const int64_t most = kSumsAtOnce / fours(std::max<int64_t>(1, d->rows)) & ~(int64_t)255;
+    return pieces_of(d->depth, d->columns, std::min<int64_t>(16384, std::max<int64_t>(1024, most)));
+}
+
+struct LossScratch {
+    Operands o;
+    LossState st;
+    int32_t *acc;
+    char *lut;
+    size_t lut_bytes, bytes;
+    bf16 *straight, *turned, *x_turned, *kernel;
+    float *column_partials, *kernel_partials, *input_partials;
+};
+static int carve_loss(const axc_dense_desc *d, bool gradients, void *base, LossScratch *s)
+{
+    if (d->rows > kMostGradientRows)
+        return api_fail(AXC_UNIMPLEMENTED, "a loss of more than 4194176 rows");
+    const Pieces pc = loss_pieces(d);
+    Carver c(base);
+    s->o = carve_operands(c, d, pc, true, true);
+    float **const state[] = {&s->st.top, &s->st.sum, &s->st.at, &s->st.lse, &s->st.rows, &s->st.coefficient};
+    for (float **p : state)
+        *p = c.take<float>((size_t)d->rows);
+    s->st.factor = c.take<float>(1);
+    if (int rc = sums_workspace(d->rows, pc, &s->lut_bytes))
+        return rc;
+    s->acc = c.take<int32_t>(sums_count(d->rows, pc));
+    s->lut = c.take<char>(s->lut_bytes);
+    if (gradients) {
+        const int64_t M = product_pad(d->rows), P = product_pad(pc.width), K = product_pad(d->depth);
+        const int px = parts_of(d->input_type), pk = parts_of(d->kernel_type);
+        s->straight = c.take<bf16>((size_t)M * P * px);
+        s->turned = c.take<bf16>((size_t)M * P * pk);
+        s->x_turned = c.take<bf16>((size_t)M * K);
+        s->kernel = c.take<bf16>((size_t)K * P);
+        s->column_partials = c.take<float>((size_t)(M / 64) * P);
+        size_t most = 0;
+        for (const int width : {pc.width_of(0), pc.width_of(pc.count - 1)})
+            most = std::max(most, plan_product(d->depth, width, M, pk, false).partial_bytes);
+        s->kernel_partials = reinterpret_cast<float *>(c.take<char>(most));
+        s->input_partials = reinterpret_cast<float *>(c.take<char>(plan_product(d->rows, d->depth, P, px, true).partial_bytes));
+    }
+    s->bytes = c.bytes();
+    return AXC_OK;
+}
+
+int axc_fake_approx_cross_entropy_workspace_bytes(const axc_dense_desc *desc, int gradients, size_t *bytes)
+{
+    if (int rc = check_desc(desc))
+        return rc;
+    if (!bytes)
+        return api_fail(AXC_INVALID_ARGUMENT, "null argument");
+    *bytes = 0;
+    if (desc->rows == 0 || desc->columns == 0)
+        return AXC_OK;
+    LossScratch s;
+    if (int rc = carve_loss(desc, gradients != 0, nullptr, &s))
+        return rc;
+    *bytes = s.bytes;
+    return AXC_OK;
+}
+
+int axc_fake_approx_cross_entropy(const axc_table *table, const axc_dense_desc *desc, const void *input, const void *input_range,
+                                  const void *kernel, const void *bias, const int64_t *targets, int64_t ignore_index,
+                                  int reduction, const float *grad_loss, float *loss, void *grad_input, void *grad_kernel,
+                                  void *grad_bias, void *workspace, size_t workspace_bytes, void *stream_v)
+{
+    if (!table)
+        return api_fail(AXC_INVALID_ARGUMENT, "null argument");
+    if (int rc = check_desc(desc))
+        return rc;
+    if (desc->activation != AXC_ACT_NONE)
+        return api_fail(AXC_INVALID_ARGUMENT, "logits have no activation");
+    if (reduction != AXC_LOSS_NONE && reduction != AXC_LOSS_SUM && reduction != AXC_LOSS_MEAN)
+        return api_fail(AXC_INVALID_ARGUMENT, "unknown reduction");
+    if (desc->columns == 0)
+        return api_fail(AXC_INVALID_ARGUMENT, "a vocabulary must have at least one column");
+    if (int rc = api_check_table(table))
+        return rc;
+    hipStream_t stream = static_cast<hipStream_t>(stream_v);
+    const int64_t rows = desc->rows, K = desc->depth, V = desc->columns;
+    if (!loss && !(rows == 0 && reduction == AXC_LOSS_NONE))
+        return api_fail(AXC_INVALID_ARGUMENT, "null tensor pointer");
+    if (rows == 0) {   // empty sums
+        if (int rc = fill_zero(loss, reduction == AXC_LOSS_NONE ? 0 : 1, AXC_F32, stream))
+            return rc;
+        if (int rc = fill_zero(grad_kernel, K * V, desc->kernel_type, stream))
+            return rc;
+        return fill_zero(grad_bias, V, desc->kernel_type, stream);
+    }
+    if (!input || !kernel || !targets)
+        return api_fail(AXC_INVALID_ARGUMENT, "null tensor pointer");
+    const bool gradients = grad_input || grad_kernel || grad_bias;
+    const Pieces pc = loss_pieces(desc);
+    LossScratch s;
+    if (int rc = carve_loss(desc, gradients, workspace, &s))
+        return rc;
+    if (int rc = check_workspace(workspace, workspace_bytes, s.bytes))
+        return rc;
+    const Operands &o = s.o;
+    if (int rc = find_grids(desc, input, input_range, kernel, o, pc.Np, stream))
+        return rc;
+    if (int rc = make_codes(desc, input, kernel, o, pc, stream))
+        return rc;
+
+    TableSums sums = {};
+    auto make_sums = [&](int p) {
+        const int rc = table_sums(table, o.x_codes, rows, pc, p, o.kernel_codes, s.acc, s.lut, s.lut_bytes, stream, &sums);
+        sums.row_sums = o.row_sums;
+        sums.column_sums = o.column_sums + pc.first(p);
+        sums.table = table->dev_tableT;
+        sums.grids = o.grids;
+        sums.K = (int)K;
+        sums.pad = pc.Kp - (int)K;
+        return rc;
+    };
+    auto columns_of = [&](int p) { return std::min<int64_t>(pc.width_of(p), V - pc.first(p)); };
+    for (int p = 0; p < pc.count; ++p) {
+        if (int rc = make_sums(p))
+            return rc;
+        ApiTimer t("loss_piece", stream);
+        AXC_HIP(launch_loss_piece(sums, rows, (int)columns_of(p), pc.first(p), element(bias, pc.first(p), desc->bias_type),
+                                  desc->bias_type, targets, ignore_index, V, p == 0, p + 1 == pc.count, s.st, stream));
+    }
+    {
+        ApiTimer t("loss_out", stream);
+        AXC_HIP(launch_loss_out(s.st, targets, ignore_index, V, rows, reduction, grad_loss, loss, gradients, stream));
+    }
+    if (!gradients)
+        return AXC_OK;
+
+    const int px = parts_of(desc->input_type), pk = parts_of(desc->kernel_type);
+    const int64_t M = product_pad(rows);
+    if (grad_kernel) {
+        ApiTimer t("centered", stream);
+        AXC_HIP(launch_centered(input, desc->input_type, rows, K, K, &o.grids->in, true, s.x_turned, stream));
+    }
+    const ProductPlan input_plan = plan_product(rows, K, product_pad(pc.width), px, true);
+    const ProductOut input_out = {grad_input, desc->input_type, K, input, desc->input_type, K, &o.grids->in, &o.grids->kernel,
+                                  s.st.factor};
+    // from the last piece on, whose sums are still there
+    for (int p = pc.count - 1; p >= 0; --p) {
+        if (p + 1 < pc.count)
+            if (int rc = make_sums(p))
+                return rc;
+        const int64_t c = pc.first(p), n = columns_of(p), P = product_pad(n);
+        {
+            GradSource g = {};
+            g.sums = sums;
+            g.lse = s.st.lse;
+            g.coefficient = s.st.coefficient;
+            g.targets = targets;
+            g.bias = element(bias, c, desc->bias_type);
+            g.bias_type = desc->bias_type;
+            g.first_column = c;
+            ApiTimer t("grad_terms", stream);
+            AXC_HIP(launch_grad_terms(g, true, rows, n, 0, px, grad_input ? s.straight : nullptr, pk, grad_kernel ? s.turned : nullptr,
+                                      grad_bias ? s.column_partials : nullptr, stream));
+        }
+        if (grad_bias) {
+            ApiTimer t("column_sums", stream);
+            AXC_HIP(launch_column_sums(s.column_partials, M / 64, n, P, s.st.factor, element(grad_bias, c, desc->kernel_type),
+                                       desc->kernel_type, stream));
+        }
+        if (grad_input) {
+            {
+                ApiTimer t("centered", stream);
+                AXC_HIP(launch_centered(element(kernel, c, desc->kernel_type), desc->kernel_type, K, n, V, &o.grids->kernel, false,
+                                        s.kernel, stream));
+            }
+            ApiTimer t("grad_product", stream);
+            AXC_HIP(launch_product(s.straight, s.kernel, rows, K, P, px, true, input_plan, s.input_partials, true,
+                                   p + 1 < pc.count, input_out, stream));
+        }
+        if (grad_kernel) {
+            const ProductOut out = {element(grad_kernel, c, desc->kernel_type), desc->kernel_type, V,
+                                    element(kernel, c, desc->kernel_type), desc->kernel_type, V, &o.grids->kernel, &o.grids->in,
+                                    s.st.factor};
+            ApiTimer t("grad_product", stream);
+            AXC_HIP(launch_product(s.x_turned, s.turned, K, n, M, pk, false, plan_product(K, n, M, pk, false), s.kernel_partials,
+                                   false, false, out, stream));
+        }
+    }
+    if (grad_input) {
+        ApiTimer t("grad_product", stream);
+        AXC_HIP(launch_product_out(s.input_partials, input_plan.splits, rows, K, input_out, stream));
+    }
+    return AXC_OK;
+}
+
+// ---- residual norms ----
+static int check_norm(const axc_residual_norm_desc *d)
+{
+    if (!d)
+        return api_fail(AXC_INVALID_ARGUMENT, "null argument");
+    if (d->rows < 0 || d->width < 1 || d->gate_groups < 0)
+        return api_fail(AXC_INVALID_ARGUMENT, "rows and gate groups must not be negative, the width at least 1");
+    if (d->width > kNormMaxWidth)
+        return api_fail(AXC_UNIMPLEMENTED, "norms of more than 32768 values");
+    if (d->rows >= ((int64_t)1 << 40) / d->width)
+        return api_fail(AXC_INVALID_ARGUMENT, "tensor too large");
+    if (d->gate_groups > 0 && (d->gate_groups > d->rows || d->rows % d->gate_groups != 0) && d->rows > 0)
+        return api_fail(AXC_INVALID_ARGUMENT, "the gate's groups must divide the rows");
+    if (!known_type(d->type) || !known_type(d->vector_type))
+        return api_fail(AXC_INVALID_ARGUMENT, "unknown element type");
+    if (d->kind != AXC_NORM_RMS && d->kind != AXC_NORM_LAYER)
+        return api_fail(AXC_INVALID_ARGUMENT, "unknown norm");
+    if (!(d->eps >= 0.0f))
+        return api_fail(AXC_INVALID_ARGUMENT, "eps must not be negative");
+    return AXC_OK;
+}
+
+static int norm_params(const axc_residual_norm_desc *d, const axc_residual_norm_tensors *in, NormParams *p)
+{
+    if (!in)
+        return api_fail(AXC_INVALID_ARGUMENT, "null argument");
+    if (!in->weight)
+        return api_fail(AXC_INVALID_ARGUMENT, "null tensor pointer");
+    if (!in->block && (in->gate || in->scale || in->post_weight))
+        return api_fail(AXC_INVALID_ARGUMENT, "a gate, a scale and a weight of the block's norm need a block");
+    if ((in->gate != nullptr) != (d->gate_groups > 0))
+        return api_fail(AXC_INVALID_ARGUMENT, "a gate and its number of groups go together");
+    *p = NormParams{};
+    p->rows = d->rows;
+    p->width = d->width;
+    p->gate_groups = d->gate_groups;
+    p->type = d->type;
+    p->vector_type = d->vector_type;
+    p->layer = d->kind == AXC_NORM_LAYER;
+    p->eps = d->eps;
+    p->x = in->x;
+    p->block = in->block;
+    p->weight = in->weight;
+    p->bias = in->bias;
+    p->gate = in->gate;
+    p->scale = in->scale;
+    p->post_weight = in->post_weight;
+    return AXC_OK;
+}
+
+int axc_residual_norm(const axc_residual_norm_desc *desc, const axc_residual_norm_tensors *in, void *h, void *y,
+                      void *output_range, void *stream_v)
+{
+    if (int rc = check_norm(desc))
+        return rc;
+    NormParams p;
+    if (int rc = norm_params(desc, in, &p))
+        return rc;
+    if (desc->rows == 0) {
+        if (output_range)
+            return api_fail(AXC_INVALID_ARGUMENT, "no rows have no range");
+        return AXC_OK;
+    }
+    if (!p.x || !y || (p.block && !h))
+        return api_fail(AXC_INVALID_ARGUMENT, "null tensor pointer");
+    if (((uintptr_t)output_range & 7) != 0)
+        return api_fail(AXC_INVALID_ARGUMENT, "a range must be 8-byte aligned");
+    p.h = h;
+    p.y = y;
+    p.range = static_cast<float *>(output_range);
+    hipStream_t stream = static_cast<hipStream_t>(stream_v);
+    ApiTimer t("residual_norm", stream);
+    AXC_HIP(launch_norm(p, stream));
+    return AXC_OK;
+}
+
+int axc_residual_norm_gradients_workspace_bytes(const axc_residual_norm_desc *desc, size_t *bytes)
+{
+    if (int rc = check_norm(desc))
+        return rc;
+    if (!bytes)
+        return api_fail(AXC_INVALID_ARGUMENT, "null argument");
+    NormParams p = {};
+    p.rows = desc->rows;
+    p.width = desc->width;
+    p.gate_groups = desc->gate_groups;
+    *bytes = desc->rows ? norm_partial_bytes(p) : 0;
+    return AXC_OK;
+}
+
+int axc_residual_norm_gradients(const axc_residual_norm_desc *desc, const axc_residual_norm_tensors *in, const void *h,
+                                const void *grad_h, const void *grad_y, const axc_residual_norm_gradients_out *out,
+                                void *workspace, size_t workspace_bytes, void *stream_v)
+{
+    if (int rc = check_norm(desc))
+        return rc;
+    NormParams p;
+    if (int rc = norm_params(desc, in, &p))
+        return rc;
+    if (!out)
+        return api_fail(AXC_INVALID_ARGUMENT, "null argument");
+    if ((out->bias && !in->bias) || (out->gate && !in->gate) || (out->scale && !in->scale) ||
+        (out->post_weight && !in->post_weight) || (out->block && !in->block))
+        return api_fail(AXC_INVALID_ARGUMENT, "a gradient of what did not go in");
+    hipStream_t stream = static_cast<hipStream_t>(stream_v);
+    if (desc->rows == 0) {   // empty sums
+        for (void *v : {out->weight, out->bias, out->scale, out->post_weight})
+            if (int rc = fill_zero(v, desc->width, desc->vector_type, stream))
+                return rc;
+        return fill_zero(out->gate, desc->gate_groups * desc->width, desc->type, stream);
+    }
+    if (!h || (!grad_h && !grad_y) || !out->x || (p.block && !out->block))
+        return api_fail(AXC_INVALID_ARGUMENT, "null tensor pointer");
+    if (int rc = check_workspace(workspace, workspace_bytes, norm_partial_bytes(p)))
+        return rc;
+    p.x = nullptr;
+    p.h = const_cast<void *>(h);
+    p.grad_h = grad_h;
+    p.grad_y = grad_y;
+    p.dx = out->x;
+    p.dblock = out->block;
+    p.dweight = out->weight;
+    p.dbias = out->bias;
+    p.dgate = out->gate;
+    p.dscale = out->scale;
+    p.dpost = out->post_weight;
+    p.partials = static_cast<float *>(workspace);
+    ApiTimer t("residual_norm_gradients", stream);
+    AXC_HIP(launch_norm_gradients(p, stream));
+    return AXC_OK;
+}
+
+} // extern "C"

@@ -1,0 +1,369 @@
+// Declarations shared by the translation units of the transformer layers: dense layers by table products, the loss over a
+// vocabulary, residual norms.
+#pragma once
+
+#include "axconv_internal.h"
+
+namespace axc {
+
+// ---- element types ----
+typedef __bf16 bf16;
+typedef _Float16 f16;
+typedef bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+
+__host__ __device__ inline int type_bytes(int type) { return type == AXC_F32 ? 4 : 2; }
+
+// One value of a vector whose type is only known at run time (biases, weights of norms: few, and read through the caches).
+__device__ __forceinline__ float load_any(const void *p, int64_t i, int type)
+{
+    if (type == AXC_F32)
+        return static_cast<const float *>(p)[i];
+    if (type == AXC_BF16)
+        return (float)static_cast<const bf16 *>(p)[i];
+    return (float)static_cast<const f16 *>(p)[i];
+}
+__device__ __forceinline__ void store_any(void *p, int64_t i, int type, float v)
+{
+    if (type == AXC_F32)
+        static_cast<float *>(p)[i] = v;
+    else if (type == AXC_BF16)
+        static_cast<bf16 *>(p)[i] = (bf16)v;
+    else
+        static_cast<f16 *>(p)[i] = (f16)v;
+}
+
+// V neighbouring values as floats: one access where `whole` says that all V are there and aligned, else value by value with
+// `fill` in the place of those beyond n.
+template <typename T, int V>
+__device__ __forceinline__ void load_values(const T *p, int64_t n, bool whole, float fill, float (&v)[V])
+{
+    if constexpr (V > 1) {
+        if (whole) {
+            typedef T vector __attribute__((ext_vector_type(V)));
+            const vector t = *reinterpret_cast<const vector *>(p);
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                v[i] = (float)t[i];
+            return;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        v[i] = i < n ? (float)p[i] : fill;
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_values(T *p, int64_t n, bool whole, const float (&v)[V])
+{
+    if constexpr (V > 1) {
+        if (whole) {
+            typedef T vector __attribute__((ext_vector_type(V)));
+            vector t;
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                t[i] = (T)v[i];
+            *reinterpret_cast<vector *>(p) = t;
+            return;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if (i < n)
+            p[i] = (T)v[i];
+}
+
+// ---- the 8-bit grid of a tensor ----
+// What fake quantization with a range gives (Nudge, tf2/src/approx_ops_types.h:29-49): value = scale * (code - zero).
+struct Grid {
+    float scale, inv_scale, low, high;   // low, high: the nudged range
+    int32_t zero;                        // code of 0.0f
+    int32_t pad[3];
+};
+struct Grids {                           // of a layer, in device memory
+    Grid in, kernel;
+};
+
+// Every operation rounded on its own, as tensor_quant_device (prepass_kernels.hip) has it for the convolutions.
+__device__ inline Grid grid_of_range(float mn, float mx)
+{
+    Grid g = {};
+    if (mn == 0.0f && mx == 0.0f)
+        return g;
+    const float sc = __fdiv_rn(__fsub_rn(mx, mn), 255.0f);
+    const float from_min = __fsub_rn(0.0f, __fdiv_rn(mn, sc));
+    const int zp = from_min < 0.0f ? 0 : from_min > 255.0f ? 255 : from_min == from_min ? (int)roundf(from_min) : 0;
+    g.scale = sc;
+    g.inv_scale = __fdiv_rn(1.0f, sc);
+    g.low = __fmul_rn(__fsub_rn(0.0f, (float)zp), sc);
+    g.high = __fmul_rn(__fsub_rn(255.0f, (float)zp), sc);
+    g.zero = zp;
+    return g;
+}
+// The grid's code of a value: that of fake_quant_value followed by quantize_code, whose round trip through the grid's float
+// changes no code (it is off by less than 2^-14 of a step).  NaN counts as the upper end, as there.
+__device__ __forceinline__ uint32_t code_of(float v, const Grid &g)
+{
+    const float c = fmaxf(fminf(v, g.high), g.low);
+    float t = floorf(__fadd_rn(__fmul_rn(__fsub_rn(c, g.low), g.inv_scale), 0.5f));
+    t = t > 0.0f ? t : 0.0f;          // NaN (a grid of no width, or of no end) too
+    return g.scale == 0.0f ? 0u : (uint32_t)(t < 255.0f ? t : 255.0f);
+}
+__device__ __forceinline__ bool inside(float v, const Grid &g) { return v >= g.low && v <= g.high; }
+
+// ---- reductions ----
+__device__ __forceinline__ float wave_sum(float v)
+{
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1)
+        v += __shfl_xor(v, s);
+    return v;
+}
+__device__ __forceinline__ int32_t wave_sum(int32_t v)
+{
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1)
+        v += __shfl_xor(v, s);
+    return v;
+}
+__device__ __forceinline__ float wave_max(float v)
+{
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1)
+        v = fmaxf(v, __shfl_xor(v, s));
+    return v;
+}
+__device__ __forceinline__ float wave_min(float v)
+{
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1)
+        v = fminf(v, __shfl_xor(v, s));
+    return v;
+}
+// Smallest and largest over a workgroup, in every thread.  red: 2 * waves floats of LDS, free before and after.
+__device__ __forceinline__ void block_range(float &lo, float &hi, float *red)
+{
+    const int wave = threadIdx.x / 64, waves = blockDim.x / 64;
+    lo = wave_min(lo);
+    hi = wave_max(hi);
+    if ((threadIdx.x & 63) == 0) {
+        red[2 * wave] = lo;
+        red[2 * wave + 1] = hi;
+    }
+    __syncthreads();
+    for (int i = 0; i < waves; ++i) {
+        lo = fminf(lo, red[2 * i]);
+        hi = fmaxf(hi, red[2 * i + 1]);
+    }
+    __syncthreads();
+}
+
+// ---- activations ----
+__device__ __forceinline__ float activate(float z, int activation)
+{
+    switch (activation) {
+    case AXC_ACT_RELU: return z > 0.0f ? z : z == z ? 0.0f : z;
+    case AXC_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+    case AXC_ACT_GELU_TANH: {   // 0.5 z (1 + tanh(u)) = z / (1 + exp(-2u))
+        const float u = 0.79788456080286536f * (z + 0.044715f * z * z * z);
+        return z == -INFINITY ? -0.0f : z / (1.0f + expf(-2.0f * u));
+    }
+    case AXC_ACT_SILU: return z == -INFINITY ? -0.0f : z / (1.0f + expf(-z));
+    default: return z;
+    }
+}
+__device__ __forceinline__ float activation_slope(float z, int activation)
+{
+    switch (activation) {
+    case AXC_ACT_RELU: return z > 0.0f ? 1.0f : z == z ? 0.0f : z;
+    case AXC_ACT_GELU: return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) +
+                              (fabsf(z) < 14.0f ? z * expf(-0.5f * z * z) * 0.39894228040143268f : 0.0f * z);
+    case AXC_ACT_GELU_TANH: {
+        if (fabsf(z) > 1e6f)
+            return z > 0.0f ? 1.0f : 0.0f;
+        const float u = 0.79788456080286536f * (z + 0.044715f * z * z * z);
+        const float s = 1.0f / (1.0f + expf(-2.0f * u));
+        return s + 2.0f * z * s * (1.0f - s) * 0.79788456080286536f * (1.0f + 0.134145f * z * z);
+    }
+    case AXC_ACT_SILU: {
+        if (fabsf(z) > 1e6f)
+            return z > 0.0f ? 1.0f : 0.0f;
+        const float s = 1.0f / (1.0f + expf(-z));
+        return s * (1.0f + z * (1.0f - s));
+    }
+    default: return 1.0f;
+    }
+}
+
+// ---- dense layers ----
+// Operands as codes, padded: input [rows][Kp], Kp the depth in fours; kernel in pieces of columns, each [Kp][width], the columns
+// in fours.  Pad codes are 0: every pad element of the depth adds T[0][0] to a sum, which the epilogue takes away again.
+struct Pieces {
+    int64_t Np;            // columns, in fours
+    int32_t Kp;
+    int32_t width;         // of all pieces but the last
+    int32_t count;
+    __host__ __device__ int64_t first(int p) const { return (int64_t)p * width; }
+    __host__ __device__ int width_of(int p) const { return p + 1 < count ? width : (int)(Np - (int64_t)(count - 1) * width); }
+    __host__ __device__ size_t offset(int p) const { return (size_t)Kp * first(p); }   // of a piece's codes, in bytes
+    size_t bytes() const { return (size_t)Kp * Np; }
+};
+
+constexpr int kRangeBlocks = 256;        // pairs that the range pass leaves per tensor, at most
+constexpr int kFewRows = 8;              // rows that the kernel for few rows takes at a time
+struct RangeSource {                     // where a tensor's smallest and largest value come from
+    const float *pairs;                  // (smallest, largest) pairs, or null
+    int count;                           // of the pairs; null and 0: lo and hi, known to the caller; null and -1: not known yet
+    float lo, hi;
+};
+
+// Sums of table entries as a consumer finds them, of one piece and one run of rows: `splits` partial sums of [rows][pitch] int32.
+struct TableSums {
+    const int32_t *acc;
+    int64_t split_stride;
+    int splits, pitch;
+    const int32_t *row_sums;             // sums of the input's codes, of the run's first row on
+    const int32_t *column_sums;          // sums of the kernel's codes, of the piece's first column on
+    const uint16_t *table;               // its first entry is T[0][0]
+    const Grids *grids;
+    int K, pad;                          // depth, and pad elements behind it
+};
+
+// What takes the two zero points and the padding out of a sum, of row r; for column c: whole - in.zero * column_sums[c].
+__device__ __forceinline__ int64_t row_term(const TableSums &s, int64_t r)
+{
+    const int64_t zi = s.grids->in.zero, zk = s.grids->kernel.zero;
+    return (int64_t)s.K * zi * zk - zk * (int64_t)s.row_sums[r] - (int64_t)s.pad * s.table[0];
+}
+
+hipError_t launch_range(const void *x, int x_type, int64_t nx, const void *kernel, int kernel_type, int64_t nk, float *x_pairs,
+                        float *kernel_pairs, int32_t *zeros, int64_t n_zeros, int *x_count, int *kernel_count, hipStream_t stream);
+hipError_t launch_grids(const RangeSource &in, const RangeSource &kernel, bool has_in, bool has_kernel, Grids *grids,
+                        hipStream_t stream);
+hipError_t launch_input_codes(const void *x, int type, int64_t rows, int K, int Kp, const Grids *grids, uint8_t *codes,
+                              int32_t *row_sums, hipStream_t stream);
+hipError_t launch_kernel_codes(const void *kernel, int type, int K, int64_t N, const Pieces &pieces, const Grids *grids,
+                               uint8_t *codes, int32_t *column_sums, hipStream_t stream);
+// Few rows: range (where src says so), grid, codes and their sums of the input in one launch; kernel_grid is copied next to it.
+hipError_t launch_few_codes(const void *x, int type, int rows, int K, int Kp, const RangeSource &src, const Grid *kernel_grid,
+                            Grids *grids, uint8_t *codes, int32_t *row_sums, hipStream_t stream);
+int few_rows_splits(int64_t rows, int K, int width);
+hipError_t launch_few_rows(const uint16_t *tableI, const uint8_t *x_codes, int rows, int Kp, const uint8_t *kernel_codes, int width,
+                           int splits, int32_t *acc, hipStream_t stream);
+struct DenseOut {
+    const void *bias, *residual;         // of the piece's / run's first element
+    void *out, *pre;
+    int bias_type, type, activation;
+    int64_t ld;                          // columns of the layer
+};
+hipError_t launch_zero(void *p, int64_t bytes, hipStream_t stream);   // a kernel: callers may capture it
+hipError_t launch_dense_out(const TableSums &s, int64_t rows, int columns, const DenseOut &o, hipStream_t stream);
+
+// ---- products of gradients with codes (gradient_kernels.hip) ----
+// Operands in bfloat16, rows and depth padded to kProductTile.  Codes minus their zero point are whole numbers below 256 and
+// exact in bfloat16; the other operand is split into `parts` terms of 8 bits each.
+constexpr int kProductTile = 128;
+inline int64_t product_pad(int64_t n) { return (n + kProductTile - 1) / kProductTile * kProductTile; }
+inline int parts_of(int type) { return type == AXC_F32 ? 3 : type == AXC_F16 ? 2 : 1; }
+
+struct GradSource {                      // where the gradient behind the product comes from
+    const void *grad, *pre;              // dense: gradient of the output, what the activation was given (or null)
+    int type, activation;
+    // loss: sums of a piece, log of each row's sum of exponentials, its coefficient and target
+    TableSums sums;
+    const float *lse, *coefficient;
+    const int64_t *targets;
+    const void *bias;
+    int bias_type;
+    int64_t first_column;
+};
+// [rows_pad][parts][cols_pad], [cols_pad][parts][rows_pad], and per 64 rows the sums over them (each may be null)
+hipError_t launch_grad_terms(const GradSource &g, bool loss, int64_t rows, int64_t cols, int64_t ld, int straight_parts,
+                             bf16 *straight, int turned_parts, bf16 *turned, float *column_partials, hipStream_t stream);
+hipError_t launch_centered(const void *v, int type, int64_t rows, int64_t cols, int64_t ld, const Grid *grid, bool turn, bf16 *out,
+                           hipStream_t stream);
+struct ProductOut {
+    void *out;                           // rows x cols, leading dimension ld; null: partial sums only
+    int type;
+    int64_t ld;
+    const void *values;                  // like out: those outside `grid` get 0
+    int values_type;
+    int64_t values_ld;
+    const Grid *grid, *scale;            // scale->scale times the sums
+    const float *factor;                 // not null: times *factor
+};
+struct ProductPlan {
+    int splits;
+    size_t partial_bytes;                // [splits][rows_pad][cols_pad] float
+};
+ProductPlan plan_product(int64_t rows, int64_t cols, int64_t depth_pad, int parts, bool keep);
+// out[r][c] = sum over parts and l of a[r][..l] * b[c][..l]; the operand with the parts is a where split_a, else b.
+// accumulate: add to the partial sums that are there.
+hipError_t launch_product(const bf16 *a, const bf16 *b, int64_t rows, int64_t cols, int64_t depth_pad, int parts, bool split_a,
+                          const ProductPlan &plan, float *partials, bool keep, bool accumulate, const ProductOut &o,
+                          hipStream_t stream);
+hipError_t launch_product_out(const float *partials, int splits, int64_t rows, int64_t cols, const ProductOut &o,
+                              hipStream_t stream);
+hipError_t launch_column_sums(const float *partials, int64_t count, int64_t cols, int64_t pitch, const float *factor, void *out,
+                              int type, hipStream_t stream);
+
+// ---- loss (loss_kernels.hip) ----
+struct LossState {                       // per row
+    float *top, *sum, *at;               // running maximum and sum of exponentials; the target's logit
+    float *lse, *rows;                   // log of the whole sum; the row's loss
+    float *coefficient, *factor;         // a row's gradient is multiplied by coefficient[row] * *factor
+};
+hipError_t launch_loss_piece(const TableSums &s, int64_t rows, int columns, int64_t first_column, const void *bias, int bias_type,
+                             const int64_t *targets, int64_t ignore, int64_t V, bool first, bool last, const LossState &st,
+                             hipStream_t stream);
+hipError_t launch_loss_out(const LossState &st, const int64_t *targets, int64_t ignore, int64_t V, int64_t rows, int reduction,
+                           const float *grad_loss, float *loss, bool gradients, hipStream_t stream);
+
+// ---- residual norms (norm_kernels.hip) ----
+struct NormParams {
+    int64_t rows, width, gate_groups;    // gate_groups: 0 = no gate; rows / gate_groups neighbouring rows share one
+    int type, layer;                     // layer: 1 = LayerNorm, 0 = RMSNorm
+    float eps;
+    const void *x, *block, *weight, *bias, *gate, *scale, *post_weight;
+    int vector_type;                     // of weight, bias, scale, post_weight
+    void *h, *y;
+    float *range;                        // kRangePairs pairs, or null
+    // backwards: h is read; gradients in, gradients out (any may be null)
+    const void *grad_h, *grad_y;
+    void *dx, *dblock;
+    void *dweight, *dbias, *dgate, *dscale, *dpost;
+    float *partials;
+};
+constexpr int kNormMaxWidth = 32768;
+hipError_t launch_norm(const NormParams &p, hipStream_t stream);
+size_t norm_partial_bytes(const NormParams &p);
+hipError_t launch_norm_gradients(const NormParams &p, hipStream_t stream);
+
+} // namespace axc
+
+// The table as its owner has it (axconv_api.hip).
+struct axc_table {
+    uint16_t *dev_tableT; // [257 filter code][256 input code]; row 256 is zero
+    uint16_t *dev_tableF; // behind it in the same allocation: the same with the top bit of every byte flipped,
+    uint16_t *dev_tableS; // and [257 input code][256 filter code], flipped too
+    uint16_t *dev_tableI; // [256 input code][64][4]: entry [l][i] is that of filter code l + 64 i
+    int device;
+};
+
+namespace axc {
+// What the entry points of axconv_api.hip use, for those of layers_api.hip.
+int api_fail(int status, const char *msg);
+int api_fail_hip(hipError_t e, const char *what);
+int api_check_table(const axc_table *table);
+class ApiTimer {   // brackets launches while the timers run
+public:
+    ApiTimer(const char *name, hipStream_t stream);
+    ~ApiTimer();
+    ApiTimer(const ApiTimer &) = delete;
+    ApiTimer &operator=(const ApiTimer &) = delete;
+
+private:
+    void *scope_;
+};
+} // namespace axc
