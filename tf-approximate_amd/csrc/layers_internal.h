@@ -113,12 +113,26 @@ __device__ __forceinline__ uint32_t code_of(float v, const Grid &g)
 __device__ __forceinline__ bool inside(float v, const Grid &g) { return v >= g.low && v <= g.high; }
 
 // ---- reductions ----
+// Sum over a wavefront, in every lane: within rows of 16 lanes, then row to row, by the vector ALU's own lane moves, which take a
+// few cycles each where a move through the LDS takes a hundred.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float add_moved(float v)
+{
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, true));
+}
+__device__ __forceinline__ float row_of_lanes_sum(float v)   // in lane 15 of each row
+{
+    v = add_moved<0x111, 0xf>(v);   // from 1, 2, 4, 8 lanes before
+    v = add_moved<0x112, 0xf>(v);
+    v = add_moved<0x114, 0xf>(v);
+    return add_moved<0x118, 0xf>(v);
+}
 __device__ __forceinline__ float wave_sum(float v)
 {
-#pragma unroll
-    for (int s = 32; s > 0; s >>= 1)
-        v += __shfl_xor(v, s);
-    return v;
+    v = row_of_lanes_sum(v);
+    v = add_moved<0x142, 0xa>(v);   // lane 15 to the next row, in rows 1 and 3
+    v = add_moved<0x143, 0xc>(v);   // lane 31 to rows 2 and 3
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 __device__ __forceinline__ int32_t wave_sum(int32_t v)
 {
