@@ -49,10 +49,12 @@ struct Reducer {
 // anywhere, so vectors are accessed as aligned as their elements are.
 //
 // Loads have no conditions: where a branch stands between a load and its use, the compiler waits for everything in flight, stores
-// included.  A vector behind the row is loaded from the row's last four values and counts as zeros; the one that ends behind the
-// row is loaded from there too, and moved.  So that rows of less than four values need no more than that, they take the place of
-// the last four values of whatever is loaded one by one (kTiny).
-enum { kEven, kOdd, kTiny };             // widths: a multiple of four, no multiple, less than four
+// included.  In rows that are no whole aligned vectors (kOdd), a vector behind the row is loaded from the row's last four values
+// and counts as zeros; the one that ends behind the row is loaded from there too, and moved.  Rows of less than four values (kTiny)
+// are loaded one by one.
+enum { kEven, kOdd, kTiny };
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ int place(int j) { return (j * (int)blockDim.x + (int)threadIdx.x) * V; }
 
 template <typename T>
@@ -78,10 +80,10 @@ template <int W, typename T>
 __device__ __forceinline__ f32x4 in_place(const T &t, int c, int width)
 {
     f32x4 v;
-    if constexpr (W == kEven) {
+    if constexpr (W == kEven) {        // (zeros as loaded)
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            v[i] = c < width ? (float)t[i] : 0.0f;
+            v[i] = (float)t[i];
     } else if constexpr (W == kTiny) {
 #pragma unroll
         for (int i = 0; i < V; ++i)
@@ -116,6 +118,20 @@ __device__ __forceinline__ void store_four(T *p, int c, int width, const float (
     }
 }
 
+// Rows of a tensor.  Aligned rows of whole vectors go through buffer descriptors, which give zeros for what lies behind a row (or
+// for all of one that is not there, of no bytes) and drop stores there, so that neither needs a condition.
+template <int W, typename T>
+struct Rows {
+    T *base;
+    int width;
+    bool there;
+    __device__ __forceinline__ Rows(const void *p, int w) : base(static_cast<T *>(const_cast<void *>(p))), width(w), there(p != nullptr) {}
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t row(int64_t r) const
+    {
+        return __builtin_amdgcn_make_buffer_rsrc(base + r * width, 0, there ? width * (int)sizeof(T) : 0, 0x00020000);
+    }
+};
+
 template <int NV>
 struct Row {
     float v[NV][V];
@@ -125,11 +141,24 @@ struct Raw {               // a row as it was loaded
     typename Vector<T>::four v[NV];
 };
 template <int W, typename T, int NV>
-__device__ __forceinline__ void load_row(const T *p, int width, Raw<T, NV> &r)
+__device__ __forceinline__ void load_row(const Rows<W, T> &t, int64_t row, Raw<T, NV> &r)
 {
+    if constexpr (W == kEven) {
+        const __amdgpu_buffer_rsrc_t from = t.row(row);
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-        r.v[j] = load_four<W>(p, place(j), width);
+        for (int j = 0; j < NV; ++j) {
+            if constexpr (sizeof(T) == 4)
+                r.v[j] = __builtin_bit_cast(typename Vector<T>::four,
+                                            __builtin_amdgcn_raw_buffer_load_b128(from, place(j) * (int)sizeof(T), 0, 0));
+            else
+                r.v[j] = __builtin_bit_cast(typename Vector<T>::four,
+                                            __builtin_amdgcn_raw_buffer_load_b64(from, place(j) * (int)sizeof(T), 0, 0));
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            r.v[j] = load_four<W>(t.base + row * t.width, place(j), t.width);
+    }
 }
 template <int W, typename T, int NV>
 __device__ __forceinline__ Row<NV> widen(const Raw<T, NV> &r, int width)
@@ -145,11 +174,26 @@ __device__ __forceinline__ Row<NV> widen(const Raw<T, NV> &r, int width)
     return w;
 }
 template <int W, typename T, int NV>
-__device__ __forceinline__ void store_row(T *p, int width, const Row<NV> &r)
+__device__ __forceinline__ void store_row(const Rows<W, T> &t, int64_t row, const Row<NV> &r)
 {
+    if constexpr (W == kEven) {
+        const __amdgpu_buffer_rsrc_t to = t.row(row);
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-        store_four<W>(p, place(j), width, r.v[j]);
+        for (int j = 0; j < NV; ++j) {
+            typename Vector<T>::four v;
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                v[i] = (T)r.v[j][i];
+            if constexpr (sizeof(T) == 4)
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), to, place(j) * (int)sizeof(T), 0, 0);
+            else
+                __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, v), to, place(j) * (int)sizeof(T), 0, 0);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+            store_four<W>(t.base + row * t.width, place(j), t.width, r.v[j]);
+    }
 }
 template <int NV>
 __device__ __forceinline__ void scale_row(Row<NV> &r, float f)
@@ -223,11 +267,12 @@ struct Kept {
     {
         const void *const p = vectors[which];
         const int c = place(j);
+        constexpr int L = W == kTiny ? kTiny : kOdd;   // (may be aligned as their elements only)
         if (type == AXC_F32)
-            return in_place<W>(load_four<W>(static_cast<const float *>(p), c, width), c, width);
+            return in_place<L>(load_four<L>(static_cast<const float *>(p), c, width), c, width);
         if (type == AXC_BF16)
-            return in_place<W>(load_four<W>(static_cast<const bf16 *>(p), c, width), c, width);
-        return in_place<W>(load_four<W>(static_cast<const f16 *>(p), c, width), c, width);
+            return in_place<L>(load_four<L>(static_cast<const bf16 *>(p), c, width), c, width);
+        return in_place<L>(load_four<L>(static_cast<const f16 *>(p), c, width), c, width);
     }
     // Vectors that are not there are ones.
     __device__ __forceinline__ void fill()
@@ -263,19 +308,19 @@ __global__ void __launch_bounds__(most_threads(NV)) norm_kernel(NormParams p)
     const int width = (int)p.width;
     const int64_t group_rows = p.gate_groups ? p.rows / p.gate_groups : 1;
     Kept<W, NV, 4> kept = {kept_lds, {p.weight, p.scale, p.post_weight, p.bias}, p.vector_type, width};
-    const T *const x = static_cast<const T *>(p.x);
-    const T *const block = static_cast<const T *>(p.block ? p.block : p.x);   // (loaded in any case, for nothing without a block)
-    const T *const gate = static_cast<const T *>(p.gate);
+    // (what is not there is loaded in any case, for nothing)
+    const Rows<W, T> x(p.x, width), block(W == kEven || p.block ? p.block : p.x, width), gate(p.gate, width), hs(p.h, width),
+        ys(p.y, width);
     float lo = INFINITY, hi = -INFINITY;
     // the gate group of the row that is loaded, and the row's place in it; a step of the loop further on
     int64_t group = (int64_t)blockIdx.x / group_rows, in_group = (int64_t)blockIdx.x - group * group_rows;
     const int64_t more_groups = (int64_t)gridDim.x / group_rows, more_rows = (int64_t)gridDim.x - more_groups * group_rows;
     Raw<T, NV> xr, br, gr = {};
     auto load = [&](int64_t r) {
-        load_row<W>(x + r * width, width, xr);
-        load_row<W>(block + r * width, width, br);
-        if (gate)
-            load_row<W>(gate + group * width, width, gr);
+        load_row(x, r, xr);
+        load_row(block, p.block ? r : 0, br);
+        if (p.gate)
+            load_row(gate, group, gr);
         group += more_groups;
         in_group += more_rows;
         if (in_group >= group_rows) {
@@ -300,7 +345,7 @@ __global__ void __launch_bounds__(most_threads(NV)) norm_kernel(NormParams p)
 #pragma unroll
                 for (int i = 0; i < V; ++i)
                     u.v[j][i] *= post[i];
-                if (gate) {
+                if (p.gate) {
                     const f32x4 g = in_place<W>(ga.v[j], place(j), width);
 #pragma unroll
                     for (int i = 0; i < V; ++i)
@@ -312,7 +357,7 @@ __global__ void __launch_bounds__(most_threads(NV)) norm_kernel(NormParams p)
                     h.v[j][i] = place(j) + (W == kEven ? 0 : i) < width ? (float)(T)s : 0.0f;
                 }
             }
-            store_row<W>(static_cast<T *>(p.h) + r * width, width, h);
+            store_row(hs, r, h);
         }
         normalize<W>(h, p, red);
 #pragma unroll
@@ -335,7 +380,7 @@ __global__ void __launch_bounds__(most_threads(NV)) norm_kernel(NormParams p)
                 hi = fmaxf(hi, there ? y : -INFINITY);
             }
         }
-        store_row<W>(static_cast<T *>(p.y) + r * width, width, h);
+        store_row(ys, r, h);
     }
     if (!p.range)
         return;
@@ -359,7 +404,7 @@ struct NormRuns {
     int64_t per_group;      // workgroups of a gate group; 0: a workgroup takes whole groups, or there is no gate
     int64_t blocks;
 };
-constexpr int64_t kRunBlocks = 1024;     // about as many workgroups, four a CU
+constexpr int64_t kRunBlocks = 768;      // about as many workgroups, three a CU: what is resident
 NormRuns norm_runs(int64_t rows, int64_t groups)
 {
     NormRuns n = {};
@@ -399,18 +444,19 @@ __global__ void __launch_bounds__(most_threads(NV)) norm_grad_kernel(NormParams 
         group = first / group_rows;
         left = group_rows;
     }
-    // (what is not there is loaded from h, for nothing, and counts as zeros, a gate as ones)
-    const T *const hs = static_cast<const T *>(p.h);
-    const T *const gys = p.grad_y ? static_cast<const T *>(p.grad_y) : hs, *const ghs = p.grad_h ? static_cast<const T *>(p.grad_h) : hs;
-    const T *const blocks = p.block ? static_cast<const T *>(p.block) : hs, *const gates = static_cast<const T *>(p.gate);
+    // (what is not there is loaded in any case, as zeros or from h for nothing; a gate that is not there counts as ones)
+    const void *const other = W == kEven ? nullptr : p.h;
+    const Rows<W, T> hs(p.h, width), gys(p.grad_y ? p.grad_y : other, width), ghs(p.grad_h ? p.grad_h : other, width),
+        blocks(p.block ? p.block : other, width), gates(p.gate, width), dxs(p.dx, width), dblocks(p.dblock, width),
+        dgates(p.dgate, width);
     Raw<T, NV> hr, gyr, ghr, br, gr = {};
     auto load = [&](int64_t r, int64_t of) {
-        load_row<W>(hs + r * width, width, hr);
-        load_row<W>(gys + r * width, width, gyr);
-        load_row<W>(ghs + r * width, width, ghr);
-        load_row<W>(blocks + r * width, width, br);
-        if (gates)
-            load_row<W>(gates + of * width, width, gr);
+        load_row(hs, r, hr);
+        load_row(gys, W == kEven && !p.grad_y ? 0 : r, gyr);
+        load_row(ghs, W == kEven && !p.grad_h ? 0 : r, ghr);
+        load_row(blocks, W == kEven && !p.block ? 0 : r, br);
+        if (p.gate)
+            load_row(gates, of, gr);
     };
     constexpr bool kAhead = NV <= 2;   // the next row's loads ahead of all reductions; of wider rows once registers are free
     Row<NV> sw = {}, sb = {}, ss = {}, sp = {}, sg = {};
@@ -428,8 +474,11 @@ __global__ void __launch_bounds__(most_threads(NV)) norm_grad_kernel(NormParams 
         const Raw<T, NV> gate = gr;
         if (kAhead && r + 1 < last)
             load(r + 1, group);
-        scale_row(dh, p.grad_y ? 1.0f : 0.0f);
-        scale_row(gh, p.grad_h ? 1.0f : 0.0f);
+        if constexpr (W != kEven) {
+            scale_row(dh, p.grad_y ? 1.0f : 0.0f);
+            if (!p.grad_h)
+                gh = {};
+        }
         if (p.layer) {
             float s[2] = {row_sum(n), row_sum(b)};
             red.sum(s);
@@ -460,7 +509,7 @@ __global__ void __launch_bounds__(most_threads(NV)) norm_grad_kernel(NormParams 
             }
         if (!p.grad_y)                 // (rather than 0 times what may be infinite)
             dh = gh;
-        store_row<W>(static_cast<T *>(p.dx) + r * width, width, dh);
+        store_row(dxs, r, dh);
         if (!kAhead && r + 1 < last)
             load(r + 1, group);
         if (!p.block)
@@ -472,7 +521,7 @@ __global__ void __launch_bounds__(most_threads(NV)) norm_grad_kernel(NormParams 
         for (int j = 0; j < NV; ++j) {
             const f32x4 w = kept.get(kPost, j), sc = kept.get(kScale, j);
             f32x4 ga = {1.0f, 1.0f, 1.0f, 1.0f};
-            if (gates)
+            if (p.gate)
                 ga = in_place<W>(gate.v[j], place(j), width);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
@@ -495,23 +544,24 @@ __global__ void __launch_bounds__(most_threads(NV)) norm_grad_kernel(NormParams 
                 for (int i = 0; i < V; ++i)
                     dh.v[j][i] = (dh.v[j][i] - b.v[j][i] * mtn - mt) * rb;
         }
-        store_row<W>(static_cast<T *>(p.dblock) + r * width, width, dh);
+        store_row(dblocks, r, dh);
         if (p.dgate && !runs.per_group && ends) {
-            store_row<W>(static_cast<T *>(p.dgate) + of * width, width, sg);
+            store_row(dgates, of, sg);
             sg = {};
         }
     }
-    float *const to = p.partials + (int64_t)blockIdx.x * kSums * width;
+    const Rows<W, float> to(p.partials, width);
+    const int64_t at = (int64_t)blockIdx.x * kSums;
     if (p.dweight)
-        store_row<W>(to + (int64_t)kSumWeight * width, width, sw);
+        store_row(to, at + kSumWeight, sw);
     if (p.dbias)
-        store_row<W>(to + (int64_t)kSumBias * width, width, sb);
+        store_row(to, at + kSumBias, sb);
     if (p.dscale)
-        store_row<W>(to + (int64_t)kSumScale * width, width, ss);
+        store_row(to, at + kSumScale, ss);
     if (p.dpost)
-        store_row<W>(to + (int64_t)kSumPost * width, width, sp);
+        store_row(to, at + kSumPost, sp);
     if (p.dgate && runs.per_group)
-        store_row<W>(to + (int64_t)kSumGate * width, width, sg);
+        store_row(to, at + kSumGate, sg);
 }
 
 struct ColumnSums {
@@ -548,6 +598,18 @@ __global__ void __launch_bounds__(512) norm_column_kernel(const float *__restric
         store_any(sums.out[which], c, vector_type, sum);
 }
 
+bool whole_vectors(const NormParams &p)
+{
+    const uintptr_t mask = (uintptr_t)(V * type_bytes(p.type) - 1);
+    if (p.width % V)
+        return false;
+    for (const void *q : {p.x, p.block, p.gate, (const void *)p.h, (const void *)p.y, p.grad_h, p.grad_y, (const void *)p.dx,
+                          (const void *)p.dblock, (const void *)p.dgate})
+        if ((uintptr_t)q & mask)
+            return false;
+    return true;
+}
+
 // Two vectors a thread up to 4096 values, in steps of a wavefront; then four, and eight of 1024 threads.
 template <template <typename, int, int> class Launch, typename T, int W>
 hipError_t by_vectors(const NormParams &p, hipStream_t stream)
@@ -567,7 +629,7 @@ hipError_t by_width(const NormParams &p, hipStream_t stream)
 {
     if (p.width < V)
         return Launch<T, 1, kTiny>::go(p, 64, stream);
-    return p.width % V ? by_vectors<Launch, T, kOdd>(p, stream) : by_vectors<Launch, T, kEven>(p, stream);
+    return whole_vectors(p) ? by_vectors<Launch, T, kEven>(p, stream) : by_vectors<Launch, T, kOdd>(p, stream);
 }
 template <template <typename, int, int> class Launch>
 hipError_t by_type(const NormParams &p, hipStream_t stream)
