@@ -1317,7 +1317,7 @@ int run_dense(const axc_table *table, const axc_conv2d_desc *desc, const float *
               void *workspace, size_t workspace_bytes, void *stream_v, bool layer_mode = false,
               const float *bias = nullptr, int activation = AXC_ACT_NONE, const int *pad_before_override = nullptr,
               const int32_t *tf1_offset_filter = nullptr, axc_layer_ranges *ranges = nullptr,
-              const float *addend = nullptr)
+              const float *addend = nullptr, RawSums *raw = nullptr)
 {
     if (!table || !desc)
         return fail(AXC_INVALID_ARGUMENT, "null argument");
@@ -1570,6 +1570,10 @@ int run_dense(const axc_table *table, const axc_conv2d_desc *desc, const float *
             ProfScope ps("lutgemm_mx", stream);
             AXC_HIP(launch_dense_mx_expand(m, stream));
         }
+        if (raw) {
+            *raw = {part, (int64_t)g.Co * m_pitch, mx->k_splits, m_pitch, 1};
+            return AXC_OK;
+        }
         {
             ProfScope ps("splitk_epilogue", stream);
             p.g = g;
@@ -1668,6 +1672,11 @@ int run_dense(const axc_table *table, const axc_conv2d_desc *desc, const float *
             ProfScope ps("lutgemm_mx", stream, mx->expand ? nullptr : "lutgemm_px");
             AXC_HIP(mx->expand ? launch_dense_mx_expand(m, stream) : launch_dense_mx(m, stream));
         }
+        if (raw) {
+            const bool parts = mx->k_splits > 1;
+            *raw = {parts ? part : out_i, (int64_t)g.M * g.Co, mx->k_splits, g.Co, 0};
+            return AXC_OK;
+        }
         if (mx->k_splits > 1) {
             p.plan.k_splits = mx->k_splits;
             ProfScope ps("splitk_epilogue", stream);
@@ -1731,6 +1740,10 @@ int run_dense(const axc_table *table, const axc_conv2d_desc *desc, const float *
     } else {
         ProfScope ps("lutgemm_expand", stream);
         AXC_HIP(launch_dense(p, p.out_i != nullptr, stream));
+    }
+    if (raw) {
+        *raw = {splits ? part : out_i, (int64_t)g.M * g.Co, pd.plan.k_splits, g.Co, 0};
+        return AXC_OK;
     }
     if (splits) {
         ProfScope ps("splitk_epilogue", stream);
@@ -1857,6 +1870,12 @@ namespace axc {
 int api_fail(int status, const char *msg) { return fail(status, msg); }
 int api_fail_hip(hipError_t e, const char *what) { return fail_hip(e, what); }
 int api_check_table(const axc_table *table) { return check_table_device(table); }
+int api_codes_sums(const axc_table *table, const axc_conv2d_desc *desc, const uint8_t *input_codes, const uint8_t *filter_codes,
+                   int32_t *acc, void *workspace, size_t workspace_bytes, void *stream, RawSums *raw)
+{
+    return run_dense(table, desc, nullptr, nullptr, input_codes, filter_codes, 0, 0.0f, 0.0f, 0.0f, 0.0f, nullptr, acc, workspace,
+                     workspace_bytes, stream, false, nullptr, AXC_ACT_NONE, nullptr, nullptr, nullptr, nullptr, raw);
+}
 ApiTimer::ApiTimer(const char *name, hipStream_t stream) : scope_(g_prof_enabled.load() ? new ProfScope(name, stream) : nullptr) {}
 ApiTimer::~ApiTimer() { delete static_cast<ProfScope *>(scope_); }
 } // namespace axc

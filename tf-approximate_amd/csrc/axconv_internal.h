@@ -350,6 +350,14 @@ __device__ __forceinline__ void fetch_arguments()
                    "n"((kLines > 4 ? 4 : 0) * 64), "n"((kLines > 5 ? 5 : 0) * 64));
 }
 
+// Sums of a codes call as its LUT-GEMM leaves them, for a caller that reads them once more anyway: the sum of `splits` parts,
+// `split_stride` apart, of value (pixel m, column c) at m * pitch + c, or c * pitch + m where they are `turned`.
+struct RawSums {
+    const int32_t *acc;
+    int64_t split_stride;
+    int splits, pitch, turned;
+};
+
 int device_cus();   // compute units of the current device (cached)
 int device_lds_bytes();    // LDS one workgroup may take on the current device (cached)
 double device_clock_hz();  // shader clock of the current device (cached)

@@ -137,25 +137,6 @@ __device__ __forceinline__ int32_t row_codes_any(const void *x, int type, int64_
     return row_codes(static_cast<const f16 *>(x) + at, K, Kp, whole, g, codes, thread, threads);
 }
 
-// A wavefront a row; rows up to the next multiple of four are pad rows, of code 0.
-__global__ void __launch_bounds__(256) input_codes_kernel(const void *x, int type, int64_t rows, int K, int Kp, const Grids *grids,
-                                                          uint8_t *codes, int32_t *row_sums)
-{
-    const int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
-    const int lane = threadIdx.x & 63;
-    if (r >= rows) {
-        for (int k = 4 * lane; k < Kp; k += 256)
-            *reinterpret_cast<uint32_t *>(codes + r * Kp + k) = 0u;
-        if (lane == 0)
-            row_sums[r] = 0;
-        return;
-    }
-    const Grid g = grids->in;
-    const int32_t sum = wave_sum(row_codes_any(x, type, r * K, K, Kp, g, codes + r * Kp, lane, 64));
-    if (lane == 0)
-        row_sums[r] = sum;
-}
-
 // Few rows: every workgroup finds the range itself, of all rows, and then takes its own row.
 __global__ void __launch_bounds__(512) few_codes_kernel(const void *x, int type, int rows, int K, int Kp, RangeSource src,
                                                         const Grid *kernel_grid, Grids *grids, uint8_t *codes, int32_t *row_sums)
@@ -189,18 +170,16 @@ __global__ void __launch_bounds__(512) few_codes_kernel(const void *x, int type,
     }
 }
 
-constexpr int kSlab = 64;   // depth a workgroup of kernel_codes_kernel takes
-
 template <typename T>
 __device__ void kernel_slab(const T *__restrict__ w, int K, int64_t N, const Pieces &pc, const Grid &g, uint8_t *__restrict__ codes,
-                            int64_t c, int k0, int (&sum)[4])
+                            int64_t c, int k0, int lines, int (&sum)[4])
 {
     const int piece = (int)(c / pc.width);
     uint8_t *const to = codes + pc.offset(piece) + (c - pc.first(piece));
     const int pitch = pc.width_of(piece);
     const bool whole = c + 4 <= N && (N & 3) == 0 && ((uintptr_t)w & (4 * sizeof(T) - 1)) == 0;
 #pragma unroll 4
-    for (int i = 0; i < kSlab / 4; ++i) {
+    for (int i = 0; i < lines; ++i) {
         const int k = k0 + 4 * i;
         if (k >= pc.Kp)
             break;
@@ -219,32 +198,62 @@ __device__ void kernel_slab(const T *__restrict__ w, int K, int64_t N, const Pie
     }
 }
 
-// 256 columns (four a lane) by kSlab of the depth (a wavefront takes every fourth); column sums are added to what the launch
-// before cleared, as whole numbers, so in any order.
-__global__ void __launch_bounds__(256) kernel_codes_kernel(const void *w, int type, int K, int64_t N, Pieces pc, const Grids *grids,
-                                                           uint8_t *codes, int32_t *column_sums)
+// The first x_blocks workgroups take four rows of the input each, a wavefront a row (rows up to the next multiple of four are pad
+// rows, of code 0).  The others take 256 columns of the kernel, four a lane, by 4 * lines of the depth, a wavefront every fourth;
+// column sums are added to what the launch before cleared, as whole numbers, so in any order.  Every workgroup makes the grid it
+// needs out of the range's pairs itself: a launch for that alone would be longer than folding 256 of them.
+__global__ void __launch_bounds__(256) codes_kernel(CodesJob job, int x_blocks, int column_blocks, int lines)
 {
+    __shared__ float ends[8];
     __shared__ int32_t red[4][256];
     const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
-    const int64_t c = ((int64_t)blockIdx.x * 64 + lane) * 4;
-    int sum[4] = {};
-    if (c < pc.Np) {
-        const Grid g = grids->kernel;
-        const int k0 = (int)blockIdx.y * kSlab + wave;
-        if (type == AXC_F32)
-            kernel_slab(static_cast<const float *>(w), K, N, pc, g, codes, c, k0, sum);
-        else if (type == AXC_BF16)
-            kernel_slab(static_cast<const bf16 *>(w), K, N, pc, g, codes, c, k0, sum);
+    float lo, hi;
+    if ((int)blockIdx.x < x_blocks) {
+        fold(job.x_range, lo, hi, ends);
+        const Grid g = grid_of_range(lo, hi);
+        if (blockIdx.x == 0 && threadIdx.x == 0) {
+            job.grids->in = g;
+            if (!job.kernel)
+                job.grids->kernel = *job.kernel_grid;
+        }
+        const int64_t r = (int64_t)blockIdx.x * 4 + wave;
+        const int Kp = job.pieces.Kp;
+        uint8_t *const codes = job.x_codes + r * Kp;
+        int32_t sum = 0;
+        if (r < job.rows)
+            sum = row_codes_any(job.x, job.x_type, r * job.K, job.K, Kp, g, codes, lane, 64);
         else
-            kernel_slab(static_cast<const f16 *>(w), K, N, pc, g, codes, c, k0, sum);
+            for (int k = 4 * lane; k < Kp; k += 256)
+                *reinterpret_cast<uint32_t *>(codes + k) = 0u;
+        sum = wave_sum(sum);
+        if (lane == 0)
+            job.row_sums[r] = sum;
+        return;
+    }
+    fold(job.kernel_range, lo, hi, ends);
+    const Grid g = grid_of_range(lo, hi);
+    const int block = (int)blockIdx.x - x_blocks, slab = block / column_blocks;
+    const int64_t first = (int64_t)(block - slab * column_blocks) * 256, c = first + 4 * lane;
+    if (block == 0 && threadIdx.x == 0)
+        job.grids->kernel = g;
+    int sum[4] = {};
+    if (c < job.pieces.Np) {
+        const int k0 = slab * 4 * lines + wave;
+        if (job.kernel_type == AXC_F32)
+            kernel_slab(static_cast<const float *>(job.kernel), job.K, job.N, job.pieces, g, job.kernel_codes, c, k0, lines, sum);
+        else if (job.kernel_type == AXC_BF16)
+            kernel_slab(static_cast<const bf16 *>(job.kernel), job.K, job.N, job.pieces, g, job.kernel_codes, c, k0, lines, sum);
+        else
+            kernel_slab(static_cast<const f16 *>(job.kernel), job.K, job.N, job.pieces, g, job.kernel_codes, c, k0, lines, sum);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j)
         red[wave][4 * lane + j] = sum[j];
     __syncthreads();
-    const int64_t column = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (column < pc.Np)
-        atomicAdd(column_sums + column, red[0][threadIdx.x] + red[1][threadIdx.x] + red[2][threadIdx.x] + red[3][threadIdx.x]);
+    const int64_t column = first + threadIdx.x;
+    if (column < job.pieces.Np)
+        atomicAdd(job.column_sums + column,
+                  red[0][threadIdx.x] + red[1][threadIdx.x] + red[2][threadIdx.x] + red[3][threadIdx.x]);
 }
 
 // ---- sums of few rows ----
@@ -360,56 +369,134 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const uint16_t *__restric
 }
 
 // ---- what is made of the sums ----
-// residual + activation(product + bias), four columns a lane, a wavefront a row at a time.  Products and everything behind them
-// are in float32, rounded once to the output's type (`pre`, what the activation is given, once more).
+// residual + activation(product + bias), four neighbouring values of a row.  Products and everything behind them are in float32,
+// rounded once to the output's type (`pre`, what the activation is given, once more).
+template <typename T, typename I>
+__device__ __forceinline__ void dense_four(const int32_t (&sum)[4], I row, const I (&column)[4], const float (&bias)[4], float scale,
+                                           int64_t r, int c, int columns, bool whole, const DenseOut &o)
+{
+    float z[4], y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        z[j] = __fmul_rn(Bracket<I>::value(sum[j], row, column[j]), scale);
+        if (o.bias)
+            z[j] = __fadd_rn(z[j], bias[j]);
+    }
+    activate_four(z, y, o.activation);
+    const int64_t to = r * o.ld + c;
+    if (o.pre)
+        store_values<T, 4>(static_cast<T *>(o.pre) + to, columns - c, whole, z);
+    if (o.residual) {
+        float v[4];
+        load_values<T, 4>(static_cast<const T *>(o.residual) + to, columns - c, whole, 0.0f, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            y[j] = __fadd_rn(y[j], v[j]);
+    }
+    store_values<T, 4>(static_cast<T *>(o.out) + to, columns - c, whole, y);
+}
 template <typename T>
+__device__ __forceinline__ bool whole_fours(int c, int columns, const DenseOut &o)
+{
+    return c + 4 <= columns && (o.ld & 3) == 0 &&
+           (((uintptr_t)o.out | (uintptr_t)o.residual | (uintptr_t)o.pre) & (4 * sizeof(T) - 1)) == 0;
+}
+template <typename I>
+__device__ __forceinline__ void column_terms(const TableSums &s, const Bracket<I> &b, int c, int columns, const DenseOut &o,
+                                             I (&column)[4], float (&bias)[4])
+{
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const bool there = c + j < columns;
+        column[j] = there ? b.column(s.column_sums[c + j]) : (I)0;
+        bias[j] = there && o.bias ? load_any(o.bias, c + j, o.bias_type) : 0.0f;
+    }
+}
+
+// Sums by rows: four columns a lane, a wavefront a row at a time.
+template <typename T, typename I>
 __global__ void __launch_bounds__(256) dense_out_kernel(TableSums s, int64_t rows, int columns, DenseOut o)
 {
     const int c = ((int)blockIdx.x * 64 + (threadIdx.x & 63)) * 4;
     if (c >= columns)
         return;
     const float scale = __fmul_rn(s.grids->in.scale, s.grids->kernel.scale);
-    const int64_t zi = s.grids->in.zero;
-    const bool whole = c + 4 <= columns && (o.ld & 3) == 0 && ((uintptr_t)o.out & (4 * sizeof(T) - 1)) == 0 &&
-                       ((uintptr_t)o.residual & (4 * sizeof(T) - 1)) == 0 && ((uintptr_t)o.pre & (4 * sizeof(T) - 1)) == 0;
-    int64_t column[4];
+    const Bracket<I> b(s);
+    const bool whole = whole_fours<T>(c, columns, o);
+    I column[4];
     float bias[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const bool there = c + j < columns;
-        column[j] = there ? zi * s.column_sums[c + j] : 0;
-        bias[j] = there && o.bias ? load_any(o.bias, c + j, o.bias_type) : 0.0f;
-    }
+    column_terms(s, b, c, columns, o, column, bias);
     for (int64_t r = (int64_t)blockIdx.y * 4 + threadIdx.x / 64; r < rows; r += (int64_t)gridDim.y * 4) {
-        const int64_t at = r * s.pitch + c;
-        int32_t t[4] = {};
+        const i32x4 t = four_sums(s.raw, r, c);
+        const int32_t sum[4] = {t[0], t[1], t[2], t[3]};
+        dense_four<T, I>(sum, b.row(s.row_sums[r]), column, bias, scale, r, c, columns, whole, o);
+    }
+}
+
+// Sums by rows of few rows, in many parts: the four wavefronts take a quarter of the parts each.
+template <typename T, typename I>
+__global__ void __launch_bounds__(256) dense_out_parts_kernel(TableSums s, int columns, DenseOut o)
+{
+    __shared__ i32x4 red[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+    const int c = ((int)blockIdx.x * 64 + lane) * 4;
+    const int64_t r = blockIdx.y;
+    i32x4 t = {};
+    if (c < columns) {
+        const int32_t *const p = s.raw.acc + r * s.raw.pitch + c;
 #pragma unroll 8
-        for (int i = 0; i < s.splits; ++i) {
-            const i32x4 v = *reinterpret_cast<const i32x4 *>(s.acc + i * s.split_stride + at);
+        for (int i = wave; i < s.raw.splits; i += 4)
+            t += *reinterpret_cast<const i32x4 *>(p + i * s.raw.split_stride);
+    }
+    red[wave][lane] = t;
+    __syncthreads();
+    if (wave != 0 || c >= columns)
+        return;
+    t = red[0][lane] + red[1][lane] + red[2][lane] + red[3][lane];
+    const int32_t sum[4] = {t[0], t[1], t[2], t[3]};
+    const Bracket<I> b(s);
+    I column[4];
+    float bias[4];
+    column_terms(s, b, c, columns, o, column, bias);
+    dense_four<T, I>(sum, b.row(s.row_sums[r]), column, bias, __fmul_rn(s.grids->in.scale, s.grids->kernel.scale), r, c, columns,
+                     whole_fours<T>(c, columns, o), o);
+}
+
+// Turned sums: 64 rows by 64 columns through LDS.
+template <typename T, typename I>
+__global__ void __launch_bounds__(256) dense_out_turned_kernel(TableSums s, int64_t rows, int columns, DenseOut o)
+{
+    __shared__ int32_t tile[64][65];
+    const int quad = (threadIdx.x & 15) * 4, line = threadIdx.x / 16;
+    const int c0 = (int)blockIdx.x * 64;
+    const int64_t r0 = (int64_t)blockIdx.y * 64;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int c = c0 + line + 16 * i;
+        if (c < columns && r0 + quad < rows) {
+            const i32x4 t = four_sums(s.raw, r0 + quad, c);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                t[j] += v[j];
+                tile[quad + j][line + 16 * i] = t[j];
         }
-        const int64_t row = row_term(s, r);
-        float z[4], y[4];
+    }
+    __syncthreads();
+    const int c = c0 + quad;
+    if (c >= columns)
+        return;
+    const float scale = __fmul_rn(s.grids->in.scale, s.grids->kernel.scale);
+    const Bracket<I> b(s);
+    const bool whole = whole_fours<T>(c, columns, o);
+    I column[4];
+    float bias[4];
+    column_terms(s, b, c, columns, o, column, bias);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            z[j] = __fmul_rn((float)((int64_t)t[j] + row - column[j]), scale);
-            if (o.bias)
-                z[j] = __fadd_rn(z[j], bias[j]);
-            y[j] = activate(z[j], o.activation);
+    for (int i = 0; i < 4; ++i) {
+        const int at = line + 16 * i;
+        if (r0 + at < rows) {
+            const int32_t sum[4] = {tile[at][quad], tile[at][quad + 1], tile[at][quad + 2], tile[at][quad + 3]};
+            dense_four<T, I>(sum, b.row(s.row_sums[r0 + at]), column, bias, scale, r0 + at, c, columns, whole, o);
         }
-        const int64_t to = r * o.ld + c;
-        if (o.pre)
-            store_values<T, 4>(static_cast<T *>(o.pre) + to, columns - c, whole, z);
-        if (o.residual) {
-            float v[4];
-            load_values<T, 4>(static_cast<const T *>(o.residual) + to, columns - c, whole, 0.0f, v);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                y[j] = __fadd_rn(y[j], v[j]);
-        }
-        store_values<T, 4>(static_cast<T *>(o.out) + to, columns - c, whole, y);
     }
 }
 
@@ -455,14 +542,6 @@ hipError_t launch_grids(const RangeSource &in, const RangeSource &kernel, bool h
     return hipGetLastError();
 }
 
-hipError_t launch_input_codes(const void *x, int type, int64_t rows, int K, int Kp, const Grids *grids, uint8_t *codes,
-                              int32_t *row_sums, hipStream_t stream)
-{
-    hipLaunchKernelGGL(input_codes_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, x, type, rows, K, Kp, grids,
-                       codes, row_sums);
-    return hipGetLastError();
-}
-
 hipError_t launch_few_codes(const void *x, int type, int rows, int K, int Kp, const RangeSource &src, const Grid *kernel_grid,
                             Grids *grids, uint8_t *codes, int32_t *row_sums, hipStream_t stream)
 {
@@ -471,11 +550,18 @@ hipError_t launch_few_codes(const void *x, int type, int rows, int K, int Kp, co
     return hipGetLastError();
 }
 
-hipError_t launch_kernel_codes(const void *kernel, int type, int K, int64_t N, const Pieces &pieces, const Grids *grids,
-                               uint8_t *codes, int32_t *column_sums, hipStream_t stream)
+hipError_t launch_codes(const CodesJob &job, hipStream_t stream)
 {
-    hipLaunchKernelGGL(kernel_codes_kernel, dim3((unsigned)((pieces.Np + 255) / 256), (unsigned)((pieces.Kp + kSlab - 1) / kSlab)),
-                       dim3(256), 0, stream, kernel, type, K, N, pieces, grids, codes, column_sums);
+    const int x_blocks = job.x ? (int)((job.rows + 3) / 4) : 0;
+    const int column_blocks = job.kernel ? (int)((job.pieces.Np + 255) / 256) : 1;
+    // a wavefront 16 lines of the depth, fewer where that would leave CUs without work
+    int lines = 16;
+    auto slabs = [&] { return (job.pieces.Kp + 4 * lines - 1) / (4 * lines); };
+    while (lines > 4 && (int64_t)slabs() * column_blocks < 1024)
+        lines /= 2;
+    const int64_t kernel_blocks = job.kernel ? (int64_t)slabs() * column_blocks : 0;
+    hipLaunchKernelGGL(codes_kernel, dim3((unsigned)(x_blocks + kernel_blocks)), dim3(256), 0, stream, job, x_blocks, column_blocks,
+                       lines);
     return hipGetLastError();
 }
 
@@ -504,17 +590,36 @@ hipError_t launch_few_rows(const uint16_t *tableI, const uint8_t *x_codes, int r
     return hipGetLastError();
 }
 
+template <typename T, typename I>
+static hipError_t dense_out(const TableSums &s, int64_t rows, int columns, const DenseOut &o, hipStream_t stream)
+{
+    if (s.raw.turned) {
+        hipLaunchKernelGGL((dense_out_turned_kernel<T, I>), dim3((unsigned)((columns + 63) / 64), (unsigned)((rows + 63) / 64)),
+                           dim3(256), 0, stream, s, rows, columns, o);
+    } else if (s.raw.splits >= 8 && rows <= 64) {
+        hipLaunchKernelGGL((dense_out_parts_kernel<T, I>), dim3((unsigned)((columns + 255) / 256), (unsigned)rows), dim3(256), 0,
+                           stream, s, columns, o);
+    } else {
+        const int64_t by = (rows + 3) / 4;
+        hipLaunchKernelGGL((dense_out_kernel<T, I>), dim3((unsigned)((columns + 255) / 256), (unsigned)(by > 4096 ? 4096 : by)),
+                           dim3(256), 0, stream, s, rows, columns, o);
+    }
+    return hipGetLastError();
+}
+template <typename T>
+static hipError_t dense_out(const TableSums &s, int64_t rows, int columns, const DenseOut &o, hipStream_t stream)
+{
+    return s.K > kNarrowDepth ? dense_out<T, int64_t>(s, rows, columns, o, stream)
+                              : dense_out<T, uint32_t>(s, rows, columns, o, stream);
+}
+
 hipError_t launch_dense_out(const TableSums &s, int64_t rows, int columns, const DenseOut &o, hipStream_t stream)
 {
-    const int64_t by = (rows + 3) / 4;
-    const dim3 grid((unsigned)((columns + 255) / 256), (unsigned)(by > 4096 ? 4096 : by));
     if (o.type == AXC_F32)
-        hipLaunchKernelGGL(dense_out_kernel<float>, grid, dim3(256), 0, stream, s, rows, columns, o);
-    else if (o.type == AXC_BF16)
-        hipLaunchKernelGGL(dense_out_kernel<bf16>, grid, dim3(256), 0, stream, s, rows, columns, o);
-    else
-        hipLaunchKernelGGL(dense_out_kernel<f16>, grid, dim3(256), 0, stream, s, rows, columns, o);
-    return hipGetLastError();
+        return dense_out<float>(s, rows, columns, o, stream);
+    if (o.type == AXC_BF16)
+        return dense_out<bf16>(s, rows, columns, o, stream);
+    return dense_out<f16>(s, rows, columns, o, stream);
 }
 
 } // namespace axc

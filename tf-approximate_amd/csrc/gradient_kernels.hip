@@ -58,88 +58,139 @@ __device__ __forceinline__ void store_terms(bf16 *p, int parts, int64_t pitch, f
     }
 }
 
-// Gradient in front of the product, 64 x 64 of it a workgroup: straight, turned through LDS, and summed by columns.
-template <bool LOSS>
-__global__ void __launch_bounds__(256) grad_terms_kernel(GradSource g, int64_t rows, int64_t cols, int64_t ld,
-                                                         int straight_parts, bf16 *__restrict__ straight, int turned_parts,
-                                                         bf16 *__restrict__ turned, float *__restrict__ column_partials)
+// What a logit's sum says of its gradient: coefficient (softmax - one-hot).
+template <typename I>
+struct LogitTerms {
+    Bracket<I> b;
+    float scale;
+    const GradSource &g;
+    __device__ __forceinline__ explicit LogitTerms(const GradSource &source)
+        : b(source.sums), scale(__fmul_rn(source.sums.grids->in.scale, source.sums.grids->kernel.scale)), g(source)
+    {
+    }
+    struct Line {                        // of a row
+        I term;
+        float share, lse;
+        int64_t target;
+    };
+    __device__ __forceinline__ Line line(int64_t r) const
+    {
+        return {b.row(g.sums.row_sums[r]), g.coefficient[r], g.lse[r], g.targets[r] - g.first_column};
+    }
+    __device__ __forceinline__ float bias(int64_t c) const { return g.bias ? load_any(g.bias, c, g.bias_type) : 0.0f; }
+    __device__ __forceinline__ I column(int64_t c) const { return b.column(g.sums.column_sums[c]); }
+    __device__ __forceinline__ float operator()(int32_t sum, const Line &l, I column, float bias, int64_t c) const
+    {
+        float z = __fmul_rn(Bracket<I>::value(sum, l.term, column), scale);
+        if (g.bias)
+            z = __fadd_rn(z, bias);
+        const float p = __expf(z - l.lse);
+        // a row that does not count has no gradient, whatever its logits are
+        return l.share == 0.0f ? 0.0f : l.share * (c == l.target ? p - 1.0f : p);
+    }
+};
+
+// Gradient in front of the product, 64 x 64 of it a workgroup: into LDS, and from there out straight, turned, and summed by columns.
+// SOURCE 0: dense; 1: logits' sums by rows, 2: turned.  `first`: the run's first row, in units of 64.
+template <int SOURCE, typename I>
+__global__ void __launch_bounds__(256) grad_terms_kernel(GradSource g, int64_t first, int64_t rows, int64_t rows_pad, int64_t cols,
+                                                         int64_t ld, int straight_parts, bf16 *__restrict__ straight,
+                                                         int turned_parts, bf16 *__restrict__ turned,
+                                                         float *__restrict__ column_partials)
 {
     __shared__ float tile[64][65];
     const int64_t r0 = (int64_t)blockIdx.y * 64, c0 = (int64_t)blockIdx.x * 64;
-    const int64_t rows_pad = (int64_t)gridDim.y * 64, cols_pad = (int64_t)gridDim.x * 64;
+    const int64_t cols_pad = (int64_t)gridDim.x * 64;
     const int quad = (threadIdx.x & 15) * 4, line = threadIdx.x / 16;
-    const int64_t c = c0 + quad;
-    float scale = 0.0f, bias[4] = {};
-    int64_t column[4] = {};
-    if constexpr (LOSS) {
-        scale = __fmul_rn(g.sums.grids->in.scale, g.sums.grids->kernel.scale);
+    if constexpr (SOURCE == 2) {         // a thread four rows of a column
+        const LogitTerms<I> at(g);
+        typename LogitTerms<I>::Line lines[4] = {};
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (c + j < cols) {
-                column[j] = (int64_t)g.sums.grids->in.zero * g.sums.column_sums[c + j];
-                bias[j] = g.bias ? load_any(g.bias, c + j, g.bias_type) : 0.0f;
-            }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t r = r0 + line + 16 * i;
-        float v[4] = {};
-        if (r < rows && c < cols) {
-            if constexpr (LOSS) {
-                const float share = g.coefficient[r], lse = g.lse[r];
-                if (share != 0.0f) {   // a row that does not count has no gradient, whatever its logits are
-                    const int64_t row = row_term(g.sums, r), target = g.targets[r] - g.first_column;
-                    const int32_t *const acc = g.sums.acc + r * g.sums.pitch + c;
-                    int32_t t[4] = {};
-                    for (int k = 0; k < g.sums.splits; ++k) {
-                        const i32x4 a = *reinterpret_cast<const i32x4 *>(acc + k * g.sums.split_stride);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            t[j] += a[j];
-                    }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        float z = __fmul_rn((float)((int64_t)t[j] + row - column[j]), scale);
-                        if (g.bias)
-                            z = __fadd_rn(z, bias[j]);
-                        const float p = expf(z - lse);
-                        v[j] = c + j < cols ? share * (c + j == target ? p - 1.0f : p) : 0.0f;
-                    }
-                }
-            } else {
-                load4_any(g.grad, r * ld + c, cols - c, g.type, v);
-                if (g.pre) {
-                    float z[4];
-                    load4_any(g.pre, r * ld + c, cols - c, g.type, z);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (c + j < cols)
-                            v[j] *= activation_slope(z[j], g.activation);
-                }
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            tile[line + 16 * i][quad + j] = v[j];
-        if (straight)
-            store_terms(straight + r * straight_parts * cols_pad + c, straight_parts, cols_pad, v);
-    }
-    __syncthreads();
-    if (turned)
+            if (r0 + quad + j < rows)
+                lines[j] = at.line(r0 + quad + j);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int col = line + 16 * i;
-            float v[4];
+            const int64_t c = c0 + line + 16 * i;
+            const bool there = c < cols && r0 + quad < rows;
+            i32x4 sum = {};
+            I column = 0;
+            float bias = 0.0f;
+            if (there) {
+                sum = four_sums(g.sums.raw, r0 + quad, c);
+                column = at.column(c);
+                bias = at.bias(c);
+            }
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                v[j] = tile[quad + j][col];
-            store_terms(turned + (c0 + col) * turned_parts * rows_pad + r0 + quad, turned_parts, rows_pad, v);
+                tile[quad + j][line + 16 * i] = there && r0 + quad + j < rows ? at(sum[j], lines[j], column, bias, c) : 0.0f;
         }
+    } else {
+        const int64_t c = c0 + quad;
+        I column[4] = {};
+        float bias[4] = {};
+        if constexpr (SOURCE == 1) {
+            const LogitTerms<I> at(g);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (c + j < cols) {
+                    column[j] = at.column(c + j);
+                    bias[j] = at.bias(c + j);
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t r = r0 + line + 16 * i;
+            float v[4] = {};
+            if (r < rows && c < cols) {
+                if constexpr (SOURCE == 1) {
+                    const LogitTerms<I> at(g);
+                    const typename LogitTerms<I>::Line l = at.line(r);
+                    const i32x4 sum = four_sums(g.sums.raw, r, c);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        v[j] = c + j < cols ? at(sum[j], l, column[j], bias[j], c + j) : 0.0f;
+                } else {
+                    load4_any(g.grad, r * ld + c, cols - c, g.type, v);
+                    if (g.pre) {
+                        float z[4];
+                        load4_any(g.pre, r * ld + c, cols - c, g.type, z);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (c + j < cols)
+                                v[j] *= activation_slope(z[j], g.activation);
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                tile[line + 16 * i][quad + j] = v[j];
+        }
+    }
+    __syncthreads();
+    const int64_t above = first * 64;    // rows of earlier runs
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int at = line + 16 * i;
+        float v[4];
+        if (straight) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                v[j] = tile[at][quad + j];
+            store_terms(straight + (above + r0 + at) * straight_parts * cols_pad + c0 + quad, straight_parts, cols_pad, v);
+        }
+        if (turned) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                v[j] = tile[quad + j][at];
+            store_terms(turned + (c0 + at) * turned_parts * rows_pad + above + r0 + quad, turned_parts, rows_pad, v);
+        }
+    }
     if (column_partials && threadIdx.x < 64) {
         float sum = 0.0f;
         for (int i = 0; i < 64; ++i)
             sum += tile[i][threadIdx.x];
-        column_partials[(int64_t)blockIdx.y * cols_pad + c0 + threadIdx.x] = sum;
+        column_partials[(first + blockIdx.y) * cols_pad + c0 + threadIdx.x] = sum;
     }
 }
 
@@ -334,16 +385,29 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const float *__restric
 
 } // namespace
 
-hipError_t launch_grad_terms(const GradSource &g, bool loss, int64_t rows, int64_t cols, int64_t ld, int straight_parts,
-                             bf16 *straight, int turned_parts, bf16 *turned, float *column_partials, hipStream_t stream)
+hipError_t launch_grad_terms(const GradSource &of_run, bool loss, int64_t first, int64_t run_rows, int64_t rows, int64_t cols,
+                             int64_t ld, int straight_parts, bf16 *straight, int turned_parts, bf16 *turned, float *column_partials,
+                             hipStream_t stream)
 {
-    const dim3 grid((unsigned)(product_pad(cols) / 64), (unsigned)(product_pad(rows) / 64));
-    if (loss)
-        hipLaunchKernelGGL(grad_terms_kernel<true>, grid, dim3(256), 0, stream, g, rows, cols, ld, straight_parts, straight,
-                           turned_parts, turned, column_partials);
+    const int64_t rows_pad = product_pad(rows);
+    // the last run makes the pad rows too
+    const int64_t high = first + run_rows < rows ? run_rows : rows_pad - first;
+    const dim3 grid((unsigned)(product_pad(cols) / 64), (unsigned)(high / 64));
+#define AXC_TERMS(SOURCE, I)                                                                                                       \
+    hipLaunchKernelGGL((grad_terms_kernel<SOURCE, I>), grid, dim3(256), 0, stream, of_run, first / 64, run_rows, rows_pad, cols, ld, \
+                       straight_parts, straight, turned_parts, turned, column_partials)
+    const bool narrow = of_run.sums.K <= kNarrowDepth;
+    if (!loss)
+        AXC_TERMS(0, uint32_t);
+    else if (of_run.sums.raw.turned && narrow)
+        AXC_TERMS(2, uint32_t);
+    else if (of_run.sums.raw.turned)
+        AXC_TERMS(2, int64_t);
+    else if (narrow)
+        AXC_TERMS(1, uint32_t);
     else
-        hipLaunchKernelGGL(grad_terms_kernel<false>, grid, dim3(256), 0, stream, g, rows, cols, ld, straight_parts, straight,
-                           turned_parts, turned, column_partials);
+        AXC_TERMS(1, int64_t);
+#undef AXC_TERMS
     return hipGetLastError();
 }
 

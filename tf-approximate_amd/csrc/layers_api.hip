@@ -110,59 +110,39 @@ axc_conv2d_desc conv_desc(int64_t rows, int Kp, int width)
     return c;
 }
 
-// What the sums of `rows` rows (of up to kRowRun at a time) and any piece need beside their own memory.
-int sums_workspace(int64_t rows, const Pieces &pc, size_t *bytes)
+// What the sums of a run of rows (kRowRun at most) and any piece need: int32 values of their own, and scratch bytes.
+int sums_workspace(int64_t rows, const Pieces &pc, size_t *count, size_t *bytes)
 {
-    *bytes = 0;
-    if (few_rows(rows))
-        return AXC_OK;
-    const int64_t runs[2] = {std::min(fours(rows), kRowRun), fours(rows) % kRowRun};
-    const int widths[2] = {pc.width_of(0), pc.width_of(pc.count - 1)};
-    for (const int64_t run : runs)
-        for (const int width : widths) {
-            if (run == 0)
-                continue;
-            const axc_conv2d_desc c = conv_desc(run, pc.Kp, width);
-            size_t need = 0;
-            if (int rc = axc_conv2d_workspace_bytes(&c, &need))
-                return rc;
-            *bytes = std::max(*bytes, need);
+    for (const int width : {pc.width_of(0), pc.width_of(pc.count - 1)}) {
+        if (few_rows(rows)) {
+            *count = std::max(*count, (size_t)few_rows_splits(rows, pc.Kp, width) * rows * width);
+            continue;
         }
+        const axc_conv2d_desc c = conv_desc(fours(rows), pc.Kp, width);
+        size_t need = 0;
+        if (int rc = axc_conv2d_workspace_bytes(&c, &need))
+            return rc;
+        *count = std::max(*count, (size_t)fours(rows) * width);
+        *bytes = std::max(*bytes, need);
+    }
     return AXC_OK;
 }
-size_t sums_count(int64_t rows, const Pieces &pc)   // int32 values
-{
-    if (!few_rows(rows))
-        return (size_t)fours(rows) * pc.width;
-    size_t most = 0;
-    for (const int width : {pc.width_of(0), pc.width_of(pc.count - 1)})
-        most = std::max(most, (size_t)few_rows_splits(rows, pc.Kp, width) * rows * width);
-    return most;
-}
 
-// Sums of `rows` rows and piece p into acc.
+// Sums of a run of rows and piece p: in acc or in the scratch.
 int table_sums(const axc_table *table, const uint8_t *input_codes, int64_t rows, const Pieces &pc, int p, const uint8_t *kernel_codes,
-               int32_t *acc, void *ws, size_t ws_bytes, hipStream_t stream, TableSums *out)
+               int32_t *acc, void *ws, size_t ws_bytes, hipStream_t stream, RawSums *out)
 {
     const int width = pc.width_of(p);
     const uint8_t *const codes = kernel_codes + pc.offset(p);
-    out->acc = acc;
-    out->pitch = width;
-    out->splits = 1;
-    out->split_stride = 0;
     if (few_rows(rows)) {
-        out->splits = few_rows_splits(rows, pc.Kp, width);
-        out->split_stride = rows * width;
+        const int splits = few_rows_splits(rows, pc.Kp, width);
+        *out = {acc, rows * width, splits, width, 0};
         ApiTimer t("few_rows", stream);
-        AXC_HIP(launch_few_rows(table->dev_tableI, input_codes, (int)rows, pc.Kp, codes, width, out->splits, acc, stream));
+        AXC_HIP(launch_few_rows(table->dev_tableI, input_codes, (int)rows, pc.Kp, codes, width, splits, acc, stream));
         return AXC_OK;
     }
-    for (int64_t r = 0; r < fours(rows); r += kRowRun) {
-        const axc_conv2d_desc c = conv_desc(std::min(kRowRun, fours(rows) - r), pc.Kp, width);
-        if (int rc = axc_conv2d_codes_acc_i32(table, &c, input_codes + r * pc.Kp, codes, 0, acc + r * width, ws, ws_bytes, stream))
-            return rc;
-    }
-    return AXC_OK;
+    const axc_conv2d_desc c = conv_desc(fours(rows), pc.Kp, width);
+    return api_codes_sums(table, &c, input_codes, codes, acc, ws, ws_bytes, stream, out);
 }
 
 // ---- operands ----
@@ -199,34 +179,82 @@ RangeSource input_source(const axc_dense_desc *d, const void *range)
     return {nullptr, -1, 0.0f, 0.0f};
 }
 
-// Grids of input and kernel (kernel_grid: it is known already), and the column sums cleared.
-int find_grids(const axc_dense_desc *d, const void *input, const void *range, const void *kernel, const Operands &o, int64_t Np,
-               hipStream_t stream)
+// The ranges that have to be looked for, into pairs; clears the column sums of a kernel whose codes are to be made.
+int find_ranges(const axc_dense_desc *d, const void *input, const void *range, const void *kernel, float *x_pairs, float *kernel_pairs,
+                int32_t *zeros, int64_t n_zeros, RangeSource *in, RangeSource *k, hipStream_t stream)
 {
-    RangeSource in = input_source(d, range), k = {o.kernel_pairs, 0, 0.0f, 0.0f};
-    const bool look = !in.pairs && in.count < 0;
+    *in = input ? input_source(d, range) : RangeSource{};
+    const bool look = !in->pairs && in->count < 0;
     int x_count = 0, k_count = 0;
     {
         ApiTimer t("layer_range", stream);
         AXC_HIP(launch_range(look ? input : nullptr, d->input_type, d->rows * d->depth, kernel, d->kernel_type,
-                             d->depth * d->columns, o.x_pairs, o.kernel_pairs, o.column_sums, o.column_sums ? Np : 0, &x_count,
-                             &k_count, stream));
+                             d->depth * d->columns, x_pairs, kernel_pairs, zeros, n_zeros, &x_count, &k_count, stream));
     }
     if (look)
-        in = {o.x_pairs, x_count, 0.0f, 0.0f};
-    k.count = k_count;
+        *in = {x_pairs, x_count, 0.0f, 0.0f};
+    *k = {kernel_pairs, k_count, 0.0f, 0.0f};
+    return AXC_OK;
+}
+
+int make_codes(const axc_dense_desc *d, const void *input, const RangeSource &in, const void *kernel, const RangeSource &k,
+               const Grid *kernel_grid, const Operands &o, const Pieces &pc, hipStream_t stream)
+{
+    CodesJob job = {};
+    job.x = input;
+    job.kernel = kernel;
+    job.x_type = d->input_type;
+    job.kernel_type = d->kernel_type;
+    job.rows = d->rows;
+    job.N = d->columns;
+    job.K = (int)d->depth;
+    job.x_range = in;
+    job.kernel_range = k;
+    job.kernel_grid = kernel_grid;
+    job.pieces = pc;
+    job.grids = o.grids;
+    job.x_codes = o.x_codes;
+    job.kernel_codes = o.kernel_codes;
+    job.row_sums = o.row_sums;
+    job.column_sums = o.column_sums;
+    ApiTimer t("layer_codes", stream);
+    AXC_HIP(launch_codes(job, stream));
+    return AXC_OK;
+}
+
+// Ranges, grids, codes and their sums of both operands.
+int find_codes(const axc_dense_desc *d, const void *input, const void *range, const void *kernel, const Operands &o, const Pieces &pc,
+               hipStream_t stream)
+{
+    RangeSource in, k;
+    if (int rc = find_ranges(d, input, range, kernel, o.x_pairs, o.kernel_pairs, o.column_sums, pc.Np, &in, &k, stream))
+        return rc;
+    return make_codes(d, input, in, kernel, k, nullptr, o, pc, stream);
+}
+// The grids alone.
+int find_grids(const axc_dense_desc *d, const void *input, const void *range, const void *kernel, const Operands &o, hipStream_t stream)
+{
+    RangeSource in, k;
+    if (int rc = find_ranges(d, input, range, kernel, o.x_pairs, o.kernel_pairs, nullptr, 0, &in, &k, stream))
+        return rc;
     ApiTimer t("layer_grids", stream);
     AXC_HIP(launch_grids(in, k, true, true, o.grids, stream));
     return AXC_OK;
 }
 
-int make_codes(const axc_dense_desc *d, const void *input, const void *kernel, const Operands &o, const Pieces &pc, hipStream_t stream)
+// What a consumer of the sums of piece p and the run of rows from r on is given.
+TableSums sums_of(const axc_table *table, const axc_dense_desc *d, const Operands &o, const Pieces &pc, int p, int64_t r,
+                  const RawSums &raw)
 {
-    ApiTimer t("layer_codes", stream);
-    AXC_HIP(launch_input_codes(input, d->input_type, d->rows, (int)d->depth, pc.Kp, o.grids, o.x_codes, o.row_sums, stream));
-    AXC_HIP(launch_kernel_codes(kernel, d->kernel_type, (int)d->depth, d->columns, pc, o.grids, o.kernel_codes, o.column_sums,
-                                stream));
-    return AXC_OK;
+    TableSums s = {};
+    s.raw = raw;
+    s.row_sums = o.row_sums + r;
+    s.column_sums = o.column_sums + pc.first(p);
+    s.table = table->dev_tableT;
+    s.grids = o.grids;
+    s.K = (int)d->depth;
+    s.pad = pc.Kp - (int)d->depth;
+    return s;
 }
 
 // ---- dense ----
@@ -254,7 +282,15 @@ Packed packed_parts(const Pieces &pc, void *base)
 int64_t dense_run(int64_t rows, const Pieces &pc)   // rows whose sums are in the workspace at a time
 {
     const int64_t run = std::min(kRowRun, std::max<int64_t>(1024, kSumsAtOnce / pc.width & ~(int64_t)3));
-    return std::min(fours(rows), run);
+    return std::min(rows, run);
+}
+// Sums and scratch of `rows` rows, a run at a time.
+int runs_workspace(int64_t rows, int64_t run, const Pieces &pc, size_t *count, size_t *bytes)
+{
+    *count = *bytes = 0;
+    if (int rc = sums_workspace(run, pc, count, bytes))
+        return rc;
+    return rows % run ? sums_workspace(rows % run, pc, count, bytes) : AXC_OK;
 }
 
 struct DenseScratch {
@@ -268,18 +304,9 @@ int carve_dense(const axc_dense_desc *d, bool packed, void *base, DenseScratch *
     const Pieces pc = pieces_of(d->depth, d->columns, kDensePiece);
     Carver c(base);
     s->o = carve_operands(c, d, pc, !packed, true);
-    s->lut_bytes = 0;
     size_t count = 0;
-    const int64_t run = dense_run(d->rows, pc), rest = run ? d->rows % run : 0;
-    for (const int64_t rows : {few_rows(d->rows) ? d->rows : run, rest}) {
-        if (rows == 0)
-            continue;
-        size_t need = 0;
-        if (int rc = sums_workspace(rows, pc, &need))
-            return rc;
-        s->lut_bytes = std::max(s->lut_bytes, need);
-        count = std::max(count, sums_count(rows, pc));
-    }
+    if (int rc = runs_workspace(d->rows, dense_run(d->rows, pc), pc, &count, &s->lut_bytes))
+        return rc;
     s->acc = c.take<int32_t>(count);
     s->lut = c.take<char>(s->lut_bytes);
     s->bytes = c.bytes();
@@ -320,14 +347,14 @@ int axc_dense_pack(const axc_dense_desc *desc, const void *kernel, void *packed,
     hipStream_t stream = static_cast<hipStream_t>(stream_v);
     const Pieces pc = pieces_of(desc->depth, desc->columns, kDensePiece);
     const Packed p = packed_parts(pc, packed);
-    int unused = 0, count = 0;
-    ApiTimer t("dense_pack", stream);
-    AXC_HIP(launch_range(nullptr, AXC_F32, 0, kernel, desc->kernel_type, desc->depth * desc->columns, nullptr, p.pairs,
-                         p.column_sums, pc.Np, &unused, &count, stream));
-    AXC_HIP(launch_grids({}, {p.pairs, count, 0.0f, 0.0f}, false, true, p.grids, stream));
-    AXC_HIP(launch_kernel_codes(kernel, desc->kernel_type, (int)desc->depth, desc->columns, pc, p.grids, p.codes, p.column_sums,
-                                stream));
-    return AXC_OK;
+    RangeSource in, k;
+    if (int rc = find_ranges(desc, nullptr, nullptr, kernel, nullptr, p.pairs, p.column_sums, pc.Np, &in, &k, stream))
+        return rc;
+    Operands o = {};
+    o.grids = p.grids;
+    o.kernel_codes = p.codes;
+    o.column_sums = p.column_sums;
+    return make_codes(desc, nullptr, in, kernel, k, nullptr, o, pc, stream);
 }
 
 int axc_fake_approx_dense_workspace_bytes(const axc_dense_desc *desc, int packed, size_t *bytes)
@@ -375,55 +402,35 @@ int axc_fake_approx_dense(const axc_table *table, const axc_dense_desc *desc, co
         const Packed p = packed_parts(pc, const_cast<void *>(packed));
         o.kernel_codes = p.codes;
         o.column_sums = p.column_sums;
-        RangeSource in = input_source(desc, input_range);
         if (few_rows(desc->rows)) {
             ApiTimer t("layer_codes", stream);
-            AXC_HIP(launch_few_codes(input, desc->input_type, (int)desc->rows, K, pc.Kp, in, &p.grids->kernel, o.grids, o.x_codes,
-                                     o.row_sums, stream));
+            AXC_HIP(launch_few_codes(input, desc->input_type, (int)desc->rows, K, pc.Kp, input_source(desc, input_range),
+                                     &p.grids->kernel, o.grids, o.x_codes, o.row_sums, stream));
         } else {
-            if (!in.pairs && in.count < 0) {
-                int count = 0, unused = 0;
-                ApiTimer t("layer_range", stream);
-                AXC_HIP(launch_range(input, desc->input_type, desc->rows * desc->depth, nullptr, AXC_F32, 0, o.x_pairs, nullptr,
-                                     nullptr, 0, &count, &unused, stream));
-                in = {o.x_pairs, count, 0.0f, 0.0f};
-            }
-            {
-                // (the kernel's range as pairs again: what it was packed with)
-                const int64_t n = desc->depth * desc->columns;
-                const int count = (int)std::min<int64_t>((n + 16383) / 16384, kRangeBlocks);
-                ApiTimer t("layer_grids", stream);
-                AXC_HIP(launch_grids(in, {p.pairs, count, 0.0f, 0.0f}, true, true, o.grids, stream));
-            }
-            ApiTimer t("layer_codes", stream);
-            AXC_HIP(launch_input_codes(input, desc->input_type, desc->rows, K, pc.Kp, o.grids, o.x_codes, o.row_sums, stream));
+            RangeSource in, none;
+            if (int rc = find_ranges(desc, input, input_range, nullptr, o.x_pairs, nullptr, nullptr, 0, &in, &none, stream))
+                return rc;
+            if (int rc = make_codes(desc, input, in, nullptr, none, &p.grids->kernel, o, pc, stream))
+                return rc;
         }
-    } else {
-        if (int rc = find_grids(desc, input, input_range, kernel, o, pc.Np, stream))
-            return rc;
-        if (int rc = make_codes(desc, input, kernel, o, pc, stream))
-            return rc;
+    } else if (int rc = find_codes(desc, input, input_range, kernel, o, pc, stream)) {
+        return rc;
     }
-    const int64_t run = few_rows(desc->rows) ? desc->rows : dense_run(desc->rows, pc);
+    const int64_t run = dense_run(desc->rows, pc);
     for (int p = 0; p < pc.count; ++p)
         for (int64_t r = 0; r < desc->rows; r += run) {
             const int64_t rows = std::min(run, desc->rows - r), c = pc.first(p);
-            TableSums sums = {};
+            RawSums raw = {};
             if (int rc = table_sums(table, o.x_codes + r * pc.Kp, rows, pc, p, o.kernel_codes, s.acc, s.lut, s.lut_bytes, stream,
-                                    &sums))
+                                    &raw))
                 return rc;
-            sums.row_sums = o.row_sums + r;
-            sums.column_sums = o.column_sums + c;
-            sums.table = table->dev_tableT;
-            sums.grids = o.grids;
-            sums.K = K;
-            sums.pad = pc.Kp - K;
             const int64_t at = r * desc->columns + c;
             const DenseOut out = {element(bias, c, desc->bias_type), element(residual, at, desc->input_type),
                                   element(output, at, desc->input_type), element(pre, at, desc->input_type), desc->bias_type,
                                   desc->input_type, desc->activation, desc->columns};
             ApiTimer t("dense_out", stream);
-            AXC_HIP(launch_dense_out(sums, rows, (int)std::min<int64_t>(pc.width_of(p), desc->columns - c), out, stream));
+            AXC_HIP(launch_dense_out(sums_of(table, desc, o, pc, p, r, raw), rows,
+                                     (int)std::min<int64_t>(pc.width_of(p), desc->columns - c), out, stream));
         }
     return AXC_OK;
 }
@@ -498,7 +505,7 @@ int axc_fake_approx_dense_gradients(const axc_dense_desc *desc, const void *grad
         return AXC_OK;
     const int64_t rows = desc->rows, K = desc->depth, N = desc->columns;
     const int px = parts_of(desc->input_type), pk = parts_of(desc->kernel_type);
-    if (int rc = find_grids(desc, input, input_range, kernel, s.o, 0, stream))
+    if (int rc = find_grids(desc, input, input_range, kernel, s.o, stream))
         return rc;
     {
         GradSource g = {};
@@ -507,8 +514,8 @@ int axc_fake_approx_dense_gradients(const axc_dense_desc *desc, const void *grad
         g.type = desc->input_type;
         g.activation = desc->activation;
         ApiTimer t("grad_terms", stream);
-        AXC_HIP(launch_grad_terms(g, false, rows, N, N, px, grad_input ? s.straight : nullptr, pk, grad_kernel ? s.turned : nullptr,
-                                  grad_bias ? s.column_partials : nullptr, stream));
+        AXC_HIP(launch_grad_terms(g, false, 0, rows, rows, N, N, px, grad_input ? s.straight : nullptr, pk,
+                                  grad_kernel ? s.turned : nullptr, grad_bias ? s.column_partials : nullptr, stream));
     }
     if (grad_bias) {
         ApiTimer t("column_sums", stream);
@@ -563,13 +570,15 @@ static int carve_loss(const axc_dense_desc *d, bool gradients, void *base, LossS
     const Pieces pc = loss_pieces(d);
     Carver c(base);
     s->o = carve_operands(c, d, pc, true, true);
-    float **const state[] = {&s->st.top, &s->st.sum, &s->st.at, &s->st.lse, &s->st.rows, &s->st.coefficient};
+    float **const state[] = {&s->st.at, &s->st.lse, &s->st.rows, &s->st.coefficient};
     for (float **p : state)
         *p = c.take<float>((size_t)d->rows);
     s->st.factor = c.take<float>(1);
-    if (int rc = sums_workspace(d->rows, pc, &s->lut_bytes))
+    s->st.parts = c.take<float2>((size_t)pc.count * ((pc.width + kLossChunk - 1) / kLossChunk) * d->rows);
+    size_t count = 0;
+    if (int rc = runs_workspace(d->rows, std::min(d->rows, kRowRun), pc, &count, &s->lut_bytes))
         return rc;
-    s->acc = c.take<int32_t>(sums_count(d->rows, pc));
+    s->acc = c.take<int32_t>(count);
     s->lut = c.take<char>(s->lut_bytes);
     if (gradients) {
         const int64_t M = product_pad(d->rows), P = product_pad(pc.width), K = product_pad(d->depth);
@@ -643,29 +652,31 @@ int axc_fake_approx_cross_entropy(const axc_table *table, const axc_dense_desc *
     if (int rc = check_workspace(workspace, workspace_bytes, s.bytes))
         return rc;
     const Operands &o = s.o;
-    if (int rc = find_grids(desc, input, input_range, kernel, o, pc.Np, stream))
-        return rc;
-    if (int rc = make_codes(desc, input, kernel, o, pc, stream))
+    if (int rc = find_codes(desc, input, input_range, kernel, o, pc, stream))
         return rc;
 
-    TableSums sums = {};
-    auto make_sums = [&](int p) {
-        const int rc = table_sums(table, o.x_codes, rows, pc, p, o.kernel_codes, s.acc, s.lut, s.lut_bytes, stream, &sums);
-        sums.row_sums = o.row_sums;
-        sums.column_sums = o.column_sums + pc.first(p);
-        sums.table = table->dev_tableT;
-        sums.grids = o.grids;
-        sums.K = (int)K;
-        sums.pad = pc.Kp - (int)K;
-        return rc;
+    const int64_t run = std::min(rows, kRowRun);
+    RawSums raw = {};
+    auto make_sums = [&](int p, int64_t r) {
+        return table_sums(table, o.x_codes + r * pc.Kp, std::min(run, rows - r), pc, p, o.kernel_codes, s.acc, s.lut, s.lut_bytes,
+                          stream, &raw);
     };
     auto columns_of = [&](int p) { return std::min<int64_t>(pc.width_of(p), V - pc.first(p)); };
-    for (int p = 0; p < pc.count; ++p) {
-        if (int rc = make_sums(p))
-            return rc;
-        ApiTimer t("loss_piece", stream);
-        AXC_HIP(launch_loss_piece(sums, rows, (int)columns_of(p), pc.first(p), element(bias, pc.first(p), desc->bias_type),
-                                  desc->bias_type, targets, ignore_index, V, p == 0, p + 1 == pc.count, s.st, stream));
+    for (int64_t r = 0; r < rows; r += run) {
+        const int64_t run_rows = std::min(run, rows - r);
+        int chunk = 0;
+        for (int p = 0; p < pc.count; ++p) {
+            if (int rc = make_sums(p, r))
+                return rc;
+            int more = 0;
+            ApiTimer t("loss_piece", stream);
+            AXC_HIP(launch_loss_piece(sums_of(table, desc, o, pc, p, r, raw), r, run_rows, rows, (int)columns_of(p), pc.first(p),
+                                      element(bias, pc.first(p), desc->bias_type), desc->bias_type, targets, chunk, &more, s.st,
+                                      stream));
+            chunk += more;
+        }
+        ApiTimer t("loss_rows", stream);
+        AXC_HIP(launch_loss_rows(s.st, targets, ignore_index, V, r, run_rows, rows, chunk, stream));
     }
     {
         ApiTimer t("loss_out", stream);
@@ -683,24 +694,26 @@ int axc_fake_approx_cross_entropy(const axc_table *table, const axc_dense_desc *
     const ProductPlan input_plan = plan_product(rows, K, product_pad(pc.width), px, true);
     const ProductOut input_out = {grad_input, desc->input_type, K, input, desc->input_type, K, &o.grids->in, &o.grids->kernel,
                                   s.st.factor};
-    // from the last piece on, whose sums are still there
+    // from the last piece on, whose last run's sums are still there
+    bool made = true;
     for (int p = pc.count - 1; p >= 0; --p) {
-        if (p + 1 < pc.count)
-            if (int rc = make_sums(p))
-                return rc;
         const int64_t c = pc.first(p), n = columns_of(p), P = product_pad(n);
-        {
+        for (int64_t r = (rows - 1) / run * run; r >= 0; r -= run) {
+            if (!made)
+                if (int rc = make_sums(p, r))
+                    return rc;
+            made = false;
             GradSource g = {};
-            g.sums = sums;
-            g.lse = s.st.lse;
-            g.coefficient = s.st.coefficient;
-            g.targets = targets;
+            g.sums = sums_of(table, desc, o, pc, p, r, raw);
+            g.lse = s.st.lse + r;
+            g.coefficient = s.st.coefficient + r;
+            g.targets = targets + r;
             g.bias = element(bias, c, desc->bias_type);
             g.bias_type = desc->bias_type;
             g.first_column = c;
             ApiTimer t("grad_terms", stream);
-            AXC_HIP(launch_grad_terms(g, true, rows, n, 0, px, grad_input ? s.straight : nullptr, pk, grad_kernel ? s.turned : nullptr,
-                                      grad_bias ? s.column_partials : nullptr, stream));
+            AXC_HIP(launch_grad_terms(g, true, r, std::min(run, rows - r), rows, n, 0, px, grad_input ? s.straight : nullptr, pk,
+                                      grad_kernel ? s.turned : nullptr, grad_bias ? s.column_partials : nullptr, stream));
         }
         if (grad_bias) {
             ApiTimer t("column_sums", stream);

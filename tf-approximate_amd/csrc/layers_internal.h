@@ -174,36 +174,78 @@ __device__ __forceinline__ void block_range(float &lo, float &hi, float *red)
 }
 
 // ---- activations ----
+// Phi(z), the normal distribution, and its density phi(z).  Both tails come from one exponential: Abramowitz & Stegun, Handbook of
+// Mathematical Functions, 7.1.26, erfc(x) = t (a1 + t (a2 + t (a3 + t (a4 + t a5)))) exp(-x^2), t = 1 / (1 + 0.3275911 x), x >= 0,
+// off by 1.5e-7 at most.  The library's erff has two ranges, which a wavefront goes through both: an epilogue of 16.8 M values took
+// 46 us with it and 64-bit whole numbers, more than its 100 MB.
+__device__ __forceinline__ void normal(float z, float &cumulative, float &density)
+{
+    const float x = fabsf(z) * 0.70710678118654752f;
+    const float e = __expf(-x * x);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.0f));
+    const float poly = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+    const float tail = 0.5f * poly * e;          // Phi(-|z|)
+    cumulative = z > 0.0f ? 1.0f - tail : tail;
+    density = 0.39894228040143268f * e;
+}
+__device__ __forceinline__ float gelu(float z)
+{
+    float c, d;
+    normal(z, c, d);
+    return z == -INFINITY ? -0.0f : z * c;
+}
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + __expf(-z)); }
 __device__ __forceinline__ float activate(float z, int activation)
 {
     switch (activation) {
     case AXC_ACT_RELU: return z > 0.0f ? z : z == z ? 0.0f : z;
-    case AXC_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-    case AXC_ACT_GELU_TANH: {   // 0.5 z (1 + tanh(u)) = z / (1 + exp(-2u))
-        const float u = 0.79788456080286536f * (z + 0.044715f * z * z * z);
-        return z == -INFINITY ? -0.0f : z / (1.0f + expf(-2.0f * u));
-    }
-    case AXC_ACT_SILU: return z == -INFINITY ? -0.0f : z / (1.0f + expf(-z));
+    case AXC_ACT_GELU: return gelu(z);
+    case AXC_ACT_GELU_TANH:   // 0.5 z (1 + tanh(u)) = z sigmoid(2u)
+        return z == -INFINITY ? -0.0f : z * sigmoid(1.5957691216057308f * (z + 0.044715f * z * z * z));
+    case AXC_ACT_SILU: return z == -INFINITY ? -0.0f : z * sigmoid(z);
     default: return z;
+    }
+}
+// One look at which activation it is for four values.
+__device__ __forceinline__ void activate_four(const float (&z)[4], float (&y)[4], int activation)
+{
+    switch (activation) {
+#define AXC_FOUR(which)                  \
+    case which:                          \
+        _Pragma("unroll")                \
+        for (int j = 0; j < 4; ++j)      \
+            y[j] = activate(z[j], which); \
+        break;
+        AXC_FOUR(AXC_ACT_RELU)
+        AXC_FOUR(AXC_ACT_GELU)
+        AXC_FOUR(AXC_ACT_GELU_TANH)
+        AXC_FOUR(AXC_ACT_SILU)
+    default:
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            y[j] = z[j];
+#undef AXC_FOUR
     }
 }
 __device__ __forceinline__ float activation_slope(float z, int activation)
 {
     switch (activation) {
     case AXC_ACT_RELU: return z > 0.0f ? 1.0f : z == z ? 0.0f : z;
-    case AXC_ACT_GELU: return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) +
-                              (fabsf(z) < 14.0f ? z * expf(-0.5f * z * z) * 0.39894228040143268f : 0.0f * z);
+    case AXC_ACT_GELU: {
+        float c, d;
+        normal(z, c, d);
+        return fabsf(z) < 14.0f ? fmaf(z, d, c) : z > 0.0f ? 1.0f : z == z ? 0.0f : z;
+    }
     case AXC_ACT_GELU_TANH: {
         if (fabsf(z) > 1e6f)
             return z > 0.0f ? 1.0f : 0.0f;
-        const float u = 0.79788456080286536f * (z + 0.044715f * z * z * z);
-        const float s = 1.0f / (1.0f + expf(-2.0f * u));
+        const float s = sigmoid(1.5957691216057308f * (z + 0.044715f * z * z * z));
         return s + 2.0f * z * s * (1.0f - s) * 0.79788456080286536f * (1.0f + 0.134145f * z * z);
     }
     case AXC_ACT_SILU: {
         if (fabsf(z) > 1e6f)
             return z > 0.0f ? 1.0f : 0.0f;
-        const float s = 1.0f / (1.0f + expf(-z));
+        const float s = sigmoid(z);
         return s * (1.0f + z * (1.0f - s));
     }
     default: return 1.0f;
@@ -232,11 +274,9 @@ struct RangeSource {                     // where a tensor's smallest and larges
     float lo, hi;
 };
 
-// Sums of table entries as a consumer finds them, of one piece and one run of rows: `splits` partial sums of [rows][pitch] int32.
+// Sums of table entries as a consumer finds them, of one piece and one run of rows.
 struct TableSums {
-    const int32_t *acc;
-    int64_t split_stride;
-    int splits, pitch;
+    RawSums raw;                         // (every fourth row and column begins 16-byte aligned)
     const int32_t *row_sums;             // sums of the input's codes, of the run's first row on
     const int32_t *column_sums;          // sums of the kernel's codes, of the piece's first column on
     const uint16_t *table;               // its first entry is T[0][0]
@@ -244,21 +284,60 @@ struct TableSums {
     int K, pad;                          // depth, and pad elements behind it
 };
 
-// What takes the two zero points and the padding out of a sum, of row r; for column c: whole - in.zero * column_sums[c].
-__device__ __forceinline__ int64_t row_term(const TableSums &s, int64_t r)
+// A product in front of its scales, sum - z_k row_sums - z_in column_sums + K z_in z_k, without the pad elements: each of the K
+// elements contributes between -65025 and 65535 + 65025.  Up to this depth it fits 32 bits, and so may be computed modulo 2^32
+// whatever its parts are; in a longer one all of it is 64 bits wide.
+constexpr int kNarrowDepth = 16384;      // 16384 * 130560 < 2^31
+template <typename I>                    // uint32_t or int64_t
+struct Bracket {
+    I whole, zi, zk;
+    __device__ __forceinline__ explicit Bracket(const TableSums &s)
+        : zi((I)s.grids->in.zero), zk((I)s.grids->kernel.zero)
+    {
+        whole = (I)s.K * zi * zk - (I)s.pad * (I)s.table[0];
+    }
+    __device__ __forceinline__ I row(int32_t row_sum) const { return whole - zk * (I)row_sum; }
+    __device__ __forceinline__ I column(int32_t column_sum) const { return zi * (I)column_sum; }
+    // of the sum of table entries, which is 0 or more and below 2^31
+    __device__ __forceinline__ static float value(int32_t sum, I row, I column)
+    {
+        if constexpr (sizeof(I) == 4)
+            return (float)(int32_t)((I)sum + row - column);
+        else
+            return (float)((I)sum + row - column);
+    }
+};
+
+// Four neighbouring sums, at (r, c) to (r, c + 3), or to (r + 3, c) where they are turned.
+__device__ __forceinline__ i32x4 four_sums(const RawSums &s, int64_t r, int64_t c)
 {
-    const int64_t zi = s.grids->in.zero, zk = s.grids->kernel.zero;
-    return (int64_t)s.K * zi * zk - zk * (int64_t)s.row_sums[r] - (int64_t)s.pad * s.table[0];
+    const int32_t *const p = s.acc + (s.turned ? c * s.pitch + r : r * s.pitch + c);
+    i32x4 t = {};
+#pragma unroll 8
+    for (int i = 0; i < s.splits; ++i)
+        t += *reinterpret_cast<const i32x4 *>(p + i * s.split_stride);
+    return t;
 }
 
 hipError_t launch_range(const void *x, int x_type, int64_t nx, const void *kernel, int kernel_type, int64_t nk, float *x_pairs,
                         float *kernel_pairs, int32_t *zeros, int64_t n_zeros, int *x_count, int *kernel_count, hipStream_t stream);
 hipError_t launch_grids(const RangeSource &in, const RangeSource &kernel, bool has_in, bool has_kernel, Grids *grids,
                         hipStream_t stream);
-hipError_t launch_input_codes(const void *x, int type, int64_t rows, int K, int Kp, const Grids *grids, uint8_t *codes,
-                              int32_t *row_sums, hipStream_t stream);
-hipError_t launch_kernel_codes(const void *kernel, int type, int K, int64_t N, const Pieces &pieces, const Grids *grids,
-                               uint8_t *codes, int32_t *column_sums, hipStream_t stream);
+// Codes of both operands and their sums, and the grids they are on.  x null: only the kernel's; kernel null: only the input's,
+// and the kernel's grid is that of kernel_grid.
+struct CodesJob {
+    const void *x, *kernel;
+    int x_type, kernel_type;
+    int64_t rows, N;
+    int K;
+    RangeSource x_range, kernel_range;
+    const Grid *kernel_grid;
+    Pieces pieces;
+    Grids *grids;
+    uint8_t *x_codes, *kernel_codes;
+    int32_t *row_sums, *column_sums;     // (those of the columns are added to)
+};
+hipError_t launch_codes(const CodesJob &job, hipStream_t stream);
 // Few rows: range (where src says so), grid, codes and their sums of the input in one launch; kernel_grid is copied next to it.
 hipError_t launch_few_codes(const void *x, int type, int rows, int K, int Kp, const RangeSource &src, const Grid *kernel_grid,
                             Grids *grids, uint8_t *codes, int32_t *row_sums, hipStream_t stream);
@@ -292,9 +371,11 @@ struct GradSource {                      // where the gradient behind the produc
     int bias_type;
     int64_t first_column;
 };
-// [rows_pad][parts][cols_pad], [cols_pad][parts][rows_pad], and per 64 rows the sums over them (each may be null)
-hipError_t launch_grad_terms(const GradSource &g, bool loss, int64_t rows, int64_t cols, int64_t ld, int straight_parts,
-                             bf16 *straight, int turned_parts, bf16 *turned, float *column_partials, hipStream_t stream);
+// [rows_pad][parts][cols_pad], [cols_pad][parts][rows_pad], and per 64 rows the sums over them (each may be null), of the run of
+// rows from `first` on (a multiple of kProductTile) out of `rows`; `of_run` describes its gradient, of run_rows rows.
+hipError_t launch_grad_terms(const GradSource &of_run, bool loss, int64_t first, int64_t run_rows, int64_t rows, int64_t cols,
+                             int64_t ld, int straight_parts, bf16 *straight, int turned_parts, bf16 *turned, float *column_partials,
+                             hipStream_t stream);
 hipError_t launch_centered(const void *v, int type, int64_t rows, int64_t cols, int64_t ld, const Grid *grid, bool turn, bf16 *out,
                            hipStream_t stream);
 struct ProductOut {
@@ -323,14 +404,19 @@ hipError_t launch_column_sums(const float *partials, int64_t count, int64_t cols
                               int type, hipStream_t stream);
 
 // ---- loss (loss_kernels.hip) ----
-struct LossState {                       // per row
-    float *top, *sum, *at;               // running maximum and sum of exponentials; the target's logit
+constexpr int kLossChunk = 512;          // columns at least that leave a maximum and a sum
+struct LossState {
+    float2 *parts;                       // [chunk][rows]: the largest logit and the sum of exponentials around it
+    float *at;                           // per row: the target's logit
     float *lse, *rows;                   // log of the whole sum; the row's loss
     float *coefficient, *factor;         // a row's gradient is multiplied by coefficient[row] * *factor
 };
-hipError_t launch_loss_piece(const TableSums &s, int64_t rows, int columns, int64_t first_column, const void *bias, int bias_type,
-                             const int64_t *targets, int64_t ignore, int64_t V, bool first, bool last, const LossState &st,
+// Of a run of rows from `first_row` on, into parts from `chunk` on; returns how many chunks in *chunks.
+hipError_t launch_loss_piece(const TableSums &s, int64_t first_row, int64_t run_rows, int64_t rows, int columns, int64_t first_column,
+                             const void *bias, int bias_type, const int64_t *targets, int chunk, int *chunks, const LossState &st,
                              hipStream_t stream);
+hipError_t launch_loss_rows(const LossState &st, const int64_t *targets, int64_t ignore, int64_t V, int64_t first_row, int64_t run_rows,
+                            int64_t rows, int chunks, hipStream_t stream);
 hipError_t launch_loss_out(const LossState &st, const int64_t *targets, int64_t ignore, int64_t V, int64_t rows, int reduction,
                            const float *grad_loss, float *loss, bool gradients, hipStream_t stream);
 
@@ -370,6 +456,9 @@ namespace axc {
 int api_fail(int status, const char *msg);
 int api_fail_hip(hipError_t e, const char *what);
 int api_check_table(const axc_table *table);
+// axc_conv2d_codes_acc_i32 without the pass that would put its sums in order; *raw is filled, unless there are no sums.
+int api_codes_sums(const axc_table *table, const axc_conv2d_desc *desc, const uint8_t *input_codes, const uint8_t *filter_codes,
+                   int32_t *acc, void *workspace, size_t workspace_bytes, void *stream, RawSums *raw);
 class ApiTimer {   // brackets launches while the timers run
 public:
     ApiTimer(const char *name, hipStream_t stream);

@@ -2,91 +2,162 @@
 //
 //   loss[m] = log sum_v exp(z[m][v]) - z[m][target[m]]
 //
-// Per row a running maximum t and sum s of exp(z - t), in float32: a piece with maximum p makes them max(t, p) and
-// s exp(t - max) + its own sum.  A row whose logits so far are all -infinity has s = 0 and t = -infinity.
+// A chunk of columns leaves its largest logit t and s = sum exp(z - t), in float32; two of them make max(t, t') and
+// s exp(t - max) + s' exp(t' - max).  Chunks whose logits are all -infinity have t = -infinity and s = 0.
 #include "layers_internal.h"
 
 namespace axc {
 namespace {
 
-// (t, s) and (p, q) together
-__device__ __forceinline__ void join(float &t, float &s, float p, float q)
-{
-    const float m = fmaxf(t, p);
-    // (equal maxima, infinite ones among them, need no factor: infinity minus itself is NaN)
-    s = (t == m ? s : s * expf(t - m)) + (p == m ? q : q * expf(p - m));
-    t = m;
-}
+struct Exponentials {
+    float top, sum;
+    __device__ __forceinline__ Exponentials() : top(-INFINITY), sum(0.0f) {}
+    __device__ __forceinline__ void join(float t, float s)
+    {
+        const float m = fmaxf(top, t);
+        // (equal maxima, infinite ones among them, need no factor: infinity minus itself is NaN)
+        sum = (top == m ? sum : sum * __expf(top - m)) + (t == m ? s : s * __expf(t - m));
+        top = m;
+    }
+    template <int N>
+    __device__ __forceinline__ void add(const float (&z)[N])
+    {
+        float m = top, undefined = 0.0f;
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            m = fmaxf(m, z[j]);
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            undefined += z[j] != z[j] ? z[j] : 0.0f;   // (fmaxf passes over NaN, which nothing else below may)
+        if (m > -INFINITY) {
+            float s = top == m ? sum : sum * __expf(top - m);
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                s += z[j] == m ? 1.0f : __expf(z[j] - m);
+            sum = s;
+            top = m;
+        }
+        sum += undefined;
+    }
+};
 
-// A workgroup a row: the piece's logits out of the sums, four at a time, joined with what earlier pieces left.
-__global__ void __launch_bounds__(1024) loss_piece_kernel(TableSums s, int columns, int64_t first_column, const void *bias,
-                                                          int bias_type, const int64_t *targets, int64_t ignore, int64_t V,
-                                                          int first, int last, LossState st)
+// Sums by rows: a workgroup a row and kRowChunk columns, four neighbours a thread.
+constexpr int kRowChunk = 2048;
+template <typename I>
+__global__ void __launch_bounds__(256) loss_piece_kernel(TableSums s, int64_t first_row, int64_t rows, int columns,
+                                                         int64_t first_column, const void *bias, int bias_type,
+                                                         const int64_t *__restrict__ targets, int chunk, LossState st)
 {
-    __shared__ float tops[16], sums[16];
+    __shared__ float tops[4], sums[4];
     const int64_t r = blockIdx.x;
     const float scale = __fmul_rn(s.grids->in.scale, s.grids->kernel.scale);
-    const int64_t zi = s.grids->in.zero, row = row_term(s, r);
-    const int64_t target = targets[r];
-    const int32_t *const acc = s.acc + r * s.pitch;
-    float top = -INFINITY, sum = 0.0f;
-    bool undefined = false;
-    for (int c = 4 * threadIdx.x; c < columns; c += 4 * blockDim.x) {
-        int32_t t[4] = {};
-        for (int k = 0; k < s.splits; ++k) {
-            const i32x4 a = *reinterpret_cast<const i32x4 *>(acc + k * s.split_stride + c);
+    const Bracket<I> b(s);
+    const I row = b.row(s.row_sums[r]);
+    const int64_t target = targets[first_row + r] - first_column;
+    Exponentials e;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                t[j] += a[j];
-        }
-        float z[4], most = top;
+    for (int i = 0; i < kRowChunk / 1024; ++i) {
+        const int c = (int)blockIdx.y * kRowChunk + i * 1024 + 4 * (int)threadIdx.x;
+        if (c >= columns)
+            continue;
+        const i32x4 t = four_sums(s.raw, r, c);
+        float z[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             z[j] = -INFINITY;
             if (c + j < columns) {
-                z[j] = __fmul_rn((float)((int64_t)t[j] + row - zi * s.column_sums[c + j]), scale);
+                z[j] = __fmul_rn(Bracket<I>::value(t[j], row, b.column(s.column_sums[c + j])), scale);
                 if (bias)
                     z[j] = __fadd_rn(z[j], load_any(bias, c + j, bias_type));
-                if (first_column + c + j == target)
-                    st.at[r] = z[j];
-                undefined |= z[j] != z[j];
+                if (c + j == target)
+                    st.at[first_row + r] = z[j];
             }
-            most = fmaxf(most, z[j]);
         }
-        if (most > -INFINITY) {
-            sum = top == most ? sum : sum * expf(top - most);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                sum += z[j] == most ? 1.0f : expf(z[j] - most);
-            top = most;
-        }
+        e.add(z);
     }
-    if (undefined)
-        sum = NAN;
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) {
-        const float p = __shfl_xor(top, d), q = __shfl_xor(sum, d);
-        join(top, sum, p, q);
+        const float t = __shfl_xor(e.top, d), q = __shfl_xor(e.sum, d);
+        e.join(t, q);
     }
     if ((threadIdx.x & 63) == 0) {
-        tops[threadIdx.x / 64] = top;
-        sums[threadIdx.x / 64] = sum;
+        tops[threadIdx.x / 64] = e.top;
+        sums[threadIdx.x / 64] = e.sum;
     }
-    __syncthreads();   // (and what the thread with the target has stored is there to be read)
+    __syncthreads();
     if (threadIdx.x != 0)
         return;
-    top = first ? -INFINITY : st.top[r];
-    sum = first ? 0.0f : st.sum[r];
-    for (int i = 0; i < (int)blockDim.x / 64; ++i)
-        join(top, sum, tops[i], sums[i]);
-    st.top[r] = top;
-    st.sum[r] = sum;
-    if (last) {
-        const float lse = top + logf(sum);
-        st.lse[r] = lse;
-        // a target that is no column of the vocabulary has no loss
-        st.rows[r] = target == ignore ? 0.0f : target >= 0 && target < V ? lse - st.at[r] : NAN;
+    for (int i = 1; i < 4; ++i)
+        e.join(tops[i], sums[i]);
+    st.parts[(chunk + blockIdx.y) * rows + first_row + r] = make_float2(e.top, e.sum);
+}
+
+// Turned sums: a workgroup 64 rows, a lane each, and kLossChunk columns, a quarter for each wavefront.  A lane goes through its row's
+// logits by itself; what belongs to a column is the same for all lanes.
+template <typename I>
+__global__ void __launch_bounds__(256) loss_turned_kernel(TableSums s, int64_t first_row, int64_t run_rows, int64_t rows, int columns,
+                                                          int64_t first_column, const void *bias, int bias_type,
+                                                          const int64_t *__restrict__ targets, int chunk, LossState st)
+{
+    constexpr int N = 8;
+    __shared__ float tops[4][64], sums[4][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int64_t at = (int64_t)blockIdx.y * 64 + lane;
+    const int64_t r = at < run_rows ? at : run_rows - 1;   // (lanes behind the rows repeat the last; nobody stores them)
+    const float scale = __fmul_rn(s.grids->in.scale, s.grids->kernel.scale);
+    const Bracket<I> b(s);
+    const I row = b.row(s.row_sums[r]);
+    const int64_t target = targets[first_row + r] - first_column;
+    const int c0 = (int)blockIdx.x * kLossChunk + wave * (kLossChunk / 4);
+    const int end = c0 + kLossChunk / 4 < columns ? c0 + kLossChunk / 4 : columns;
+    Exponentials e;
+    for (int c = c0; c < end; c += N) {
+        int32_t t[N] = {};
+        for (int k = 0; k < s.raw.splits; ++k)
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+                t[j] += s.raw.acc[k * s.raw.split_stride + (int64_t)(c + j < end ? c + j : end - 1) * s.raw.pitch + r];
+        float z[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int of = c + j < end ? c + j : end - 1;
+            z[j] = __fmul_rn(Bracket<I>::value(t[j], row, b.column(s.column_sums[of])), scale);
+            if (bias)
+                z[j] = __fadd_rn(z[j], load_any(bias, of, bias_type));
+            if (of == target)
+                st.at[first_row + r] = z[j];
+            z[j] = c + j < end ? z[j] : -INFINITY;
+        }
+        e.add(z);
     }
+    tops[wave][lane] = e.top;
+    sums[wave][lane] = e.sum;
+    __syncthreads();
+    if (wave != 0 || at >= run_rows)
+        return;
+    for (int i = 1; i < 4; ++i)
+        e.join(tops[i][lane], sums[i][lane]);
+    st.parts[(chunk + blockIdx.x) * rows + first_row + at] = make_float2(e.top, e.sum);
+}
+
+// A row a thread, over what the chunks have left.
+__global__ void __launch_bounds__(64) loss_rows_kernel(LossState st, const int64_t *__restrict__ targets, int64_t ignore, int64_t V,
+                                                       int64_t first_row, int64_t run_rows, int64_t rows, int chunks)
+{
+    const int64_t i = (int64_t)blockIdx.x * 64 + threadIdx.x, r = first_row + i;
+    if (i >= run_rows)
+        return;
+    Exponentials e;
+#pragma unroll 8
+    for (int c = 0; c < chunks; ++c) {
+        const float2 p = st.parts[c * rows + r];
+        e.join(p.x, p.y);
+    }
+    const float lse = e.top + logf(e.sum);
+    const int64_t t = targets[r];
+    st.lse[r] = lse;
+    // a target that is no column of the vocabulary has no loss
+    st.rows[r] = t == ignore ? 0.0f : t >= 0 && t < V ? lse - st.at[r] : NAN;
 }
 
 // The loss out of the rows', in one order, and what each row's gradient is multiplied by.
@@ -154,13 +225,38 @@ __global__ void __launch_bounds__(1024) loss_out_kernel(LossState st, const int6
 
 } // namespace
 
-hipError_t launch_loss_piece(const TableSums &s, int64_t rows, int columns, int64_t first_column, const void *bias, int bias_type,
-                             const int64_t *targets, int64_t ignore, int64_t V, bool first, bool last, const LossState &st,
+hipError_t launch_loss_piece(const TableSums &s, int64_t first_row, int64_t run_rows, int64_t rows, int columns, int64_t first_column,
+                             const void *bias, int bias_type, const int64_t *targets, int chunk, int *chunks, const LossState &st,
                              hipStream_t stream)
 {
-    // many rows have wavefronts enough; few rows need theirs long
-    hipLaunchKernelGGL(loss_piece_kernel, dim3((unsigned)rows), dim3(rows >= 1024 ? 256 : 1024), 0, stream, s, columns, first_column,
-                       bias, bias_type, targets, ignore, V, (int)first, (int)last, st);
+    const bool narrow = s.K <= kNarrowDepth;
+    if (s.raw.turned) {
+        *chunks = (columns + kLossChunk - 1) / kLossChunk;
+        const dim3 grid((unsigned)*chunks, (unsigned)((run_rows + 63) / 64));
+        if (narrow)
+            hipLaunchKernelGGL(loss_turned_kernel<uint32_t>, grid, dim3(256), 0, stream, s, first_row, run_rows, rows, columns,
+                               first_column, bias, bias_type, targets, chunk, st);
+        else
+            hipLaunchKernelGGL(loss_turned_kernel<int64_t>, grid, dim3(256), 0, stream, s, first_row, run_rows, rows, columns,
+                               first_column, bias, bias_type, targets, chunk, st);
+    } else {
+        *chunks = (columns + kRowChunk - 1) / kRowChunk;
+        const dim3 grid((unsigned)run_rows, (unsigned)*chunks);
+        if (narrow)
+            hipLaunchKernelGGL(loss_piece_kernel<uint32_t>, grid, dim3(256), 0, stream, s, first_row, rows, columns, first_column, bias,
+                               bias_type, targets, chunk, st);
+        else
+            hipLaunchKernelGGL(loss_piece_kernel<int64_t>, grid, dim3(256), 0, stream, s, first_row, rows, columns, first_column, bias,
+                               bias_type, targets, chunk, st);
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_loss_rows(const LossState &st, const int64_t *targets, int64_t ignore, int64_t V, int64_t first_row, int64_t run_rows,
+                            int64_t rows, int chunks, hipStream_t stream)
+{
+    hipLaunchKernelGGL(loss_rows_kernel, dim3((unsigned)((run_rows + 63) / 64)), dim3(64), 0, stream, st, targets, ignore, V, first_row,
+                       run_rows, rows, chunks);
     return hipGetLastError();
 }
 
