@@ -257,46 +257,84 @@ __global__ void __launch_bounds__(256) codes_kernel(CodesJob job, int x_blocks, 
 }
 
 // ---- sums of few rows ----
-// A wavefront takes MT rows, 512 columns (eight a lane) and one element of the depth at a time.  It turns the MT table rows that
-// the rows' codes name into R[b] = entries of filter code b for all MT rows, in LDS of its own, and a lane then reads the entries
-// of all MT rows for one weight with one access of 2 MT bytes.  Sums of two rows share a dword as they come: one register adds
-// whole dwords modulo 2^32, another the upper halves.  Building costs 256 entries a row and element where the lookups are 512.
+// A pair of wavefronts takes MT rows, 1024 columns (eight a lane) and two elements of the depth at a time.  Each of the two turns the
+// MT table rows that the rows' codes name at one of the elements into R[b] = entries of filter code b for all MT rows, in LDS; a lane
+// then reads the entries of all MT rows for one weight with one access of 2 MT bytes.  Sums of two rows share a dword as they come:
+// one register adds whole dwords modulo 2^32, another the upper halves, three instructions for two dwords.
+// Eight pairs make a workgroup, which adds up their sums in LDS before it leaves them to the others' (parts of the depth).
+// What bounds it for eight rows: lookups at random among 256 places of 16 bytes, 3 of 16 lanes on the busiest of 16 groups of banks
+// (25 T/s), and the table rows out of the L2, 4 KiB for every element and 1024 columns.
+constexpr int kFewGroups = 8;            // pairs of wavefronts
+constexpr int kFewColumns = 1024;
+constexpr int kFewRowsAtOnce = 4;        // whose sums are added up in LDS
 template <int MT>
-__global__ void __launch_bounds__(256) few_rows_kernel(const uint16_t *__restrict__ tableI, const uint8_t *__restrict__ x_codes,
-                                                       int rows, int Kp, const uint8_t *__restrict__ kernel_codes, int width,
-                                                       int32_t *__restrict__ acc)
+constexpr int few_lds_bytes()            // two buffers of table rows; then the sums of 16 wavefronts
 {
-    constexpr int H = (MT + 1) / 2;   // dwords of an entry
-    constexpr int kRowBytes = 256 * 2 * MT;
-    __shared__ __align__(16) unsigned char lds[4 * (kRowBytes > 2048 ? kRowBytes : 2048)];
+    constexpr int table_rows = 2 * 2 * kFewGroups * 512 * MT, sums = 16 * 512 * 4 * (MT < kFewRowsAtOnce ? MT : kFewRowsAtOnce);
+    return table_rows > sums ? table_rows : sums;
+}
+
+template <int MT>
+__global__ void __launch_bounds__(1024) few_rows_kernel(const uint16_t *__restrict__ tableI, const uint8_t *__restrict__ x_codes,
+                                                        int rows, int Kp, const uint8_t *__restrict__ kernel_codes, int width,
+                                                        int32_t *__restrict__ acc)
+{
+    constexpr int H = (MT + 1) / 2;      // dwords of an entry
+    constexpr int kRowBytes = 512 * MT;  // of R
+    extern __shared__ __align__(16) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    unsigned char *const R = lds + wave * kRowBytes;
-    const int c = (int)blockIdx.x * 512 + lane * 8;
+    const int group = wave >> 1, half = wave & 1;
+    const int c = (int)blockIdx.x * kFewColumns + half * 512 + lane * 8;
     const int row0 = (int)blockIdx.z * MT;
-    const int quads = Kp / 4, splits = gridDim.y;
-    const int q_end = (int)((int64_t)quads * (blockIdx.y + 1) / splits);
+    const int pairs = Kp / 2;
+    const int first = (int)((int64_t)pairs * blockIdx.y / gridDim.y), last = (int)((int64_t)pairs * (blockIdx.y + 1) / gridDim.y);
+    const int steps = (last - first + kFewGroups - 1) / kFewGroups;
     const bool in0 = c < width, in1 = c + 4 < width;
 
-    uint32_t even[8][H] = {}, odd[8][H] = {};
-    for (int q = (int)((int64_t)quads * blockIdx.y / splits) + wave; q < q_end; q += 4) {
-        uint32_t a[MT];
+    uint2 t[MT];                         // table rows of this wavefront's element, four entries a lane
+    uint32_t b[2][2];                    // weights of both elements, eight codes a lane
+    auto load = [&](int step) {
+        const int pair = first + step * kFewGroups + group;
+        if (pair >= last)                // (uniform; what is there is not used)
+            return;
+        const int k = 2 * pair + half;
 #pragma unroll
-        for (int m = 0; m < MT; ++m)   // (rows beyond the last repeat it; nobody stores them)
-            a[m] = *reinterpret_cast<const uint32_t *>(x_codes + (int64_t)min(row0 + m, rows - 1) * Kp + 4 * q);
-        uint32_t b[4][2];
+        for (int m = 0; m < MT; ++m) {   // (rows beyond the last repeat it; nobody stores them)
+            const uint32_t four = *reinterpret_cast<const uint32_t *>(x_codes + (int64_t)min(row0 + m, rows - 1) * Kp + (k & ~3));
+            t[m] = *reinterpret_cast<const uint2 *>(tableI + ((four >> (8 * (k & 3))) & 255u) * 256u + lane * 4);
+        }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint8_t *const p = kernel_codes + (size_t)(4 * q + j) * width + c;
+        for (int j = 0; j < 2; ++j) {
+            const uint8_t *const p = kernel_codes + (size_t)(2 * pair + j) * width + c;
             b[j][0] = in0 ? *reinterpret_cast<const uint32_t *>(p) : 0u;
             b[j][1] = in1 ? *reinterpret_cast<const uint32_t *>(p + 4) : 0u;
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            uint2 t[MT];
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-                t[m] = *reinterpret_cast<const uint2 *>(tableI + ((a[m] >> (8 * j)) & 255u) * 256u + lane * 4);
-            __builtin_amdgcn_wave_barrier();
+    };
+    auto entry = [&](const unsigned char *R, uint32_t code, uint32_t (&e)[H]) {
+        const unsigned char *const from = R + code * (2 * MT);
+        if constexpr (MT == 1) {
+            e[0] = *reinterpret_cast<const uint16_t *>(from);
+        } else if constexpr (MT == 2) {
+            e[0] = *reinterpret_cast<const uint32_t *>(from);
+        } else if constexpr (MT == 4) {
+            const uint2 v = *reinterpret_cast<const uint2 *>(from);
+            e[0] = v.x;
+            e[1] = v.y;
+        } else {
+            const uint4 v = *reinterpret_cast<const uint4 *>(from);
+            e[0] = v.x;
+            e[1] = v.y;
+            e[2] = v.z;
+            e[3] = v.w;
+        }
+    };
+
+    uint32_t even[8][H] = {}, odd[8][H] = {};
+    load(0);
+    for (int step = 0; step < steps; ++step) {
+        const bool there = first + step * kFewGroups + group < last;
+        unsigned char *const R = lds + ((step & 1) * kFewGroups + group) * 2 * kRowBytes;
+        if (there) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {   // filter code lane + 64 i
                 const uint32_t sel = i & 1 ? 0x07060302u : 0x05040100u;
@@ -307,7 +345,7 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const uint16_t *__restric
                     const uint32_t hi = MT == 1 ? 0u : i < 2 ? t[(2 * h + 1) % MT].x : t[(2 * h + 1) % MT].y;
                     e[h] = __builtin_amdgcn_perm(hi, lo, sel);
                 }
-                unsigned char *const to = R + (lane + 64 * i) * (2 * MT);
+                unsigned char *const to = R + half * kRowBytes + (lane + 64 * i) * (2 * MT);
                 if constexpr (MT == 1)
                     *reinterpret_cast<uint16_t *>(to) = (uint16_t)e[0];
                 else if constexpr (MT == 2)
@@ -317,54 +355,53 @@ __global__ void __launch_bounds__(256) few_rows_kernel(const uint16_t *__restric
                 else
                     *reinterpret_cast<uint4 *>(to) = make_uint4(e[0], e[1], e[2], e[3]);
             }
-            __builtin_amdgcn_wave_barrier();
+        }
+        uint32_t w[2][2] = {{b[0][0], b[0][1]}, {b[1][0], b[1][1]}};
+        if (step + 1 < steps)
+            load(step + 1);
+        __syncthreads();   // both rows are there, and the other buffer's are no longer read
+        if (there) {
 #pragma unroll
             for (int n = 0; n < 8; ++n) {
-                const unsigned char *const from = R + ((b[j][n / 4] >> (8 * (n & 3))) & 255u) * (2 * MT);
-                uint32_t e[H];
-                if constexpr (MT == 1) {
-                    e[0] = *reinterpret_cast<const uint16_t *>(from);
-                } else if constexpr (MT == 2) {
-                    e[0] = *reinterpret_cast<const uint32_t *>(from);
-                } else if constexpr (MT == 4) {
-                    const uint2 v = *reinterpret_cast<const uint2 *>(from);
-                    e[0] = v.x;
-                    e[1] = v.y;
-                } else {
-                    const uint4 v = *reinterpret_cast<const uint4 *>(from);
-                    e[0] = v.x;
-                    e[1] = v.y;
-                    e[2] = v.z;
-                    e[3] = v.w;
-                }
+                uint32_t e0[H], e1[H];
+                entry(R, (w[0][n / 4] >> (8 * (n & 3))) & 255u, e0);
+                entry(R + kRowBytes, (w[1][n / 4] >> (8 * (n & 3))) & 255u, e1);
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
-                    even[n][h] += e[h];
+                    even[n][h] += e0[h] + e1[h];
                     if constexpr (MT > 1)
-                        odd[n][h] += e[h] >> 16;
+                        odd[n][h] += (e0[h] >> 16) + (e1[h] >> 16);
                 }
             }
         }
     }
-    // the four wavefronts' sums, a row at a time through LDS
+    // the pairs' sums, four rows at a time
     int32_t *const red = reinterpret_cast<int32_t *>(lds);
+    constexpr int N = MT < kFewRowsAtOnce ? MT : kFewRowsAtOnce;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
+    for (int m0 = 0; m0 < MT; m0 += N) {
         __syncthreads();
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
-            const uint32_t v = m & 1 ? odd[n][m / 2] : even[n][m / 2] - (MT > 1 ? odd[n][m / 2] << 16 : 0u);
-            red[wave * 512 + n * 64 + lane] = (int32_t)v;
-        }
-        __syncthreads();
-        if (row0 + m < rows) {
-            int32_t *const to = acc + ((int64_t)blockIdx.y * rows + row0 + m) * width;
-            for (int i = threadIdx.x; i < 512; i += 256) {   // column 8 * lane + n stands at n * 64 + lane
-                const int col = (int)blockIdx.x * 512 + i, at = (i & 7) * 64 + i / 8;
-                if (col < width)
-                    to[col] = red[at] + red[512 + at] + red[1024 + at] + red[1536 + at];
+        for (int m = 0; m < N; ++m)
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                const int of = m0 + m;
+                const uint32_t v = of & 1 ? odd[n][of / 2] : even[n][of / 2] - (MT > 1 ? odd[n][of / 2] << 16 : 0u);
+                red[(wave * N + m) * 512 + n * 64 + lane] = (int32_t)v;
             }
-        }
+        __syncthreads();
+        // column 8 l + n of a half stands at 64 n + l
+        const int at = (threadIdx.x & 7) * 64 + (threadIdx.x & 511) / 8, of_half = threadIdx.x / 512;
+        const int col = (int)blockIdx.x * kFewColumns + (int)threadIdx.x;
+#pragma unroll
+        for (int m = 0; m < N; ++m)
+            if (row0 + m0 + m < rows && col < width) {
+                int32_t sum = 0;
+#pragma unroll
+                for (int g = 0; g < kFewGroups; ++g)
+                    sum += red[((2 * g + of_half) * N + m) * 512 + at];
+                acc[((int64_t)blockIdx.y * rows + row0 + m0 + m) * width + col] = sum;
+            }
     }
 }
 
@@ -565,29 +602,38 @@ hipError_t launch_codes(const CodesJob &job, hipStream_t stream)
     return hipGetLastError();
 }
 
-// Enough workgroups for the chip, four a CU, but at least two quads of the depth for every wavefront.
+// A workgroup a CU, but at least two steps of the depth each.
 int few_rows_splits(int64_t rows, int K, int width)
 {
-    const int64_t groups = (rows + kFewRows - 1) / kFewRows * ((width + 511) / 512);
-    const int64_t want = 1024 / groups, most = ((K + 3) / 4) / 8;
+    const int64_t groups = (rows + kFewRows - 1) / kFewRows * ((width + kFewColumns - 1) / kFewColumns);
+    const int64_t want = device_cus() / groups, most = (K + 3) / 4 * 2 / (2 * kFewGroups);
     const int64_t s = want < most ? want : most;
     return (int)(s < 1 ? 1 : s);
+}
+
+template <int MT>
+static hipError_t few_rows(const uint16_t *tableI, const uint8_t *x_codes, int rows, int Kp, const uint8_t *kernel_codes, int width,
+                           int splits, int32_t *acc, hipStream_t stream)
+{
+    constexpr int bytes = few_lds_bytes<MT>();
+    if (hipError_t e = set_max_dynamic_lds_once(reinterpret_cast<const void *>(&few_rows_kernel<MT>), bytes))
+        return e;
+    hipLaunchKernelGGL(few_rows_kernel<MT>,
+                       dim3((unsigned)((width + kFewColumns - 1) / kFewColumns), (unsigned)splits, (unsigned)((rows + MT - 1) / MT)),
+                       dim3(1024), bytes, stream, tableI, x_codes, rows, Kp, kernel_codes, width, acc);
+    return hipGetLastError();
 }
 
 hipError_t launch_few_rows(const uint16_t *tableI, const uint8_t *x_codes, int rows, int Kp, const uint8_t *kernel_codes, int width,
                            int splits, int32_t *acc, hipStream_t stream)
 {
-    const int mt = rows == 1 ? 1 : rows == 2 ? 2 : rows <= 4 ? 4 : 8;
-    const dim3 grid((unsigned)((width + 511) / 512), (unsigned)splits, (unsigned)((rows + mt - 1) / mt));
-    if (mt == 1)
-        hipLaunchKernelGGL(few_rows_kernel<1>, grid, dim3(256), 0, stream, tableI, x_codes, rows, Kp, kernel_codes, width, acc);
-    else if (mt == 2)
-        hipLaunchKernelGGL(few_rows_kernel<2>, grid, dim3(256), 0, stream, tableI, x_codes, rows, Kp, kernel_codes, width, acc);
-    else if (mt == 4)
-        hipLaunchKernelGGL(few_rows_kernel<4>, grid, dim3(256), 0, stream, tableI, x_codes, rows, Kp, kernel_codes, width, acc);
-    else
-        hipLaunchKernelGGL(few_rows_kernel<8>, grid, dim3(256), 0, stream, tableI, x_codes, rows, Kp, kernel_codes, width, acc);
-    return hipGetLastError();
+    if (rows == 1)
+        return few_rows<1>(tableI, x_codes, rows, Kp, kernel_codes, width, splits, acc, stream);
+    if (rows == 2)
+        return few_rows<2>(tableI, x_codes, rows, Kp, kernel_codes, width, splits, acc, stream);
+    if (rows <= 4)
+        return few_rows<4>(tableI, x_codes, rows, Kp, kernel_codes, width, splits, acc, stream);
+    return few_rows<8>(tableI, x_codes, rows, Kp, kernel_codes, width, splits, acc, stream);
 }
 
 template <typename T, typename I>
@@ -600,9 +646,10 @@ static hipError_t dense_out(const TableSums &s, int64_t rows, int columns, const
         hipLaunchKernelGGL((dense_out_parts_kernel<T, I>), dim3((unsigned)((columns + 255) / 256), (unsigned)rows), dim3(256), 0,
                            stream, s, columns, o);
     } else {
-        const int64_t by = (rows + 3) / 4;
-        hipLaunchKernelGGL((dense_out_kernel<T, I>), dim3((unsigned)((columns + 255) / 256), (unsigned)(by > 4096 ? 4096 : by)),
-                           dim3(256), 0, stream, s, rows, columns, o);
+        // several rows a wavefront, so that what belongs to the columns is loaded once for them
+        const int64_t bx = (columns + 255) / 256, most = (4096 + bx - 1) / bx, by = (rows + 3) / 4;
+        hipLaunchKernelGGL((dense_out_kernel<T, I>), dim3((unsigned)bx, (unsigned)(by > most ? most : by)), dim3(256), 0, stream, s,
+                           rows, columns, o);
     }
     return hipGetLastError();
 }

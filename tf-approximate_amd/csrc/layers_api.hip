@@ -574,7 +574,7 @@ static int carve_loss(const axc_dense_desc *d, bool gradients, void *base, LossS
     for (float **p : state)
         *p = c.take<float>((size_t)d->rows);
     s->st.factor = c.take<float>(1);
-    s->st.parts = c.take<float2>((size_t)pc.count * ((pc.width + kLossChunk - 1) / kLossChunk) * d->rows);
+    s->st.parts = c.take<float2>((size_t)pc.count * ((pc.width + loss_chunk(d->rows) - 1) / loss_chunk(d->rows)) * d->rows);
     size_t count = 0;
     if (int rc = runs_workspace(d->rows, std::min(d->rows, kRowRun), pc, &count, &s->lut_bytes))
         return rc;

@@ -404,7 +404,8 @@ hipError_t launch_column_sums(const float *partials, int64_t count, int64_t cols
                               int type, hipStream_t stream);
 
 // ---- loss (loss_kernels.hip) ----
-constexpr int kLossChunk = 512;          // columns at least that leave a maximum and a sum
+// Columns at least that leave a maximum and a sum: fewer where few rows would leave CUs without work.
+inline int loss_chunk(int64_t rows) { return rows >= 2048 ? 512 : rows >= 512 ? 256 : 64; }
 struct LossState {
     float2 *parts;                       // [chunk][rows]: the largest logit and the sum of exponentials around it
     float *at;                           // per row: the target's logit

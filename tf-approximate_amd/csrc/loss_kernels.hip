@@ -92,12 +92,12 @@ __global__ void __launch_bounds__(256) loss_piece_kernel(TableSums s, int64_t fi
     st.parts[(chunk + blockIdx.y) * rows + first_row + r] = make_float2(e.top, e.sum);
 }
 
-// Turned sums: a workgroup 64 rows, a lane each, and kLossChunk columns, a quarter for each wavefront.  A lane goes through its row's
+// Turned sums: a workgroup 64 rows, a lane each, and `size` columns, a quarter for each wavefront.  A lane goes through its row's
 // logits by itself; what belongs to a column is the same for all lanes.
 template <typename I>
 __global__ void __launch_bounds__(256) loss_turned_kernel(TableSums s, int64_t first_row, int64_t run_rows, int64_t rows, int columns,
                                                           int64_t first_column, const void *bias, int bias_type,
-                                                          const int64_t *__restrict__ targets, int chunk, LossState st)
+                                                          const int64_t *__restrict__ targets, int chunk, int size, LossState st)
 {
     constexpr int N = 8;
     __shared__ float tops[4][64], sums[4][64];
@@ -108,8 +108,8 @@ __global__ void __launch_bounds__(256) loss_turned_kernel(TableSums s, int64_t f
     const Bracket<I> b(s);
     const I row = b.row(s.row_sums[r]);
     const int64_t target = targets[first_row + r] - first_column;
-    const int c0 = (int)blockIdx.x * kLossChunk + wave * (kLossChunk / 4);
-    const int end = c0 + kLossChunk / 4 < columns ? c0 + kLossChunk / 4 : columns;
+    const int c0 = (int)blockIdx.x * size + wave * (size / 4);
+    const int end = c0 + size / 4 < columns ? c0 + size / 4 : columns;
     Exponentials e;
     for (int c = c0; c < end; c += N) {
         int32_t t[N] = {};
@@ -231,14 +231,15 @@ hipError_t launch_loss_piece(const TableSums &s, int64_t first_row, int64_t run_
 {
     const bool narrow = s.K <= kNarrowDepth;
     if (s.raw.turned) {
-        *chunks = (columns + kLossChunk - 1) / kLossChunk;
+        const int size = loss_chunk(rows);
+        *chunks = (columns + size - 1) / size;
         const dim3 grid((unsigned)*chunks, (unsigned)((run_rows + 63) / 64));
         if (narrow)
             hipLaunchKernelGGL(loss_turned_kernel<uint32_t>, grid, dim3(256), 0, stream, s, first_row, run_rows, rows, columns,
-                               first_column, bias, bias_type, targets, chunk, st);
+                               first_column, bias, bias_type, targets, chunk, size, st);
         else
             hipLaunchKernelGGL(loss_turned_kernel<int64_t>, grid, dim3(256), 0, stream, s, first_row, run_rows, rows, columns,
-                               first_column, bias, bias_type, targets, chunk, st);
+                               first_column, bias, bias_type, targets, chunk, size, st);
     } else {
         *chunks = (columns + kRowChunk - 1) / kRowChunk;
         const dim3 grid((unsigned)run_rows, (unsigned)*chunks);
