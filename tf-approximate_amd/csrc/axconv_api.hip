@@ -1901,7 +1901,7 @@ int axc_table_create(const uint16_t *host_table, axc_table **out)
         return fail(AXC_INVALID_ARGUMENT, "null argument");
     // weight-code major: tableT[b][a] = T[(a << 8) | b], in squares that the first-level cache holds by row and by column, and
     // the two flipped copies by whole vectors (us a table with its upload, on one machine: entry by entry 143 for the first
-    // alone, 181 for three; 42); behind them input-code major rows for dense layers of few rows
+    // alone, 181 for three; 42); behind them the caller's own order, for dense layers of few rows
     const size_t entries = (size_t)kTableRows * 256, used = 65536;   // row 256: the null weight's, zeros
     std::vector<uint16_t> t(4 * entries);
     uint16_t *const T = t.data(), *const F = T + entries, *const S = F + entries, *const I = S + entries;
@@ -1916,10 +1916,7 @@ int axc_table_create(const uint16_t *host_table, axc_table **out)
         S[i] = host_table[i] ^ 0x8080u;
     for (size_t i = used; i < entries; ++i)
         S[i] = 0x8080u;
-    for (int a = 0; a < 256; ++a)   // entry 4 l + i is that of filter code l + 64 i: what a lane loads at once
-        for (int l = 0; l < 64; ++l)
-            for (int i = 0; i < 4; ++i)
-                I[a * 256 + 4 * l + i] = host_table[a * 256 + l + 64 * i];
+    memcpy(I, host_table, used * sizeof(uint16_t));
     axc_table *tab = new axc_table;
     tab->dev_tableT = nullptr;
     hipError_t e = hipGetDevice(&tab->device);

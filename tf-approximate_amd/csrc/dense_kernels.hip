@@ -137,8 +137,21 @@ __device__ __forceinline__ int32_t row_codes_any(const void *x, int type, int64_
     return row_codes(static_cast<const f16 *>(x) + at, K, Kp, whole, g, codes, thread, threads);
 }
 
-// Few rows: every workgroup finds the range itself, of all rows, and then takes its own row.
-__global__ void __launch_bounds__(512) few_codes_kernel(const void *x, int type, int rows, int K, int Kp, RangeSource src,
+// Few rows, in groups of eight: every workgroup finds the range itself, of all rows, and then takes its own row
+// (of rows that are not there the codes are what the memory held: any byte is one, and nobody stores what comes of them).
+template <typename T>
+__device__ int32_t column_codes(const T *__restrict__ x, int K, int Kb, const Grid &g, uint8_t *__restrict__ codes)
+{
+    int32_t sum = 0;
+#pragma unroll 4
+    for (int k = threadIdx.x; k < Kb; k += 512) {
+        const uint32_t c = k < K ? code_of((float)x[k], g) : 0u;
+        codes[(int64_t)k * 8] = (uint8_t)c;
+        sum += (int32_t)c;
+    }
+    return sum;
+}
+__global__ void __launch_bounds__(512) few_codes_kernel(const void *x, int type, int rows, int K, int Kb, RangeSource src,
                                                         const Grid *kernel_grid, Grids *grids, uint8_t *codes, int32_t *row_sums)
 {
     __shared__ float red[16];
@@ -154,7 +167,15 @@ __global__ void __launch_bounds__(512) few_codes_kernel(const void *x, int type,
     }
     const Grid g = grid_of_range(lo, hi);
     const int64_t r = blockIdx.x;
-    const int32_t part = wave_sum(row_codes_any(x, type, r * K, K, Kp, g, codes + r * Kp, (int)threadIdx.x, 512));
+    uint8_t *const to = codes + (r & ~7) * Kb + (r & 7);
+    int32_t part = 0;
+    if (type == AXC_F32)
+        part = column_codes(static_cast<const float *>(x) + r * K, K, Kb, g, to);
+    else if (type == AXC_BF16)
+        part = column_codes(static_cast<const bf16 *>(x) + r * K, K, Kb, g, to);
+    else
+        part = column_codes(static_cast<const f16 *>(x) + r * K, K, Kb, g, to);
+    part = wave_sum(part);
     if ((threadIdx.x & 63) == 0)
         sums[threadIdx.x / 64] = part;
     __syncthreads();
@@ -165,14 +186,18 @@ __global__ void __launch_bounds__(512) few_codes_kernel(const void *x, int type,
         row_sums[r] = sum;
         if (r == 0) {
             grids->in = g;
-            grids->kernel = *kernel_grid;
+            if (kernel_grid)
+                grids->kernel = *kernel_grid;
         }
     }
 }
 
+constexpr int kSlab = 64;   // most of the depth that a workgroup of codes_kernel takes
+
+// tile: not null: the codes go there too, [element of the slab][column of the workgroup].
 template <typename T>
 __device__ void kernel_slab(const T *__restrict__ w, int K, int64_t N, const Pieces &pc, const Grid &g, uint8_t *__restrict__ codes,
-                            int64_t c, int k0, int lines, int (&sum)[4])
+                            uint32_t (*tile)[64], int64_t c, int first, int wave, int lines, int (&sum)[4])
 {
     const int piece = (int)(c / pc.width);
     uint8_t *const to = codes + pc.offset(piece) + (c - pc.first(piece));
@@ -180,9 +205,7 @@ __device__ void kernel_slab(const T *__restrict__ w, int K, int64_t N, const Pie
     const bool whole = c + 4 <= N && (N & 3) == 0 && ((uintptr_t)w & (4 * sizeof(T) - 1)) == 0;
 #pragma unroll 4
     for (int i = 0; i < lines; ++i) {
-        const int k = k0 + 4 * i;
-        if (k >= pc.Kp)
-            break;
+        const int k = first + wave + 4 * i;
         float v[4];
         uint32_t word = 0;
         if (k < K) {
@@ -194,7 +217,10 @@ __device__ void kernel_slab(const T *__restrict__ w, int K, int64_t N, const Pie
                 sum[j] += (int)q;
             }
         }
-        *reinterpret_cast<uint32_t *>(to + (size_t)k * pitch) = word;
+        if (codes && k < pc.Kp)
+            *reinterpret_cast<uint32_t *>(to + (size_t)k * pitch) = word;
+        if (tile)
+            tile[wave + 4 * i][threadIdx.x & 63] = word;
     }
 }
 
@@ -206,6 +232,7 @@ __global__ void __launch_bounds__(256) codes_kernel(CodesJob job, int x_blocks, 
 {
     __shared__ float ends[8];
     __shared__ int32_t red[4][256];
+    __shared__ uint32_t tile[kSlab][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
     float lo, hi;
     if ((int)blockIdx.x < x_blocks) {
@@ -237,14 +264,18 @@ __global__ void __launch_bounds__(256) codes_kernel(CodesJob job, int x_blocks, 
     if (block == 0 && threadIdx.x == 0)
         job.grids->kernel = g;
     int sum[4] = {};
+    const int k0 = slab * 4 * lines;
+    uint32_t(*const turn)[64] = job.kernel_blocks ? tile : nullptr;
     if (c < job.pieces.Np) {
-        const int k0 = slab * 4 * lines + wave;
         if (job.kernel_type == AXC_F32)
-            kernel_slab(static_cast<const float *>(job.kernel), job.K, job.N, job.pieces, g, job.kernel_codes, c, k0, lines, sum);
+            kernel_slab(static_cast<const float *>(job.kernel), job.K, job.N, job.pieces, g, job.kernel_codes, turn, c, k0, wave,
+                        lines, sum);
         else if (job.kernel_type == AXC_BF16)
-            kernel_slab(static_cast<const bf16 *>(job.kernel), job.K, job.N, job.pieces, g, job.kernel_codes, c, k0, lines, sum);
+            kernel_slab(static_cast<const bf16 *>(job.kernel), job.K, job.N, job.pieces, g, job.kernel_codes, turn, c, k0, wave,
+                        lines, sum);
         else
-            kernel_slab(static_cast<const f16 *>(job.kernel), job.K, job.N, job.pieces, g, job.kernel_codes, c, k0, lines, sum);
+            kernel_slab(static_cast<const f16 *>(job.kernel), job.K, job.N, job.pieces, g, job.kernel_codes, turn, c, k0, wave, lines,
+                        sum);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -254,155 +285,148 @@ __global__ void __launch_bounds__(256) codes_kernel(CodesJob job, int x_blocks, 
     if (column < job.pieces.Np)
         atomicAdd(job.column_sums + column,
                   red[0][threadIdx.x] + red[1][threadIdx.x] + red[2][threadIdx.x] + red[3][threadIdx.x]);
+    if (!turn || column >= job.pieces.Np)
+        return;
+    // a column a thread: its codes of a block, begun at element n & 15
+    const int piece = (int)(column / job.pieces.width), n = (int)(column - job.pieces.first(piece));
+    uint8_t *const to = job.kernel_blocks + job.pieces.block_offset(piece) + (size_t)n * 16;
+    const size_t pitch = (size_t)job.pieces.width_of(piece) * 16;
+    for (int block_k = 0; block_k < 4 * lines && k0 + block_k < job.pieces.Kb; block_k += 16) {
+        uint32_t word[4] = {};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const uint32_t four = tile[block_k + ((n + i) & 15)][threadIdx.x / 4];
+            word[i / 4] |= (four >> (8 * (threadIdx.x & 3)) & 255u) << (8 * (i & 3));
+        }
+        *reinterpret_cast<uint4 *>(to + (size_t)(k0 + block_k) / 16 * pitch) = make_uint4(word[0], word[1], word[2], word[3]);
+    }
 }
 
 // ---- sums of few rows ----
-// A pair of wavefronts takes MT rows, 1024 columns (eight a lane) and two elements of the depth at a time.  Each of the two turns the
-// MT table rows that the rows' codes name at one of the elements into R[b] = entries of filter code b for all MT rows, in LDS; a lane
-// then reads the entries of all MT rows for one weight with one access of 2 MT bytes.  Sums of two rows share a dword as they come:
-// one register adds whole dwords modulo 2^32, another the upper halves, three instructions for two dwords.
-// Eight pairs make a workgroup, which adds up their sums in LDS before it leaves them to the others' (parts of the depth).
-// What bounds it for eight rows: lookups at random among 256 places of 16 bytes, 3 of 16 lanes on the busiest of 16 groups of banks
-// (25 T/s), and the table rows out of the L2, 4 KiB for every element and 1024 columns.
-constexpr int kFewGroups = 8;            // pairs of wavefronts
+// A workgroup takes MT rows, 1024 columns (one a lane) and 16 elements of the depth at a time.  For those elements it lays out in LDS
+//   R[b][e] = entries of filter code b for all MT rows, at element e of the block: 16 places of 16 bytes, a row of 256 bytes,
+// and every lane looks its column's 16 weights up in it, 2 MT bytes an access.  Which row that is, is anybody's guess, but the place
+// in it decides the banks: at step s lane l takes element (l + s) & 15, so that any 16 lanes meet 16 different groups of banks,
+// whatever their weights are (as all elements go into the same sum, their order does not matter; the codes are laid out in it).
+// Building R takes 8 to 64 KiB of table rows for the block and 1024 columns, through a first-level cache that takes an address for
+// every 64 neighbouring bytes a cycle: four neighbouring lanes read on in one table row, of one element, and the next four in
+// another's (a different row for each lane, whose stores would meet no bank twice, took 64 addresses a load: 23 us instead of 13.8
+// for 8 rows by 4096 by 4096).  Sums of two rows share a dword as they come: one register adds whole dwords modulo 2^32, another the
+// upper halves, three instructions for two dwords.
 constexpr int kFewColumns = 1024;
-constexpr int kFewRowsAtOnce = 4;        // whose sums are added up in LDS
-template <int MT>
-constexpr int few_lds_bytes()            // two buffers of table rows; then the sums of 16 wavefronts
-{
-    constexpr int table_rows = 2 * 2 * kFewGroups * 512 * MT, sums = 16 * 512 * 4 * (MT < kFewRowsAtOnce ? MT : kFewRowsAtOnce);
-    return table_rows > sums ? table_rows : sums;
-}
+constexpr int kFewLdsBytes = 2 * 65536;  // R twice: one is built while the other is read
 
 template <int MT>
 __global__ void __launch_bounds__(1024) few_rows_kernel(const uint16_t *__restrict__ tableI, const uint8_t *__restrict__ x_codes,
-                                                        int rows, int Kp, const uint8_t *__restrict__ kernel_codes, int width,
+                                                        int rows, int Kb, const uint8_t *__restrict__ kernel_blocks, int width,
                                                         int32_t *__restrict__ acc)
 {
-    constexpr int H = (MT + 1) / 2;      // dwords of an entry
-    constexpr int kRowBytes = 512 * MT;  // of R
+    constexpr int H = (MT + 1) / 2;      // dwords of a place that are used
+    constexpr int kOf = MT < 4 ? MT : 4; // rows that a wavefront takes table entries of
+    constexpr int kEntries = MT == 8 ? 8 : 4;   // of neighbouring filter codes that a lane takes: eight rows are two wavefronts' work
+    typedef uint32_t Words __attribute__((ext_vector_type(kEntries / 2)));
     extern __shared__ __align__(16) unsigned char lds[];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const int group = wave >> 1, half = wave & 1;
-    const int c = (int)blockIdx.x * kFewColumns + half * 512 + lane * 8;
-    const int row0 = (int)blockIdx.z * MT;
-    const int pairs = Kp / 2;
-    const int first = (int)((int64_t)pairs * blockIdx.y / gridDim.y), last = (int)((int64_t)pairs * (blockIdx.y + 1) / gridDim.y);
-    const int steps = (last - first + kFewGroups - 1) / kFewGroups;
-    const bool in0 = c < width, in1 = c + 4 < width;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+    const int c = (int)blockIdx.x * kFewColumns + (int)threadIdx.x;
+    const int at = c < width ? c : width - 1;   // (lanes behind the columns repeat the last, at its place; nobody stores them)
+    const int row0 = (int)blockIdx.z * 8;
+    const int blocks = Kb / 16;
+    const int first = (int)((int64_t)blocks * blockIdx.y / gridDim.y), last = (int)((int64_t)blocks * (blockIdx.y + 1) / gridDim.y);
+    // this lane's part of R: filter codes b0 on, at element lane >> 2, rows `half` on
+    const int half = MT == 8 ? (wave & 1) * 4 : 0;
+    const int b0 = (MT == 8 ? (wave >> 1) * 32 : wave * 16) + (lane & 3) * kEntries;
+    const uint8_t *const xs = x_codes + (int64_t)row0 * Kb + (lane >> 2) * 8 + half;
 
-    uint2 t[MT];                         // table rows of this wavefront's element, four entries a lane
-    uint32_t b[2][2];                    // weights of both elements, eight codes a lane
-    auto load = [&](int step) {
-        const int pair = first + step * kFewGroups + group;
-        if (pair >= last)                // (uniform; what is there is not used)
-            return;
-        const int k = 2 * pair + half;
+    uint32_t a;                          // the rows' codes at that element
+    Words t[kOf];                        // table entries
+    uint4 w;                             // the column's 16 weights
+    auto load_codes = [&](int block) { a = *reinterpret_cast<const uint32_t *>(xs + (int64_t)block * 128); };
+    auto load_entries = [&] {
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {   // (rows beyond the last repeat it; nobody stores them)
-            const uint32_t four = *reinterpret_cast<const uint32_t *>(x_codes + (int64_t)min(row0 + m, rows - 1) * Kp + (k & ~3));
-            t[m] = *reinterpret_cast<const uint2 *>(tableI + ((four >> (8 * (k & 3))) & 255u) * 256u + lane * 4);
-        }
+        for (int m = 0; m < kOf; ++m)
+            t[m] = *reinterpret_cast<const Words *>(tableI + ((a >> (8 * m)) & 255u) * 256u + b0);
+    };
+    auto load_weights = [&](int block) {
+        w = *reinterpret_cast<const uint4 *>(kernel_blocks + ((int64_t)block * width + at) * 16);
+    };
+    uint32_t chunk[4];                   // where step 4 i + j reads in a row, in bytes: byte j of chunk[i]
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const uint8_t *const p = kernel_codes + (size_t)(2 * pair + j) * width + c;
-            b[j][0] = in0 ? *reinterpret_cast<const uint32_t *>(p) : 0u;
-            b[j][1] = in1 ? *reinterpret_cast<const uint32_t *>(p + 4) : 0u;
-        }
-    };
-    auto entry = [&](const unsigned char *R, uint32_t code, uint32_t (&e)[H]) {
-        const unsigned char *const from = R + code * (2 * MT);
-        if constexpr (MT == 1) {
-            e[0] = *reinterpret_cast<const uint16_t *>(from);
-        } else if constexpr (MT == 2) {
-            e[0] = *reinterpret_cast<const uint32_t *>(from);
-        } else if constexpr (MT == 4) {
-            const uint2 v = *reinterpret_cast<const uint2 *>(from);
-            e[0] = v.x;
-            e[1] = v.y;
-        } else {
-            const uint4 v = *reinterpret_cast<const uint4 *>(from);
-            e[0] = v.x;
-            e[1] = v.y;
-            e[2] = v.z;
-            e[3] = v.w;
-        }
-    };
+    for (int i = 0; i < 4; ++i) {
+        chunk[i] = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            chunk[i] |= (uint32_t)(((at + 4 * i + j) & 15) * 16) << (8 * j);
+    }
 
-    uint32_t even[8][H] = {}, odd[8][H] = {};
-    load(0);
-    for (int step = 0; step < steps; ++step) {
-        const bool there = first + step * kFewGroups + group < last;
-        unsigned char *const R = lds + ((step & 1) * kFewGroups + group) * 2 * kRowBytes;
-        if (there) {
+    uint32_t even[H] = {}, odd[H] = {};
+    if (first < last) {
+        load_codes(first);
+        load_entries();
+        load_weights(first);
+        if (first + 1 < last)
+            load_codes(first + 1);
+    }
+    for (int block = first; block < last; ++block) {
+        unsigned char *const R = lds + ((block - first) & 1) * 65536;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {   // filter code lane + 64 i
-                const uint32_t sel = i & 1 ? 0x07060302u : 0x05040100u;
-                uint32_t e[H];
+        for (int i = 0; i < kEntries; ++i) {
+            const uint32_t sel = i & 1 ? 0x07060302u : 0x05040100u;
+            uint32_t e[2] = {};
 #pragma unroll
-                for (int h = 0; h < H; ++h) {
-                    const uint32_t lo = i < 2 ? t[2 * h].x : t[2 * h].y;
-                    const uint32_t hi = MT == 1 ? 0u : i < 2 ? t[(2 * h + 1) % MT].x : t[(2 * h + 1) % MT].y;
-                    e[h] = __builtin_amdgcn_perm(hi, lo, sel);
+            for (int h = 0; h < (kOf + 1) / 2; ++h)
+                e[h] = __builtin_amdgcn_perm(MT == 1 ? 0u : t[(2 * h + 1) % kOf][i / 2], t[2 * h][i / 2], sel);
+            unsigned char *const to = R + (b0 + i) * 256 + (lane >> 2) * 16 + half * 2;
+            if constexpr (H == 1)
+                *reinterpret_cast<uint32_t *>(to) = e[0];
+            else
+                *reinterpret_cast<uint2 *>(to) = make_uint2(e[0], e[1]);
+        }
+        const uint32_t weights[4] = {w.x, w.y, w.z, w.w};
+        if (block + 1 < last) {
+            load_entries();
+            load_weights(block + 1);
+            if (block + 2 < last)
+                load_codes(block + 2);
+        }
+        __syncthreads();   // R is whole, and the other one is no longer read
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t e[4][H];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                // byte 1: the weight, byte 0: the place
+                const unsigned char *const from = R + __builtin_amdgcn_perm(weights[i], chunk[i], 0x0c0c0400u + 0x0101u * j);
+                if constexpr (H == 1) {
+                    e[j][0] = *reinterpret_cast<const uint32_t *>(from);
+                } else if constexpr (H == 2) {
+                    const uint2 v = *reinterpret_cast<const uint2 *>(from);
+                    e[j][0] = v.x;
+                    e[j][1] = v.y;
+                } else {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(from);
+                    e[j][0] = v.x;
+                    e[j][1] = v.y;
+                    e[j][2] = v.z;
+                    e[j][3] = v.w;
                 }
-                unsigned char *const to = R + half * kRowBytes + (lane + 64 * i) * (2 * MT);
-                if constexpr (MT == 1)
-                    *reinterpret_cast<uint16_t *>(to) = (uint16_t)e[0];
-                else if constexpr (MT == 2)
-                    *reinterpret_cast<uint32_t *>(to) = e[0];
-                else if constexpr (MT == 4)
-                    *reinterpret_cast<uint2 *>(to) = make_uint2(e[0], e[1]);
-                else
-                    *reinterpret_cast<uint4 *>(to) = make_uint4(e[0], e[1], e[2], e[3]);
             }
-        }
-        uint32_t w[2][2] = {{b[0][0], b[0][1]}, {b[1][0], b[1][1]}};
-        if (step + 1 < steps)
-            load(step + 1);
-        __syncthreads();   // both rows are there, and the other buffer's are no longer read
-        if (there) {
 #pragma unroll
-            for (int n = 0; n < 8; ++n) {
-                uint32_t e0[H], e1[H];
-                entry(R, (w[0][n / 4] >> (8 * (n & 3))) & 255u, e0);
-                entry(R + kRowBytes, (w[1][n / 4] >> (8 * (n & 3))) & 255u, e1);
+            for (int j = 0; j < 4; j += 2)
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
-                    even[n][h] += e0[h] + e1[h];
+                    even[h] += e[j][h] + e[j + 1][h];
                     if constexpr (MT > 1)
-                        odd[n][h] += (e0[h] >> 16) + (e1[h] >> 16);
+                        odd[h] += (e[j][h] >> 16) + (e[j + 1][h] >> 16);
                 }
-            }
         }
     }
-    // the pairs' sums, four rows at a time
-    int32_t *const red = reinterpret_cast<int32_t *>(lds);
-    constexpr int N = MT < kFewRowsAtOnce ? MT : kFewRowsAtOnce;
+    if (c >= width)
+        return;
 #pragma unroll
-    for (int m0 = 0; m0 < MT; m0 += N) {
-        __syncthreads();
-#pragma unroll
-        for (int m = 0; m < N; ++m)
-#pragma unroll
-            for (int n = 0; n < 8; ++n) {
-                const int of = m0 + m;
-                const uint32_t v = of & 1 ? odd[n][of / 2] : even[n][of / 2] - (MT > 1 ? odd[n][of / 2] << 16 : 0u);
-                red[(wave * N + m) * 512 + n * 64 + lane] = (int32_t)v;
-            }
-        __syncthreads();
-        // column 8 l + n of a half stands at 64 n + l
-        const int at = (threadIdx.x & 7) * 64 + (threadIdx.x & 511) / 8, of_half = threadIdx.x / 512;
-        const int col = (int)blockIdx.x * kFewColumns + (int)threadIdx.x;
-#pragma unroll
-        for (int m = 0; m < N; ++m)
-            if (row0 + m0 + m < rows && col < width) {
-                int32_t sum = 0;
-#pragma unroll
-                for (int g = 0; g < kFewGroups; ++g)
-                    sum += red[((2 * g + of_half) * N + m) * 512 + at];
-                acc[((int64_t)blockIdx.y * rows + row0 + m0 + m) * width + col] = sum;
-            }
-    }
+    for (int m = 0; m < MT; ++m)
+        if (row0 + m < rows)
+            acc[((int64_t)blockIdx.y * rows + row0 + m) * width + c] =
+                (int32_t)(m & 1 ? odd[m / 2] : even[m / 2] - (MT > 1 ? odd[m / 2] << 16 : 0u));
 }
 
 // ---- what is made of the sums ----
@@ -579,10 +603,10 @@ hipError_t launch_grids(const RangeSource &in, const RangeSource &kernel, bool h
     return hipGetLastError();
 }
 
-hipError_t launch_few_codes(const void *x, int type, int rows, int K, int Kp, const RangeSource &src, const Grid *kernel_grid,
+hipError_t launch_few_codes(const void *x, int type, int rows, int K, int Kb, const RangeSource &src, const Grid *kernel_grid,
                             Grids *grids, uint8_t *codes, int32_t *row_sums, hipStream_t stream)
 {
-    hipLaunchKernelGGL(few_codes_kernel, dim3(rows), dim3(512), 0, stream, x, type, rows, K, Kp, src, kernel_grid, grids, codes,
+    hipLaunchKernelGGL(few_codes_kernel, dim3(rows), dim3(512), 0, stream, x, type, rows, K, Kb, src, kernel_grid, grids, codes,
                        row_sums);
     return hipGetLastError();
 }
@@ -592,8 +616,9 @@ hipError_t launch_codes(const CodesJob &job, hipStream_t stream)
     const int x_blocks = job.x ? (int)((job.rows + 3) / 4) : 0;
     const int column_blocks = job.kernel ? (int)((job.pieces.Np + 255) / 256) : 1;
     // a wavefront 16 lines of the depth, fewer where that would leave CUs without work
-    int lines = 16;
-    auto slabs = [&] { return (job.pieces.Kp + 4 * lines - 1) / (4 * lines); };
+    int lines = kSlab / 4;
+    const int depth = job.kernel_blocks ? job.pieces.Kb : job.pieces.Kp;
+    auto slabs = [&] { return (depth + 4 * lines - 1) / (4 * lines); };
     while (lines > 4 && (int64_t)slabs() * column_blocks < 1024)
         lines /= 2;
     const int64_t kernel_blocks = job.kernel ? (int64_t)slabs() * column_blocks : 0;
@@ -602,38 +627,37 @@ hipError_t launch_codes(const CodesJob &job, hipStream_t stream)
     return hipGetLastError();
 }
 
-// A workgroup a CU, but at least two steps of the depth each.
-int few_rows_splits(int64_t rows, int K, int width)
+// A workgroup a CU, but at least two blocks of the depth each.
+int few_rows_splits(int64_t rows, int Kb, int width)
 {
-    const int64_t groups = (rows + kFewRows - 1) / kFewRows * ((width + kFewColumns - 1) / kFewColumns);
-    const int64_t want = device_cus() / groups, most = (K + 3) / 4 * 2 / (2 * kFewGroups);
+    const int64_t groups = (rows + 7) / 8 * ((width + kFewColumns - 1) / kFewColumns);
+    const int64_t want = device_cus() / groups, most = Kb / 32;
     const int64_t s = want < most ? want : most;
     return (int)(s < 1 ? 1 : s);
 }
 
 template <int MT>
-static hipError_t few_rows(const uint16_t *tableI, const uint8_t *x_codes, int rows, int Kp, const uint8_t *kernel_codes, int width,
+static hipError_t few_rows(const uint16_t *tableI, const uint8_t *x_codes, int rows, int Kb, const uint8_t *kernel_blocks, int width,
                            int splits, int32_t *acc, hipStream_t stream)
 {
-    constexpr int bytes = few_lds_bytes<MT>();
-    if (hipError_t e = set_max_dynamic_lds_once(reinterpret_cast<const void *>(&few_rows_kernel<MT>), bytes))
+    if (hipError_t e = set_max_dynamic_lds_once(reinterpret_cast<const void *>(&few_rows_kernel<MT>), kFewLdsBytes))
         return e;
     hipLaunchKernelGGL(few_rows_kernel<MT>,
-                       dim3((unsigned)((width + kFewColumns - 1) / kFewColumns), (unsigned)splits, (unsigned)((rows + MT - 1) / MT)),
-                       dim3(1024), bytes, stream, tableI, x_codes, rows, Kp, kernel_codes, width, acc);
+                       dim3((unsigned)((width + kFewColumns - 1) / kFewColumns), (unsigned)splits, (unsigned)((rows + 7) / 8)),
+                       dim3(1024), kFewLdsBytes, stream, tableI, x_codes, rows, Kb, kernel_blocks, width, acc);
     return hipGetLastError();
 }
 
-hipError_t launch_few_rows(const uint16_t *tableI, const uint8_t *x_codes, int rows, int Kp, const uint8_t *kernel_codes, int width,
+hipError_t launch_few_rows(const uint16_t *tableI, const uint8_t *x_codes, int rows, int Kb, const uint8_t *kernel_blocks, int width,
                            int splits, int32_t *acc, hipStream_t stream)
 {
     if (rows == 1)
-        return few_rows<1>(tableI, x_codes, rows, Kp, kernel_codes, width, splits, acc, stream);
+        return few_rows<1>(tableI, x_codes, rows, Kb, kernel_blocks, width, splits, acc, stream);
     if (rows == 2)
-        return few_rows<2>(tableI, x_codes, rows, Kp, kernel_codes, width, splits, acc, stream);
+        return few_rows<2>(tableI, x_codes, rows, Kb, kernel_blocks, width, splits, acc, stream);
     if (rows <= 4)
-        return few_rows<4>(tableI, x_codes, rows, Kp, kernel_codes, width, splits, acc, stream);
-    return few_rows<8>(tableI, x_codes, rows, Kp, kernel_codes, width, splits, acc, stream);
+        return few_rows<4>(tableI, x_codes, rows, Kb, kernel_blocks, width, splits, acc, stream);
+    return few_rows<8>(tableI, x_codes, rows, Kb, kernel_blocks, width, splits, acc, stream);
 }
 
 template <typename T, typename I>

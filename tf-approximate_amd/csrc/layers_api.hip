@@ -78,6 +78,7 @@ Pieces pieces_of(int64_t depth, int64_t columns, int64_t most)
     Pieces p = {};
     p.Np = fours(columns);
     p.Kp = (int32_t)fours(depth);
+    p.Kb = (int32_t)((depth + 15) & ~(int64_t)15);
     const int64_t count = std::max<int64_t>(1, (p.Np + most - 1) / most);
     const int64_t each = (p.Np + count - 1) / count;
     p.width = (int32_t)std::min<int64_t>(std::max<int64_t>(4, p.Np), (each + 63) / 64 * 64);
@@ -85,7 +86,7 @@ Pieces pieces_of(int64_t depth, int64_t columns, int64_t most)
     return p;
 }
 
-// ---- sums of table entries: input codes [rows][Kp] by a piece of the kernel's ----
+// ---- sums of table entries: input codes by a piece of the kernel's ----
 constexpr int64_t kRowRun = 16384;       // rows a LUT-GEMM call takes (its rows must be below 32768)
 constexpr int64_t kSumsAtOnce = (int64_t)1 << 25;   // int32 sums in the workspace: 128 MiB, half the memory-side cache
 constexpr int64_t kFewRowsMost = 16;
@@ -110,12 +111,13 @@ axc_conv2d_desc conv_desc(int64_t rows, int Kp, int width)
     return c;
 }
 
-// What the sums of a run of rows (kRowRun at most) and any piece need: int32 values of their own, and scratch bytes.
-int sums_workspace(int64_t rows, const Pieces &pc, size_t *count, size_t *bytes)
+// What the sums of a run of rows (kRowRun at most) and any piece need: int32 values of their own, and scratch bytes.  few: the call
+// has few rows altogether.
+int sums_workspace(bool few, int64_t rows, const Pieces &pc, size_t *count, size_t *bytes)
 {
     for (const int width : {pc.width_of(0), pc.width_of(pc.count - 1)}) {
-        if (few_rows(rows)) {
-            *count = std::max(*count, (size_t)few_rows_splits(rows, pc.Kp, width) * rows * width);
+        if (few) {
+            *count = std::max(*count, (size_t)few_rows_splits(rows, pc.Kb, width) * rows * width);
             continue;
         }
         const axc_conv2d_desc c = conv_desc(fours(rows), pc.Kp, width);
@@ -128,28 +130,11 @@ int sums_workspace(int64_t rows, const Pieces &pc, size_t *count, size_t *bytes)
     return AXC_OK;
 }
 
-// Sums of a run of rows and piece p: in acc or in the scratch.
-int table_sums(const axc_table *table, const uint8_t *input_codes, int64_t rows, const Pieces &pc, int p, const uint8_t *kernel_codes,
-               int32_t *acc, void *ws, size_t ws_bytes, hipStream_t stream, RawSums *out)
-{
-    const int width = pc.width_of(p);
-    const uint8_t *const codes = kernel_codes + pc.offset(p);
-    if (few_rows(rows)) {
-        const int splits = few_rows_splits(rows, pc.Kp, width);
-        *out = {acc, rows * width, splits, width, 0};
-        ApiTimer t("few_rows", stream);
-        AXC_HIP(launch_few_rows(table->dev_tableI, input_codes, (int)rows, pc.Kp, codes, width, splits, acc, stream));
-        return AXC_OK;
-    }
-    const axc_conv2d_desc c = conv_desc(fours(rows), pc.Kp, width);
-    return api_codes_sums(table, &c, input_codes, codes, acc, ws, ws_bytes, stream, out);
-}
-
 // ---- operands ----
 struct Operands {
     Grids *grids;
     float *x_pairs, *kernel_pairs;
-    uint8_t *x_codes, *kernel_codes;
+    uint8_t *x_codes, *kernel_codes, *kernel_blocks;
     int32_t *row_sums, *column_sums;
 };
 
@@ -160,11 +145,15 @@ Operands carve_operands(Carver &c, const axc_dense_desc *d, const Pieces &pc, bo
     o.x_pairs = c.take<float>(2 * kRangeBlocks);
     o.kernel_pairs = c.take<float>(2 * kRangeBlocks);
     if (codes) {
-        o.x_codes = c.take<uint8_t>((size_t)fours(d->rows) * pc.Kp);
+        o.x_codes = few_rows(d->rows) ? c.take<uint8_t>((size_t)(d->rows + 7) / 8 * 8 * pc.Kb)
+                                      : c.take<uint8_t>((size_t)fours(d->rows) * pc.Kp);
         o.row_sums = c.take<int32_t>((size_t)fours(d->rows));
     }
     if (codes && with_kernel) {
-        o.kernel_codes = c.take<uint8_t>(pc.bytes());
+        if (few_rows(d->rows))
+            o.kernel_blocks = c.take<uint8_t>(pc.block_bytes());
+        else
+            o.kernel_codes = c.take<uint8_t>(pc.bytes());
         o.column_sums = c.take<int32_t>((size_t)pc.Np);
     }
     return o;
@@ -215,6 +204,7 @@ int make_codes(const axc_dense_desc *d, const void *input, const RangeSource &in
     job.grids = o.grids;
     job.x_codes = o.x_codes;
     job.kernel_codes = o.kernel_codes;
+    job.kernel_blocks = o.kernel_blocks;
     job.row_sums = o.row_sums;
     job.column_sums = o.column_sums;
     ApiTimer t("layer_codes", stream);
@@ -222,14 +212,27 @@ int make_codes(const axc_dense_desc *d, const void *input, const RangeSource &in
     return AXC_OK;
 }
 
+// Few rows of the input, against a kernel whose grid is known (null: it stands in the grids already).
+int make_few_codes(const axc_dense_desc *d, const void *input, const void *range, const Grid *kernel_grid, const Operands &o,
+                   const Pieces &pc, hipStream_t stream)
+{
+    ApiTimer t("layer_codes", stream);
+    AXC_HIP(launch_few_codes(input, d->input_type, (int)d->rows, (int)d->depth, pc.Kb, input_source(d, range), kernel_grid, o.grids,
+                             o.x_codes, o.row_sums, stream));
+    return AXC_OK;
+}
+
 // Ranges, grids, codes and their sums of both operands.
 int find_codes(const axc_dense_desc *d, const void *input, const void *range, const void *kernel, const Operands &o, const Pieces &pc,
                hipStream_t stream)
 {
+    const bool few = few_rows(d->rows);
     RangeSource in, k;
-    if (int rc = find_ranges(d, input, range, kernel, o.x_pairs, o.kernel_pairs, o.column_sums, pc.Np, &in, &k, stream))
+    if (int rc = find_ranges(d, few ? nullptr : input, range, kernel, o.x_pairs, o.kernel_pairs, o.column_sums, pc.Np, &in, &k, stream))
         return rc;
-    return make_codes(d, input, in, kernel, k, nullptr, o, pc, stream);
+    if (int rc = make_codes(d, few ? nullptr : input, in, kernel, k, nullptr, o, pc, stream))
+        return rc;
+    return few ? make_few_codes(d, input, range, nullptr, o, pc, stream) : AXC_OK;
 }
 // The grids alone.
 int find_grids(const axc_dense_desc *d, const void *input, const void *range, const void *kernel, const Operands &o, hipStream_t stream)
@@ -242,19 +245,29 @@ int find_grids(const axc_dense_desc *d, const void *input, const void *range, co
     return AXC_OK;
 }
 
-// What a consumer of the sums of piece p and the run of rows from r on is given.
-TableSums sums_of(const axc_table *table, const axc_dense_desc *d, const Operands &o, const Pieces &pc, int p, int64_t r,
-                  const RawSums &raw)
+// Sums of the run of rows from r on and piece p, in acc or in the scratch, as their consumer is given them.
+int table_sums(const axc_table *table, const axc_dense_desc *d, const Operands &o, const Pieces &pc, int p, int64_t r, int64_t rows,
+               int32_t *acc, void *ws, size_t ws_bytes, hipStream_t stream, TableSums *out)
 {
-    TableSums s = {};
-    s.raw = raw;
-    s.row_sums = o.row_sums + r;
-    s.column_sums = o.column_sums + pc.first(p);
-    s.table = table->dev_tableT;
-    s.grids = o.grids;
-    s.K = (int)d->depth;
-    s.pad = pc.Kp - (int)d->depth;
-    return s;
+    const bool few = few_rows(d->rows);
+    const int width = pc.width_of(p);
+    *out = {};
+    out->row_sums = o.row_sums + r;
+    out->column_sums = o.column_sums + pc.first(p);
+    out->table = table->dev_tableT;
+    out->grids = o.grids;
+    out->K = (int)d->depth;
+    out->pad = (few ? pc.Kb : pc.Kp) - (int)d->depth;
+    if (few) {
+        const int splits = few_rows_splits(rows, pc.Kb, width);
+        out->raw = {acc, rows * width, splits, width, 0};
+        ApiTimer t("few_rows", stream);
+        AXC_HIP(launch_few_rows(table->dev_tableI, o.x_codes, (int)rows, pc.Kb, o.kernel_blocks + pc.block_offset(p), width, splits,
+                                acc, stream));
+        return AXC_OK;
+    }
+    const axc_conv2d_desc c = conv_desc(fours(rows), pc.Kp, width);
+    return api_codes_sums(table, &c, o.x_codes + r * pc.Kp, o.kernel_codes + pc.offset(p), acc, ws, ws_bytes, stream, &out->raw);
 }
 
 // ---- dense ----
@@ -264,7 +277,7 @@ struct Packed {                          // a packed kernel
     Grids *grids;
     float *pairs;
     int32_t *column_sums;
-    uint8_t *codes;
+    uint8_t *codes, *blocks;             // for many rows, for few
     size_t bytes;
 };
 Packed packed_parts(const Pieces &pc, void *base)
@@ -275,6 +288,7 @@ Packed packed_parts(const Pieces &pc, void *base)
     p.pairs = c.take<float>(2 * kRangeBlocks);
     p.column_sums = c.take<int32_t>((size_t)pc.Np);
     p.codes = c.take<uint8_t>(pc.bytes());
+    p.blocks = c.take<uint8_t>(pc.block_bytes());
     p.bytes = c.bytes();
     return p;
 }
@@ -287,10 +301,11 @@ int64_t dense_run(int64_t rows, const Pieces &pc)   // rows whose sums are in th
 // Sums and scratch of `rows` rows, a run at a time.
 int runs_workspace(int64_t rows, int64_t run, const Pieces &pc, size_t *count, size_t *bytes)
 {
+    const bool few = few_rows(rows);
     *count = *bytes = 0;
-    if (int rc = sums_workspace(run, pc, count, bytes))
+    if (int rc = sums_workspace(few, run, pc, count, bytes))
         return rc;
-    return rows % run ? sums_workspace(rows % run, pc, count, bytes) : AXC_OK;
+    return rows % run ? sums_workspace(few, rows % run, pc, count, bytes) : AXC_OK;
 }
 
 struct DenseScratch {
@@ -353,6 +368,7 @@ int axc_dense_pack(const axc_dense_desc *desc, const void *kernel, void *packed,
     Operands o = {};
     o.grids = p.grids;
     o.kernel_codes = p.codes;
+    o.kernel_blocks = p.blocks;
     o.column_sums = p.column_sums;
     return make_codes(desc, nullptr, in, kernel, k, nullptr, o, pc, stream);
 }
@@ -401,11 +417,11 @@ int axc_fake_approx_dense(const axc_table *table, const axc_dense_desc *desc, co
     if (packed) {
         const Packed p = packed_parts(pc, const_cast<void *>(packed));
         o.kernel_codes = p.codes;
+        o.kernel_blocks = p.blocks;
         o.column_sums = p.column_sums;
         if (few_rows(desc->rows)) {
-            ApiTimer t("layer_codes", stream);
-            AXC_HIP(launch_few_codes(input, desc->input_type, (int)desc->rows, K, pc.Kp, input_source(desc, input_range),
-                                     &p.grids->kernel, o.grids, o.x_codes, o.row_sums, stream));
+            if (int rc = make_few_codes(desc, input, input_range, &p.grids->kernel, o, pc, stream))
+                return rc;
         } else {
             RangeSource in, none;
             if (int rc = find_ranges(desc, input, input_range, nullptr, o.x_pairs, nullptr, nullptr, 0, &in, &none, stream))
@@ -420,17 +436,15 @@ int axc_fake_approx_dense(const axc_table *table, const axc_dense_desc *desc, co
     for (int p = 0; p < pc.count; ++p)
         for (int64_t r = 0; r < desc->rows; r += run) {
             const int64_t rows = std::min(run, desc->rows - r), c = pc.first(p);
-            RawSums raw = {};
-            if (int rc = table_sums(table, o.x_codes + r * pc.Kp, rows, pc, p, o.kernel_codes, s.acc, s.lut, s.lut_bytes, stream,
-                                    &raw))
+            TableSums sums;
+            if (int rc = table_sums(table, desc, o, pc, p, r, rows, s.acc, s.lut, s.lut_bytes, stream, &sums))
                 return rc;
             const int64_t at = r * desc->columns + c;
             const DenseOut out = {element(bias, c, desc->bias_type), element(residual, at, desc->input_type),
                                   element(output, at, desc->input_type), element(pre, at, desc->input_type), desc->bias_type,
                                   desc->input_type, desc->activation, desc->columns};
             ApiTimer t("dense_out", stream);
-            AXC_HIP(launch_dense_out(sums_of(table, desc, o, pc, p, r, raw), rows,
-                                     (int)std::min<int64_t>(pc.width_of(p), desc->columns - c), out, stream));
+            AXC_HIP(launch_dense_out(sums, rows, (int)std::min<int64_t>(pc.width_of(p), desc->columns - c), out, stream));
         }
     return AXC_OK;
 }
@@ -656,10 +670,9 @@ int axc_fake_approx_cross_entropy(const axc_table *table, const axc_dense_desc *
         return rc;
 
     const int64_t run = std::min(rows, kRowRun);
-    RawSums raw = {};
+    TableSums sums;
     auto make_sums = [&](int p, int64_t r) {
-        return table_sums(table, o.x_codes + r * pc.Kp, std::min(run, rows - r), pc, p, o.kernel_codes, s.acc, s.lut, s.lut_bytes,
-                          stream, &raw);
+        return table_sums(table, desc, o, pc, p, r, std::min(run, rows - r), s.acc, s.lut, s.lut_bytes, stream, &sums);
     };
     auto columns_of = [&](int p) { return std::min<int64_t>(pc.width_of(p), V - pc.first(p)); };
     for (int64_t r = 0; r < rows; r += run) {
@@ -670,7 +683,7 @@ int axc_fake_approx_cross_entropy(const axc_table *table, const axc_dense_desc *
                 return rc;
             int more = 0;
             ApiTimer t("loss_piece", stream);
-            AXC_HIP(launch_loss_piece(sums_of(table, desc, o, pc, p, r, raw), r, run_rows, rows, (int)columns_of(p), pc.first(p),
+            AXC_HIP(launch_loss_piece(sums, r, run_rows, rows, (int)columns_of(p), pc.first(p),
                                       element(bias, pc.first(p), desc->bias_type), desc->bias_type, targets, chunk, &more, s.st,
                                       stream));
             chunk += more;
@@ -704,7 +717,7 @@ int axc_fake_approx_cross_entropy(const axc_table *table, const axc_dense_desc *
                     return rc;
             made = false;
             GradSource g = {};
-            g.sums = sums_of(table, desc, o, pc, p, r, raw);
+            g.sums = sums;
             g.lse = s.st.lse + r;
             g.coefficient = s.st.coefficient + r;
             g.targets = targets + r;

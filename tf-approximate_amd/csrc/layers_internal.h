@@ -254,16 +254,20 @@ __device__ __forceinline__ float activation_slope(float z, int activation)
 
 // ---- dense layers ----
 // Operands as codes, padded: input [rows][Kp], Kp the depth in fours; kernel in pieces of columns, each [Kp][width], the columns
-// in fours.  Pad codes are 0: every pad element of the depth adds T[0][0] to a sum, which the epilogue takes away again.
+// in fours.  For few_rows_kernel the depth is padded to blocks of 16: input [groups of 8 rows][Kb][8]; kernel, in each piece,
+// [block][width] of 16 codes, those of column n begun at element n & 15 of the block and gone on round it.
+// Pad codes are 0: every pad element of the depth adds T[0][0] to a sum, which the epilogue takes away again.
 struct Pieces {
     int64_t Np;            // columns, in fours
-    int32_t Kp;
+    int32_t Kp, Kb;
     int32_t width;         // of all pieces but the last
     int32_t count;
     __host__ __device__ int64_t first(int p) const { return (int64_t)p * width; }
     __host__ __device__ int width_of(int p) const { return p + 1 < count ? width : (int)(Np - (int64_t)(count - 1) * width); }
     __host__ __device__ size_t offset(int p) const { return (size_t)Kp * first(p); }   // of a piece's codes, in bytes
+    __host__ __device__ size_t block_offset(int p) const { return (size_t)Kb * first(p); }
     size_t bytes() const { return (size_t)Kp * Np; }
+    size_t block_bytes() const { return (size_t)Kb * Np; }
 };
 
 constexpr int kRangeBlocks = 256;        // pairs that the range pass leaves per tensor, at most
@@ -335,14 +339,16 @@ struct CodesJob {
     Pieces pieces;
     Grids *grids;
     uint8_t *x_codes, *kernel_codes;
+    uint8_t *kernel_blocks;              // kernel_codes and kernel_blocks: the two layouts, either may be null
     int32_t *row_sums, *column_sums;     // (those of the columns are added to)
 };
 hipError_t launch_codes(const CodesJob &job, hipStream_t stream);
-// Few rows: range (where src says so), grid, codes and their sums of the input in one launch; kernel_grid is copied next to it.
-hipError_t launch_few_codes(const void *x, int type, int rows, int K, int Kp, const RangeSource &src, const Grid *kernel_grid,
+// Few rows: range (where src says so), grid, codes and their sums of the input in one launch; a kernel_grid that is not null is
+// copied next to it.
+hipError_t launch_few_codes(const void *x, int type, int rows, int K, int Kb, const RangeSource &src, const Grid *kernel_grid,
                             Grids *grids, uint8_t *codes, int32_t *row_sums, hipStream_t stream);
-int few_rows_splits(int64_t rows, int K, int width);
-hipError_t launch_few_rows(const uint16_t *tableI, const uint8_t *x_codes, int rows, int Kp, const uint8_t *kernel_codes, int width,
+int few_rows_splits(int64_t rows, int Kb, int width);
+hipError_t launch_few_rows(const uint16_t *tableI, const uint8_t *x_codes, int rows, int Kb, const uint8_t *kernel_blocks, int width,
                            int splits, int32_t *acc, hipStream_t stream);
 struct DenseOut {
     const void *bias, *residual;         // of the piece's / run's first element
@@ -448,7 +454,7 @@ struct axc_table {
     uint16_t *dev_tableT; // [257 filter code][256 input code]; row 256 is zero
     uint16_t *dev_tableF; // behind it in the same allocation: the same with the top bit of every byte flipped,
     uint16_t *dev_tableS; // and [257 input code][256 filter code], flipped too
-    uint16_t *dev_tableI; // [256 input code][64][4]: entry [l][i] is that of filter code l + 64 i
+    uint16_t *dev_tableI; // [256 input code][256 filter code], as the caller gave it
     int device;
 };
 
