@@ -310,16 +310,19 @@ __global__ void __launch_bounds__(256) codes_kernel(CodesJob job, int x_blocks, 
 // whatever their weights are (as all elements go into the same sum, their order does not matter; the codes are laid out in it).
 // Building R takes 8 to 64 KiB of table rows for the block and 1024 columns, through a first-level cache that takes an address for
 // every 64 neighbouring bytes a cycle: four neighbouring lanes read on in one table row, of one element, and the next four in
-// another's (a different row for each lane, whose stores would meet no bank twice, took 64 addresses a load: 23 us instead of 13.8
-// for 8 rows by 4096 by 4096).  Sums of two rows share a dword as they come: one register adds whole dwords modulo 2^32, another the
+// another's (a different row for each lane, whose stores would meet no bank twice, took 64 addresses a load: 23.5 us instead of
+// 15.8 for 8 rows by 4096 by 4096).  Sums of two rows share a dword as they come: one register adds whole dwords modulo 2^32, another the
 // upper halves, three instructions for two dwords.
+// RAW: the input comes as it is.  Every workgroup finds its range and its grid itself and makes the codes of its own part of the
+// depth, into LDS; one of them the rows' sums and the grids for the launch behind this one.
 constexpr int kFewColumns = 1024;
+constexpr int kFewBlocks = 192;          // of the depth, a workgroup at most where it makes codes: 128 bytes of LDS each
 constexpr int kFewLdsBytes = 2 * 65536;  // R twice: one is built while the other is read
 
-template <int MT>
+template <int MT, bool RAW>
 __global__ void __launch_bounds__(1024) few_rows_kernel(const uint16_t *__restrict__ tableI, const uint8_t *__restrict__ x_codes,
-                                                        int rows, int Kb, const uint8_t *__restrict__ kernel_blocks, int width,
-                                                        int32_t *__restrict__ acc)
+                                                        FewInput in, int rows, int Kb, const uint8_t *__restrict__ kernel_blocks,
+                                                        int width, int32_t *__restrict__ acc)
 {
     constexpr int H = (MT + 1) / 2;      // dwords of a place that are used
     constexpr int kOf = MT < 4 ? MT : 4; // rows that a wavefront takes table entries of
@@ -340,7 +343,13 @@ __global__ void __launch_bounds__(1024) few_rows_kernel(const uint16_t *__restri
     uint32_t a;                          // the rows' codes at that element
     Words t[kOf];                        // table entries
     uint4 w;                             // the column's 16 weights
-    auto load_codes = [&](int block) { a = *reinterpret_cast<const uint32_t *>(xs + (int64_t)block * 128); };
+    unsigned char *const own_codes = lds + kFewLdsBytes;   // RAW: [element of this part][8 rows]
+    auto load_codes = [&](int block) {
+        if constexpr (RAW)
+            a = *reinterpret_cast<const uint32_t *>(own_codes + (block - first) * 128 + (lane >> 2) * 8 + half);
+        else
+            a = *reinterpret_cast<const uint32_t *>(xs + (int64_t)block * 128);
+    };
     auto load_entries = [&] {
 #pragma unroll
         for (int m = 0; m < kOf; ++m)
@@ -358,11 +367,63 @@ __global__ void __launch_bounds__(1024) few_rows_kernel(const uint16_t *__restri
             chunk[i] |= (uint32_t)(((at + 4 * i + j) & 15) * 16) << (8 * j);
     }
 
+    if (first < last)
+        load_weights(first);
+    if constexpr (RAW) {
+        __shared__ float ends[32];
+        __shared__ int32_t part[16][8];
+        float lo, hi;
+        if (!in.range.pairs && in.range.count < 0) {
+            lo = INFINITY;
+            hi = -INFINITY;
+            range_of_any(in.x, in.type, (int64_t)rows * in.K, threadIdx.x, 1024, lo, hi);
+            block_range(lo, hi, ends);
+        } else {
+            fold(in.range, lo, hi, ends);
+        }
+        const Grid g = grid_of_range(lo, hi);
+        const int here = rows - row0 < 8 ? rows - row0 : 8, k0 = first * 16, many = (last - first) * 16;
+        for (int i = (int)threadIdx.x; i < many * 8; i += 1024) {
+            const int m = i & 7, k = k0 + (i >> 3);
+            own_codes[i] = (unsigned char)(m < here && k < in.K
+                                               ? code_of(load_any(in.x, (int64_t)(row0 + m) * in.K + k, in.type), g)
+                                               : 0u);
+        }
+        if (blockIdx.x == 0 && blockIdx.y == 0) {
+            int32_t sums[MT] = {};
+            for (int k = 4 * (int)threadIdx.x; k < in.K; k += 4096)
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    float v[4] = {};
+                    load_four_any(in.x, (int64_t)(row0 + (m < here ? m : 0)) * in.K + k, in.K - k, in.type, v);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        sums[m] += k + j < in.K ? (int32_t)code_of(v[j], g) : 0;
+                }
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                sums[m] = wave_sum(sums[m]);
+                if (lane == 0)
+                    part[wave][m] = sums[m];
+            }
+            __syncthreads();
+            if ((int)threadIdx.x < here) {
+                int32_t sum = 0;
+                for (int i = 0; i < 16; ++i)
+                    sum += part[i][threadIdx.x];
+                in.row_sums[row0 + threadIdx.x] = sum;
+            }
+            if (blockIdx.z == 0 && threadIdx.x == 0) {
+                in.grids->in = g;
+                in.grids->kernel = *in.kernel_grid;
+            }
+        }
+        __syncthreads();
+    }
     uint32_t even[H] = {}, odd[H] = {};
     if (first < last) {
         load_codes(first);
         load_entries();
-        load_weights(first);
         if (first + 1 < last)
             load_codes(first + 1);
     }
@@ -627,37 +688,43 @@ hipError_t launch_codes(const CodesJob &job, hipStream_t stream)
     return hipGetLastError();
 }
 
-// A workgroup a CU, but at least two blocks of the depth each.
+// A workgroup a CU, but at least two blocks of the depth each, and at most kFewBlocks.
 int few_rows_splits(int64_t rows, int Kb, int width)
 {
     const int64_t groups = (rows + 7) / 8 * ((width + kFewColumns - 1) / kFewColumns);
-    const int64_t want = device_cus() / groups, most = Kb / 32;
+    const int64_t want = device_cus() / groups, most = Kb / 32, least = (Kb / 16 + kFewBlocks - 1) / kFewBlocks;
     const int64_t s = want < most ? want : most;
-    return (int)(s < 1 ? 1 : s);
+    return (int)(s < least ? least : s);
 }
 
-template <int MT>
-static hipError_t few_rows(const uint16_t *tableI, const uint8_t *x_codes, int rows, int Kb, const uint8_t *kernel_blocks, int width,
-                           int splits, int32_t *acc, hipStream_t stream)
+template <int MT, bool RAW>
+static hipError_t few_rows(const uint16_t *tableI, const uint8_t *x_codes, const FewInput &in, int rows, int Kb,
+                           const uint8_t *kernel_blocks, int width, int splits, int32_t *acc, hipStream_t stream)
 {
-    if (hipError_t e = set_max_dynamic_lds_once(reinterpret_cast<const void *>(&few_rows_kernel<MT>), kFewLdsBytes))
+    const int bytes = kFewLdsBytes + (RAW ? kFewBlocks * 128 : 0);
+    if (hipError_t e = set_max_dynamic_lds_once(reinterpret_cast<const void *>(&few_rows_kernel<MT, RAW>), bytes))
         return e;
-    hipLaunchKernelGGL(few_rows_kernel<MT>,
+    hipLaunchKernelGGL((few_rows_kernel<MT, RAW>),
                        dim3((unsigned)((width + kFewColumns - 1) / kFewColumns), (unsigned)splits, (unsigned)((rows + 7) / 8)),
-                       dim3(1024), kFewLdsBytes, stream, tableI, x_codes, rows, Kb, kernel_blocks, width, acc);
+                       dim3(1024), bytes, stream, tableI, x_codes, in, rows, Kb, kernel_blocks, width, acc);
     return hipGetLastError();
 }
 
-hipError_t launch_few_rows(const uint16_t *tableI, const uint8_t *x_codes, int rows, int Kb, const uint8_t *kernel_blocks, int width,
-                           int splits, int32_t *acc, hipStream_t stream)
+hipError_t launch_few_rows(const uint16_t *tableI, const uint8_t *x_codes, const FewInput *raw, int rows, int Kb,
+                           const uint8_t *kernel_blocks, int width, int splits, int32_t *acc, hipStream_t stream)
 {
+    const FewInput in = raw ? *raw : FewInput{};
+#define AXC_FEW(MT)                                                                                                         \
+    return raw ? few_rows<MT, true>(tableI, x_codes, in, rows, Kb, kernel_blocks, width, splits, acc, stream)              \
+               : few_rows<MT, false>(tableI, x_codes, in, rows, Kb, kernel_blocks, width, splits, acc, stream)
     if (rows == 1)
-        return few_rows<1>(tableI, x_codes, rows, Kb, kernel_blocks, width, splits, acc, stream);
+        AXC_FEW(1);
     if (rows == 2)
-        return few_rows<2>(tableI, x_codes, rows, Kb, kernel_blocks, width, splits, acc, stream);
+        AXC_FEW(2);
     if (rows <= 4)
-        return few_rows<4>(tableI, x_codes, rows, Kb, kernel_blocks, width, splits, acc, stream);
-    return few_rows<8>(tableI, x_codes, rows, Kb, kernel_blocks, width, splits, acc, stream);
+        AXC_FEW(4);
+    AXC_FEW(8);
+#undef AXC_FEW
 }
 
 template <typename T, typename I>

@@ -17,33 +17,6 @@
 namespace axc {
 namespace {
 
-__device__ __forceinline__ void load4_any(const void *p, int64_t at, int64_t n, int type, float (&v)[4])
-{
-    if (type == AXC_F32) {
-        const float *const q = static_cast<const float *>(p) + at;
-        load_values<float, 4>(q, n, n >= 4 && ((uintptr_t)q & 15) == 0, 0.0f, v);
-    } else if (type == AXC_BF16) {
-        const bf16 *const q = static_cast<const bf16 *>(p) + at;
-        load_values<bf16, 4>(q, n, n >= 4 && ((uintptr_t)q & 7) == 0, 0.0f, v);
-    } else {
-        const f16 *const q = static_cast<const f16 *>(p) + at;
-        load_values<f16, 4>(q, n, n >= 4 && ((uintptr_t)q & 7) == 0, 0.0f, v);
-    }
-}
-__device__ __forceinline__ void store4_any(void *p, int64_t at, int64_t n, int type, const float (&v)[4])
-{
-    if (type == AXC_F32) {
-        float *const q = static_cast<float *>(p) + at;
-        store_values<float, 4>(q, n, n >= 4 && ((uintptr_t)q & 15) == 0, v);
-    } else if (type == AXC_BF16) {
-        bf16 *const q = static_cast<bf16 *>(p) + at;
-        store_values<bf16, 4>(q, n, n >= 4 && ((uintptr_t)q & 7) == 0, v);
-    } else {
-        f16 *const q = static_cast<f16 *>(p) + at;
-        store_values<f16, 4>(q, n, n >= 4 && ((uintptr_t)q & 7) == 0, v);
-    }
-}
-
 // Four neighbouring values as `parts` terms, `pitch` elements from one term to the next.
 __device__ __forceinline__ void store_terms(bf16 *p, int parts, int64_t pitch, float (&v)[4])
 {
@@ -151,10 +124,10 @@ __global__ void __launch_bounds__(256) grad_terms_kernel(GradSource g, int64_t f
                     for (int j = 0; j < 4; ++j)
                         v[j] = c + j < cols ? at(sum[j], l, column[j], bias[j], c + j) : 0.0f;
                 } else {
-                    load4_any(g.grad, r * ld + c, cols - c, g.type, v);
+                    load_four_any(g.grad, r * ld + c, cols - c, g.type, v);
                     if (g.pre) {
                         float z[4];
-                        load4_any(g.pre, r * ld + c, cols - c, g.type, z);
+                        load_four_any(g.pre, r * ld + c, cols - c, g.type, z);
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
                             if (c + j < cols)
@@ -208,7 +181,7 @@ __global__ void __launch_bounds__(256) centered_kernel(const void *values, int t
         const int64_t r = r0 + line + 16 * i, c = c0 + quad;
         float v[4] = {};
         if (r < rows && c < cols) {
-            load4_any(values, r * ld + c, cols - c, type, v);
+            load_four_any(values, r * ld + c, cols - c, type, v);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 v[j] = c + j < cols ? (float)((int)code_of(v[j], g) - g.zero) : 0.0f;
@@ -244,12 +217,12 @@ __device__ __forceinline__ void store_result(const ProductOut &o, int64_t r, int
 {
     const float scale = o.factor ? o.scale->scale * *o.factor : o.scale->scale;
     float at[4];
-    load4_any(o.values, r * o.values_ld + c, cols - c, o.values_type, at);
+    load_four_any(o.values, r * o.values_ld + c, cols - c, o.values_type, at);
     const Grid g = *o.grid;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
         v[j] = inside(at[j], g) ? v[j] * scale : 0.0f;
-    store4_any(o.out, r * o.ld + c, cols - c, o.type, v);
+    store_four_any(o.out, r * o.ld + c, cols - c, o.type, v);
 }
 
 constexpr int kStep = 64;   // of the depth

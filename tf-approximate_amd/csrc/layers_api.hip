@@ -89,7 +89,9 @@ Pieces pieces_of(int64_t depth, int64_t columns, int64_t most)
 // ---- sums of table entries: input codes by a piece of the kernel's ----
 constexpr int64_t kRowRun = 16384;       // rows a LUT-GEMM call takes (its rows must be below 32768)
 constexpr int64_t kSumsAtOnce = (int64_t)1 << 25;   // int32 sums in the workspace: 128 MiB, half the memory-side cache
-constexpr int64_t kFewRowsMost = 16;
+// Up to here few_rows_kernel is the shorter one, by rows (us, packed 4096 -> 4096: 16 rows 33, 63 by the kernels of many rows, 32 rows
+// 50 and 65, 64 rows 90 and 76; 4096 -> 14336, 16 rows 84 and 131, 32 rows 145 and 141).
+constexpr int64_t kFewRowsMost = 32;
 
 bool few_rows(int64_t rows) { return rows <= kFewRowsMost; }
 
@@ -136,6 +138,7 @@ struct Operands {
     float *x_pairs, *kernel_pairs;
     uint8_t *x_codes, *kernel_codes, *kernel_blocks;
     int32_t *row_sums, *column_sums;
+    const FewInput *raw;                 // not null: few_rows_kernel makes the input's codes itself
 };
 
 Operands carve_operands(Carver &c, const axc_dense_desc *d, const Pieces &pc, bool with_kernel, bool codes)
@@ -262,8 +265,8 @@ int table_sums(const axc_table *table, const axc_dense_desc *d, const Operands &
         const int splits = few_rows_splits(rows, pc.Kb, width);
         out->raw = {acc, rows * width, splits, width, 0};
         ApiTimer t("few_rows", stream);
-        AXC_HIP(launch_few_rows(table->dev_tableI, o.x_codes, (int)rows, pc.Kb, o.kernel_blocks + pc.block_offset(p), width, splits,
-                                acc, stream));
+        AXC_HIP(launch_few_rows(table->dev_tableI, o.x_codes, o.raw, (int)rows, pc.Kb, o.kernel_blocks + pc.block_offset(p), width,
+                                splits, acc, stream));
         return AXC_OK;
     }
     const axc_conv2d_desc c = conv_desc(fours(rows), pc.Kp, width);
@@ -414,13 +417,17 @@ int axc_fake_approx_dense(const axc_table *table, const axc_dense_desc *desc, co
     hipStream_t stream = static_cast<hipStream_t>(stream_v);
     const int K = (int)desc->depth;
     Operands &o = s.o;
+    FewInput raw = {};
     if (packed) {
         const Packed p = packed_parts(pc, const_cast<void *>(packed));
         o.kernel_codes = p.codes;
         o.kernel_blocks = p.blocks;
         o.column_sums = p.column_sums;
         if (few_rows(desc->rows)) {
-            if (int rc = make_few_codes(desc, input, input_range, &p.grids->kernel, o, pc, stream))
+            raw = {input, desc->input_type, K, input_source(desc, input_range), &p.grids->kernel, o.grids, o.row_sums};
+            if (desc->rows * desc->depth <= kFewRawValues || raw.range.count >= 0)
+                o.raw = &raw;
+            else if (int rc = make_few_codes(desc, input, input_range, &p.grids->kernel, o, pc, stream))
                 return rc;
         } else {
             RangeSource in, none;

@@ -74,6 +74,34 @@ __device__ __forceinline__ void store_values(T *p, int64_t n, bool whole, const 
             p[i] = (T)v[i];
 }
 
+// Four neighbouring values of a tensor whose type is only known at run time, as many of them as there are (n).
+__device__ __forceinline__ void load_four_any(const void *p, int64_t at, int64_t n, int type, float (&v)[4])
+{
+    if (type == AXC_F32) {
+        const float *const q = static_cast<const float *>(p) + at;
+        load_values<float, 4>(q, n, n >= 4 && ((uintptr_t)q & 15) == 0, 0.0f, v);
+    } else if (type == AXC_BF16) {
+        const bf16 *const q = static_cast<const bf16 *>(p) + at;
+        load_values<bf16, 4>(q, n, n >= 4 && ((uintptr_t)q & 7) == 0, 0.0f, v);
+    } else {
+        const f16 *const q = static_cast<const f16 *>(p) + at;
+        load_values<f16, 4>(q, n, n >= 4 && ((uintptr_t)q & 7) == 0, 0.0f, v);
+    }
+}
+__device__ __forceinline__ void store_four_any(void *p, int64_t at, int64_t n, int type, const float (&v)[4])
+{
+    if (type == AXC_F32) {
+        float *const q = static_cast<float *>(p) + at;
+        store_values<float, 4>(q, n, n >= 4 && ((uintptr_t)q & 15) == 0, v);
+    } else if (type == AXC_BF16) {
+        bf16 *const q = static_cast<bf16 *>(p) + at;
+        store_values<bf16, 4>(q, n, n >= 4 && ((uintptr_t)q & 7) == 0, v);
+    } else {
+        f16 *const q = static_cast<f16 *>(p) + at;
+        store_values<f16, 4>(q, n, n >= 4 && ((uintptr_t)q & 7) == 0, v);
+    }
+}
+
 // ---- the 8-bit grid of a tensor ----
 // What fake quantization with a range gives (Nudge, tf2/src/approx_ops_types.h:29-49): value = scale * (code - zero).
 struct Grid {
@@ -348,8 +376,19 @@ hipError_t launch_codes(const CodesJob &job, hipStream_t stream);
 hipError_t launch_few_codes(const void *x, int type, int rows, int K, int Kb, const RangeSource &src, const Grid *kernel_grid,
                             Grids *grids, uint8_t *codes, int32_t *row_sums, hipStream_t stream);
 int few_rows_splits(int64_t rows, int Kb, int width);
-hipError_t launch_few_rows(const uint16_t *tableI, const uint8_t *x_codes, int rows, int Kb, const uint8_t *kernel_blocks, int width,
-                           int splits, int32_t *acc, hipStream_t stream);
+struct FewInput {                        // for few_rows_kernel where it makes the codes of the input itself
+    const void *x;
+    int type, K;
+    RangeSource range;
+    const Grid *kernel_grid;
+    Grids *grids;
+    int32_t *row_sums;
+};
+// Where every workgroup may read all of the input for its range: beyond that a launch of its own is as short (us a call with and
+// without one, 4096 -> 4096: 1 row 17.8 and 14.4, 4 rows 19.4 and 18.1, 8 rows 25; 4096 -> 14336, 4 rows: 41.4 and 44.7).
+constexpr int64_t kFewRawValues = 8192;
+hipError_t launch_few_rows(const uint16_t *tableI, const uint8_t *x_codes, const FewInput *raw, int rows, int Kb,
+                           const uint8_t *kernel_blocks, int width, int splits, int32_t *acc, hipStream_t stream);
 struct DenseOut {
     const void *bias, *residual;         // of the piece's / run's first element
     void *out, *pre;

@@ -125,6 +125,19 @@ class FakeApproxDense:
         self.table = _table_of(mul_map_file, num_bits)
         self.activation = _ACTIVATIONS[activation]
         self.input_minmax = _minmax_of(input_minmax)
+        self._descs = {}
+
+    def _desc(self, inputs, depth, columns, kernel_dtype, bias):
+        """(description, reference to it) of a call: made once for its shapes and types."""
+        key = (inputs.shape, inputs.dtype, depth, columns, kernel_dtype, None if bias is None else bias.dtype)
+        found = self._descs.get(key)
+        if found is None:
+            desc = _dense_desc(inputs, depth, columns, kernel_dtype, bias, self.activation, self.input_minmax)
+            found = desc, ctypes.byref(desc), inputs.shape[:-1] + (columns,)
+            if len(self._descs) >= 256:
+                self._descs.clear()
+            self._descs[key] = found
+        return found
 
     def pack(self, kernel):
         """The kernel as codes, for calls with the same kernel."""
@@ -163,11 +176,9 @@ class FakeApproxDense:
             (depth, columns), kernel_dtype = kernel.shape, kernel.dtype
         if bias is not None:
             bias = _require(bias, "bias", device, shape=(columns,))
-        out_shape = inputs.shape[:-1] + (columns,)
+        _, ref, out_shape = self._desc(inputs, depth, columns, kernel_dtype, bias)
         if residual is not None:
             residual = _require(residual, "residual", device, inputs.dtype, out_shape)
-        desc = _dense_desc(inputs, depth, columns, kernel_dtype, bias, self.activation, self.input_minmax)
-        ref = ctypes.byref(desc)
         nbytes = ctypes.c_size_t()
         _check(lib.axc_fake_approx_dense_workspace_bytes(ref, packed, ctypes.byref(nbytes)))
         ws = _scratch(nbytes.value, device)
@@ -192,12 +203,10 @@ class FakeApproxDense:
         depth, columns = kernel.shape
         if not set(want) <= {"inputs", "kernel", "bias"}:
             raise InvalidArgumentError("want: 'inputs', 'kernel', 'bias'")
-        desc = _dense_desc(inputs, depth, columns, kernel.dtype, None, self.activation, self.input_minmax)
-        out_shape = inputs.shape[:-1] + (columns,)
+        _, ref, out_shape = self._desc(inputs, depth, columns, kernel.dtype, None)
         grad_output = _require(grad_output, "grad_output", device, inputs.dtype, out_shape)
         if pre is not None:
             pre = _require(pre, "pre", device, inputs.dtype, out_shape)
-        ref = ctypes.byref(desc)
         nbytes = ctypes.c_size_t()
         _check(lib.axc_fake_approx_dense_gradients_workspace_bytes(ref, ctypes.byref(nbytes)))
         ws = _scratch(nbytes.value, device)
