@@ -212,20 +212,51 @@ __global__ void __launch_bounds__(256) centered_kernel(const void *values, int t
     }
 }
 
-// Four results that the product or the pass over its partial sums has at (r, c).
-__device__ __forceinline__ void store_result(const ProductOut &o, int64_t r, int64_t c, int64_t cols, float (&v)[4])
-{
-    const float scale = o.factor ? o.scale->scale * *o.factor : o.scale->scale;
-    float at[4];
-    load_four_any(o.values, r * o.values_ld + c, cols - c, o.values_type, at);
-    const Grid g = *o.grid;
+// Results that the product or the pass over its partial sums has, of type T, as the values that decide where there is a gradient.
+template <typename T>
+struct Results {
+    typedef T four __attribute__((ext_vector_type(4)));
+    T *out;
+    const T *values;
+    int64_t ld, values_ld;
+    Grid grid;
+    float scale;
+    bool aligned;                        // every fourth column, in every row
+    __device__ __forceinline__ explicit Results(const ProductOut &o)
+        : out(static_cast<T *>(o.out)), values(static_cast<const T *>(o.values)), ld(o.ld), values_ld(o.values_ld), grid(*o.grid),
+          scale(o.factor ? o.scale->scale * *o.factor : o.scale->scale)
+    {
+        aligned = ((ld | values_ld) & 3) == 0 && (((uintptr_t)out | (uintptr_t)values) & (4 * sizeof(T) - 1)) == 0;
+    }
+    __device__ __forceinline__ four values_at(int64_t r, int64_t c) const
+    {
+        return *reinterpret_cast<const four *>(values + r * values_ld + c);
+    }
+    __device__ __forceinline__ void store(int64_t r, int64_t c, const four &at, const f32x4 &v) const
+    {
+        four t;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-        v[j] = inside(at[j], g) ? v[j] * scale : 0.0f;
-    store_four_any(o.out, r * o.ld + c, cols - c, o.type, v);
-}
+        for (int j = 0; j < 4; ++j)
+            t[j] = (T)(inside((float)at[j], grid) ? v[j] * scale : 0.0f);
+        *reinterpret_cast<four *>(out + r * ld + c) = t;
+    }
+    __device__ __forceinline__ void store_some(int64_t r, int64_t c, int64_t cols, const f32x4 &v) const
+    {
+        if (aligned && c + 4 <= cols) {
+            store(r, c, values_at(r, c), v);
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (c + j < cols)
+                out[r * ld + c + j] = (T)(inside((float)values[r * values_ld + c + j], grid) ? v[j] * scale : 0.0f);
+    }
+};
 
 constexpr int kStep = 64;   // of the depth
+constexpr int kGroups = 2;  // of four wavefronts, which take the steps in turn
+constexpr int kProductThreads = kGroups * 256;
+constexpr int kProductLds = kGroups * 2 * 2 * kProductTile * kStep * 2;
 
 __device__ __forceinline__ void load_to_lds(const bf16 *from, bf16 *to)
 {
@@ -234,17 +265,20 @@ __device__ __forceinline__ void load_to_lds(const bf16 *from, bf16 *to)
                                      (__attribute__((address_space(3))) uint32_t *)to, 16, 0, 0);
 }
 
-// A tile of 128 x 128 by four wavefronts, 64 x 64 each; two buffers of 64 of the depth in LDS, filled straight from memory while
-// the other is multiplied.  In LDS a line of 64 elements is eight chunks of 16 bytes, chunk q of line r in place q ^ (r & 7): the
-// 16 lanes that read neighbouring lines then meet different banks.  The loads write LDS in order, so it is their addresses that
-// are exchanged.  PARTIAL: sums go to `partials` (added to what is there with `accumulate`).
-template <bool PARTIAL>
-__global__ void __launch_bounds__(256, 2) product_kernel(const bf16 *__restrict__ a, const bf16 *__restrict__ b, int64_t rows,
+// A tile of 128 x 128 by two groups of four wavefronts, each of which multiplies every other step of the depth, 64 x 64 a wavefront,
+// and has two buffers of 64 of the depth in LDS, filled straight from memory while the other is multiplied: two wavefronts a SIMD, so
+// that one reads while the other multiplies, where there are no more tiles than CUs.  At the end the groups exchange half of their
+// sums each.
+// In LDS a line of 64 elements is eight chunks of 16 bytes, chunk q of line r in place q ^ (r & 7): the 16 lanes that read
+// neighbouring lines then meet different banks.  The loads write LDS in order, so it is their addresses that are exchanged.
+// PARTIAL: sums go to `partials` (added to what is there with `accumulate`).
+template <typename T, bool PARTIAL>
+__global__ void __launch_bounds__(kProductThreads) product_kernel(const bf16 *__restrict__ a, const bf16 *__restrict__ b, int64_t rows,
                                                          int64_t cols, int row_tiles, int col_tiles, int depth, int parts,
                                                          int split_a, int splits, float *__restrict__ partials, int accumulate,
                                                          ProductOut o)
 {
-    __shared__ __align__(16) bf16 lds[2][2][kProductTile * kStep];
+    extern __shared__ __align__(16) bf16 lds_raw[];
     // Workgroups go round the eight XCDs; each XCD gets a run of neighbouring tiles, in bands of eight row tiles, so that its L2
     // serves them.
     const int tiles = row_tiles * col_tiles * splits;
@@ -259,7 +293,8 @@ __global__ void __launch_bounds__(256, 2) product_kernel(const bf16 *__restrict_
     const int band_rows = row_tiles - band * 8 < 8 ? row_tiles - band * 8 : 8;
     const int row_tile = band * 8 + in_band % band_rows, col_tile = in_band / band_rows;
 
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int lane = threadIdx.x & 63, wave8 = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wave = wave8 & 3, part = wave8 >> 2;
+    bf16(*const lds)[2][kProductTile * kStep] = reinterpret_cast<bf16(*)[2][kProductTile * kStep]>(lds_raw) + part * 2;
     const int per_part = depth / kStep, steps = per_part * parts;
     const int first = (int)((int64_t)steps * split / splits), last = (int)((int64_t)steps * (split + 1) / splits);
     const int64_t lda = split_a ? (int64_t)depth * parts : depth, ldb = split_a ? depth : (int64_t)depth * parts;
@@ -279,16 +314,18 @@ __global__ void __launch_bounds__(256, 2) product_kernel(const bf16 *__restrict_
 
     f32x4 acc[4][4] = {};
     const int wr = (wave >> 1) * 64, wc = (wave & 1) * 64, in_line = lane & 15, group = lane >> 4;
-    if (first < last)
-        fetch(first, 0);
-    for (int step = first; step < last; ++step) {
-        const int buffer = (step - first) & 1;
-        // This buffer is full, by all wavefronts' loads (a barrier alone does not wait for loads into LDS), and the other is no
-        // longer read.
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (step + 1 < last)
-            fetch(step + 1, buffer ^ 1);
+    const int rounds = (last - first + kGroups - 1) / kGroups;
+    if (first + part < last)
+        fetch(first + part, 0);
+    for (int round = 0; round < rounds; ++round) {
+        const int step = first + round * kGroups + part, buffer = round & 1;
+        // This buffer is full once the loads of all of its wavefronts have come (a barrier alone does not wait for loads into LDS), and
+        // nobody reads the other any more.
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (step + kGroups < last)
+            fetch(step + kGroups, buffer ^ 1);
+        if (step >= last)
+            continue;
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
             bf16x8 fa[4], fb[4];
@@ -305,37 +342,83 @@ __global__ void __launch_bounds__(256, 2) product_kernel(const bf16 *__restrict_
                     acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j], fa[i], acc[i][j], 0, 0, 0);
         }
     }
-    const int64_t rows_pad = (int64_t)row_tiles * kProductTile, cols_pad = (int64_t)col_tiles * kProductTile;
+    // the other group's half of the sums for this one's: rows 0 and 1 of four for the first group
+    f32x4 *const give = reinterpret_cast<f32x4 *>(lds_raw) + (wave * 8) * 64 + lane;   // [wavefront][8][64], twice
+    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int64_t r = (int64_t)row_tile * kProductTile + wr + i * 16 + in_line;
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t c = (int64_t)col_tile * kProductTile + wc + j * 16 + group * 4;
-            if constexpr (PARTIAL) {
-                f32x4 *const to = reinterpret_cast<f32x4 *>(partials + ((int64_t)split * rows_pad + r) * cols_pad + c);
-                *to = accumulate ? *to + acc[i][j] : acc[i][j];
-            } else if (r < rows && c < cols) {
-                float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-                store_result(o, r, c, cols, v);
-            }
+        for (int j = 0; j < 4; ++j)
+            give[part * 2048 + (i * 4 + j) * 64] = part == 0 ? acc[i + 2][j] : acc[i][j];
+    __syncthreads();
+    f32x4 sum[2][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            sum[i][j] = (part == 0 ? acc[i][j] : acc[i + 2][j]) + give[(1 - part) * 2048 + (i * 4 + j) * 64];
+    // What is read for the results is read all at once, where the tile has no edge: value by value it took as long as the product.
+    const int64_t r0 = (int64_t)row_tile * kProductTile + wr + part * 32 + in_line, c0 = (int64_t)col_tile * kProductTile + wc + group * 4;
+    if constexpr (PARTIAL) {
+        const int64_t rows_pad = (int64_t)row_tiles * kProductTile, cols_pad = (int64_t)col_tiles * kProductTile;
+        float *const to = partials + ((int64_t)split * rows_pad + r0) * cols_pad + c0;
+        if (accumulate) {
+            f32x4 was[2][4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    was[i][j] = *reinterpret_cast<const f32x4 *>(to + i * 16 * cols_pad + j * 16);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    sum[i][j] += was[i][j];
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<f32x4 *>(to + i * 16 * cols_pad + j * 16) = sum[i][j];
+    } else {
+        const Results<T> results(o);
+        if (results.aligned && (int64_t)(row_tile + 1) * kProductTile <= rows && (int64_t)(col_tile + 1) * kProductTile <= cols) {
+            typename Results<T>::four at[2][4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    at[i][j] = results.values_at(r0 + i * 16, c0 + j * 16);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    results.store(r0 + i * 16, c0 + j * 16, at[i][j], sum[i][j]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (r0 + i * 16 < rows && c0 + j * 16 < cols)
+                        results.store_some(r0 + i * 16, c0 + j * 16, cols, sum[i][j]);
         }
     }
 }
 
+template <typename T>
 __global__ void __launch_bounds__(256) product_out_kernel(const float *__restrict__ partials, int splits, int64_t rows, int64_t cols,
                                                           int64_t rows_pad, int64_t cols_pad, ProductOut o)
 {
     const int64_t c = ((int64_t)blockIdx.x * 64 + (threadIdx.x & 63)) * 4;
     if (c >= cols)
         return;
+    const Results<T> results(o);
     for (int64_t r = (int64_t)blockIdx.y * 4 + threadIdx.x / 64; r < rows; r += (int64_t)gridDim.y * 4) {
         f32x4 sum = {};
-#pragma unroll 4
+#pragma unroll 8
         for (int s = 0; s < splits; ++s)
             sum += *reinterpret_cast<const f32x4 *>(partials + ((int64_t)s * rows_pad + r) * cols_pad + c);
-        float v[4] = {sum[0], sum[1], sum[2], sum[3]};
-        store_result(o, r, c, cols, v);
+        results.store_some(r, c, cols, sum);
     }
 }
 
@@ -410,30 +493,49 @@ ProductPlan plan_product(int64_t rows, int64_t cols, int64_t depth_pad, int part
     return plan;
 }
 
+template <typename T, bool PARTIAL>
+static hipError_t product(const bf16 *a, const bf16 *b, int64_t rows, int64_t cols, int64_t depth_pad, int parts, bool split_a,
+                          int splits, float *partials, bool accumulate, const ProductOut &o, hipStream_t stream)
+{
+    const int row_tiles = (int)(product_pad(rows) / kProductTile), col_tiles = (int)(product_pad(cols) / kProductTile);
+    if (hipError_t e = set_max_dynamic_lds_once(reinterpret_cast<const void *>(&product_kernel<T, PARTIAL>), kProductLds))
+        return e;
+    hipLaunchKernelGGL((product_kernel<T, PARTIAL>), dim3((unsigned)((int64_t)row_tiles * col_tiles * splits)), dim3(kProductThreads),
+                       kProductLds,
+                       stream, a, b, rows, cols, row_tiles, col_tiles, (int)depth_pad, parts, (int)split_a, splits, partials,
+                       (int)accumulate, o);
+    return hipGetLastError();
+}
+
 hipError_t launch_product(const bf16 *a, const bf16 *b, int64_t rows, int64_t cols, int64_t depth_pad, int parts, bool split_a,
                           const ProductPlan &plan, float *partials, bool keep, bool accumulate, const ProductOut &o,
                           hipStream_t stream)
 {
-    const int row_tiles = (int)(product_pad(rows) / kProductTile), col_tiles = (int)(product_pad(cols) / kProductTile);
-    const dim3 grid((unsigned)((int64_t)row_tiles * col_tiles * plan.splits));
     if (plan.splits > 1 || keep) {
-        hipLaunchKernelGGL(product_kernel<true>, grid, dim3(256), 0, stream, a, b, rows, cols, row_tiles, col_tiles, (int)depth_pad,
-                           parts, (int)split_a, plan.splits, partials, (int)accumulate, o);
-        if (hipError_t e = hipGetLastError())
+        if (hipError_t e = product<float, true>(a, b, rows, cols, depth_pad, parts, split_a, plan.splits, partials, accumulate, o,
+                                                stream))
             return e;
         return keep ? hipSuccess : launch_product_out(partials, plan.splits, rows, cols, o, stream);
     }
-    hipLaunchKernelGGL(product_kernel<false>, grid, dim3(256), 0, stream, a, b, rows, cols, row_tiles, col_tiles, (int)depth_pad,
-                       parts, (int)split_a, 1, partials, 0, o);
-    return hipGetLastError();
+    if (o.type == AXC_F32)
+        return product<float, false>(a, b, rows, cols, depth_pad, parts, split_a, 1, nullptr, false, o, stream);
+    if (o.type == AXC_BF16)
+        return product<bf16, false>(a, b, rows, cols, depth_pad, parts, split_a, 1, nullptr, false, o, stream);
+    return product<f16, false>(a, b, rows, cols, depth_pad, parts, split_a, 1, nullptr, false, o, stream);
 }
 
 hipError_t launch_product_out(const float *partials, int splits, int64_t rows, int64_t cols, const ProductOut &o,
                               hipStream_t stream)
 {
     const int64_t by = (rows + 3) / 4;
-    hipLaunchKernelGGL(product_out_kernel, dim3((unsigned)((cols + 255) / 256), (unsigned)(by > 16384 ? 16384 : by)), dim3(256), 0,
-                       stream, partials, splits, rows, cols, product_pad(rows), product_pad(cols), o);
+    const dim3 grid((unsigned)((cols + 255) / 256), (unsigned)(by > 16384 ? 16384 : by));
+    const int64_t rows_pad = product_pad(rows), cols_pad = product_pad(cols);
+    if (o.type == AXC_F32)
+        hipLaunchKernelGGL(product_out_kernel<float>, grid, dim3(256), 0, stream, partials, splits, rows, cols, rows_pad, cols_pad, o);
+    else if (o.type == AXC_BF16)
+        hipLaunchKernelGGL(product_out_kernel<bf16>, grid, dim3(256), 0, stream, partials, splits, rows, cols, rows_pad, cols_pad, o);
+    else
+        hipLaunchKernelGGL(product_out_kernel<f16>, grid, dim3(256), 0, stream, partials, splits, rows, cols, rows_pad, cols_pad, o);
     return hipGetLastError();
 }
 

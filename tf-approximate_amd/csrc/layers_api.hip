@@ -548,7 +548,7 @@ int axc_fake_approx_dense_gradients(const axc_dense_desc *desc, const void *grad
             ApiTimer t("centered", stream);
             AXC_HIP(launch_centered(kernel, desc->kernel_type, K, N, N, &s.o.grids->kernel, false, s.kernel, stream));
         }
-        const ProductOut o = {grad_input, desc->input_type, K, input, desc->input_type, K, &s.o.grids->in, &s.o.grids->kernel,
+        const ProductOut o = {grad_input, desc->input_type, K, input, K, &s.o.grids->in, &s.o.grids->kernel,
                               nullptr};
         ApiTimer t("grad_product", stream);
         AXC_HIP(launch_product(s.straight, s.kernel, rows, K, product_pad(N), px, true, plan_product(rows, K, product_pad(N), px, false),
@@ -559,7 +559,7 @@ int axc_fake_approx_dense_gradients(const axc_dense_desc *desc, const void *grad
             ApiTimer t("centered", stream);
             AXC_HIP(launch_centered(input, desc->input_type, rows, K, K, &s.o.grids->in, true, s.x_turned, stream));
         }
-        const ProductOut o = {grad_kernel, desc->kernel_type, N, kernel, desc->kernel_type, N, &s.o.grids->kernel, &s.o.grids->in,
+        const ProductOut o = {grad_kernel, desc->kernel_type, N, kernel, N, &s.o.grids->kernel, &s.o.grids->in,
                               nullptr};
         ApiTimer t("grad_product", stream);
         AXC_HIP(launch_product(s.x_turned, s.turned, K, N, product_pad(rows), pk, false,
@@ -712,7 +712,7 @@ int axc_fake_approx_cross_entropy(const axc_table *table, const axc_dense_desc *
         AXC_HIP(launch_centered(input, desc->input_type, rows, K, K, &o.grids->in, true, s.x_turned, stream));
     }
     const ProductPlan input_plan = plan_product(rows, K, product_pad(pc.width), px, true);
-    const ProductOut input_out = {grad_input, desc->input_type, K, input, desc->input_type, K, &o.grids->in, &o.grids->kernel,
+    const ProductOut input_out = {grad_input, desc->input_type, K, input, K, &o.grids->in, &o.grids->kernel,
                                   s.st.factor};
     // from the last piece on, whose last run's sums are still there
     bool made = true;
@@ -752,7 +752,7 @@ int axc_fake_approx_cross_entropy(const axc_table *table, const axc_dense_desc *
         }
         if (grad_kernel) {
             const ProductOut out = {element(grad_kernel, c, desc->kernel_type), desc->kernel_type, V,
-                                    element(kernel, c, desc->kernel_type), desc->kernel_type, V, &o.grids->kernel, &o.grids->in,
+                                    element(kernel, c, desc->kernel_type), V, &o.grids->kernel, &o.grids->in,
                                     s.st.factor};
             ApiTimer t("grad_product", stream);
             AXC_HIP(launch_product(s.x_turned, s.turned, K, n, M, pk, false, plan_product(K, n, M, pk, false), s.kernel_partials,

@@ -424,11 +424,10 @@ hipError_t launch_grad_terms(const GradSource &of_run, bool loss, int64_t first,
 hipError_t launch_centered(const void *v, int type, int64_t rows, int64_t cols, int64_t ld, const Grid *grid, bool turn, bf16 *out,
                            hipStream_t stream);
 struct ProductOut {
-    void *out;                           // rows x cols, leading dimension ld; null: partial sums only
+    void *out;                           // rows x cols, leading dimension ld
     int type;
     int64_t ld;
-    const void *values;                  // like out: those outside `grid` get 0
-    int values_type;
+    const void *values;                  // like out, of its type: where they are outside `grid`, out gets 0
     int64_t values_ld;
     const Grid *grid, *scale;            // scale->scale times the sums
     const float *factor;                 // not null: times *factor
