@@ -72,38 +72,6 @@ __global__ void __launch_bounds__(1024) range_kernel(const void *x, int x_type, 
     }
 }
 
-__device__ void fold(const RangeSource &src, float &lo, float &hi, float *red)
-{
-    lo = src.lo;
-    hi = src.hi;
-    if (src.pairs) {
-        lo = INFINITY;
-        hi = -INFINITY;
-        for (int i = threadIdx.x; i < src.count; i += blockDim.x) {
-            const float2 p = reinterpret_cast<const float2 *>(src.pairs)[i];
-            lo = fminf(lo, p.x);
-            hi = fmaxf(hi, p.y);
-        }
-        block_range(lo, hi, red);
-    }
-}
-
-__global__ void __launch_bounds__(256) grids_kernel(RangeSource in, RangeSource kernel, int has_in, int has_kernel, Grids *grids)
-{
-    __shared__ float red[8];
-    float lo, hi;
-    if (has_in) {
-        fold(in, lo, hi, red);
-        if (threadIdx.x == 0)
-            grids->in = grid_of_range(lo, hi);
-    }
-    if (has_kernel) {
-        fold(kernel, lo, hi, red);
-        if (threadIdx.x == 0)
-            grids->kernel = grid_of_range(lo, hi);
-    }
-}
-
 // ---- codes ----
 // Codes of one row by a group of `threads` threads, and this thread's part of their sum.  Behind the depth come pad codes, 0.
 template <typename T>
@@ -584,25 +552,28 @@ __global__ void __launch_bounds__(256) dense_out_parts_kernel(TableSums s, int c
                      whole_fours<T>(c, columns, o), o);
 }
 
-// Turned sums: 64 rows by 64 columns through LDS.
-template <typename T, typename I>
+// Turned sums: 64 rows by CT columns through LDS.
+template <typename T, typename I, int CT>
 __global__ void __launch_bounds__(256) dense_out_turned_kernel(TableSums s, int64_t rows, int columns, DenseOut o)
 {
-    __shared__ int32_t tile[64][65];
-    const int quad = (threadIdx.x & 15) * 4, line = threadIdx.x / 16;
-    const int c0 = (int)blockIdx.x * 64;
+    __shared__ int32_t tile[64][CT + 1];
+    const int c0 = (int)blockIdx.x * CT;
     const int64_t r0 = (int64_t)blockIdx.y * 64;
+    {
+        const int quad = (threadIdx.x & 15) * 4, line = threadIdx.x / 16;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int c = c0 + line + 16 * i;
-        if (c < columns && r0 + quad < rows) {
-            const i32x4 t = four_sums(s.raw, r0 + quad, c);
+        for (int i = 0; i < CT / 16; ++i) {
+            const int c = c0 + line + 16 * i;
+            if (c < columns && r0 + quad < rows) {
+                const i32x4 t = four_sums(s.raw, r0 + quad, c);
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                tile[quad + j][line + 16 * i] = t[j];
+                for (int j = 0; j < 4; ++j)
+                    tile[quad + j][line + 16 * i] = t[j];
+            }
         }
     }
     __syncthreads();
+    const int quad = (int)threadIdx.x % (CT / 4) * 4, line = (int)threadIdx.x / (CT / 4);
     const int c = c0 + quad;
     if (c >= columns)
         return;
@@ -613,8 +584,8 @@ __global__ void __launch_bounds__(256) dense_out_turned_kernel(TableSums s, int6
     float bias[4];
     column_terms(s, b, c, columns, o, column, bias);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int at = line + 16 * i;
+    for (int i = 0; i < CT / 16; ++i) {
+        const int at = line + 1024 / CT * i;
         if (r0 + at < rows) {
             const int32_t sum[4] = {tile[at][quad], tile[at][quad + 1], tile[at][quad + 2], tile[at][quad + 3]};
             dense_four<T, I>(sum, b.row(s.row_sums[r0 + at]), column, bias, scale, r0 + at, c, columns, whole, o);
@@ -654,13 +625,6 @@ hipError_t launch_range(const void *x, int x_type, int64_t nx, const void *kerne
         return hipSuccess;
     hipLaunchKernelGGL(range_kernel, dim3(total), dim3(1024), 0, stream, x, x_type, nx, bx, kernel, kernel_type, nk, x_pairs,
                        kernel_pairs, zeros, n_zeros);
-    return hipGetLastError();
-}
-
-hipError_t launch_grids(const RangeSource &in, const RangeSource &kernel, bool has_in, bool has_kernel, Grids *grids,
-                        hipStream_t stream)
-{
-    hipLaunchKernelGGL(grids_kernel, dim3(1), dim3(256), 0, stream, in, kernel, (int)has_in, (int)has_kernel, grids);
     return hipGetLastError();
 }
 
@@ -731,8 +695,14 @@ template <typename T, typename I>
 static hipError_t dense_out(const TableSums &s, int64_t rows, int columns, const DenseOut &o, hipStream_t stream)
 {
     if (s.raw.turned) {
-        hipLaunchKernelGGL((dense_out_turned_kernel<T, I>), dim3((unsigned)((columns + 63) / 64), (unsigned)((rows + 63) / 64)),
-                           dim3(256), 0, stream, s, rows, columns, o);
+        // tiles of fewer columns where those of 64 would leave CUs without work
+        const unsigned by = (unsigned)((rows + 63) / 64);
+        if ((int64_t)by * ((columns + 63) / 64) >= 1024)
+            hipLaunchKernelGGL((dense_out_turned_kernel<T, I, 64>), dim3((unsigned)((columns + 63) / 64), by), dim3(256), 0, stream, s,
+                               rows, columns, o);
+        else
+            hipLaunchKernelGGL((dense_out_turned_kernel<T, I, 16>), dim3((unsigned)((columns + 15) / 16), by), dim3(256), 0, stream, s,
+                               rows, columns, o);
     } else if (s.raw.splits >= 8 && rows <= 64) {
         hipLaunchKernelGGL((dense_out_parts_kernel<T, I>), dim3((unsigned)((columns + 255) / 256), (unsigned)rows), dim3(256), 0,
                            stream, s, columns, o);

@@ -66,14 +66,13 @@ struct LogitTerms {
 // Gradient in front of the product, 64 x 64 of it a workgroup: into LDS, and from there out straight, turned, and summed by columns.
 // SOURCE 0: dense; 1: logits' sums by rows, 2: turned.  `first`: the run's first row, in units of 64.
 template <int SOURCE, typename I>
-__global__ void __launch_bounds__(256) grad_terms_kernel(GradSource g, int64_t first, int64_t rows, int64_t rows_pad, int64_t cols,
-                                                         int64_t ld, int straight_parts, bf16 *__restrict__ straight,
-                                                         int turned_parts, bf16 *__restrict__ turned,
-                                                         float *__restrict__ column_partials)
+__device__ __forceinline__ void terms_tile(const GradSource &g, int tile_row, int tile_col, int64_t first, int64_t rows,
+                                           int64_t rows_pad, int64_t cols, int64_t ld, int straight_parts,
+                                           bf16 *__restrict__ straight, int turned_parts, bf16 *__restrict__ turned,
+                                           float *__restrict__ column_partials, float (&tile)[64][65])
 {
-    __shared__ float tile[64][65];
-    const int64_t r0 = (int64_t)blockIdx.y * 64, c0 = (int64_t)blockIdx.x * 64;
-    const int64_t cols_pad = (int64_t)gridDim.x * 64;
+    const int64_t r0 = (int64_t)tile_row * 64, c0 = (int64_t)tile_col * 64;
+    const int64_t cols_pad = product_pad(cols);
     const int quad = (threadIdx.x & 15) * 4, line = threadIdx.x / 16;
     if constexpr (SOURCE == 2) {         // a thread four rows of a column
         const LogitTerms<I> at(g);
@@ -163,28 +162,26 @@ __global__ void __launch_bounds__(256) grad_terms_kernel(GradSource g, int64_t f
         float sum = 0.0f;
         for (int i = 0; i < 64; ++i)
             sum += tile[i][threadIdx.x];
-        column_partials[(first + blockIdx.y) * cols_pad + c0 + threadIdx.x] = sum;
+        column_partials[(first + tile_row) * cols_pad + c0 + threadIdx.x] = sum;
     }
 }
 
-// Codes minus zero point of a tensor, straight or turned, 64 x 64 a workgroup; pads are zeros.
+// Codes minus zero point of a tensor, straight or turned, a tile of 64 x 64; pads are zeros.
 template <bool TURN>
-__global__ void __launch_bounds__(256) centered_kernel(const void *values, int type, int64_t rows, int64_t cols, int64_t ld,
-                                                       const Grid *grid, bf16 *__restrict__ out)
+__device__ __forceinline__ void centered_tile(const CenteredJob &job, const Grid &g, int tile_row, int tile_col, float (&tile)[64][65])
 {
-    __shared__ float tile[TURN ? 64 : 1][65];
-    const int64_t r0 = (int64_t)blockIdx.y * 64, c0 = (int64_t)blockIdx.x * 64;
+    const int64_t r0 = (int64_t)tile_row * 64, c0 = (int64_t)tile_col * 64;
+    const int64_t rows_pad = product_pad(job.rows), cols_pad = product_pad(job.cols);
     const int quad = (threadIdx.x & 15) * 4, line = threadIdx.x / 16;
-    const Grid g = *grid;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int64_t r = r0 + line + 16 * i, c = c0 + quad;
         float v[4] = {};
-        if (r < rows && c < cols) {
-            load_four_any(values, r * ld + c, cols - c, type, v);
+        if (r < job.rows && c < job.cols) {
+            load_four_any(job.values, r * job.ld + c, job.cols - c, job.type, v);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                v[j] = c + j < cols ? (float)((int)code_of(v[j], g) - g.zero) : 0.0f;
+                v[j] = c + j < job.cols ? (float)((int)code_of(v[j], g) - g.zero) : 0.0f;
         }
         if constexpr (TURN) {
 #pragma unroll
@@ -195,7 +192,7 @@ __global__ void __launch_bounds__(256) centered_kernel(const void *values, int t
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 b[j] = (bf16)v[j];
-            *reinterpret_cast<bf16x4 *>(out + r * ((int64_t)gridDim.x * 64) + c) = b;
+            *reinterpret_cast<bf16x4 *>(job.out + r * cols_pad + c) = b;
         }
     }
     if constexpr (TURN) {
@@ -207,9 +204,53 @@ __global__ void __launch_bounds__(256) centered_kernel(const void *values, int t
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 b[j] = (bf16)tile[quad + j][col];
-            *reinterpret_cast<bf16x4 *>(out + (c0 + col) * ((int64_t)gridDim.y * 64) + r0 + quad) = b;
+            *reinterpret_cast<bf16x4 *>(job.out + (c0 + col) * rows_pad + r0 + quad) = b;
         }
     }
+}
+
+__device__ __forceinline__ Grid own_grid(const RangeSource &range, float *ends)
+{
+    float lo, hi;
+    fold(range, lo, hi, ends);
+    return grid_of_range(lo, hi);
+}
+
+// Everything that stands in front of the products, in one launch: the gradient's tiles (in lines of term_cols), then those of the
+// input's codes and of the kernel's.  With `ranges` the workgroups of codes make their grids out of the ranges' pairs themselves, and
+// the first of all of them both for the launches behind.
+template <int SOURCE, typename I>
+__global__ void __launch_bounds__(256) grad_prep_kernel(GradSource g, int term_rows, int term_cols, int64_t first, int64_t rows,
+                                                        int64_t rows_pad, int64_t cols, int64_t ld, int straight_parts,
+                                                        bf16 *__restrict__ straight, int turned_parts, bf16 *__restrict__ turned,
+                                                        float *__restrict__ column_partials, CenteredJob x, int x_rows, int x_cols,
+                                                        CenteredJob k, int k_cols, RangeSource x_range, RangeSource k_range, int ranges,
+                                                        Grids *grids)
+{
+    __shared__ float tile[64][65];
+    __shared__ float ends[8];
+    int block = (int)blockIdx.x;
+    if (ranges && block == 0) {
+        const Grid in = own_grid(x_range, ends), kernel = own_grid(k_range, ends);
+        if (threadIdx.x == 0) {
+            grids->in = in;
+            grids->kernel = kernel;
+        }
+    }
+    if (block < term_rows * term_cols) {
+        terms_tile<SOURCE, I>(g, block / term_cols, block % term_cols, first, rows, rows_pad, cols, ld, straight_parts, straight,
+                              turned_parts, turned, column_partials, tile);
+        return;
+    }
+    block -= term_rows * term_cols;
+    if (block < x_rows * x_cols) {
+        const Grid of = ranges ? own_grid(x_range, ends) : grids->in;
+        centered_tile<true>(x, of, block / x_cols, block % x_cols, tile);
+        return;
+    }
+    block -= x_rows * x_cols;
+    const Grid of = ranges ? own_grid(k_range, ends) : grids->kernel;
+    centered_tile<false>(k, of, block / k_cols, block % k_cols, tile);
 }
 
 // Results that the product or the pass over its partial sums has, of type T, as the values that decide where there is a gradient.
@@ -265,24 +306,53 @@ __device__ __forceinline__ void load_to_lds(const bf16 *from, bf16 *to)
                                      (__attribute__((address_space(3))) uint32_t *)to, 16, 0, 0);
 }
 
+// Sums of the column partials, 64 columns a workgroup, in one order.
+__device__ void column_sums(const ColumnJob &job, int block, float *red)
+{
+    const int column = threadIdx.x & 63, line = threadIdx.x / 64, lines = blockDim.x / 64;
+    const int64_t c = (int64_t)block * 64 + column;
+    float sum = 0.0f;
+    if (c < job.cols)
+#pragma unroll 8
+        for (int64_t i = line; i < job.count; i += lines)
+            sum += job.partials[i * job.pitch + c];
+    red[line * 64 + column] = sum;
+    __syncthreads();
+    if (line == 0 && c < job.cols) {
+        sum = 0.0f;
+        for (int i = 0; i < lines; ++i)
+            sum += red[i * 64 + column];
+        store_any(job.out, c, job.type, job.factor ? sum * *job.factor : sum);
+    }
+}
+__global__ void __launch_bounds__(512) column_sums_kernel(ColumnJob job)
+{
+    __shared__ float red[512];
+    column_sums(job, (int)blockIdx.x, red);
+}
+
 // A tile of 128 x 128 by two groups of four wavefronts, each of which multiplies every other step of the depth, 64 x 64 a wavefront,
 // and has two buffers of 64 of the depth in LDS, filled straight from memory while the other is multiplied: two wavefronts a SIMD, so
 // that one reads while the other multiplies, where there are no more tiles than CUs.  At the end the groups exchange half of their
 // sums each.
 // In LDS a line of 64 elements is eight chunks of 16 bytes, chunk q of line r in place q ^ (r & 7): the 16 lanes that read
 // neighbouring lines then meet different banks.  The loads write LDS in order, so it is their addresses that are exchanged.
-// PARTIAL: sums go to `partials` (added to what is there with `accumulate`).
+// PARTIAL: sums go to `partials` (added to what is there with `accumulate`).  Workgroups behind the tiles add up the columns of `job`.
 template <typename T, bool PARTIAL>
 __global__ void __launch_bounds__(kProductThreads) product_kernel(const bf16 *__restrict__ a, const bf16 *__restrict__ b, int64_t rows,
                                                          int64_t cols, int row_tiles, int col_tiles, int depth, int parts,
                                                          int split_a, int splits, float *__restrict__ partials, int accumulate,
-                                                         ProductOut o)
+                                                         ProductOut o, ColumnJob job)
 {
     extern __shared__ __align__(16) bf16 lds_raw[];
     // Workgroups go round the eight XCDs; each XCD gets a run of neighbouring tiles, in bands of eight row tiles, so that its L2
     // serves them.
     const int tiles = row_tiles * col_tiles * splits;
     int id = (int)blockIdx.x;
+    if (id >= tiles) {
+        column_sums(job, id - tiles, reinterpret_cast<float *>(lds_raw));
+        return;
+    }
     {
         const int per = tiles / 8, more = tiles % 8, xcd = id % 8;
         id = xcd * per + (xcd < more ? xcd : more) + id / 8;
@@ -422,59 +492,40 @@ __global__ void __launch_bounds__(256) product_out_kernel(const float *__restric
     }
 }
 
-// Sums of the column partials, 64 columns a workgroup, in one order.
-__global__ void __launch_bounds__(256) column_sums_kernel(const float *__restrict__ partials, int64_t count, int64_t cols,
-                                                          int64_t pitch, const float *factor, void *out, int type)
-{
-    __shared__ float red[4][64];
-    const int64_t c = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
-    float sum = 0.0f;
-    if (c < cols)
-        for (int64_t i = threadIdx.x / 64; i < count; i += 4)
-            sum += partials[i * pitch + c];
-    red[threadIdx.x / 64][threadIdx.x & 63] = sum;
-    __syncthreads();
-    if (threadIdx.x < 64 && c < cols)
-        store_any(out, c, type, ((red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x])) *
-                                    (factor ? *factor : 1.0f));
-}
-
 } // namespace
 
-hipError_t launch_grad_terms(const GradSource &of_run, bool loss, int64_t first, int64_t run_rows, int64_t rows, int64_t cols,
-                             int64_t ld, int straight_parts, bf16 *straight, int turned_parts, bf16 *turned, float *column_partials,
-                             hipStream_t stream)
+hipError_t launch_grad_prep(const GradSource &of_run, bool loss, int64_t first, int64_t run_rows, int64_t rows, int64_t cols,
+                            int64_t ld, int straight_parts, bf16 *straight, int turned_parts, bf16 *turned, float *column_partials,
+                            const CenteredJob &x, const CenteredJob &kernel, const RangeSource *ranges, Grids *grids,
+                            hipStream_t stream)
 {
     const int64_t rows_pad = product_pad(rows);
     // the last run makes the pad rows too
     const int64_t high = first + run_rows < rows ? run_rows : rows_pad - first;
-    const dim3 grid((unsigned)(product_pad(cols) / 64), (unsigned)(high / 64));
-#define AXC_TERMS(SOURCE, I)                                                                                                       \
-    hipLaunchKernelGGL((grad_terms_kernel<SOURCE, I>), grid, dim3(256), 0, stream, of_run, first / 64, run_rows, rows_pad, cols, ld, \
-                       straight_parts, straight, turned_parts, turned, column_partials)
+    const int term_rows = (int)(high / 64), term_cols = (int)(product_pad(cols) / 64);
+    auto tiles = [](int64_t n) { return (int)(product_pad(n) / 64); };
+    const int x_rows = x.out ? tiles(x.rows) : 0, x_cols = x.out ? tiles(x.cols) : 1;
+    const int k_rows = kernel.out ? tiles(kernel.rows) : 0, k_cols = kernel.out ? tiles(kernel.cols) : 1;
+    const int64_t blocks = (int64_t)term_rows * term_cols + (int64_t)x_rows * x_cols + (int64_t)k_rows * k_cols;
+    if (blocks >= (int64_t)1 << 31)
+        return hipErrorInvalidConfiguration;
+#define AXC_PREP(SOURCE, I)                                                                                                        \
+    hipLaunchKernelGGL((grad_prep_kernel<SOURCE, I>), dim3((unsigned)blocks), dim3(256), 0, stream, of_run, term_rows, term_cols,  \
+                       first / 64, run_rows, rows_pad, cols, ld, straight_parts, straight, turned_parts, turned, column_partials,  \
+                       x, x_rows, x_cols, kernel, k_cols, ranges ? ranges[0] : RangeSource{}, ranges ? ranges[1] : RangeSource{},  \
+                       ranges != nullptr, grids)
     const bool narrow = of_run.sums.K <= kNarrowDepth;
     if (!loss)
-        AXC_TERMS(0, uint32_t);
+        AXC_PREP(0, uint32_t);
     else if (of_run.sums.raw.turned && narrow)
-        AXC_TERMS(2, uint32_t);
+        AXC_PREP(2, uint32_t);
     else if (of_run.sums.raw.turned)
-        AXC_TERMS(2, int64_t);
+        AXC_PREP(2, int64_t);
     else if (narrow)
-        AXC_TERMS(1, uint32_t);
+        AXC_PREP(1, uint32_t);
     else
-        AXC_TERMS(1, int64_t);
-#undef AXC_TERMS
-    return hipGetLastError();
-}
-
-hipError_t launch_centered(const void *v, int type, int64_t rows, int64_t cols, int64_t ld, const Grid *grid, bool turn, bf16 *out,
-                           hipStream_t stream)
-{
-    const dim3 blocks((unsigned)(product_pad(cols) / 64), (unsigned)(product_pad(rows) / 64));
-    if (turn)
-        hipLaunchKernelGGL(centered_kernel<true>, blocks, dim3(256), 0, stream, v, type, rows, cols, ld, grid, out);
-    else
-        hipLaunchKernelGGL(centered_kernel<false>, blocks, dim3(256), 0, stream, v, type, rows, cols, ld, grid, out);
+        AXC_PREP(1, int64_t);
+#undef AXC_PREP
     return hipGetLastError();
 }
 
@@ -482,7 +533,7 @@ ProductPlan plan_product(int64_t rows, int64_t cols, int64_t depth_pad, int part
 {
     const int64_t tiles = (product_pad(rows) / kProductTile) * (product_pad(cols) / kProductTile);
     const int64_t steps = depth_pad / kStep * parts;
-    int64_t splits = tiles >= 256 ? 1 : 512 / tiles;
+    int64_t splits = tiles >= 256 ? 1 : 256 / tiles;
     if (splits > steps / 4)
         splits = steps / 4;
     if (splits < 1)
@@ -495,33 +546,35 @@ ProductPlan plan_product(int64_t rows, int64_t cols, int64_t depth_pad, int part
 
 template <typename T, bool PARTIAL>
 static hipError_t product(const bf16 *a, const bf16 *b, int64_t rows, int64_t cols, int64_t depth_pad, int parts, bool split_a,
-                          int splits, float *partials, bool accumulate, const ProductOut &o, hipStream_t stream)
+                          int splits, float *partials, bool accumulate, const ProductOut &o, const ColumnJob &job,
+                          hipStream_t stream)
 {
     const int row_tiles = (int)(product_pad(rows) / kProductTile), col_tiles = (int)(product_pad(cols) / kProductTile);
     if (hipError_t e = set_max_dynamic_lds_once(reinterpret_cast<const void *>(&product_kernel<T, PARTIAL>), kProductLds))
         return e;
-    hipLaunchKernelGGL((product_kernel<T, PARTIAL>), dim3((unsigned)((int64_t)row_tiles * col_tiles * splits)), dim3(kProductThreads),
+    hipLaunchKernelGGL((product_kernel<T, PARTIAL>), dim3((unsigned)((int64_t)row_tiles * col_tiles * splits + job.blocks())),
+                       dim3(kProductThreads),
                        kProductLds,
                        stream, a, b, rows, cols, row_tiles, col_tiles, (int)depth_pad, parts, (int)split_a, splits, partials,
-                       (int)accumulate, o);
+                       (int)accumulate, o, job);
     return hipGetLastError();
 }
 
 hipError_t launch_product(const bf16 *a, const bf16 *b, int64_t rows, int64_t cols, int64_t depth_pad, int parts, bool split_a,
                           const ProductPlan &plan, float *partials, bool keep, bool accumulate, const ProductOut &o,
-                          hipStream_t stream)
+                          const ColumnJob &job, hipStream_t stream)
 {
     if (plan.splits > 1 || keep) {
         if (hipError_t e = product<float, true>(a, b, rows, cols, depth_pad, parts, split_a, plan.splits, partials, accumulate, o,
-                                                stream))
+                                                job, stream))
             return e;
         return keep ? hipSuccess : launch_product_out(partials, plan.splits, rows, cols, o, stream);
     }
     if (o.type == AXC_F32)
-        return product<float, false>(a, b, rows, cols, depth_pad, parts, split_a, 1, nullptr, false, o, stream);
+        return product<float, false>(a, b, rows, cols, depth_pad, parts, split_a, 1, nullptr, false, o, job, stream);
     if (o.type == AXC_BF16)
-        return product<bf16, false>(a, b, rows, cols, depth_pad, parts, split_a, 1, nullptr, false, o, stream);
-    return product<f16, false>(a, b, rows, cols, depth_pad, parts, split_a, 1, nullptr, false, o, stream);
+        return product<bf16, false>(a, b, rows, cols, depth_pad, parts, split_a, 1, nullptr, false, o, job, stream);
+    return product<f16, false>(a, b, rows, cols, depth_pad, parts, split_a, 1, nullptr, false, o, job, stream);
 }
 
 hipError_t launch_product_out(const float *partials, int splits, int64_t rows, int64_t cols, const ProductOut &o,
@@ -539,11 +592,9 @@ hipError_t launch_product_out(const float *partials, int splits, int64_t rows, i
     return hipGetLastError();
 }
 
-hipError_t launch_column_sums(const float *partials, int64_t count, int64_t cols, int64_t pitch, const float *factor, void *out,
-                              int type, hipStream_t stream)
+hipError_t launch_column_sums(const ColumnJob &job, hipStream_t stream)
 {
-    hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)((cols + 63) / 64)), dim3(256), 0, stream, partials, count, cols, pitch,
-                       factor, out, type);
+    hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)job.blocks()), dim3(512), 0, stream, job);
     return hipGetLastError();
 }
 

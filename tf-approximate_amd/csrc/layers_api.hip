@@ -237,17 +237,6 @@ int find_codes(const axc_dense_desc *d, const void *input, const void *range, co
         return rc;
     return few ? make_few_codes(d, input, range, nullptr, o, pc, stream) : AXC_OK;
 }
-// The grids alone.
-int find_grids(const axc_dense_desc *d, const void *input, const void *range, const void *kernel, const Operands &o, hipStream_t stream)
-{
-    RangeSource in, k;
-    if (int rc = find_ranges(d, input, range, kernel, o.x_pairs, o.kernel_pairs, nullptr, 0, &in, &k, stream))
-        return rc;
-    ApiTimer t("layer_grids", stream);
-    AXC_HIP(launch_grids(in, k, true, true, o.grids, stream));
-    return AXC_OK;
-}
-
 // Sums of the run of rows from r on and piece p, in acc or in the scratch, as their consumer is given them.
 int table_sums(const axc_table *table, const axc_dense_desc *d, const Operands &o, const Pieces &pc, int p, int64_t r, int64_t rows,
                int32_t *acc, void *ws, size_t ws_bytes, hipStream_t stream, TableSums *out)
@@ -526,7 +515,9 @@ int axc_fake_approx_dense_gradients(const axc_dense_desc *desc, const void *grad
         return AXC_OK;
     const int64_t rows = desc->rows, K = desc->depth, N = desc->columns;
     const int px = parts_of(desc->input_type), pk = parts_of(desc->kernel_type);
-    if (int rc = find_grids(desc, input, input_range, kernel, s.o, stream))
+    RangeSource ranges[2];
+    if (int rc = find_ranges(desc, input, input_range, kernel, s.o.x_pairs, s.o.kernel_pairs, nullptr, 0, &ranges[0], &ranges[1],
+                             stream))
         return rc;
     {
         GradSource g = {};
@@ -534,36 +525,30 @@ int axc_fake_approx_dense_gradients(const axc_dense_desc *desc, const void *grad
         g.pre = desc->activation == AXC_ACT_NONE ? nullptr : pre;
         g.type = desc->input_type;
         g.activation = desc->activation;
-        ApiTimer t("grad_terms", stream);
-        AXC_HIP(launch_grad_terms(g, false, 0, rows, rows, N, N, px, grad_input ? s.straight : nullptr, pk,
-                                  grad_kernel ? s.turned : nullptr, grad_bias ? s.column_partials : nullptr, stream));
+        ApiTimer t("grad_prep", stream);
+        AXC_HIP(launch_grad_prep(g, false, 0, rows, rows, N, N, px, grad_input ? s.straight : nullptr, pk,
+                                 grad_kernel ? s.turned : nullptr, grad_bias ? s.column_partials : nullptr,
+                                 {input, desc->input_type, rows, K, K, grad_kernel ? s.x_turned : nullptr},
+                                 {kernel, desc->kernel_type, K, N, N, grad_input ? s.kernel : nullptr}, ranges, s.o.grids, stream));
     }
-    if (grad_bias) {
-        ApiTimer t("column_sums", stream);
-        AXC_HIP(launch_column_sums(s.column_partials, product_pad(rows) / 64, N, product_pad(N), nullptr, grad_bias,
-                                   desc->kernel_type, stream));
-    }
+    ColumnJob job = {s.column_partials, product_pad(rows) / 64, N, product_pad(N), nullptr, grad_bias, desc->kernel_type};
     if (grad_input) {
-        {
-            ApiTimer t("centered", stream);
-            AXC_HIP(launch_centered(kernel, desc->kernel_type, K, N, N, &s.o.grids->kernel, false, s.kernel, stream));
-        }
-        const ProductOut o = {grad_input, desc->input_type, K, input, K, &s.o.grids->in, &s.o.grids->kernel,
-                              nullptr};
+        const ProductOut o = {grad_input, desc->input_type, K, input, K, &s.o.grids->in, &s.o.grids->kernel, nullptr};
         ApiTimer t("grad_product", stream);
         AXC_HIP(launch_product(s.straight, s.kernel, rows, K, product_pad(N), px, true, plan_product(rows, K, product_pad(N), px, false),
-                               s.partials, false, false, o, stream));
+                               s.partials, false, false, o, job, stream));
+        job.out = nullptr;
     }
     if (grad_kernel) {
-        {
-            ApiTimer t("centered", stream);
-            AXC_HIP(launch_centered(input, desc->input_type, rows, K, K, &s.o.grids->in, true, s.x_turned, stream));
-        }
-        const ProductOut o = {grad_kernel, desc->kernel_type, N, kernel, N, &s.o.grids->kernel, &s.o.grids->in,
-                              nullptr};
+        const ProductOut o = {grad_kernel, desc->kernel_type, N, kernel, N, &s.o.grids->kernel, &s.o.grids->in, nullptr};
         ApiTimer t("grad_product", stream);
         AXC_HIP(launch_product(s.x_turned, s.turned, K, N, product_pad(rows), pk, false,
-                               plan_product(K, N, product_pad(rows), pk, false), s.partials, false, false, o, stream));
+                               plan_product(K, N, product_pad(rows), pk, false), s.partials, false, false, o, job, stream));
+        job.out = nullptr;
+    }
+    if (job.out) {
+        ApiTimer t("column_sums", stream);
+        AXC_HIP(launch_column_sums(job, stream));
     }
     return AXC_OK;
 }
@@ -707,10 +692,6 @@ int axc_fake_approx_cross_entropy(const axc_table *table, const axc_dense_desc *
 
     const int px = parts_of(desc->input_type), pk = parts_of(desc->kernel_type);
     const int64_t M = product_pad(rows);
-    if (grad_kernel) {
-        ApiTimer t("centered", stream);
-        AXC_HIP(launch_centered(input, desc->input_type, rows, K, K, &o.grids->in, true, s.x_turned, stream));
-    }
     const ProductPlan input_plan = plan_product(rows, K, product_pad(pc.width), px, true);
     const ProductOut input_out = {grad_input, desc->input_type, K, input, K, &o.grids->in, &o.grids->kernel,
                                   s.st.factor};
@@ -731,32 +712,35 @@ int axc_fake_approx_cross_entropy(const axc_table *table, const axc_dense_desc *
             g.bias = element(bias, c, desc->bias_type);
             g.bias_type = desc->bias_type;
             g.first_column = c;
-            ApiTimer t("grad_terms", stream);
-            AXC_HIP(launch_grad_terms(g, true, r, std::min(run, rows - r), rows, n, 0, px, grad_input ? s.straight : nullptr, pk,
-                                      grad_kernel ? s.turned : nullptr, grad_bias ? s.column_partials : nullptr, stream));
+            // the kernel's codes of the piece, and once the input's, go with the first run
+            const bool first_run = r == (rows - 1) / run * run;
+            ApiTimer t("grad_prep", stream);
+            AXC_HIP(launch_grad_prep(g, true, r, std::min(run, rows - r), rows, n, 0, px, grad_input ? s.straight : nullptr, pk,
+                                     grad_kernel ? s.turned : nullptr, grad_bias ? s.column_partials : nullptr,
+                                     {input, desc->input_type, rows, K, K,
+                                      grad_kernel && first_run && p + 1 == pc.count ? s.x_turned : nullptr},
+                                     {element(kernel, c, desc->kernel_type), desc->kernel_type, K, n, V,
+                                      grad_input && first_run ? s.kernel : nullptr},
+                                     nullptr, o.grids, stream));
         }
-        if (grad_bias) {
-            ApiTimer t("column_sums", stream);
-            AXC_HIP(launch_column_sums(s.column_partials, M / 64, n, P, s.st.factor, element(grad_bias, c, desc->kernel_type),
-                                       desc->kernel_type, stream));
-        }
+        ColumnJob job = {s.column_partials, M / 64, n, P, s.st.factor, element(grad_bias, c, desc->kernel_type), desc->kernel_type};
         if (grad_input) {
-            {
-                ApiTimer t("centered", stream);
-                AXC_HIP(launch_centered(element(kernel, c, desc->kernel_type), desc->kernel_type, K, n, V, &o.grids->kernel, false,
-                                        s.kernel, stream));
-            }
             ApiTimer t("grad_product", stream);
             AXC_HIP(launch_product(s.straight, s.kernel, rows, K, P, px, true, input_plan, s.input_partials, true,
-                                   p + 1 < pc.count, input_out, stream));
+                                   p + 1 < pc.count, input_out, job, stream));
+            job.out = nullptr;
         }
         if (grad_kernel) {
             const ProductOut out = {element(grad_kernel, c, desc->kernel_type), desc->kernel_type, V,
-                                    element(kernel, c, desc->kernel_type), V, &o.grids->kernel, &o.grids->in,
-                                    s.st.factor};
+                                    element(kernel, c, desc->kernel_type), V, &o.grids->kernel, &o.grids->in, s.st.factor};
             ApiTimer t("grad_product", stream);
             AXC_HIP(launch_product(s.x_turned, s.turned, K, n, M, pk, false, plan_product(K, n, M, pk, false), s.kernel_partials,
-                                   false, false, out, stream));
+                                   false, false, out, job, stream));
+            job.out = nullptr;
+        }
+        if (job.out) {
+            ApiTimer t("column_sums", stream);
+            AXC_HIP(launch_column_sums(job, stream));
         }
     }
     if (grad_input) {

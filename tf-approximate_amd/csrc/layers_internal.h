@@ -140,6 +140,12 @@ __device__ __forceinline__ uint32_t code_of(float v, const Grid &g)
 }
 __device__ __forceinline__ bool inside(float v, const Grid &g) { return v >= g.low && v <= g.high; }
 
+struct RangeSource {                     // where a tensor's smallest and largest value come from
+    const float *pairs;                  // (smallest, largest) pairs, or null
+    int count;                           // of the pairs; null and 0: lo and hi, known to the caller; null and -1: not known yet
+    float lo, hi;
+};
+
 // ---- reductions ----
 // Sum over a wavefront, in every lane: within rows of 16 lanes, then row to row, by the vector ALU's own lane moves, which take a
 // few cycles each where a move through the LDS takes a hundred.
@@ -199,6 +205,23 @@ __device__ __forceinline__ void block_range(float &lo, float &hi, float *red)
         hi = fmaxf(hi, red[2 * i + 1]);
     }
     __syncthreads();
+}
+
+// The range that a source stands for, in every thread.  red: 2 * waves floats of LDS, free before and after.
+__device__ __forceinline__ void fold(const RangeSource &src, float &lo, float &hi, float *red)
+{
+    lo = src.lo;
+    hi = src.hi;
+    if (src.pairs) {
+        lo = INFINITY;
+        hi = -INFINITY;
+        for (int i = threadIdx.x; i < src.count; i += blockDim.x) {
+            const float2 p = reinterpret_cast<const float2 *>(src.pairs)[i];
+            lo = fminf(lo, p.x);
+            hi = fmaxf(hi, p.y);
+        }
+        block_range(lo, hi, red);
+    }
 }
 
 // ---- activations ----
@@ -300,11 +323,6 @@ struct Pieces {
 
 constexpr int kRangeBlocks = 256;        // pairs that the range pass leaves per tensor, at most
 constexpr int kFewRows = 8;              // rows that the kernel for few rows takes at a time
-struct RangeSource {                     // where a tensor's smallest and largest value come from
-    const float *pairs;                  // (smallest, largest) pairs, or null
-    int count;                           // of the pairs; null and 0: lo and hi, known to the caller; null and -1: not known yet
-    float lo, hi;
-};
 
 // Sums of table entries as a consumer finds them, of one piece and one run of rows.
 struct TableSums {
@@ -353,8 +371,6 @@ __device__ __forceinline__ i32x4 four_sums(const RawSums &s, int64_t r, int64_t 
 
 hipError_t launch_range(const void *x, int x_type, int64_t nx, const void *kernel, int kernel_type, int64_t nk, float *x_pairs,
                         float *kernel_pairs, int32_t *zeros, int64_t n_zeros, int *x_count, int *kernel_count, hipStream_t stream);
-hipError_t launch_grids(const RangeSource &in, const RangeSource &kernel, bool has_in, bool has_kernel, Grids *grids,
-                        hipStream_t stream);
 // Codes of both operands and their sums, and the grids they are on.  x null: only the kernel's; kernel null: only the input's,
 // and the kernel's grid is that of kernel_grid.
 struct CodesJob {
@@ -402,7 +418,7 @@ hipError_t launch_dense_out(const TableSums &s, int64_t rows, int columns, const
 // Operands in bfloat16, rows and depth padded to kProductTile.  Codes minus their zero point are whole numbers below 256 and
 // exact in bfloat16; the other operand is split into `parts` terms of 8 bits each.
 constexpr int kProductTile = 128;
-inline int64_t product_pad(int64_t n) { return (n + kProductTile - 1) / kProductTile * kProductTile; }
+__host__ __device__ inline int64_t product_pad(int64_t n) { return (n + kProductTile - 1) / kProductTile * kProductTile; }
 inline int parts_of(int type) { return type == AXC_F32 ? 3 : type == AXC_F16 ? 2 : 1; }
 
 struct GradSource {                      // where the gradient behind the product comes from
@@ -416,13 +432,29 @@ struct GradSource {                      // where the gradient behind the produc
     int bias_type;
     int64_t first_column;
 };
-// [rows_pad][parts][cols_pad], [cols_pad][parts][rows_pad], and per 64 rows the sums over them (each may be null), of the run of
-// rows from `first` on (a multiple of kProductTile) out of `rows`; `of_run` describes its gradient, of run_rows rows.
-hipError_t launch_grad_terms(const GradSource &of_run, bool loss, int64_t first, int64_t run_rows, int64_t rows, int64_t cols,
-                             int64_t ld, int straight_parts, bf16 *straight, int turned_parts, bf16 *turned, float *column_partials,
-                             hipStream_t stream);
-hipError_t launch_centered(const void *v, int type, int64_t rows, int64_t cols, int64_t ld, const Grid *grid, bool turn, bf16 *out,
-                           hipStream_t stream);
+struct CenteredJob {                     // codes minus zero point of a tensor; out null: not wanted
+    const void *values;
+    int type;
+    int64_t rows, cols, ld;
+    bf16 *out;
+};
+// What stands in front of the products: of the gradient [rows_pad][parts][cols_pad], [cols_pad][parts][rows_pad] and per 64 rows the
+// sums over them (each may be null), for the run of rows from `first` on (a multiple of kProductTile) out of `rows`, of_run describing
+// its run_rows rows; of the input's codes [cols_pad][rows_pad], of the kernel's [rows_pad][cols_pad].  ranges (of input and kernel):
+// the grids are not made yet, and this launch does.
+hipError_t launch_grad_prep(const GradSource &of_run, bool loss, int64_t first, int64_t run_rows, int64_t rows, int64_t cols,
+                            int64_t ld, int straight_parts, bf16 *straight, int turned_parts, bf16 *turned, float *column_partials,
+                            const CenteredJob &x, const CenteredJob &kernel, const RangeSource *ranges, Grids *grids,
+                            hipStream_t stream);
+struct ColumnJob {                       // out[c] = sum over i of partials[i * pitch + c], times *factor
+    const float *partials;
+    int64_t count, cols, pitch;
+    const float *factor;
+    void *out;
+    int type;
+    int64_t blocks() const { return out ? (cols + 63) / 64 : 0; }
+};
+hipError_t launch_column_sums(const ColumnJob &job, hipStream_t stream);
 struct ProductOut {
     void *out;                           // rows x cols, leading dimension ld
     int type;
@@ -438,15 +470,12 @@ struct ProductPlan {
 };
 ProductPlan plan_product(int64_t rows, int64_t cols, int64_t depth_pad, int parts, bool keep);
 // out[r][c] = sum over parts and l of a[r][..l] * b[c][..l]; the operand with the parts is a where split_a, else b.
-// accumulate: add to the partial sums that are there.
+// accumulate: add to the partial sums that are there.  job: column sums that the launch makes too.
 hipError_t launch_product(const bf16 *a, const bf16 *b, int64_t rows, int64_t cols, int64_t depth_pad, int parts, bool split_a,
                           const ProductPlan &plan, float *partials, bool keep, bool accumulate, const ProductOut &o,
-                          hipStream_t stream);
+                          const ColumnJob &job, hipStream_t stream);
 hipError_t launch_product_out(const float *partials, int splits, int64_t rows, int64_t cols, const ProductOut &o,
                               hipStream_t stream);
-hipError_t launch_column_sums(const float *partials, int64_t count, int64_t cols, int64_t pitch, const float *factor, void *out,
-                              int type, hipStream_t stream);
-
 // ---- loss (loss_kernels.hip) ----
 // Columns at least that leave a maximum and a sum: fewer where few rows would leave CUs without work.
 inline int loss_chunk(int64_t rows) { return rows >= 2048 ? 512 : rows >= 512 ? 256 : 64; }
