@@ -554,10 +554,14 @@ int axc_fake_approx_dense_gradients(const axc_dense_desc *desc, const void *grad
 }
 
 // ---- loss ----
-static Pieces loss_pieces(const axc_dense_desc *d)
+// Columns whose sums are in the workspace at a time.  With gradients twice as many: the last piece's sums need not be made again for
+// them, and making them takes longer than reading 256 MiB from beyond the memory-side cache.
+static Pieces loss_pieces(const axc_dense_desc *d, bool gradients)
 {
-    const int64_t most = kSumsAtOnce / fours(std::max<int64_t>(1, d->rows)) & ~(int64_t)255;
-    return pieces_of(d->depth, d->columns, std::min<int64_t>(16384, std::max<int64_t>(1024, most)));
+    const int64_t sums = gradients ? 2 * kSumsAtOnce : kSumsAtOnce;
+    const int64_t most = sums / fours(std::max<int64_t>(1, d->rows)) & ~(int64_t)255;
+    const int64_t codes = ((int64_t)1 << 29) / fours(d->depth) & ~(int64_t)255;   // the LUT-GEMM's offsets have 32 bits
+    return pieces_of(d->depth, d->columns, std::min(codes, std::min<int64_t>(65536, std::max<int64_t>(1024, most))));
 }
 
 struct LossScratch {
@@ -573,7 +577,7 @@ static int carve_loss(const axc_dense_desc *d, bool gradients, void *base, LossS
 {
     if (d->rows > kMostGradientRows)
         return api_fail(AXC_UNIMPLEMENTED, "a loss of more than 4194176 rows");
-    const Pieces pc = loss_pieces(d);
+    const Pieces pc = loss_pieces(d, gradients);
     Carver c(base);
     s->o = carve_operands(c, d, pc, true, true);
     float **const state[] = {&s->st.at, &s->st.lse, &s->st.rows, &s->st.coefficient};
@@ -651,7 +655,7 @@ int axc_fake_approx_cross_entropy(const axc_table *table, const axc_dense_desc *
     if (!input || !kernel || !targets)
         return api_fail(AXC_INVALID_ARGUMENT, "null tensor pointer");
     const bool gradients = grad_input || grad_kernel || grad_bias;
-    const Pieces pc = loss_pieces(desc);
+    const Pieces pc = loss_pieces(desc, gradients);
     LossScratch s;
     if (int rc = carve_loss(desc, gradients, workspace, &s))
         return rc;
