@@ -279,7 +279,7 @@ enum { AXC_ACT_GELU = 2, AXC_ACT_GELU_TANH = 3, AXC_ACT_SILU = 4 };   /* dense l
 /* A dense layer: input [rows][depth], kernel [depth][columns] as Keras has it, output [rows][columns].  Both operands are
  * quantized to the 8-bit grid of their (smallest, largest) value, with a = code of the input and b = code of the kernel
  *   product = s_in s_k sum over depth of (T[a][b] - z_k a - z_in b + z_in z_k),
- * the brackets in whole numbers, what follows in float32, rounded once to the output's type.  depth below 32768.
+ * the brackets in whole numbers, what follows in float32, rounded once to the output's type.  depth from 1 to 32764.
  * The kernel's range is its own; the input's is its own, or what a call before has reported of it (`input_range`,
  * AXC_RANGE_BYTES, as in axc_layer_ranges), or fixed by the caller (range_known), in this order of precedence: fixed, reported,
  * its own.  NaN in an operand counts as the upper end of its range, as in the convolutions. */
@@ -293,7 +293,7 @@ typedef struct axc_dense_desc {
     float input_min, input_max;
 } axc_dense_desc;
 
-/* The kernel's codes, laid out once for many calls (rows of the desc does not matter): device memory of this size, 256-byte
+/* The kernel's codes, laid out once for many calls (the desc's rows do not matter), two bytes a weight: device memory of this size, 256-byte
  * aligned, which the call fills and axc_fake_approx_dense reads in the kernel's place. */
 int axc_dense_packed_bytes(const axc_dense_desc *desc, size_t *bytes);
 int axc_dense_pack(const axc_dense_desc *desc, const void *kernel, void *packed, void *stream);

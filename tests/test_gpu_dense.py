@@ -31,7 +31,9 @@ SIZES = [
     # many rows
     (17, 1, 3), (18, 7, 2), (33, 66, 65), (64, 255, 129), (130, 64, 1), (131, 1001, 70), (257, 96, 333), (515, 40, 1030),
     # several runs of rows, the last of few; several pieces of columns
-    (16389, 5, 3), (20, 12, 8201), (3, 9, 16400),
+    (16389, 5, 3), (20, 12, 8201), (40, 12, 8201), (3, 9, 16400), (50, 9, 16400),
+    # brackets that need 64 bits, at the largest depths
+    (2, 20001, 33), (40, 20001, 33), (3, 32764, 20), (35, 32764, 20),
 ]
 
 
@@ -279,6 +281,60 @@ def test_in_a_graph_and_on_streams(pkg, tables):
     torch.cuda.synchronize()
     for g, want in zip(got, wants):
         assert all(torch.equal(a, b) for a, b in zip(g, want))
+
+
+PINS = [("set_matrix_rows", v) for v in (1, 2, 3)] + [("set_preexpand", v) for v in (1, -1)] + \
+    [("set_tile_columns", v) for v in (16, 32, 64)] + [("set_merged_launches", v) for v in (1, -1)]
+
+
+@pytest.mark.parametrize("pin", PINS, ids=str)
+def test_every_form_of_the_sums(pkg, tables, pin):
+    """The kernels that make the sums of many rows leave them in order, in parts or turned: the same comes of them."""
+    layer = pkg.FakeApproxDense(tables["random"][1], "relu")
+    loss = pkg.FakeApproxCrossEntropy(tables["noisy"][1])
+    cases = []
+    for rows, depth, columns in ((40, 70, 130), (1000, 300, 72), (260, 1024, 96)):
+        x, k = make((rows, depth), rows), make((depth, columns), depth)
+        t = torch.arange(rows, device=DEV) % columns
+        cases.append((x, k, t, layer(x, k), loss.loss_and_gradients(x, k, t, reduction="none")))
+    getattr(pkg.ops, pin[0])(pin[1])
+    try:
+        for x, k, t, y, (l, g) in cases:
+            assert torch.equal(layer(x, k), y)
+            l2, g2 = loss.loss_and_gradients(x, k, t, reduction="none")
+            # (exponentials are summed chunk by chunk: in another order where the sums come in another one)
+            assert (l2 - l).abs().max() <= 2 * ref.E * (256 + 8 * float(l.abs().max()))
+            for a, b in zip(g2, g):
+                assert b is None or (a - b).abs().max() <= 1e-4 * b.abs().max()
+    finally:
+        getattr(pkg.ops, pin[0])(0)
+
+
+def test_gradients_of_many_rows(pkg, tables):
+    """As many rows as there may be, operands of more than 2^31 elements: the last rows alone, and sums over all of them."""
+    rows, depth, columns = 4194176, 520, 3
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(1)
+    x = torch.randint(-127, 129, (rows, depth), device=DEV, generator=gen, dtype=torch.int16).to(BF16)
+    x[0, 0], x[0, 1] = -127, 128           # the grid is the whole numbers
+    k, gy = make((depth, columns), 2, BF16), make((rows, columns), 3, BF16)
+    layer = pkg.FakeApproxDense(tables["noisy"][1])
+    g = layer.gradients(gy, x, k)
+    assert x.numel() > 2 ** 31
+    kg = ref.Grid(pkg, k)
+    for first in (0, rows // 2, rows - 50):
+        part = gy[first:first + 50].double()
+        want = part @ kg.values.t()
+        size = part.abs() @ kg.values.abs().t()
+        ref.check(g.inputs[first:first + 50], want, ref.rounded(want, 2.0 ** -7 * size, BF16))
+    total, size = torch.zeros((depth, columns), dtype=torch.float64, device=DEV), 0
+    for part in range(0, rows, 1 << 18):
+        a, b = x[part:part + (1 << 18)].double().t().contiguous(), gy[part:part + (1 << 18)].double()
+        total += a @ b
+        size = size + a.abs() @ b.abs()
+    # float32 sums of 4.2 M terms in 16 384 steps and more of matrix instructions of 32: off by the square root of their number,
+    # in steps of the largest partial sum, which is below the sum of the terms' sizes
+    ref.check(g.kernel, total * kg.inside, ref.rounded(total, (2.0 ** -7 / 64 + 64 * ref.E) * size, BF16))
 
 
 def test_far_offsets(pkg, tables):

@@ -31,7 +31,9 @@ def noisy(pkg):
 
 
 SIZES = [(1, 4, 1), (1, 32, 5003), (2, 7, 9), (5, 64, 1000), (16, 50, 2049), (17, 20, 3), (70, 33, 257), (129, 64, 5003),
-         (300, 48, 16390), (1100, 17, 1025)]
+         (300, 48, 16390), (1100, 17, 1025),
+         # several pieces of the vocabulary; several runs of rows; both
+         (2000, 20, 70001), (16500, 9, 100), (16500, 5, 5000), (3, 20, 70001), (40, 16500, 50)]
 
 
 def reference(pkg, noisy, x, k, bias, t, reduction, grad_loss):

@@ -218,6 +218,22 @@ def test_alignment_and_strides(pkg):
         assert torch.equal(norm(apart[:, 1], *c.args())[1], want[1])
 
 
+def test_far_rows(pkg):
+    """More than 2^31 elements: the last rows, against a call on those alone."""
+    norm = pkg.ResidualNorm("rms", EPS)
+    rows, width = 270000, 8192
+    x, w = make((rows, width), 1, BF16), make((width,), 2, BF16, 0.1, 1.0)
+    assert x.numel() > 2 ** 31
+    _, y, seen = norm.call_in_turn(x, x, w)
+    h, last = norm(x[-30:], x[-30:], w)
+    assert torch.equal(y[-30:], last)
+    g = norm.gradients(y, y, x, None, w)
+    assert torch.equal(g.x[-30:], norm.gradients(y[-30:], y[-30:], x[-30:], None, w).x)
+    pairs = seen.view(-1, 2)
+    lo, hi = torch.aminmax(y)
+    assert float(pairs[:, 0].min()) == float(lo) and float(pairs[:, 1].max()) == float(hi)
+
+
 def test_gates_of_a_batch(pkg):
     norm = pkg.ResidualNorm("layer", EPS)
     x, b, w = make((3, 5, 32), 1), make((3, 5, 32), 2), make((32,), 3)

@@ -13,7 +13,7 @@ def norm(pkg, rows=4, width=8, groups=0, types=(0, 0), kind=0, eps=1e-6):
     return pkg._lib.ResidualNormDesc(rows, width, groups, *types, kind, eps)
 
 
-BAD_DENSE = [dict(rows=-1), dict(columns=-1), dict(depth=0), dict(depth=-3), dict(depth=32768), dict(rows=1 << 31),
+BAD_DENSE = [dict(rows=-1), dict(columns=-1), dict(depth=0), dict(depth=-3), dict(depth=32768), dict(depth=32765), dict(rows=1 << 31),
              dict(columns=1 << 31), dict(rows=1 << 21, columns=1 << 20), dict(types=(3, 0, 0)), dict(types=(0, -1, 0)),
              dict(types=(0, 0, 9)), dict(activation=5), dict(activation=-1)]
 

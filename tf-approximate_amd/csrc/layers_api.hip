@@ -16,6 +16,8 @@ namespace {
             return api_fail_hip(e_, #call);          \
     } while (0)
 
+int64_t fours(int64_t n) { return (n + 3) & ~(int64_t)3; }
+
 bool known_type(int type) { return type == AXC_F32 || type == AXC_BF16 || type == AXC_F16; }
 
 int check_desc(const axc_dense_desc *d)
@@ -26,8 +28,8 @@ int check_desc(const axc_dense_desc *d)
         return api_fail(AXC_INVALID_ARGUMENT, "rows, depth and columns must not be negative");
     if (d->depth < 1)
         return api_fail(AXC_INVALID_ARGUMENT, "depth must be at least 1");
-    if (d->depth >= 32768)   // 32768 * 65535 would overflow the int32 accumulator
-        return api_fail(AXC_INVALID_ARGUMENT, "depth must be below 32768 for int32 accumulation");
+    if (fours(d->depth) >= 32768)   // 32768 * 65535 would overflow the int32 accumulator
+        return api_fail(AXC_INVALID_ARGUMENT, "depth must be at most 32764 for int32 accumulation");
     const int64_t most = ((int64_t)1 << 31) - 256;
     if (d->rows > most || d->columns > most || d->rows * d->columns >= ((int64_t)1 << 40) ||
         d->columns * d->depth >= ((int64_t)1 << 40))
@@ -38,7 +40,7 @@ int check_desc(const axc_dense_desc *d)
         return api_fail(AXC_INVALID_ARGUMENT, "unknown activation");
     return AXC_OK;
 }
-constexpr int64_t kMostGradientRows = (int64_t)65535 * 64 / kProductTile * kProductTile;   // 64 a workgroup, in the grid's y
+constexpr int64_t kMostGradientRows = 4194176;   // 65 534 tiles of 64: with those of the columns they are counted in 32 bits
 
 // Hands out parts of a workspace; without one it only counts.
 class Carver {
@@ -69,8 +71,6 @@ int check_workspace(const void *workspace, size_t have, size_t need)
 
 const void *element(const void *p, int64_t i, int type) { return p ? static_cast<const char *>(p) + i * type_bytes(type) : nullptr; }
 void *element(void *p, int64_t i, int type) { return p ? static_cast<char *>(p) + i * type_bytes(type) : nullptr; }
-
-int64_t fours(int64_t n) { return (n + 3) & ~(int64_t)3; }
 
 // Columns in pieces of about the same width, `most` at most.
 Pieces pieces_of(int64_t depth, int64_t columns, int64_t most)
@@ -237,6 +237,7 @@ int find_codes(const axc_dense_desc *d, const void *input, const void *range, co
         return rc;
     return few ? make_few_codes(d, input, range, nullptr, o, pc, stream) : AXC_OK;
 }
+
 // Sums of the run of rows from r on and piece p, in acc or in the scratch, as their consumer is given them.
 int table_sums(const axc_table *table, const axc_dense_desc *d, const Operands &o, const Pieces &pc, int p, int64_t r, int64_t rows,
                int32_t *acc, void *ws, size_t ws_bytes, hipStream_t stream, TableSums *out)
@@ -554,12 +555,11 @@ int axc_fake_approx_dense_gradients(const axc_dense_desc *desc, const void *grad
 }
 
 // ---- loss ----
-// Columns whose sums are in the workspace at a time.  With gradients twice as many: the last piece's sums need not be made again for
-// them, and making them takes longer than reading 256 MiB from beyond the memory-side cache.
-static Pieces loss_pieces(const axc_dense_desc *d, bool gradients)
+// Columns whose sums are in the workspace at a time, 256 MiB of them: the last piece's need not be made again for the gradients, and
+// making them takes longer than reading them from beyond the memory-side cache.  The same without gradients, so that the loss is.
+static Pieces loss_pieces(const axc_dense_desc *d)
 {
-    const int64_t sums = gradients ? 2 * kSumsAtOnce : kSumsAtOnce;
-    const int64_t most = sums / fours(std::max<int64_t>(1, d->rows)) & ~(int64_t)255;
+    const int64_t most = 2 * kSumsAtOnce / fours(std::max<int64_t>(1, d->rows)) & ~(int64_t)255;
     const int64_t codes = ((int64_t)1 << 29) / fours(d->depth) & ~(int64_t)255;   // the LUT-GEMM's offsets have 32 bits
     return pieces_of(d->depth, d->columns, std::min(codes, std::min<int64_t>(65536, std::max<int64_t>(1024, most))));
 }
@@ -577,7 +577,7 @@ static int carve_loss(const axc_dense_desc *d, bool gradients, void *base, LossS
 {
     if (d->rows > kMostGradientRows)
         return api_fail(AXC_UNIMPLEMENTED, "a loss of more than 4194176 rows");
-    const Pieces pc = loss_pieces(d, gradients);
+    const Pieces pc = loss_pieces(d);
     Carver c(base);
     s->o = carve_operands(c, d, pc, true, true);
     float **const state[] = {&s->st.at, &s->st.lse, &s->st.rows, &s->st.coefficient};
@@ -655,7 +655,7 @@ int axc_fake_approx_cross_entropy(const axc_table *table, const axc_dense_desc *
     if (!input || !kernel || !targets)
         return api_fail(AXC_INVALID_ARGUMENT, "null tensor pointer");
     const bool gradients = grad_input || grad_kernel || grad_bias;
-    const Pieces pc = loss_pieces(desc, gradients);
+    const Pieces pc = loss_pieces(desc);
     LossScratch s;
     if (int rc = carve_loss(desc, gradients, workspace, &s))
         return rc;

@@ -22,22 +22,26 @@ struct Exponentials {
     template <int N>
     __device__ __forceinline__ void add(const float (&z)[N])
     {
-        float m = top, undefined = 0.0f;
+        float m = top;
 #pragma unroll
         for (int j = 0; j < N; ++j)
             m = fmaxf(m, z[j]);
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-            undefined += z[j] != z[j] ? z[j] : 0.0f;   // (fmaxf passes over NaN, which nothing else below may)
-        if (m > -INFINITY) {
-            float s = top == m ? sum : sum * __expf(top - m);
+        if (fabsf(m) < INFINITY) {       // (a NaN, over which fmaxf has passed, is in the sum then)
+            float s = sum * __expf(top - m);
 #pragma unroll
             for (int j = 0; j < N; ++j)
-                s += z[j] == m ? 1.0f : __expf(z[j] - m);
+                s += __expf(z[j] - m);
             sum = s;
             top = m;
+        } else {                         // nothing but -infinity yet, or an infinite one
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                if (z[j] > -INFINITY)
+                    join(z[j], 1.0f);
+                else if (z[j] != z[j])
+                    sum = z[j];
+            }
         }
-        sum += undefined;
     }
 };
 
@@ -140,19 +144,28 @@ __global__ void __launch_bounds__(256) loss_turned_kernel(TableSums s, int64_t f
     st.parts[(chunk + blockIdx.x) * rows + first_row + at] = make_float2(e.top, e.sum);
 }
 
-// A row a thread, over what the chunks have left.
-__global__ void __launch_bounds__(64) loss_rows_kernel(LossState st, const int64_t *__restrict__ targets, int64_t ignore, int64_t V,
-                                                       int64_t first_row, int64_t run_rows, int64_t rows, int chunks)
+// 64 rows a workgroup, over what the chunks have left: a row a lane, every eighth chunk a wavefront.
+constexpr int kRowWaves = 8;
+__global__ void __launch_bounds__(64 * kRowWaves) loss_rows_kernel(LossState st, const int64_t *__restrict__ targets, int64_t ignore,
+                                                                   int64_t V, int64_t first_row, int64_t run_rows, int64_t rows,
+                                                                   int chunks)
 {
-    const int64_t i = (int64_t)blockIdx.x * 64 + threadIdx.x, r = first_row + i;
-    if (i >= run_rows)
-        return;
+    __shared__ float2 ends[kRowWaves][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+    const int64_t i = (int64_t)blockIdx.x * 64 + lane, r = first_row + i;
     Exponentials e;
-#pragma unroll 8
-    for (int c = 0; c < chunks; ++c) {
-        const float2 p = st.parts[c * rows + r];
-        e.join(p.x, p.y);
-    }
+    if (i < run_rows)
+#pragma unroll 4
+        for (int c = wave; c < chunks; c += kRowWaves) {
+            const float2 p = st.parts[c * rows + r];
+            e.join(p.x, p.y);
+        }
+    ends[wave][lane] = make_float2(e.top, e.sum);
+    __syncthreads();
+    if (wave != 0 || i >= run_rows)
+        return;
+    for (int w = 1; w < kRowWaves; ++w)
+        e.join(ends[w][lane].x, ends[w][lane].y);
     const float lse = e.top + logf(e.sum);
     const int64_t t = targets[r];
     st.lse[r] = lse;
@@ -256,7 +269,7 @@ hipError_t launch_loss_piece(const TableSums &s, int64_t first_row, int64_t run_
 hipError_t launch_loss_rows(const LossState &st, const int64_t *targets, int64_t ignore, int64_t V, int64_t first_row, int64_t run_rows,
                             int64_t rows, int chunks, hipStream_t stream)
 {
-    hipLaunchKernelGGL(loss_rows_kernel, dim3((unsigned)((run_rows + 63) / 64)), dim3(64), 0, stream, st, targets, ignore, V, first_row,
+    hipLaunchKernelGGL(loss_rows_kernel, dim3((unsigned)((run_rows + 63) / 64)), dim3(64 * kRowWaves), 0, stream, st, targets, ignore, V, first_row,
                        run_rows, rows, chunks);
     return hipGetLastError();
 }
