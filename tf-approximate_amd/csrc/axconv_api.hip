@@ -1901,10 +1901,10 @@ int axc_table_create(const uint16_t *host_table, axc_table **out)
         return fail(AXC_INVALID_ARGUMENT, "null argument");
     // weight-code major: tableT[b][a] = T[(a << 8) | b], in squares that the first-level cache holds by row and by column, and
     // the two flipped copies by whole vectors (us a table with its upload, on one machine: entry by entry 143 for the first
-    // alone, 181 for three; 42); behind them the caller's own order, for dense layers of few rows
+    // alone, 181 for three; 42); behind them the one for dense layers of few rows
     const size_t entries = (size_t)kTableRows * 256, used = 65536;   // row 256: the null weight's, zeros
     std::vector<uint16_t> t(4 * entries);
-    uint16_t *const T = t.data(), *const F = T + entries, *const S = F + entries, *const I = S + entries;
+    uint16_t *const T = t.data(), *const F = T + entries, *const S = F + entries, *const L = S + entries;
     for (int a0 = 0; a0 < 256; a0 += 16)
         for (int b0 = 0; b0 < 256; b0 += 16)
             for (int b = b0; b < b0 + 16; ++b)
@@ -1916,7 +1916,13 @@ int axc_table_create(const uint16_t *host_table, axc_table **out)
         S[i] = host_table[i] ^ 0x8080u;
     for (size_t i = used; i < entries; ++i)
         S[i] = 0x8080u;
-    memcpy(I, host_table, used * sizeof(uint16_t));
+    for (uint32_t a = 0; a < 256; ++a) {
+        uint32_t r = 0;                  // the bits of a turned round
+        for (int bit = 0; bit < 8; ++bit)
+            r |= (a >> bit & 1u) << (7 - bit);
+        for (uint32_t b = 0; b < 256; ++b)
+            L[r * 256 + (b ^ r)] = host_table[a * 256 + b];
+    }
     axc_table *tab = new axc_table;
     tab->dev_tableT = nullptr;
     hipError_t e = hipGetDevice(&tab->device);
@@ -1926,7 +1932,7 @@ int axc_table_create(const uint16_t *host_table, axc_table **out)
         e = hipMemcpy(tab->dev_tableT, t.data(), 4 * (size_t)kTableAllocBytes, hipMemcpyHostToDevice);
     tab->dev_tableF = tab->dev_tableT + entries;
     tab->dev_tableS = tab->dev_tableF + entries;
-    tab->dev_tableI = tab->dev_tableS + entries;
+    tab->dev_tableL = tab->dev_tableS + entries;
     if (e != hipSuccess) {
         if (tab->dev_tableT)
             (void)hipFree(tab->dev_tableT);

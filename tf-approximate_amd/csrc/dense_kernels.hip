@@ -7,7 +7,8 @@
 // number and is computed as one, so a product is rounded three times: s_in s_k, the bracket, and the two multiplied.
 //
 // The sums of many rows are made by the kernels that make them for 1x1 convolutions (axc_conv2d_codes_acc_i32); those of few
-// rows, where building rows for every filter element would cost more than the lookups, by few_rows_kernel.
+// rows, where building rows for every filter element would cost more than the lookups, by few_rows_kernel; one or two rows are all
+// token_kernel's.
 #include "layers_internal.h"
 
 namespace axc {
@@ -105,44 +106,40 @@ __device__ __forceinline__ int32_t row_codes_any(const void *x, int type, int64_
     return row_codes(static_cast<const f16 *>(x) + at, K, Kp, whole, g, codes, thread, threads);
 }
 
+// The grid of an input of few rows, found by one workgroup.  red: 2 * wavefronts floats of LDS.
+__device__ __forceinline__ Grid few_grid(const FewInput &in, int rows, float *red)
+{
+    float lo, hi;
+    if (!in.range.pairs && in.range.count < 0) {
+        lo = INFINITY;
+        hi = -INFINITY;
+        range_of_any(in.x, in.type, (int64_t)rows * in.K, threadIdx.x, blockDim.x, lo, hi);
+        block_range(lo, hi, red);
+    } else {
+        fold(in.range, lo, hi, red);
+    }
+    return grid_of_range(lo, hi);
+}
 // Few rows, in groups of eight: every workgroup finds the range itself, of all rows, and then takes its own row
 // (of rows that are not there the codes are what the memory held: any byte is one, and nobody stores what comes of them).
-template <typename T>
-__device__ int32_t column_codes(const T *__restrict__ x, int K, int Kb, const Grid &g, uint8_t *__restrict__ codes)
-{
-    int32_t sum = 0;
-#pragma unroll 4
-    for (int k = threadIdx.x; k < Kb; k += 512) {
-        const uint32_t c = k < K ? code_of((float)x[k], g) : 0u;
-        codes[(int64_t)k * 8] = (uint8_t)c;
-        sum += (int32_t)c;
-    }
-    return sum;
-}
-__global__ void __launch_bounds__(512) few_codes_kernel(const void *x, int type, int rows, int K, int Kb, RangeSource src,
-                                                        const Grid *kernel_grid, Grids *grids, uint8_t *codes, int32_t *row_sums)
+__global__ void __launch_bounds__(512) few_codes_kernel(FewInput in, int rows, int Kb, Grids *grids, uint8_t *codes, int32_t *row_sums)
 {
     __shared__ float red[16];
     __shared__ int32_t sums[8];
-    float lo, hi;
-    if (!src.pairs && src.count < 0) {
-        lo = INFINITY;
-        hi = -INFINITY;
-        range_of_any(x, type, (int64_t)rows * K, threadIdx.x, 512, lo, hi);
-        block_range(lo, hi, red);
-    } else {
-        fold(src, lo, hi, red);
-    }
-    const Grid g = grid_of_range(lo, hi);
+    const Grid g = few_grid(in, rows, red);
     const int64_t r = blockIdx.x;
     uint8_t *const to = codes + (r & ~7) * Kb + (r & 7);
     int32_t part = 0;
-    if (type == AXC_F32)
-        part = column_codes(static_cast<const float *>(x) + r * K, K, Kb, g, to);
-    else if (type == AXC_BF16)
-        part = column_codes(static_cast<const bf16 *>(x) + r * K, K, Kb, g, to);
-    else
-        part = column_codes(static_cast<const f16 *>(x) + r * K, K, Kb, g, to);
+    for (int k = 4 * (int)threadIdx.x; k < Kb; k += 2048) {
+        float v[4];
+        load_four_any(in.x, r * in.K + k, in.K - k, in.type, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t c = k + j < in.K ? code_of(v[j], g) : 0u;
+            to[(int64_t)(k + j) * 8] = (uint8_t)c;
+            part += (int32_t)c;
+        }
+    }
     part = wave_sum(part);
     if ((threadIdx.x & 63) == 0)
         sums[threadIdx.x / 64] = part;
@@ -154,8 +151,8 @@ __global__ void __launch_bounds__(512) few_codes_kernel(const void *x, int type,
         row_sums[r] = sum;
         if (r == 0) {
             grids->in = g;
-            if (kernel_grid)
-                grids->kernel = *kernel_grid;
+            if (in.kernel_grid)
+                grids->kernel = *in.kernel_grid;
         }
     }
 }
@@ -271,46 +268,50 @@ __global__ void __launch_bounds__(256) codes_kernel(CodesJob job, int x_blocks, 
 }
 
 // ---- sums of few rows ----
-// A workgroup takes MT rows, 1024 columns (one a lane) and 16 elements of the depth at a time.  For those elements it lays out in LDS
-//   R[b][e] = entries of filter code b for all MT rows, at element e of the block: 16 places of 16 bytes, a row of 256 bytes,
-// and every lane looks its column's 16 weights up in it, 2 MT bytes an access.  Which row that is, is anybody's guess, but the place
-// in it decides the banks: at step s lane l takes element (l + s) & 15, so that any 16 lanes meet 16 different groups of banks,
-// whatever their weights are (as all elements go into the same sum, their order does not matter; the codes are laid out in it).
-// Building R takes 8 to 64 KiB of table rows for the block and 1024 columns, through a first-level cache that takes an address for
+// A workgroup takes eight rows, 1024 columns and 16 elements of the depth at a time.  For those elements it lays out in LDS
+//   R[b][e] = entries of filter code b for all eight rows, at element e of the block: 16 places of 16 bytes, a row of 256 bytes,
+// and looks the columns' weights up in it, 16 bytes an access.  Which row that is, is anybody's guess, but the place in it decides the
+// banks: a lane of column n takes the elements from n on, so that any 16 lanes meet 16 different groups of banks, whatever their
+// weights are (as all elements go into the same sum, their order does not matter; the codes are laid out in it).
+// The matrix cores add up what is found: a lane's 16 bytes are its column's line of the left operand, four lanes' blocks of the depth
+// of 64, and the right operand, a one where byte and result agree, adds the bytes up one by one.  They are signed bytes there, so the
+// table is the one whose bytes have their top bit flipped, 128 less each.  (The vector ALU would take three instructions
+// for two dwords, six a lookup.)
+// Building R takes 64 KiB of table rows for the block and 1024 columns, through a first-level cache that takes an address for
 // every 64 neighbouring bytes a cycle: four neighbouring lanes read on in one table row, of one element, and the next four in
-// another's (a different row for each lane, whose stores would meet no bank twice, took 64 addresses a load: 23.5 us instead of
-// 15.8 for 8 rows by 4096 by 4096).  Sums of two rows share a dword as they come: one register adds whole dwords modulo 2^32, another the
-// upper halves, three instructions for two dwords.
+// another's (a different row for each lane, whose stores would meet no bank twice, took 64 addresses a load, and half as long again).
+// So four lanes store to one place of four rows of R, which are the same banks: they store dwords, odd lanes the other of their two
+// first (8 cycles a store; both at once took 24, twice as long as all reads together; with as many dwords as there are lanes, of loads
+// half as wide, the stores took 2 and the loads more than they saved).
+// MT: 4 where there are no more rows, 8 bytes a place then.  8 rows by 4096 by 4096, four blocks a workgroup, take 17 us: 5 until the
+// first R is there (range, codes, table rows, one after the other), then 2 a block, 1.5 of them the LDS's accesses; 4 rows 15.
 // RAW: the input comes as it is.  Every workgroup finds its range and its grid itself and makes the codes of its own part of the
-// depth, into LDS; one of them the rows' sums and the grids for the launch behind this one.
+// depth, into LDS, and their sums.
 constexpr int kFewColumns = 1024;
 constexpr int kFewBlocks = 192;          // of the depth, a workgroup at most where it makes codes: 128 bytes of LDS each
 constexpr int kFewLdsBytes = 2 * 65536;  // R twice: one is built while the other is read
 
 template <int MT, bool RAW>
-__global__ void __launch_bounds__(1024) few_rows_kernel(const uint16_t *__restrict__ tableI, const uint8_t *__restrict__ x_codes,
-                                                        FewInput in, int rows, int Kb, const uint8_t *__restrict__ kernel_blocks,
-                                                        int width, int32_t *__restrict__ acc)
+__global__ void __launch_bounds__(1024) few_rows_kernel(FewJob job)
 {
-    constexpr int H = (MT + 1) / 2;      // dwords of a place that are used
-    constexpr int kOf = MT < 4 ? MT : 4; // rows that a wavefront takes table entries of
-    constexpr int kEntries = MT == 8 ? 8 : 4;   // of neighbouring filter codes that a lane takes: eight rows are two wavefronts' work
+    constexpr int kEntries = MT;
     typedef uint32_t Words __attribute__((ext_vector_type(kEntries / 2)));
     extern __shared__ __align__(16) unsigned char lds[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
-    const int c = (int)blockIdx.x * kFewColumns + (int)threadIdx.x;
-    const int at = c < width ? c : width - 1;   // (lanes behind the columns repeat the last, at its place; nobody stores them)
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int n = lane & 15, quarter = lane >> 4, width = job.width, Kb = job.Kb;
+    const int column0 = (int)blockIdx.x * kFewColumns + wave * 64;
     const int row0 = (int)blockIdx.z * 8;
     const int blocks = Kb / 16;
     const int first = (int)((int64_t)blocks * blockIdx.y / gridDim.y), last = (int)((int64_t)blocks * (blockIdx.y + 1) / gridDim.y);
-    // this lane's part of R: filter codes b0 on, at element lane >> 2, rows `half` on
+    // this lane's part of R: kEntries filter codes, b0 on, at element lane >> 2, four rows, `half` on
     const int half = MT == 8 ? (wave & 1) * 4 : 0;
     const int b0 = (MT == 8 ? (wave >> 1) * 32 : wave * 16) + (lane & 3) * kEntries;
-    const uint8_t *const xs = x_codes + (int64_t)row0 * Kb + (lane >> 2) * 8 + half;
+    const int own_place = b0 * 256 + (lane >> 2) * 16 + half * 2, odd = (lane & 1) * 4;
+    const uint8_t *const xs = job.x_codes + (int64_t)row0 * Kb + (lane >> 2) * 8 + half;
 
     uint32_t a;                          // the rows' codes at that element
-    Words t[kOf];                        // table entries
-    uint4 w;                             // the column's 16 weights
+    Words t[4];                          // table entries
+    uint32_t w[4];                       // four weights of a column in each of four groups of 16
     unsigned char *const own_codes = lds + kFewLdsBytes;   // RAW: [element of this part][8 rows]
     auto load_codes = [&](int block) {
         if constexpr (RAW)
@@ -320,75 +321,68 @@ __global__ void __launch_bounds__(1024) few_rows_kernel(const uint16_t *__restri
     };
     auto load_entries = [&] {
 #pragma unroll
-        for (int m = 0; m < kOf; ++m)
-            t[m] = *reinterpret_cast<const Words *>(tableI + ((a >> (8 * m)) & 255u) * 256u + b0);
+        for (int m = 0; m < 4; ++m)
+            t[m] = *reinterpret_cast<const Words *>(job.tableS + ((a >> (8 * m)) & 255u) * 256u + b0);
     };
-    auto load_weights = [&](int block) {
-        w = *reinterpret_cast<const uint4 *>(kernel_blocks + ((int64_t)block * width + at) * 16);
-    };
-    uint32_t chunk[4];                   // where step 4 i + j reads in a row, in bytes: byte j of chunk[i]
+    const uint8_t *from[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        chunk[i] = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            chunk[i] |= (uint32_t)(((at + 4 * i + j) & 15) * 16) << (8 * j);
+    for (int q = 0; q < 4; ++q) {        // (lanes behind the columns repeat the last; nobody stores them)
+        const int c = column0 + q * 16 + n;
+        from[q] = job.kernel_blocks + (int64_t)(c < width ? c : width - 1) * 16 + quarter * 4;
     }
+    auto load_weights = [&](int block) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            w[q] = *reinterpret_cast<const uint32_t *>(from[q] + (int64_t)block * width * 16);
+    };
+    uint32_t places = 0;                 // of this lane's four elements, in bytes
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        places |= (uint32_t)(((n + 4 * quarter + i) & 15) * 16) << (8 * i);
+    i32x4 one = {};                      // byte n of an element's 2 MT is 1
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        one[i] = n / 4 == i % (MT / 2) ? 1 << (8 * (n & 3)) : 0;
 
     if (first < last)
         load_weights(first);
     if constexpr (RAW) {
         __shared__ float ends[32];
-        __shared__ int32_t part[16][8];
-        float lo, hi;
-        if (!in.range.pairs && in.range.count < 0) {
-            lo = INFINITY;
-            hi = -INFINITY;
-            range_of_any(in.x, in.type, (int64_t)rows * in.K, threadIdx.x, 1024, lo, hi);
-            block_range(lo, hi, ends);
-        } else {
-            fold(in.range, lo, hi, ends);
-        }
-        const Grid g = grid_of_range(lo, hi);
-        const int here = rows - row0 < 8 ? rows - row0 : 8, k0 = first * 16, many = (last - first) * 16;
+        __shared__ int32_t part[8];
+        if (threadIdx.x < 8)
+            part[threadIdx.x] = 0;
+        const int here = job.rows - row0 < 8 ? job.rows - row0 : 8, k0 = first * 16, many = (last - first) * 16;
+        auto there = [&](int i) { return i < many * 8 && (i & 7) < here && k0 + (i >> 3) < job.in.K; };
+        auto bits_at = [&](int i) {
+            return there(i) ? load_bits(job.in.x, (int64_t)(row0 + (i & 7)) * job.in.K + k0 + (i >> 3), job.in.type) : 0u;
+        };
+        const uint32_t early = bits_at((int)threadIdx.x);   // (while the range is looked for)
+        const Grid g = few_grid(job.in, job.rows, ends);
+        __syncthreads();                 // (of a known range, nothing else waits for `part`)
+        int32_t sum = 0;                 // of row threadIdx.x & 7
         for (int i = (int)threadIdx.x; i < many * 8; i += 1024) {
-            const int m = i & 7, k = k0 + (i >> 3);
-            own_codes[i] = (unsigned char)(m < here && k < in.K
-                                               ? code_of(load_any(in.x, (int64_t)(row0 + m) * in.K + k, in.type), g)
-                                               : 0u);
+            const uint32_t bits = i < 1024 ? early : bits_at(i);
+            const uint32_t c = there(i) ? code_of(value_of(bits, job.in.type), g) : 0u;
+            own_codes[i] = (unsigned char)c;
+            sum += (int32_t)c;
         }
-        if (blockIdx.x == 0 && blockIdx.y == 0) {
-            int32_t sums[MT] = {};
-            for (int k = 4 * (int)threadIdx.x; k < in.K; k += 4096)
-#pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    float v[4] = {};
-                    load_four_any(in.x, (int64_t)(row0 + (m < here ? m : 0)) * in.K + k, in.K - k, in.type, v);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        sums[m] += k + j < in.K ? (int32_t)code_of(v[j], g) : 0;
-                }
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                sums[m] = wave_sum(sums[m]);
-                if (lane == 0)
-                    part[wave][m] = sums[m];
-            }
-            __syncthreads();
-            if ((int)threadIdx.x < here) {
-                int32_t sum = 0;
-                for (int i = 0; i < 16; ++i)
-                    sum += part[i][threadIdx.x];
-                in.row_sums[row0 + threadIdx.x] = sum;
-            }
-            if (blockIdx.z == 0 && threadIdx.x == 0) {
-                in.grids->in = g;
-                in.grids->kernel = *in.kernel_grid;
-            }
+        if (blockIdx.x == 0) {
+            sum += __shfl_xor(sum, 8);
+            sum += __shfl_xor(sum, 16);
+            sum += __shfl_xor(sum, 32);
+            if (lane < 8)
+                atomicAdd(&part[lane], sum);   // whole numbers, in any order
+        }
+        if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) {
+            job.grids->in = g;
+            if (job.in.kernel_grid != &job.grids->kernel)
+                job.grids->kernel = *job.in.kernel_grid;
         }
         __syncthreads();
+        if (blockIdx.x == 0 && (int)threadIdx.x < here)
+            job.acc[((int64_t)blockIdx.y * job.rows + row0 + threadIdx.x) * job.pitch + width] = part[threadIdx.x];
     }
-    uint32_t even[H] = {}, odd[H] = {};
+    i32x4 sums[4] = {};
     if (first < last) {
         load_codes(first);
         load_entries();
@@ -400,17 +394,13 @@ __global__ void __launch_bounds__(1024) few_rows_kernel(const uint16_t *__restri
 #pragma unroll
         for (int i = 0; i < kEntries; ++i) {
             const uint32_t sel = i & 1 ? 0x07060302u : 0x05040100u;
-            uint32_t e[2] = {};
-#pragma unroll
-            for (int h = 0; h < (kOf + 1) / 2; ++h)
-                e[h] = __builtin_amdgcn_perm(MT == 1 ? 0u : t[(2 * h + 1) % kOf][i / 2], t[2 * h][i / 2], sel);
-            unsigned char *const to = R + (b0 + i) * 256 + (lane >> 2) * 16 + half * 2;
-            if constexpr (H == 1)
-                *reinterpret_cast<uint32_t *>(to) = e[0];
-            else
-                *reinterpret_cast<uint2 *>(to) = make_uint2(e[0], e[1]);
+            const uint32_t e0 = __builtin_amdgcn_perm(t[1][i / 2], t[0][i / 2], sel);
+            const uint32_t e1 = __builtin_amdgcn_perm(t[3][i / 2], t[2][i / 2], sel);
+            unsigned char *const to = R + own_place + i * 256;
+            *reinterpret_cast<uint32_t *>(to + odd) = odd ? e1 : e0;
+            *reinterpret_cast<uint32_t *>(to + 4 - odd) = odd ? e0 : e1;
         }
-        const uint32_t weights[4] = {w.x, w.y, w.z, w.w};
+        const uint32_t weights[4] = {w[0], w[1], w[2], w[3]};
         if (block + 1 < last) {
             load_entries();
             load_weights(block + 1);
@@ -419,43 +409,246 @@ __global__ void __launch_bounds__(1024) few_rows_kernel(const uint16_t *__restri
         }
         __syncthreads();   // R is whole, and the other one is no longer read
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t e[4][H];
+        for (int q = 0; q < 4; ++q) {
+            // byte 1: the weight, byte 0: the place
+            auto place = [&](int i) { return R + __builtin_amdgcn_perm(weights[q], places, 0x0c0c0400u + 0x0101u * i); };
+            if constexpr (MT == 8) {
+                i32x4 found[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                // byte 1: the weight, byte 0: the place
-                const unsigned char *const from = R + __builtin_amdgcn_perm(weights[i], chunk[i], 0x0c0c0400u + 0x0101u * j);
-                if constexpr (H == 1) {
-                    e[j][0] = *reinterpret_cast<const uint32_t *>(from);
-                } else if constexpr (H == 2) {
-                    const uint2 v = *reinterpret_cast<const uint2 *>(from);
-                    e[j][0] = v.x;
-                    e[j][1] = v.y;
-                } else {
-                    const uint4 v = *reinterpret_cast<const uint4 *>(from);
-                    e[j][0] = v.x;
-                    e[j][1] = v.y;
-                    e[j][2] = v.z;
-                    e[j][3] = v.w;
+                for (int i = 0; i < 4; ++i)
+                    found[i] = *reinterpret_cast<const i32x4 *>(place(i));
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    sums[q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(found[i], one, sums[q], 0, 0, 0);
+            } else {
+                int2 found[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    found[i] = *reinterpret_cast<const int2 *>(place(i));
+#pragma unroll
+                for (int i = 0; i < 4; i += 2)
+                    sums[q] = __builtin_amdgcn_mfma_i32_16x16x64_i8(i32x4{found[i].x, found[i].y, found[i + 1].x, found[i + 1].y}, one,
+                                                                    sums[q], 0, 0, 0);
+            }
+        }
+    }
+    // sums[q][r] is byte n of column 4 * quarter + r: rows n / 2, low and high byte in neighbouring lanes
+    const int32_t flipped = (last - first) * 16 * (128 + 256 * 128);
+    const bool high = n & 1;
+    const int row = row0 + n / 2;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        i32x4 v;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int32_t other = __builtin_amdgcn_update_dpp(0, sums[q][r], 0xb1, 0xf, 0xf, true);   // of lane ^ 1
+            v[r] = (high ? other + 256 * sums[q][r] : sums[q][r] + 256 * other) + flipped;
+        }
+        const int c = column0 + q * 16 + quarter * 4;
+        if ((q & 1) == (int)high && n < 2 * MT && row < job.rows && c < width)
+            *reinterpret_cast<i32x4 *>(job.acc + ((int64_t)blockIdx.y * job.rows + row) * job.pitch + c) = v;
+    }
+}
+
+// ---- one or two rows ----
+// A workgroup holds the whole table in LDS and takes 16 columns, over all of the depth: nothing is left to be joined, and what is
+// made of the sums is made here, in one launch.  A lane has one of the columns and every 64th block of 16 elements.
+// A lookup is a read of two bytes from anywhere in LDS, 64 of which meet in the 64 banks as chance has it (about 10 a cycle and CU,
+// a tenth of what few_rows_kernel finds once R is there), and chance is what is left to them: at step s the lane of column n takes
+// element (n + s) & 15, so that lanes of one block have different input codes, and the table keeps T[a][b] at
+//   [r(a)][b ^ r(a)], r(a) the bits of a turned round,
+// so that neither codes around a mean, nor one input code throughout, make some banks busier than others.  Both bytes of such a place
+// are pairs of bytes of the codes put together, two places at once.
+// One row by 4096 by 4096 takes 11 us on its own, 4 until the input, the first weights and the table are there and 4.4 for the
+// lookups; two rows 15, as many by few_rows_kernel and the launch behind it 18.  One row to 14336 columns: 25.
+constexpr int kTokenTable = 131072;      // bytes of LDS
+constexpr int kTokenCodes = 16384;       // of the input's codes
+constexpr int kTokenColumns = 16;
+constexpr int kTokenRows = 2;
+constexpr int kTokenLds = kTokenTable + kTokenCodes + 2 * 16 * kTokenRows * kTokenColumns * 4 + 256;
+
+__device__ __forceinline__ uint32_t twice_low(uint32_t pair)    // 2 * (pair & 0xffff) and 2 * (pair >> 16)
+{
+    uint32_t r;
+    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:WORD_0" : "=v"(r) : "s"(1), "v"(pair));
+    return r;
+}
+__device__ __forceinline__ uint32_t twice_high(uint32_t pair)
+{
+    uint32_t r;
+    asm("v_lshlrev_b32_sdwa %0, %1, %2 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:WORD_1" : "=v"(r) : "s"(1), "v"(pair));
+    return r;
+}
+
+template <int MT>
+__global__ void __launch_bounds__(1024) token_kernel(TokenJob job)
+{
+    constexpr int kDepth = kTokenCodes / MT, kRounds = kTokenCodes / 4096;   // four codes a thread and round
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    extern __shared__ __align__(16) unsigned char lds[];
+    unsigned char *const codes = lds + kTokenTable;                                // [row][kDepth]
+    uint32_t *const red = reinterpret_cast<uint32_t *>(codes + kTokenCodes);       // [turn][wavefront][row][column]
+    float *const ends = reinterpret_cast<float *>(red + 2 * 16 * MT * kTokenColumns);
+    int32_t *const part = reinterpret_cast<int32_t *>(ends + 32);                  // [row][wavefront]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int n = lane & 15, own = wave * 4 + (lane >> 4);
+    const int K = job.in.K, blocks = job.pieces.Kb / 16, steps = (blocks + 255) / 256;
+    const int groups = (int)((job.columns + kTokenColumns - 1) / kTokenColumns);
+
+    // the input first: it is waited for first
+    float v[kRounds][4];
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+        const int at = (i * 1024 + (int)threadIdx.x) * 4, row = at / kDepth, k = at - row * kDepth;
+        load_four_any(job.in.x, (int64_t)row * K + k, row < MT ? K - k : 0, job.in.type, v[i]);
+    }
+    auto load_weights = [&](int group, int step, uint4(&w)[4]) {
+        const uint32_t c0 = (uint32_t)group * kTokenColumns;
+        const int p = (int)(c0 / (uint32_t)job.pieces.width), width = job.pieces.width_of(p);
+        int c = (int)(c0 - (uint32_t)job.pieces.first(p)) + n;
+        c = c < width ? c : width - 1;   // (lanes behind the columns: nobody stores them)
+        const uint8_t *const from = job.kernel_blocks + job.pieces.block_offset(p) + (size_t)c * 16;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int block = step * 256 + i * 64 + own;
+            w[i] = block < blocks ? *reinterpret_cast<const uint4 *>(from + (size_t)block * width * 16) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    int group = (int)blockIdx.x;
+    uint4 w[4], next[4] = {};
+    load_weights(group, 0, w);
+#pragma unroll
+    for (int i = 0; i < kTokenTable / 16384; ++i)
+        __builtin_amdgcn_global_load_lds(
+            (const __attribute__((address_space(1))) uint32_t *)(reinterpret_cast<const unsigned char *>(job.tableL) +
+                                                                 (i * 1024 + (int)threadIdx.x) * 16),
+            (__attribute__((address_space(3))) uint32_t *)(lds + (i * 1024 + wave * 64) * 16), 16, 0, 0);
+    float lo = INFINITY, hi = -INFINITY;
+    if (!job.in.range.pairs && job.in.range.count < 0) {
+#pragma unroll
+        for (int i = 0; i < kRounds; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if ((i * 1024 + (int)threadIdx.x) * 4 % kDepth + j < K) {
+                    lo = fminf(lo, v[i][j]);
+                    hi = fmaxf(hi, v[i][j]);
+                }
+        block_range(lo, hi, ends);
+    } else {
+        fold(job.in.range, lo, hi, ends);
+    }
+    const Grid in_grid = grid_of_range(lo, hi), kernel_grid = *job.in.kernel_grid;
+    int32_t row_part[MT] = {};
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) {
+        const int at = (i * 1024 + (int)threadIdx.x) * 4, k = at % kDepth;
+        uint32_t word = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t c = k + j < K ? code_of(v[i][j], in_grid) : 0u;
+            word |= (__builtin_bitreverse32(c) >> 24) << (8 * j);
+            row_part[i * 4096 / kDepth] += (int32_t)c;
+        }
+        *reinterpret_cast<uint32_t *>(codes + at) = word;
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        row_part[m] = wave_sum(row_part[m]);
+        if (lane == 0)
+            part[m * 16 + wave] = row_part[m];
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // a barrier alone does not wait for loads into LDS
+    __syncthreads();
+
+    const uint32_t turned = (uint32_t)n & 3u;
+    int order[4];                        // the dwords of a block's codes, this column's first one first
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        order[i] = (((n >> 2) + i) & 3) * 4;
+    for (int turn = 0; group < groups; group += (int)gridDim.x, turn ^= 1) {
+        // a thread a value at the end; what is read for it is read here
+        const int64_t c = (int64_t)group * kTokenColumns + (threadIdx.x & 15);
+        const int row = (int)threadIdx.x / 16;
+        const bool mine = row < MT && c < job.columns;
+        int32_t column_sum = 0;
+        float bias = 0.0f, residual = 0.0f;
+        if (mine) {
+            column_sum = job.column_sums[c];
+            bias = job.out.bias ? load_any(job.out.bias, c, job.out.bias_type) : 0.0f;
+            residual = job.out.residual ? load_any(job.out.residual, row * job.out.ld + c, job.out.type) : 0.0f;
+        }
+        uint32_t sum[MT] = {};
+        for (int s = 0; s < steps; ++s) {
+            const bool end = s + 1 == steps;
+            if (!end || group + (int)gridDim.x < groups)
+                load_weights(end ? group + (int)gridDim.x : group, end ? 0 : s + 1, next);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int block = s * 256 + i * 64 + own;
+                if (block >= blocks)
+                    continue;
+                const unsigned char *const x = codes + block * 16;
+                const uint32_t weights[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    uint32_t d[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        d[q] = *reinterpret_cast<const uint32_t *>(x + m * kDepth + order[q]);
+                    uint32_t found[16];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const uint32_t a = __builtin_amdgcn_alignbyte(d[(q + 1) & 3], d[q], turned);
+                        const uint32_t p = __builtin_amdgcn_perm(0u, a, 0x01010000u) ^ __builtin_amdgcn_perm(0u, weights[q], 0x0c010c00u);
+                        const uint32_t t = __builtin_amdgcn_perm(0u, a, 0x03030202u) ^ __builtin_amdgcn_perm(0u, weights[q], 0x0c030c02u);
+                        found[4 * q] = *reinterpret_cast<const uint16_t *>(lds + twice_low(p));
+                        found[4 * q + 1] = *reinterpret_cast<const uint16_t *>(lds + twice_high(p));
+                        found[4 * q + 2] = *reinterpret_cast<const uint16_t *>(lds + twice_low(t));
+                        found[4 * q + 3] = *reinterpret_cast<const uint16_t *>(lds + twice_high(t));
+                    }
+#pragma unroll
+                    for (int q = 0; q < 16; q += 2)
+                        sum[m] += found[q] + found[q + 1];
                 }
             }
 #pragma unroll
-            for (int j = 0; j < 4; j += 2)
-#pragma unroll
-                for (int h = 0; h < H; ++h) {
-                    even[h] += e[j][h] + e[j + 1][h];
-                    if constexpr (MT > 1)
-                        odd[h] += (e[j][h] >> 16) + (e[j + 1][h] >> 16);
-                }
+            for (int i = 0; i < 4; ++i)
+                w[i] = next[i];
         }
-    }
-    if (c >= width)
-        return;
+        // the four blocks of a wavefront; then, row by row, the wavefronts
+        uint32_t stored = 0;
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-        if (row0 + m < rows)
-            acc[((int64_t)blockIdx.y * rows + row0 + m) * width + c] =
-                (int32_t)(m & 1 ? odd[m / 2] : even[m / 2] - (MT > 1 ? odd[m / 2] << 16 : 0u));
+        for (int m = 0; m < MT; ++m) {
+            sum[m] += (uint32_t)__shfl_xor((int)sum[m], 16);
+            sum[m] += (uint32_t)__shfl_xor((int)sum[m], 32);
+            stored = lane >> 4 == m ? sum[m] : stored;
+        }
+        uint32_t *const to = red + turn * 16 * MT * kTokenColumns;
+        if (lane >> 4 < MT)
+            to[wave * MT * kTokenColumns + lane] = stored;
+        __syncthreads();
+        if (!mine)
+            continue;
+        uint32_t all = 0;
+        int32_t row_sum = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            all += to[i * MT * kTokenColumns + threadIdx.x];
+            row_sum += part[row * 16 + i];
+        }
+        const int64_t zi = in_grid.zero, zk = kernel_grid.zero;
+        const int64_t bracket = (int64_t)all + K * zi * zk - (int64_t)(job.pieces.Kb - K) * job.tableL[0] - zk * row_sum - zi * column_sum;
+        float z = __fmul_rn((float)bracket, __fmul_rn(in_grid.scale, kernel_grid.scale));
+        if (job.out.bias)
+            z = __fadd_rn(z, bias);
+        const int64_t at = row * job.out.ld + c;
+        if (job.out.pre)
+            store_any(job.out.pre, at, job.out.type, z);
+        float y = activate(z, job.out.activation);
+        if (job.out.residual)
+            y = __fadd_rn(y, residual);
+        store_any(job.out.out, at, job.out.type, y);
+    }
 }
 
 // ---- what is made of the sums ----
@@ -532,6 +725,14 @@ __global__ void __launch_bounds__(256) dense_out_parts_kernel(TableSums s, int c
     const int c = ((int)blockIdx.x * 64 + lane) * 4;
     const int64_t r = blockIdx.y;
     i32x4 t = {};
+    int32_t row_sum = 0;
+    if (s.row_sums) {
+        row_sum = s.row_sums[r];
+    } else {
+        for (int i = lane; i < s.raw.splits; i += 64)
+            row_sum += s.raw.acc[r * s.raw.pitch + s.sums_at + i * s.raw.split_stride];
+        row_sum = wave_sum(row_sum);
+    }
     if (c < columns) {
         const int32_t *const p = s.raw.acc + r * s.raw.pitch + c;
 #pragma unroll 8
@@ -548,7 +749,7 @@ __global__ void __launch_bounds__(256) dense_out_parts_kernel(TableSums s, int c
     I column[4];
     float bias[4];
     column_terms(s, b, c, columns, o, column, bias);
-    dense_four<T, I>(sum, b.row(s.row_sums[r]), column, bias, __fmul_rn(s.grids->in.scale, s.grids->kernel.scale), r, c, columns,
+    dense_four<T, I>(sum, b.row(row_sum), column, bias, __fmul_rn(s.grids->in.scale, s.grids->kernel.scale), r, c, columns,
                      whole_fours<T>(c, columns, o), o);
 }
 
@@ -628,11 +829,9 @@ hipError_t launch_range(const void *x, int x_type, int64_t nx, const void *kerne
     return hipGetLastError();
 }
 
-hipError_t launch_few_codes(const void *x, int type, int rows, int K, int Kb, const RangeSource &src, const Grid *kernel_grid,
-                            Grids *grids, uint8_t *codes, int32_t *row_sums, hipStream_t stream)
+hipError_t launch_few_codes(const FewInput &in, int rows, int Kb, Grids *grids, uint8_t *codes, int32_t *row_sums, hipStream_t stream)
 {
-    hipLaunchKernelGGL(few_codes_kernel, dim3(rows), dim3(512), 0, stream, x, type, rows, K, Kb, src, kernel_grid, grids, codes,
-                       row_sums);
+    hipLaunchKernelGGL(few_codes_kernel, dim3(rows), dim3(512), 0, stream, in, rows, Kb, grids, codes, row_sums);
     return hipGetLastError();
 }
 
@@ -660,35 +859,41 @@ int few_rows_splits(int64_t rows, int Kb, int width)
     const int64_t s = want < most ? want : most;
     return (int)(s < least ? least : s);
 }
-
 template <int MT, bool RAW>
-static hipError_t few_rows(const uint16_t *tableI, const uint8_t *x_codes, const FewInput &in, int rows, int Kb,
-                           const uint8_t *kernel_blocks, int width, int splits, int32_t *acc, hipStream_t stream)
+static hipError_t few_rows(const FewJob &job, hipStream_t stream)
 {
     const int bytes = kFewLdsBytes + (RAW ? kFewBlocks * 128 : 0);
     if (hipError_t e = set_max_dynamic_lds_once(reinterpret_cast<const void *>(&few_rows_kernel<MT, RAW>), bytes))
         return e;
     hipLaunchKernelGGL((few_rows_kernel<MT, RAW>),
-                       dim3((unsigned)((width + kFewColumns - 1) / kFewColumns), (unsigned)splits, (unsigned)((rows + 7) / 8)),
-                       dim3(1024), bytes, stream, tableI, x_codes, in, rows, Kb, kernel_blocks, width, acc);
+                       dim3((unsigned)((job.width + kFewColumns - 1) / kFewColumns), (unsigned)job.splits, (unsigned)((job.rows + 7) / 8)),
+                       dim3(1024), bytes, stream, job);
     return hipGetLastError();
 }
-
-hipError_t launch_few_rows(const uint16_t *tableI, const uint8_t *x_codes, const FewInput *raw, int rows, int Kb,
-                           const uint8_t *kernel_blocks, int width, int splits, int32_t *acc, hipStream_t stream)
+hipError_t launch_few_rows(const FewJob &job, hipStream_t stream)
 {
-    const FewInput in = raw ? *raw : FewInput{};
-#define AXC_FEW(MT)                                                                                                         \
-    return raw ? few_rows<MT, true>(tableI, x_codes, in, rows, Kb, kernel_blocks, width, splits, acc, stream)              \
-               : few_rows<MT, false>(tableI, x_codes, in, rows, Kb, kernel_blocks, width, splits, acc, stream)
-    if (rows == 1)
-        AXC_FEW(1);
-    if (rows == 2)
-        AXC_FEW(2);
-    if (rows <= 4)
-        AXC_FEW(4);
-    AXC_FEW(8);
-#undef AXC_FEW
+    if (job.rows <= 4)
+        return job.in.x ? few_rows<4, true>(job, stream) : few_rows<4, false>(job, stream);
+    return job.in.x ? few_rows<8, true>(job, stream) : few_rows<8, false>(job, stream);
+}
+
+bool token_fits(int64_t rows, int Kb)
+{
+    return rows <= kTokenRows && rows * Kb <= kTokenCodes;
+}
+template <int MT>
+static hipError_t token(const TokenJob &job, hipStream_t stream)
+{
+    if (hipError_t e = set_max_dynamic_lds_once(reinterpret_cast<const void *>(&token_kernel<MT>), kTokenLds))
+        return e;
+    // a workgroup a CU, and as many columns in each
+    const int64_t groups = (job.columns + kTokenColumns - 1) / kTokenColumns, each = (groups + device_cus() - 1) / device_cus();
+    hipLaunchKernelGGL(token_kernel<MT>, dim3((unsigned)((groups + each - 1) / each)), dim3(1024), kTokenLds, stream, job);
+    return hipGetLastError();
+}
+hipError_t launch_token(const TokenJob &job, hipStream_t stream)
+{
+    return job.rows == 1 ? token<1>(job, stream) : token<2>(job, stream);
 }
 
 template <typename T, typename I>
@@ -703,7 +908,7 @@ static hipError_t dense_out(const TableSums &s, int64_t rows, int columns, const
         else
             hipLaunchKernelGGL((dense_out_turned_kernel<T, I, 16>), dim3((unsigned)((columns + 15) / 16), by), dim3(256), 0, stream, s,
                                rows, columns, o);
-    } else if (s.raw.splits >= 8 && rows <= 64) {
+    } else if (!s.row_sums || (s.raw.splits >= 8 && rows <= 64)) {
         hipLaunchKernelGGL((dense_out_parts_kernel<T, I>), dim3((unsigned)((columns + 255) / 256), (unsigned)rows), dim3(256), 0,
                            stream, s, columns, o);
     } else {

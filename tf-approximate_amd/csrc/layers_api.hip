@@ -89,8 +89,8 @@ Pieces pieces_of(int64_t depth, int64_t columns, int64_t most)
 // ---- sums of table entries: input codes by a piece of the kernel's ----
 constexpr int64_t kRowRun = 16384;       // rows a LUT-GEMM call takes (its rows must be below 32768)
 constexpr int64_t kSumsAtOnce = (int64_t)1 << 25;   // int32 sums in the workspace: 128 MiB, half the memory-side cache
-// Up to here few_rows_kernel is the shorter one, by rows (us, packed 4096 -> 4096: 16 rows 33, 63 by the kernels of many rows, 32 rows
-// 50 and 65, 64 rows 90 and 76; 4096 -> 14336, 16 rows 84 and 131, 32 rows 145 and 141).
+// Up to here few_rows_kernel is the shorter one, by rows (us, packed 4096 -> 4096: 16 rows 29, 63 by the kernels of many rows, 32 rows
+// 48 and 65, 64 rows about 85 and 72; 4096 -> 14336, 32 rows 131 and 141).
 constexpr int64_t kFewRowsMost = 32;
 
 bool few_rows(int64_t rows) { return rows <= kFewRowsMost; }
@@ -119,7 +119,7 @@ int sums_workspace(bool few, int64_t rows, const Pieces &pc, size_t *count, size
 {
     for (const int width : {pc.width_of(0), pc.width_of(pc.count - 1)}) {
         if (few) {
-            *count = std::max(*count, (size_t)few_rows_splits(rows, pc.Kb, width) * rows * width);
+            *count = std::max(*count, (size_t)few_rows_splits(rows, pc.Kb, width) * rows * (width + 4));
             continue;
         }
         const axc_conv2d_desc c = conv_desc(fours(rows), pc.Kp, width);
@@ -138,7 +138,7 @@ struct Operands {
     float *x_pairs, *kernel_pairs;
     uint8_t *x_codes, *kernel_codes, *kernel_blocks;
     int32_t *row_sums, *column_sums;
-    const FewInput *raw;                 // not null: few_rows_kernel makes the input's codes itself
+    FewInput raw;                        // x not null: few_rows_kernel makes the input's codes itself
 };
 
 Operands carve_operands(Carver &c, const axc_dense_desc *d, const Pieces &pc, bool with_kernel, bool codes)
@@ -220,22 +220,33 @@ int make_few_codes(const axc_dense_desc *d, const void *input, const void *range
                    const Pieces &pc, hipStream_t stream)
 {
     ApiTimer t("layer_codes", stream);
-    AXC_HIP(launch_few_codes(input, d->input_type, (int)d->rows, (int)d->depth, pc.Kb, input_source(d, range), kernel_grid, o.grids,
-                             o.x_codes, o.row_sums, stream));
+    const FewInput in = {input, d->input_type, (int)d->depth, input_source(d, range), kernel_grid};
+    AXC_HIP(launch_few_codes(in, (int)d->rows, pc.Kb, o.grids, o.x_codes, o.row_sums, stream));
     return AXC_OK;
+}
+
+// The same of a kernel alone.
+int make_kernel_codes(const axc_dense_desc *d, const void *kernel, const Operands &o, const Pieces &pc, hipStream_t stream)
+{
+    RangeSource in, k;
+    if (int rc = find_ranges(d, nullptr, nullptr, kernel, nullptr, o.kernel_pairs, o.column_sums, pc.Np, &in, &k, stream))
+        return rc;
+    return make_codes(d, nullptr, in, kernel, k, nullptr, o, pc, stream);
 }
 
 // Ranges, grids, codes and their sums of both operands.
 int find_codes(const axc_dense_desc *d, const void *input, const void *range, const void *kernel, const Operands &o, const Pieces &pc,
                hipStream_t stream)
 {
-    const bool few = few_rows(d->rows);
+    if (few_rows(d->rows)) {
+        if (int rc = make_kernel_codes(d, kernel, o, pc, stream))
+            return rc;
+        return make_few_codes(d, input, range, nullptr, o, pc, stream);
+    }
     RangeSource in, k;
-    if (int rc = find_ranges(d, few ? nullptr : input, range, kernel, o.x_pairs, o.kernel_pairs, o.column_sums, pc.Np, &in, &k, stream))
+    if (int rc = find_ranges(d, input, range, kernel, o.x_pairs, o.kernel_pairs, o.column_sums, pc.Np, &in, &k, stream))
         return rc;
-    if (int rc = make_codes(d, few ? nullptr : input, in, kernel, k, nullptr, o, pc, stream))
-        return rc;
-    return few ? make_few_codes(d, input, range, nullptr, o, pc, stream) : AXC_OK;
+    return make_codes(d, input, in, kernel, k, nullptr, o, pc, stream);
 }
 
 // Sums of the run of rows from r on and piece p, in acc or in the scratch, as their consumer is given them.
@@ -253,10 +264,15 @@ int table_sums(const axc_table *table, const axc_dense_desc *d, const Operands &
     out->pad = (few ? pc.Kb : pc.Kp) - (int)d->depth;
     if (few) {
         const int splits = few_rows_splits(rows, pc.Kb, width);
-        out->raw = {acc, rows * width, splits, width, 0};
+        if (o.raw.x) {
+            out->row_sums = nullptr;
+            out->sums_at = width;
+        }
+        const FewJob job = {table->dev_tableS, o.raw, o.x_codes, o.grids, o.kernel_blocks + pc.block_offset(p), (int)rows, pc.Kb, width,
+                            splits, acc, width + 4};
+        out->raw = {acc, rows * job.pitch, splits, job.pitch, 0};
         ApiTimer t("few_rows", stream);
-        AXC_HIP(launch_few_rows(table->dev_tableI, o.x_codes, o.raw, (int)rows, pc.Kb, o.kernel_blocks + pc.block_offset(p), width,
-                                splits, acc, stream));
+        AXC_HIP(launch_few_rows(job, stream));
         return AXC_OK;
     }
     const axc_conv2d_desc c = conv_desc(fours(rows), pc.Kp, width);
@@ -311,6 +327,9 @@ int carve_dense(const axc_dense_desc *d, bool packed, void *base, DenseScratch *
 {
     const Pieces pc = pieces_of(d->depth, d->columns, kDensePiece);
     Carver c(base);
+    *s = {};
+    if (packed && token_fits(d->rows, pc.Kb))
+        return AXC_OK;                   // nothing is kept
     s->o = carve_operands(c, d, pc, !packed, true);
     size_t count = 0;
     if (int rc = runs_workspace(d->rows, dense_run(d->rows, pc), pc, &count, &s->lut_bytes))
@@ -355,15 +374,13 @@ int axc_dense_pack(const axc_dense_desc *desc, const void *kernel, void *packed,
     hipStream_t stream = static_cast<hipStream_t>(stream_v);
     const Pieces pc = pieces_of(desc->depth, desc->columns, kDensePiece);
     const Packed p = packed_parts(pc, packed);
-    RangeSource in, k;
-    if (int rc = find_ranges(desc, nullptr, nullptr, kernel, nullptr, p.pairs, p.column_sums, pc.Np, &in, &k, stream))
-        return rc;
     Operands o = {};
     o.grids = p.grids;
+    o.kernel_pairs = p.pairs;
     o.kernel_codes = p.codes;
     o.kernel_blocks = p.blocks;
     o.column_sums = p.column_sums;
-    return make_codes(desc, nullptr, in, kernel, k, nullptr, o, pc, stream);
+    return make_kernel_codes(desc, kernel, o, pc, stream);
 }
 
 int axc_fake_approx_dense_workspace_bytes(const axc_dense_desc *desc, int packed, size_t *bytes)
@@ -405,27 +422,38 @@ int axc_fake_approx_dense(const axc_table *table, const axc_dense_desc *desc, co
     if (int rc = check_workspace(workspace, workspace_bytes, s.bytes))
         return rc;
     hipStream_t stream = static_cast<hipStream_t>(stream_v);
-    const int K = (int)desc->depth;
     Operands &o = s.o;
-    FewInput raw = {};
+    const Grid *kernel_grid = nullptr;   // of a packed kernel
     if (packed) {
         const Packed p = packed_parts(pc, const_cast<void *>(packed));
         o.kernel_codes = p.codes;
         o.kernel_blocks = p.blocks;
         o.column_sums = p.column_sums;
-        if (few_rows(desc->rows)) {
-            raw = {input, desc->input_type, K, input_source(desc, input_range), &p.grids->kernel, o.grids, o.row_sums};
-            if (desc->rows * desc->depth <= kFewRawValues || raw.range.count >= 0)
-                o.raw = &raw;
-            else if (int rc = make_few_codes(desc, input, input_range, &p.grids->kernel, o, pc, stream))
+        kernel_grid = &p.grids->kernel;
+    }
+    if (few_rows(desc->rows)) {
+        if (!packed)
+            if (int rc = make_kernel_codes(desc, kernel, o, pc, stream))
                 return rc;
-        } else {
-            RangeSource in, none;
-            if (int rc = find_ranges(desc, input, input_range, nullptr, o.x_pairs, nullptr, nullptr, 0, &in, &none, stream))
-                return rc;
-            if (int rc = make_codes(desc, input, in, nullptr, none, &p.grids->kernel, o, pc, stream))
-                return rc;
+        const FewInput in = {input, desc->input_type, (int)desc->depth, input_source(desc, input_range),
+                             packed ? kernel_grid : &o.grids->kernel};
+        if (token_fits(desc->rows, pc.Kb)) {
+            const TokenJob job = {table->dev_tableL, in, o.kernel_blocks, o.column_sums, pc, (int)desc->rows, desc->columns,
+                                  {bias, residual, output, pre, desc->bias_type, desc->input_type, desc->activation, desc->columns}};
+            ApiTimer t("token", stream);
+            AXC_HIP(launch_token(job, stream));
+            return AXC_OK;
         }
+        if (desc->rows * desc->depth <= kFewRawValues || in.range.count >= 0)
+            o.raw = in;
+        else if (int rc = make_few_codes(desc, input, input_range, kernel_grid, o, pc, stream))
+            return rc;
+    } else     if (packed) {
+        RangeSource in, none;
+        if (int rc = find_ranges(desc, input, input_range, nullptr, o.x_pairs, nullptr, nullptr, 0, &in, &none, stream))
+            return rc;
+        if (int rc = make_codes(desc, input, in, nullptr, none, kernel_grid, o, pc, stream))
+            return rc;
     } else if (int rc = find_codes(desc, input, input_range, kernel, o, pc, stream)) {
         return rc;
     }

@@ -25,6 +25,19 @@ __device__ __forceinline__ float load_any(const void *p, int64_t i, int type)
         return (float)static_cast<const bf16 *>(p)[i];
     return (float)static_cast<const f16 *>(p)[i];
 }
+// The same in two steps: nothing waits for the first.
+__device__ __forceinline__ uint32_t load_bits(const void *p, int64_t i, int type)
+{
+    return type == AXC_F32 ? static_cast<const uint32_t *>(p)[i] : static_cast<const uint16_t *>(p)[i];
+}
+__device__ __forceinline__ float value_of(uint32_t bits, int type)
+{
+    if (type == AXC_F32)
+        return __builtin_bit_cast(float, bits);
+    if (type == AXC_BF16)
+        return __builtin_bit_cast(float, bits << 16);
+    return (float)__builtin_bit_cast(f16, (uint16_t)bits);
+}
 __device__ __forceinline__ void store_any(void *p, int64_t i, int type, float v)
 {
     if (type == AXC_F32)
@@ -175,35 +188,38 @@ __device__ __forceinline__ int32_t wave_sum(int32_t v)
         v += __shfl_xor(v, s);
     return v;
 }
+// Smallest and largest, the same way: a lane that nothing moves to keeps its own.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float moved(float v)
+{
+    const int i = __builtin_bit_cast(int, v);
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, CTRL, ROWS, 0xf, false));
+}
 __device__ __forceinline__ float wave_max(float v)
 {
-#pragma unroll
-    for (int s = 32; s > 0; s >>= 1)
-        v = fmaxf(v, __shfl_xor(v, s));
-    return v;
+    v = fmaxf(v, moved<0x111, 0xf>(v));
+    v = fmaxf(v, moved<0x112, 0xf>(v));
+    v = fmaxf(v, moved<0x114, 0xf>(v));
+    v = fmaxf(v, moved<0x118, 0xf>(v));
+    v = fmaxf(v, moved<0x142, 0xa>(v));
+    v = fmaxf(v, moved<0x143, 0xc>(v));
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
-__device__ __forceinline__ float wave_min(float v)
-{
-#pragma unroll
-    for (int s = 32; s > 0; s >>= 1)
-        v = fminf(v, __shfl_xor(v, s));
-    return v;
-}
+__device__ __forceinline__ float wave_min(float v) { return -wave_max(-v); }
 // Smallest and largest over a workgroup, in every thread.  red: 2 * waves floats of LDS, free before and after.
 __device__ __forceinline__ void block_range(float &lo, float &hi, float *red)
 {
-    const int wave = threadIdx.x / 64, waves = blockDim.x / 64;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64, waves = blockDim.x / 64;
     lo = wave_min(lo);
     hi = wave_max(hi);
-    if ((threadIdx.x & 63) == 0) {
+    if (lane == 0) {
         red[2 * wave] = lo;
         red[2 * wave + 1] = hi;
     }
     __syncthreads();
-    for (int i = 0; i < waves; ++i) {
-        lo = fminf(lo, red[2 * i]);
-        hi = fmaxf(hi, red[2 * i + 1]);
-    }
+    const int of = lane < waves ? lane : 0;
+    lo = wave_min(red[2 * of]);
+    hi = wave_max(red[2 * of + 1]);
     __syncthreads();
 }
 
@@ -322,12 +338,12 @@ struct Pieces {
 };
 
 constexpr int kRangeBlocks = 256;        // pairs that the range pass leaves per tensor, at most
-constexpr int kFewRows = 8;              // rows that the kernel for few rows takes at a time
 
 // Sums of table entries as a consumer finds them, of one piece and one run of rows.
 struct TableSums {
     RawSums raw;                         // (every fourth row and column begins 16-byte aligned)
-    const int32_t *row_sums;             // sums of the input's codes, of the run's first row on
+    const int32_t *row_sums;             // sums of the input's codes, of the run's first row on; null: a column behind the sums' last
+    int sums_at;                         // (that column)
     const int32_t *column_sums;          // sums of the kernel's codes, of the piece's first column on
     const uint16_t *table;               // its first entry is T[0][0]
     const Grids *grids;
@@ -387,30 +403,50 @@ struct CodesJob {
     int32_t *row_sums, *column_sums;     // (those of the columns are added to)
 };
 hipError_t launch_codes(const CodesJob &job, hipStream_t stream);
-// Few rows: range (where src says so), grid, codes and their sums of the input in one launch; a kernel_grid that is not null is
-// copied next to it.
-hipError_t launch_few_codes(const void *x, int type, int rows, int K, int Kb, const RangeSource &src, const Grid *kernel_grid,
-                            Grids *grids, uint8_t *codes, int32_t *row_sums, hipStream_t stream);
-int few_rows_splits(int64_t rows, int Kb, int width);
-struct FewInput {                        // for few_rows_kernel where it makes the codes of the input itself
-    const void *x;
-    int type, K;
-    RangeSource range;
-    const Grid *kernel_grid;
-    Grids *grids;
-    int32_t *row_sums;
-};
-// Where every workgroup may read all of the input for its range: beyond that a launch of its own is as short (us a call with and
-// without one, 4096 -> 4096: 1 row 17.8 and 14.4, 4 rows 19.4 and 18.1, 8 rows 25; 4096 -> 14336, 4 rows: 41.4 and 44.7).
-constexpr int64_t kFewRawValues = 8192;
-hipError_t launch_few_rows(const uint16_t *tableI, const uint8_t *x_codes, const FewInput *raw, int rows, int Kb,
-                           const uint8_t *kernel_blocks, int width, int splits, int32_t *acc, hipStream_t stream);
 struct DenseOut {
     const void *bias, *residual;         // of the piece's / run's first element
     void *out, *pre;
     int bias_type, type, activation;
     int64_t ld;                          // columns of the layer
 };
+struct FewInput {                        // few rows of an input, and where its grid and the kernel's come from
+    const void *x;
+    int type, K;
+    RangeSource range;
+    const Grid *kernel_grid;
+};
+// Range (where it is not known), grid, codes and their sums of the input in one launch; a kernel_grid that is not null is copied
+// next to it.
+hipError_t launch_few_codes(const FewInput &in, int rows, int Kb, Grids *grids, uint8_t *codes, int32_t *row_sums, hipStream_t stream);
+constexpr int kFewRowsAtOnce = 8;        // rows that a workgroup of few_rows_kernel takes
+struct FewJob {
+    const uint16_t *tableS;
+    FewInput in;                         // x not null: the input as it is, its grid and the kernel's go to *grids, else:
+    const uint8_t *x_codes;
+    Grids *grids;
+    const uint8_t *kernel_blocks;        // of a piece
+    int rows, Kb, width, splits;
+    int32_t *acc;                        // [splits][rows][pitch]; of an input as it is, the rows' sums are column `width`
+    int pitch;
+};
+// Where every workgroup may read all of the input for its range: beyond that a launch of its own is as short (us a call without and
+// with one, 4096 -> 4096: 8 rows 22 and 25).
+constexpr int64_t kFewRawValues = 65536;
+int few_rows_splits(int64_t rows, int Kb, int width);
+hipError_t launch_few_rows(const FewJob &job, hipStream_t stream);
+
+struct TokenJob {                        // one or two rows, and all that is made of them, in one launch
+    const uint16_t *tableL;
+    FewInput in;
+    const uint8_t *kernel_blocks;
+    const int32_t *column_sums;
+    Pieces pieces;
+    int rows;
+    int64_t columns;
+    DenseOut out;
+};
+bool token_fits(int64_t rows, int Kb);   // whether a workgroup has room for all of the input's codes
+hipError_t launch_token(const TokenJob &job, hipStream_t stream);
 hipError_t launch_zero(void *p, int64_t bytes, hipStream_t stream);   // a kernel: callers may capture it
 hipError_t launch_dense_out(const TableSums &s, int64_t rows, int columns, const DenseOut &o, hipStream_t stream);
 
@@ -521,7 +557,7 @@ struct axc_table {
     uint16_t *dev_tableT; // [257 filter code][256 input code]; row 256 is zero
     uint16_t *dev_tableF; // behind it in the same allocation: the same with the top bit of every byte flipped,
     uint16_t *dev_tableS; // and [257 input code][256 filter code], flipped too
-    uint16_t *dev_tableI; // [256 input code][256 filter code], as the caller gave it
+    uint16_t *dev_tableL; // T[a][b] at [r][b ^ r], r the bits of a turned round, for single tokens
     int device;
 };
 
