@@ -58,6 +58,52 @@ def test_forward(pkg, tables, size, x_dtype, k_dtype):
     assert torch.equal(layer(x, layer.pack(k), bias, residual), y)
 
 
+FEW = [
+    # one and two rows: all of the input's codes in a workgroup, and just too many; columns beyond a workgroup a CU, and of several pieces
+    (1, 16384, 50), (1, 16385, 20), (2, 8192, 40), (2, 8193, 40), (1, 4100, 4200), (1, 30, 16450), (2, 20, 8210), (2, 1030, 4110),
+    # more: parts of one block of the depth and of several, groups of eight rows that end early
+    (4, 12, 8201), (6, 4000, 70), (13, 700, 2050), (31, 17, 3000), (32, 2500, 1030), (8, 32764, 24),
+]
+
+
+@pytest.mark.parametrize("size", FEW, ids=str)
+@pytest.mark.parametrize("x_dtype", [F32, BF16], ids=str)
+def test_few_rows(pkg, tables, size, x_dtype):
+    print("size", size, x_dtype, flush=True)
+    rows, depth, columns = size
+    table, handle = tables["random"]
+    x, k = make((rows, depth), rows, x_dtype, 1.0, -0.4), make((depth, columns), columns + 1, BF16, depth ** -0.5)
+    bias, residual = make((columns,), 3, F16), make((rows, columns), 4, x_dtype)
+    layer = pkg.FakeApproxDense(handle, "gelu")
+    y, pre = layer.call_and_keep(x, layer.pack(k), bias, residual)
+    want, z, y_off, z_off = ref.dense(table, ref.Grid(pkg, x), ref.Grid(pkg, k), bias, residual, "gelu")
+    ref.check(pre, z, ref.rounded(z, z_off, x_dtype), "pre")
+    ref.check(y, want, ref.rounded(want, y_off, x_dtype), "output")
+    assert torch.equal(layer(x, k, bias, residual), y)
+
+
+@pytest.mark.parametrize("rows", [1, 2])
+def test_nan_in_a_token(pkg, tables, rows):
+    """NaN widens no range and has the upper end's code."""
+    layer = pkg.FakeApproxDense(tables["noisy"][1])
+    x, k = make((rows, 23), 1), make((23, 20), 2)
+    n, m = x.clone(), x.clone()
+    n[0, 3], m[0, 3] = float("nan"), 1e30
+    kept = torch.cat([x.flatten()[:3], x.flatten()[4:]])
+    fixed = pkg.FakeApproxDense(tables["noisy"][1], input_minmax=tuple(float(v) for v in kept.aminmax()))
+    for kernel in (k, layer.pack(k)):
+        assert torch.equal(layer(n, kernel), fixed(m, kernel))
+
+
+def test_a_range_set_later(pkg, tables):
+    layer = pkg.FakeApproxDense(tables["noisy"][1])
+    x, k = make((5, 23), 1), make((23, 20), 2)
+    own = layer(x, k)
+    layer.input_minmax = (-8.0, 8.0)
+    wide = layer(x, k)
+    assert torch.equal(wide, pkg.FakeApproxDense(tables["noisy"][1], input_minmax=(-8.0, 8.0))(x, k)) and not torch.equal(wide, own)
+
+
 @pytest.mark.parametrize("rows", [1, 4, 16, 40])
 @pytest.mark.parametrize("lo,hi", [(-1.0, 1.0), (0.0, 2.5), (0.5, 3.0), (-4.0, -0.25)])
 def test_fixed_range(pkg, tables, rows, lo, hi):

@@ -365,3 +365,17 @@ def test_together_in_a_graph(pkg):
         torch.cuda.synchronize()
         for name in s:
             assert torch.equal(s[name], want[name]), name
+
+
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+def test_no_rows(pkg, kind):
+    norm = pkg.ResidualNorm(kind, EPS)
+    x, w, gate = make((0, 3, 32), 1), make((32,), 3), make((1, 32), 4)
+    args = (x, w, w, gate, w, w)
+    h, y, seen = norm.call_in_turn(x, *args)
+    assert h.shape == x.shape and y.shape == x.shape and seen is None
+    assert norm(x, x, w, gate=make((0, 32), 4), scale=w)[0].shape == x.shape
+    g = norm.gradients(h, y, h, *args)
+    assert g.x.shape == x.shape and g.block.shape == x.shape
+    for sums in (g.weight, g.bias, g.scale, g.post_weight, g.gate):
+        assert not sums.any()

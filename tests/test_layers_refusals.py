@@ -119,3 +119,11 @@ def test_empty_calls_do_nothing(pkg):
     n = ctypes.c_size_t(5)
     assert lib.axc_fake_approx_dense_gradients_workspace_bytes(ctypes.byref(dense(pkg, rows=0)), ctypes.byref(n)) == 0
     assert n.value == 0
+
+
+def test_no_rows_have_no_block(pkg):
+    """The tensors of a call without rows hold nothing, and may stand nowhere."""
+    lib = pkg._lib.load()
+    T = pkg._lib.ResidualNormTensors
+    assert lib.axc_residual_norm(ctypes.byref(norm(pkg, rows=0)), ctypes.byref(T(None, None, 256, None, None, 256, 256)), None, None,
+                                 None, None) == 0

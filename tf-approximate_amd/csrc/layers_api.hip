@@ -810,7 +810,7 @@ static int norm_params(const axc_residual_norm_desc *d, const axc_residual_norm_
         return api_fail(AXC_INVALID_ARGUMENT, "null argument");
     if (!in->weight)
         return api_fail(AXC_INVALID_ARGUMENT, "null tensor pointer");
-    if (!in->block && (in->gate || in->scale || in->post_weight))
+    if (d->rows > 0 && !in->block && (in->gate || in->scale || in->post_weight))
         return api_fail(AXC_INVALID_ARGUMENT, "a gate, a scale and a weight of the block's norm need a block");
     if ((in->gate != nullptr) != (d->gate_groups > 0))
         return api_fail(AXC_INVALID_ARGUMENT, "a gate and its number of groups go together");

@@ -129,7 +129,8 @@ class FakeApproxDense:
 
     def _desc(self, inputs, depth, columns, kernel_dtype, bias):
         """(description, reference to it) of a call: made once for its shapes and types."""
-        key = (inputs.shape, inputs.dtype, depth, columns, kernel_dtype, None if bias is None else bias.dtype)
+        key = (inputs.shape, inputs.dtype, depth, columns, kernel_dtype, None if bias is None else bias.dtype, self.activation,
+               self.input_minmax)
         found = self._descs.get(key)
         if found is None:
             desc = _dense_desc(inputs, depth, columns, kernel_dtype, bias, self.activation, self.input_minmax)
