@@ -14,6 +14,8 @@
 // stores.
 #include "layers_internal.h"
 
+#include <algorithm>
+
 namespace axc {
 namespace {
 
@@ -295,9 +297,7 @@ struct Results {
 };
 
 constexpr int kStep = 64;   // of the depth
-constexpr int kGroups = 2;  // of four wavefronts, which take the steps in turn
-constexpr int kProductThreads = kGroups * 256;
-constexpr int kProductLds = kGroups * 2 * 2 * kProductTile * kStep * 2;
+constexpr int product_lds(int groups) { return groups * 2 * 2 * kProductTile * kStep * 2; }
 
 __device__ __forceinline__ void load_to_lds(const bf16 *from, bf16 *to)
 {
@@ -331,30 +331,59 @@ __global__ void __launch_bounds__(512) column_sums_kernel(ColumnJob job)
     column_sums(job, (int)blockIdx.x, red);
 }
 
-// A tile of 128 x 128 by two groups of four wavefronts, each of which multiplies every other step of the depth, 64 x 64 a wavefront,
-// and has two buffers of 64 of the depth in LDS, filled straight from memory while the other is multiplied: two wavefronts a SIMD, so
-// that one reads while the other multiplies, where there are no more tiles than CUs.  At the end the groups exchange half of their
-// sums each.
+// A tile of 128 x 128 by G groups of four wavefronts, each of which multiplies every G-th step of the depth, 64 x 64 a wavefront,
+// and has two buffers of 64 of the depth in LDS, filled straight from memory while the other is multiplied.  Two wavefronts a SIMD, so
+// that one reads while the other multiplies, are two workgroups of one group where there are tiles enough (one's end then goes on under
+// the other's steps), else the two groups of one, which at the end exchange half of their sums each.
 // In LDS a line of 64 elements is eight chunks of 16 bytes, chunk q of line r in place q ^ (r & 7): the 16 lanes that read
 // neighbouring lines then meet different banks.  The loads write LDS in order, so it is their addresses that are exchanged.
-// PARTIAL: sums go to `partials` (added to what is there with `accumulate`).  Workgroups behind the tiles add up the columns of `job`.
-template <typename T, bool PARTIAL>
-__global__ void __launch_bounds__(kProductThreads) product_kernel(const bf16 *__restrict__ a, const bf16 *__restrict__ b, int64_t rows,
-                                                         int64_t cols, int row_tiles, int col_tiles, int depth, int parts,
-                                                         int split_a, int splits, float *__restrict__ partials, int accumulate,
-                                                         ProductOut o, ColumnJob job)
+// One launch makes both of a layer's products, and the column sums of `job` in workgroups behind their tiles: 78 us for 4096 rows,
+// 1024 -> 4096, in bfloat16, 883 TFLOP/s (88 one after the other), 115 for a loss of 1024 rows, 512 -> 32 000 (144).
+template <typename T, typename V>
+__device__ __forceinline__ void store_tile(const Product &j, int row_tile, int col_tile, int64_t r0, int64_t c0, const V &sum)
+{
+    constexpr int R = sizeof(V) / sizeof(sum[0]);
+    const Results<T> results(j.o);
+    // What is read for the results is read all at once, where the tile has no edge: value by value it took as long as the product.
+    if (results.aligned && (int64_t)(row_tile + 1) * kProductTile <= j.rows && (int64_t)(col_tile + 1) * kProductTile <= j.cols) {
+        typename Results<T>::four at[R][4];
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                at[i][k] = results.values_at(r0 + i * 16, c0 + k * 16);
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                results.store(r0 + i * 16, c0 + k * 16, at[i][k], sum[i][k]);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (r0 + i * 16 < j.rows && c0 + k * 16 < j.cols)
+                results.store_some(r0 + i * 16, c0 + k * 16, j.cols, sum[i][k]);
+}
+template <int G>
+__global__ void __launch_bounds__(G * 256) products_kernel(Product first_product, int first_tiles, Product second_product, int tiles,
+                                                           ColumnJob job)
 {
     extern __shared__ __align__(16) bf16 lds_raw[];
-    // Workgroups go round the eight XCDs; each XCD gets a run of neighbouring tiles, in bands of eight row tiles, so that its L2
-    // serves them.
-    const int tiles = row_tiles * col_tiles * splits;
     int id = (int)blockIdx.x;
     if (id >= tiles) {
         column_sums(job, id - tiles, reinterpret_cast<float *>(lds_raw));
         return;
     }
+    const Product &j = id < first_tiles ? first_product : second_product;
+    const int row_tiles = (int)(product_pad(j.rows) / kProductTile), col_tiles = (int)(product_pad(j.cols) / kProductTile);
+    // Workgroups go round the eight XCDs; each XCD gets a run of neighbouring tiles, in bands of eight row tiles, so that its L2
+    // serves them.
     {
-        const int per = tiles / 8, more = tiles % 8, xcd = id % 8;
+        const int own = id < first_tiles ? first_tiles : tiles - first_tiles;
+        id -= id < first_tiles ? 0 : first_tiles;
+        const int per = own / 8, more = own % 8, xcd = id % 8;
         id = xcd * per + (xcd < more ? xcd : more) + id / 8;
     }
     const int split = id / (row_tiles * col_tiles);
@@ -362,6 +391,8 @@ __global__ void __launch_bounds__(kProductThreads) product_kernel(const bf16 *__
     const int band = id / (8 * col_tiles), in_band = id - band * 8 * col_tiles;
     const int band_rows = row_tiles - band * 8 < 8 ? row_tiles - band * 8 : 8;
     const int row_tile = band * 8 + in_band % band_rows, col_tile = in_band / band_rows;
+    const bf16 *const a = j.a, *const b = j.b;
+    const int depth = j.depth, parts = j.parts, split_a = j.split_a, splits = j.splits;
 
     const int lane = threadIdx.x & 63, wave8 = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wave = wave8 & 3, part = wave8 >> 2;
     bf16(*const lds)[2][kProductTile * kStep] = reinterpret_cast<bf16(*)[2][kProductTile * kStep]>(lds_raw) + part * 2;
@@ -384,16 +415,16 @@ __global__ void __launch_bounds__(kProductThreads) product_kernel(const bf16 *__
 
     f32x4 acc[4][4] = {};
     const int wr = (wave >> 1) * 64, wc = (wave & 1) * 64, in_line = lane & 15, group = lane >> 4;
-    const int rounds = (last - first + kGroups - 1) / kGroups;
+    const int rounds = (last - first + G - 1) / G;
     if (first + part < last)
         fetch(first + part, 0);
     for (int round = 0; round < rounds; ++round) {
-        const int step = first + round * kGroups + part, buffer = round & 1;
+        const int step = first + round * G + part, buffer = round & 1;
         // This buffer is full once the loads of all of its wavefronts have come (a barrier alone does not wait for loads into LDS), and
         // nobody reads the other any more.
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (step + kGroups < last)
-            fetch(step + kGroups, buffer ^ 1);
+        if (step + G < last)
+            fetch(step + G, buffer ^ 1);
         if (step >= last)
             continue;
 #pragma unroll
@@ -412,84 +443,87 @@ __global__ void __launch_bounds__(kProductThreads) product_kernel(const bf16 *__
                     acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j], fa[i], acc[i][j], 0, 0, 0);
         }
     }
-    // the other group's half of the sums for this one's: rows 0 and 1 of four for the first group
-    f32x4 *const give = reinterpret_cast<f32x4 *>(lds_raw) + (wave * 8) * 64 + lane;   // [wavefront][8][64], twice
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            give[part * 2048 + (i * 4 + j) * 64] = part == 0 ? acc[i + 2][j] : acc[i][j];
-    __syncthreads();
-    f32x4 sum[2][4];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            sum[i][j] = (part == 0 ? acc[i][j] : acc[i + 2][j]) + give[(1 - part) * 2048 + (i * 4 + j) * 64];
-    // What is read for the results is read all at once, where the tile has no edge: value by value it took as long as the product.
-    const int64_t r0 = (int64_t)row_tile * kProductTile + wr + part * 32 + in_line, c0 = (int64_t)col_tile * kProductTile + wc + group * 4;
-    if constexpr (PARTIAL) {
-        const int64_t rows_pad = (int64_t)row_tiles * kProductTile, cols_pad = (int64_t)col_tiles * kProductTile;
-        float *const to = partials + ((int64_t)split * rows_pad + r0) * cols_pad + c0;
-        if (accumulate) {
-            f32x4 was[2][4];
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    was[i][j] = *reinterpret_cast<const f32x4 *>(to + i * 16 * cols_pad + j * 16);
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    sum[i][j] += was[i][j];
-        }
+    constexpr int R = 4 / G;             // of a wavefront's rows of four by 16 columns
+    f32x4 sum[R][4];
+    if constexpr (G == 2) {
+        // the other group's half of the sums for this one's: rows 0 and 1 of four for the first group
+        f32x4 *const give = reinterpret_cast<f32x4 *>(lds_raw) + (wave * 8) * 64 + lane;   // [wavefront][8][64], twice
+        __syncthreads();
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                *reinterpret_cast<f32x4 *>(to + i * 16 * cols_pad + j * 16) = sum[i][j];
+            for (int k = 0; k < 4; ++k)
+                give[part * 2048 + (i * 4 + k) * 64] = part == 0 ? acc[i + 2][k] : acc[i][k];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                sum[i][k] = (part == 0 ? acc[i][k] : acc[i + 2][k]) + give[(1 - part) * 2048 + (i * 4 + k) * 64];
     } else {
-        const Results<T> results(o);
-        if (results.aligned && (int64_t)(row_tile + 1) * kProductTile <= rows && (int64_t)(col_tile + 1) * kProductTile <= cols) {
-            typename Results<T>::four at[2][4];
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < R; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    at[i][j] = results.values_at(r0 + i * 16, c0 + j * 16);
+            for (int k = 0; k < 4; ++k)
+                sum[i][k] = acc[i][k];
+    }
+    const int64_t r0 = (int64_t)row_tile * kProductTile + wr + part * 32 + in_line, c0 = (int64_t)col_tile * kProductTile + wc + group * 4;
+    if (j.partials) {
+        const int64_t rows_pad = (int64_t)row_tiles * kProductTile, cols_pad = (int64_t)col_tiles * kProductTile;
+        float *const to = j.partials + ((int64_t)split * rows_pad + r0) * cols_pad + c0;
+        if (j.accumulate) {
+            f32x4 was[R][4];
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < R; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    results.store(r0 + i * 16, c0 + j * 16, at[i][j], sum[i][j]);
-        } else {
+                for (int k = 0; k < 4; ++k)
+                    was[i][k] = *reinterpret_cast<const f32x4 *>(to + i * 16 * cols_pad + k * 16);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < R; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (r0 + i * 16 < rows && c0 + j * 16 < cols)
-                        results.store_some(r0 + i * 16, c0 + j * 16, cols, sum[i][j]);
+                for (int k = 0; k < 4; ++k)
+                    sum[i][k] += was[i][k];
         }
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                *reinterpret_cast<f32x4 *>(to + i * 16 * cols_pad + k * 16) = sum[i][k];
+    } else if (j.o.type == AXC_F32) {
+        store_tile<float>(j, row_tile, col_tile, r0, c0, sum);
+    } else if (j.o.type == AXC_BF16) {
+        store_tile<bf16>(j, row_tile, col_tile, r0, c0, sum);
+    } else {
+        store_tile<f16>(j, row_tile, col_tile, r0, c0, sum);
     }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) product_out_kernel(const float *__restrict__ partials, int splits, int64_t rows, int64_t cols,
-                                                          int64_t rows_pad, int64_t cols_pad, ProductOut o)
+__device__ __forceinline__ void product_out(const Product &j, int block)
 {
-    const int64_t c = ((int64_t)blockIdx.x * 64 + (threadIdx.x & 63)) * 4;
-    if (c >= cols)
+    const int64_t rows_pad = product_pad(j.rows), cols_pad = product_pad(j.cols);
+    const int across = (int)((j.cols + 255) / 256);
+    const int64_t c = ((int64_t)(block % across) * 64 + (threadIdx.x & 63)) * 4, r = (int64_t)(block / across) * 4 + threadIdx.x / 64;
+    if (c >= j.cols || r >= j.rows)
         return;
-    const Results<T> results(o);
-    for (int64_t r = (int64_t)blockIdx.y * 4 + threadIdx.x / 64; r < rows; r += (int64_t)gridDim.y * 4) {
-        f32x4 sum = {};
+    const Results<T> results(j.o);
+    f32x4 sum = {};
 #pragma unroll 8
-        for (int s = 0; s < splits; ++s)
-            sum += *reinterpret_cast<const f32x4 *>(partials + ((int64_t)s * rows_pad + r) * cols_pad + c);
-        results.store_some(r, c, cols, sum);
-    }
+    for (int s = 0; s < j.splits; ++s)
+        sum += *reinterpret_cast<const f32x4 *>(j.partials + ((int64_t)s * rows_pad + r) * cols_pad + c);
+    results.store_some(r, c, j.cols, sum);
+}
+__global__ void __launch_bounds__(256) products_out_kernel(Product first_product, int first_blocks, Product second_product)
+{
+    const bool first = (int)blockIdx.x < first_blocks;
+    const Product &j = first ? first_product : second_product;
+    const int block = first ? (int)blockIdx.x : (int)blockIdx.x - first_blocks;
+    if (j.o.type == AXC_F32)
+        product_out<float>(j, block);
+    else if (j.o.type == AXC_BF16)
+        product_out<bf16>(j, block);
+    else
+        product_out<f16>(j, block);
 }
 
 } // namespace
@@ -529,66 +563,57 @@ hipError_t launch_grad_prep(const GradSource &of_run, bool loss, int64_t first, 
     return hipGetLastError();
 }
 
-ProductPlan plan_product(int64_t rows, int64_t cols, int64_t depth_pad, int parts, bool keep)
+static int64_t product_tiles(int64_t rows, int64_t cols)
 {
-    const int64_t tiles = (product_pad(rows) / kProductTile) * (product_pad(cols) / kProductTile);
-    const int64_t steps = depth_pad / kStep * parts;
-    int64_t splits = tiles >= 256 ? 1 : 256 / tiles;
-    if (splits > steps / 4)
-        splits = steps / 4;
-    if (splits < 1)
-        splits = 1;
-    ProductPlan plan = {(int)splits, 0};
-    if (splits > 1 || keep)
-        plan.partial_bytes = (size_t)splits * product_pad(rows) * product_pad(cols) * sizeof(float);
-    return plan;
+    return (product_pad(rows) / kProductTile) * (product_pad(cols) / kProductTile);
+}
+constexpr int64_t kManyTiles = 512;      // two workgroups a CU
+void plan_products(const ProductShape *shapes, int count, ProductPlan *plans)
+{
+    int64_t tiles = 0, all = 0;
+    for (int i = 0; i < count; ++i) {
+        const int64_t t = product_tiles(shapes[i].rows, shapes[i].cols);
+        tiles += t;
+        all += t * (product_pad(shapes[i].depth) / kStep) * shapes[i].parts;
+    }
+    // steps of the depth that a workgroup takes, 4 at least
+    const int64_t each = std::max<int64_t>(4, all / (tiles >= kManyTiles ? kManyTiles : kManyTiles / 2));
+    for (int i = 0; i < count; ++i) {
+        const ProductShape &s = shapes[i];
+        const int64_t splits = std::max<int64_t>(1, product_pad(s.depth) / kStep * s.parts / each);
+        plans[i] = {(int)splits, 0};
+        if (splits > 1 || s.keep)
+            plans[i].partial_bytes = (size_t)splits * product_pad(s.rows) * product_pad(s.cols) * sizeof(float);
+    }
 }
 
-template <typename T, bool PARTIAL>
-static hipError_t product(const bf16 *a, const bf16 *b, int64_t rows, int64_t cols, int64_t depth_pad, int parts, bool split_a,
-                          int splits, float *partials, bool accumulate, const ProductOut &o, const ColumnJob &job,
-                          hipStream_t stream)
+template <int G>
+static hipError_t products(const Product *p, int count, int first_tiles, int tiles, const ColumnJob &job, hipStream_t stream)
 {
-    const int row_tiles = (int)(product_pad(rows) / kProductTile), col_tiles = (int)(product_pad(cols) / kProductTile);
-    if (hipError_t e = set_max_dynamic_lds_once(reinterpret_cast<const void *>(&product_kernel<T, PARTIAL>), kProductLds))
+    if (hipError_t e = set_max_dynamic_lds_once(reinterpret_cast<const void *>(&products_kernel<G>), product_lds(G)))
         return e;
-    hipLaunchKernelGGL((product_kernel<T, PARTIAL>), dim3((unsigned)((int64_t)row_tiles * col_tiles * splits + job.blocks())),
-                       dim3(kProductThreads),
-                       kProductLds,
-                       stream, a, b, rows, cols, row_tiles, col_tiles, (int)depth_pad, parts, (int)split_a, splits, partials,
-                       (int)accumulate, o, job);
+    hipLaunchKernelGGL(products_kernel<G>, dim3((unsigned)(tiles + job.blocks())), dim3(G * 256), product_lds(G), stream, p[0],
+                       first_tiles, p[count - 1], tiles, job);
     return hipGetLastError();
 }
-
-hipError_t launch_product(const bf16 *a, const bf16 *b, int64_t rows, int64_t cols, int64_t depth_pad, int parts, bool split_a,
-                          const ProductPlan &plan, float *partials, bool keep, bool accumulate, const ProductOut &o,
-                          const ColumnJob &job, hipStream_t stream)
+hipError_t launch_products(const Product *p, int count, const ColumnJob &job, hipStream_t stream)
 {
-    if (plan.splits > 1 || keep) {
-        if (hipError_t e = product<float, true>(a, b, rows, cols, depth_pad, parts, split_a, plan.splits, partials, accumulate, o,
-                                                job, stream))
-            return e;
-        return keep ? hipSuccess : launch_product_out(partials, plan.splits, rows, cols, o, stream);
+    int64_t plain = 0, tiles[2] = {};
+    for (int i = 0; i < count; ++i) {
+        tiles[i] = product_tiles(p[i].rows, p[i].cols) * p[i].splits;
+        plain += product_tiles(p[i].rows, p[i].cols);
     }
-    if (o.type == AXC_F32)
-        return product<float, false>(a, b, rows, cols, depth_pad, parts, split_a, 1, nullptr, false, o, job, stream);
-    if (o.type == AXC_BF16)
-        return product<bf16, false>(a, b, rows, cols, depth_pad, parts, split_a, 1, nullptr, false, o, job, stream);
-    return product<f16, false>(a, b, rows, cols, depth_pad, parts, split_a, 1, nullptr, false, o, job, stream);
+    return plain >= kManyTiles ? products<1>(p, count, (int)tiles[0], (int)(tiles[0] + tiles[1]), job, stream)
+                               : products<2>(p, count, (int)tiles[0], (int)(tiles[0] + tiles[1]), job, stream);
 }
 
-hipError_t launch_product_out(const float *partials, int splits, int64_t rows, int64_t cols, const ProductOut &o,
-                              hipStream_t stream)
+hipError_t launch_products_out(const Product *p, int count, hipStream_t stream)
 {
-    const int64_t by = (rows + 3) / 4;
-    const dim3 grid((unsigned)((cols + 255) / 256), (unsigned)(by > 16384 ? 16384 : by));
-    const int64_t rows_pad = product_pad(rows), cols_pad = product_pad(cols);
-    if (o.type == AXC_F32)
-        hipLaunchKernelGGL(product_out_kernel<float>, grid, dim3(256), 0, stream, partials, splits, rows, cols, rows_pad, cols_pad, o);
-    else if (o.type == AXC_BF16)
-        hipLaunchKernelGGL(product_out_kernel<bf16>, grid, dim3(256), 0, stream, partials, splits, rows, cols, rows_pad, cols_pad, o);
-    else
-        hipLaunchKernelGGL(product_out_kernel<f16>, grid, dim3(256), 0, stream, partials, splits, rows, cols, rows_pad, cols_pad, o);
+    int64_t blocks[2] = {};
+    for (int i = 0; i < count; ++i)
+        blocks[i] = (p[i].cols + 255) / 256 * ((p[i].rows + 3) / 4);
+    hipLaunchKernelGGL(products_out_kernel, dim3((unsigned)(blocks[0] + blocks[1])), dim3(256), 0, stream, p[0], (int)blocks[0],
+                       p[count - 1]);
     return hipGetLastError();
 }
 

@@ -344,7 +344,8 @@ int carve_dense(const axc_dense_desc *d, bool packed, void *base, DenseScratch *
 struct GradScratch {
     Operands o;
     bf16 *straight, *turned, *x_turned, *kernel;
-    float *column_partials, *partials;
+    float *column_partials, *partials[2];
+    ProductPlan plans[2];                // of the input's product and of the kernel's
 };
 
 } // namespace
@@ -489,8 +490,10 @@ static int carve_gradients(const axc_dense_desc *d, void *base, GradScratch *s, 
     s->x_turned = c.take<bf16>((size_t)M * K);
     s->kernel = c.take<bf16>((size_t)K * N);
     s->column_partials = c.take<float>((size_t)(M / 64) * N);
-    s->partials = reinterpret_cast<float *>(c.take<char>(std::max(plan_product(d->rows, d->depth, N, px, false).partial_bytes,
-                                                                  plan_product(d->depth, d->columns, M, pk, false).partial_bytes)));
+    const ProductShape shapes[2] = {{d->rows, d->depth, d->columns, px, 0}, {d->depth, d->columns, d->rows, pk, 0}};
+    plan_products(shapes, 2, s->plans);
+    for (int i = 0; i < 2; ++i)
+        s->partials[i] = s->plans[i].partial_bytes ? reinterpret_cast<float *>(c.take<char>(s->plans[i].partial_bytes)) : nullptr;
     *bytes = c.bytes();
     return AXC_OK;
 }
@@ -506,6 +509,27 @@ int axc_fake_approx_dense_gradients_workspace_bytes(const axc_dense_desc *desc, 
         return AXC_OK;
     GradScratch s;
     return carve_gradients(desc, nullptr, &s, bytes);
+}
+
+// Products, then results of those whose partial sums are whole; column sums with them, or alone.
+static int make_products(const Product *products, int count, const ColumnJob &job, hipStream_t stream)
+{
+    if (count == 0) {
+        ApiTimer t("column_sums", stream);
+        if (job.out)
+            AXC_HIP(launch_column_sums(job, stream));
+        return AXC_OK;
+    }
+    ApiTimer t("grad_product", stream);
+    AXC_HIP(launch_products(products, count, job, stream));
+    Product whole[2];
+    int left = 0;
+    for (int i = 0; i < count; ++i)
+        if (products[i].partials && products[i].o.out)
+            whole[left++] = products[i];
+    if (left)
+        AXC_HIP(launch_products_out(whole, left, stream));
+    return AXC_OK;
 }
 
 static int fill_zero(void *p, int64_t n, int type, hipStream_t stream)
@@ -561,25 +585,15 @@ int axc_fake_approx_dense_gradients(const axc_dense_desc *desc, const void *grad
                                  {kernel, desc->kernel_type, K, N, N, grad_input ? s.kernel : nullptr}, ranges, s.o.grids, stream));
     }
     ColumnJob job = {s.column_partials, product_pad(rows) / 64, N, product_pad(N), nullptr, grad_bias, desc->kernel_type};
-    if (grad_input) {
-        const ProductOut o = {grad_input, desc->input_type, K, input, K, &s.o.grids->in, &s.o.grids->kernel, nullptr};
-        ApiTimer t("grad_product", stream);
-        AXC_HIP(launch_product(s.straight, s.kernel, rows, K, product_pad(N), px, true, plan_product(rows, K, product_pad(N), px, false),
-                               s.partials, false, false, o, job, stream));
-        job.out = nullptr;
-    }
-    if (grad_kernel) {
-        const ProductOut o = {grad_kernel, desc->kernel_type, N, kernel, N, &s.o.grids->kernel, &s.o.grids->in, nullptr};
-        ApiTimer t("grad_product", stream);
-        AXC_HIP(launch_product(s.x_turned, s.turned, K, N, product_pad(rows), pk, false,
-                               plan_product(K, N, product_pad(rows), pk, false), s.partials, false, false, o, job, stream));
-        job.out = nullptr;
-    }
-    if (job.out) {
-        ApiTimer t("column_sums", stream);
-        AXC_HIP(launch_column_sums(job, stream));
-    }
-    return AXC_OK;
+    Product products[2];
+    int count = 0;
+    if (grad_input)
+        products[count++] = {s.straight, s.kernel, rows, K, (int)product_pad(N), px, 1, s.plans[0].splits, s.partials[0], 0,
+                             {grad_input, desc->input_type, K, input, K, &s.o.grids->in, &s.o.grids->kernel, nullptr}};
+    if (grad_kernel)
+        products[count++] = {s.x_turned, s.turned, K, N, (int)product_pad(rows), pk, 0, s.plans[1].splits, s.partials[1], 0,
+                             {grad_kernel, desc->kernel_type, N, kernel, N, &s.o.grids->kernel, &s.o.grids->in, nullptr}};
+    return make_products(products, count, job, stream);
 }
 
 // ---- loss ----
@@ -590,6 +604,21 @@ static Pieces loss_pieces(const axc_dense_desc *d)
     const int64_t most = 2 * kSumsAtOnce / fours(std::max<int64_t>(1, d->rows)) & ~(int64_t)255;
     const int64_t codes = ((int64_t)1 << 29) / fours(d->depth) & ~(int64_t)255;   // the LUT-GEMM's offsets have 32 bits
     return pieces_of(d->depth, d->columns, std::min(codes, std::min<int64_t>(65536, std::max<int64_t>(1024, most))));
+}
+
+// Products of a piece of so many columns; the input's is that of the first whatever the piece, as its partial sums go on.
+struct LossPlan {
+    ProductPlan input, kernel;
+};
+static LossPlan loss_plan(const axc_dense_desc *d, const Pieces &pc, int64_t columns)
+{
+    const int px = parts_of(d->input_type), pk = parts_of(d->kernel_type);
+    const ProductShape first[2] = {{d->rows, d->depth, pc.width_of(0), px, 1}, {d->depth, pc.width_of(0), d->rows, pk, 0}};
+    const ProductShape own[2] = {{d->rows, d->depth, columns, px, 1}, {d->depth, columns, d->rows, pk, 0}};
+    ProductPlan a[2], b[2];
+    plan_products(first, 2, a);
+    plan_products(own, 2, b);
+    return {a[0], b[1]};
 }
 
 struct LossScratch {
@@ -628,9 +657,9 @@ static int carve_loss(const axc_dense_desc *d, bool gradients, void *base, LossS
         s->column_partials = c.take<float>((size_t)(M / 64) * P);
         size_t most = 0;
         for (const int width : {pc.width_of(0), pc.width_of(pc.count - 1)})
-            most = std::max(most, plan_product(d->depth, width, M, pk, false).partial_bytes);
+            most = std::max(most, loss_plan(d, pc, width).kernel.partial_bytes);
         s->kernel_partials = reinterpret_cast<float *>(c.take<char>(most));
-        s->input_partials = reinterpret_cast<float *>(c.take<char>(plan_product(d->rows, d->depth, P, px, true).partial_bytes));
+        s->input_partials = reinterpret_cast<float *>(c.take<char>(loss_plan(d, pc, pc.width_of(0)).input.partial_bytes));
     }
     s->bytes = c.bytes();
     return AXC_OK;
@@ -724,9 +753,7 @@ int axc_fake_approx_cross_entropy(const axc_table *table, const axc_dense_desc *
 
     const int px = parts_of(desc->input_type), pk = parts_of(desc->kernel_type);
     const int64_t M = product_pad(rows);
-    const ProductPlan input_plan = plan_product(rows, K, product_pad(pc.width), px, true);
-    const ProductOut input_out = {grad_input, desc->input_type, K, input, K, &o.grids->in, &o.grids->kernel,
-                                  s.st.factor};
+    const ProductOut input_out = {grad_input, desc->input_type, K, input, K, &o.grids->in, &o.grids->kernel, s.st.factor};
     // from the last piece on, whose last run's sums are still there
     bool made = true;
     for (int p = pc.count - 1; p >= 0; --p) {
@@ -756,28 +783,23 @@ int axc_fake_approx_cross_entropy(const axc_table *table, const axc_dense_desc *
                                      nullptr, o.grids, stream));
         }
         ColumnJob job = {s.column_partials, M / 64, n, P, s.st.factor, element(grad_bias, c, desc->kernel_type), desc->kernel_type};
+        const LossPlan plan = loss_plan(desc, pc, n);
+        Product products[2];
+        int count = 0;
         if (grad_input) {
-            ApiTimer t("grad_product", stream);
-            AXC_HIP(launch_product(s.straight, s.kernel, rows, K, P, px, true, input_plan, s.input_partials, true,
-                                   p + 1 < pc.count, input_out, job, stream));
-            job.out = nullptr;
+            products[count] = {s.straight, s.kernel, rows, K, (int)P, px, 1, plan.input.splits, s.input_partials, p + 1 < pc.count,
+                               input_out};
+            if (p > 0)
+                products[count].o.out = nullptr;   // not yet
+            ++count;
         }
-        if (grad_kernel) {
-            const ProductOut out = {element(grad_kernel, c, desc->kernel_type), desc->kernel_type, V,
-                                    element(kernel, c, desc->kernel_type), V, &o.grids->kernel, &o.grids->in, s.st.factor};
-            ApiTimer t("grad_product", stream);
-            AXC_HIP(launch_product(s.x_turned, s.turned, K, n, M, pk, false, plan_product(K, n, M, pk, false), s.kernel_partials,
-                                   false, false, out, job, stream));
-            job.out = nullptr;
-        }
-        if (job.out) {
-            ApiTimer t("column_sums", stream);
-            AXC_HIP(launch_column_sums(job, stream));
-        }
-    }
-    if (grad_input) {
-        ApiTimer t("grad_product", stream);
-        AXC_HIP(launch_product_out(s.input_partials, input_plan.splits, rows, K, input_out, stream));
+        if (grad_kernel)
+            products[count++] = {s.x_turned, s.turned, K, n, (int)M, pk, 0, plan.kernel.splits,
+                                 plan.kernel.partial_bytes ? s.kernel_partials : nullptr, 0,
+                                 {element(grad_kernel, c, desc->kernel_type), desc->kernel_type, V,
+                                  element(kernel, c, desc->kernel_type), V, &o.grids->kernel, &o.grids->in, s.st.factor}};
+        if (int rc = make_products(products, count, job, stream))
+            return rc;
     }
     return AXC_OK;
 }

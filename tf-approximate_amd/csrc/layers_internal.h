@@ -500,18 +500,30 @@ struct ProductOut {
     const Grid *grid, *scale;            // scale->scale times the sums
     const float *factor;                 // not null: times *factor
 };
+// out[r][c] = sum over parts and l of a[r][..l] * b[c][..l]; the operand with the parts is a where split_a, else b.
+struct Product {
+    const bf16 *a, *b;
+    int64_t rows, cols;
+    int depth, parts, split_a;           // depth in whole tiles
+    int splits;                          // of the depth, by plan_products
+    float *partials;                     // [splits][rows in tiles][cols in tiles]; null: not split, and not kept
+    int accumulate;                      // add to the partial sums that are there
+    ProductOut o;
+};
+struct ProductShape {
+    int64_t rows, cols, depth;           // any; keep: its partial sums go on from launch to launch
+    int parts, keep;
+};
 struct ProductPlan {
     int splits;
-    size_t partial_bytes;                // [splits][rows_pad][cols_pad] float
+    size_t partial_bytes;
 };
-ProductPlan plan_product(int64_t rows, int64_t cols, int64_t depth_pad, int parts, bool keep);
-// out[r][c] = sum over parts and l of a[r][..l] * b[c][..l]; the operand with the parts is a where split_a, else b.
-// accumulate: add to the partial sums that are there.  job: column sums that the launch makes too.
-hipError_t launch_product(const bf16 *a, const bf16 *b, int64_t rows, int64_t cols, int64_t depth_pad, int parts, bool split_a,
-                          const ProductPlan &plan, float *partials, bool keep, bool accumulate, const ProductOut &o,
-                          const ColumnJob &job, hipStream_t stream);
-hipError_t launch_product_out(const float *partials, int splits, int64_t rows, int64_t cols, const ProductOut &o,
-                              hipStream_t stream);
+// Of one or two products that one launch makes.
+void plan_products(const ProductShape *shapes, int count, ProductPlan *plans);
+// job: column sums that the launch makes too.
+hipError_t launch_products(const Product *products, int count, const ColumnJob &job, hipStream_t stream);
+// What the partial sums of products give.
+hipError_t launch_products_out(const Product *products, int count, hipStream_t stream);
 // ---- loss (loss_kernels.hip) ----
 // Columns at least that leave a maximum and a sum: fewer where few rows would leave CUs without work.
 inline int loss_chunk(int64_t rows) { return rows >= 2048 ? 512 : rows >= 512 ? 256 : 64; }
