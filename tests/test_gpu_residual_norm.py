@@ -68,6 +68,7 @@ CASES = [
     (3, 8192, 1, ("scale",)), (3, 8193, 3, ALL), (2, 16384, 1, ALL), (2, 32768, 2, ALL), (2, 32767, 1, ALL),
     # more rows than workgroups, groups of whole runs and runs of whole groups
     (1200, 40, 2, ALL), (5000, 24, 1000, ALL), (4097, 17, 0, ALL), (3000, 36, 3000, ("scale",)),
+    (1600, 4100, 4, ALL), (1600, 4101, 1600, ("post",)), (1100, 8197, 550, ALL), (1030, 8196, 0, ("scale", "bias")),
 ]
 
 

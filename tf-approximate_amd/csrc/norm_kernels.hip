@@ -254,52 +254,59 @@ __device__ __forceinline__ void normalize(Row<NV> &r, const NormParams &p, Reduc
     scale_row(r, root(s[0], width, p.eps));
 }
 
-// The layer's vectors (weights and the like), as floats in LDS: each thread its own columns, so without a barrier.  Rows of eight
-// vectors a thread have more of them than LDS holds, and load them again for every row.
+// Four values of one of the layer's vectors, as floats; ones where it is not there.
+template <int W>
+__device__ __forceinline__ f32x4 load_vector(const void *p, int type, int c, int width)
+{
+    if (!p)
+        return f32x4{1.0f, 1.0f, 1.0f, 1.0f};
+    if (type == AXC_F32)
+        return in_place<W>(load_four<W>(static_cast<const float *>(p), c, width), c, width);
+    if (type == AXC_BF16)
+        return in_place<W>(load_four<W>(static_cast<const bf16 *>(p), c, width), c, width);
+    return in_place<W>(load_four<W>(static_cast<const f16 *>(p), c, width), c, width);
+}
+
+// The layer's vectors (weights and the like), as floats in LDS: each thread its own columns, so without a barrier.
 template <int W, int NV, int N>
 struct Kept {
     f32x4 *lds;
     const void *vectors[N];
     int type, width;
-    static constexpr bool kKeep = NV <= 4;
-    static int bytes(int threads) { return kKeep ? N * threads * NV * V * (int)sizeof(float) : 0; }
-    __device__ __forceinline__ f32x4 load(int which, int j) const
-    {
-        const void *const p = vectors[which];
-        const int c = place(j);
-        constexpr int L = W == kTiny ? kTiny : kOdd;   // (may be aligned as their elements only)
-        if (type == AXC_F32)
-            return in_place<L>(load_four<L>(static_cast<const float *>(p), c, width), c, width);
-        if (type == AXC_BF16)
-            return in_place<L>(load_four<L>(static_cast<const bf16 *>(p), c, width), c, width);
-        return in_place<L>(load_four<L>(static_cast<const f16 *>(p), c, width), c, width);
-    }
+    static int bytes(int threads) { return N * threads * NV * V * (int)sizeof(float); }
     // Vectors that are not there are ones.
     __device__ __forceinline__ void fill()
     {
-        if constexpr (!kKeep)
-            return;
 #pragma unroll
         for (int k = 0; k < N; ++k)
 #pragma unroll
             for (int j = 0; j < NV; ++j)
-                lds[(k * NV + j) * (int)blockDim.x + (int)threadIdx.x] = vectors[k] ? load(k, j) : f32x4{1.0f, 1.0f, 1.0f, 1.0f};
+                lds[(k * NV + j) * (int)blockDim.x + (int)threadIdx.x] =
+                    load_vector<W == kTiny ? kTiny : kOdd>(vectors[k], type, place(j), width);   // (may be aligned as their elements only)
     }
     __device__ __forceinline__ f32x4 get(int which, int j) const
     {
-        if constexpr (kKeep)
-            return lds[(which * NV + j) * (int)blockDim.x + (int)threadIdx.x];
-        return vectors[which] ? load(which, j) : f32x4{1.0f, 1.0f, 1.0f, 1.0f};
+        return lds[(which * NV + j) * (int)blockDim.x + (int)threadIdx.x];
     }
 };
 
-// Threads of a workgroup at most, by the vectors of a thread: 1024 threads have 128 registers each.
-constexpr int most_threads(int NV) { return NV > 4 ? 1024 : 512; }
-
 enum { kWeight, kScale, kPost, kBias };
 
+// A workgroup's pair of the range of y.
+__device__ __forceinline__ void report_range(const NormParams &p, float lo, float hi, float *ends)
+{
+    if (!p.range)
+        return;
+    block_range(lo, hi, ends);
+    if (threadIdx.x == 0)
+        reinterpret_cast<float2 *>(p.range)[blockIdx.x] = make_float2(lo, hi);
+    if (blockIdx.x == 0)   // pairs that nobody has
+        for (int i = (int)gridDim.x + (int)threadIdx.x; i < kRangePairs; i += blockDim.x)
+            reinterpret_cast<float2 *>(p.range)[i] = make_float2(INFINITY, -INFINITY);
+}
+
 template <typename T, int NV, int W>
-__global__ void __launch_bounds__(most_threads(NV)) norm_kernel(NormParams p)
+__global__ void __launch_bounds__(512) norm_kernel(NormParams p)
 {
     __shared__ float lds[2][kMaxWaves][4];
     __shared__ float ends[2 * kMaxWaves];
@@ -382,14 +389,98 @@ __global__ void __launch_bounds__(most_threads(NV)) norm_kernel(NormParams p)
         }
         store_row(ys, r, h);
     }
-    if (!p.range)
-        return;
-    block_range(lo, hi, ends);
-    if (threadIdx.x == 0)
-        reinterpret_cast<float2 *>(p.range)[blockIdx.x] = make_float2(lo, hi);
-    if (blockIdx.x == 0)   // pairs that nobody has
-        for (int i = (int)gridDim.x + (int)threadIdx.x; i < kRangePairs; i += blockDim.x)
-            reinterpret_cast<float2 *>(p.range)[i] = make_float2(INFINITY, -INFINITY);
+    report_range(p, lo, hi, ends);
+}
+
+// Rows of more than 8192 values do not stay in registers: every sum goes over the row again, out of the caches, and four workgroups a
+// CU take the place of loads ahead.  16 384 values of bfloat16, 33.6 M altogether, take 88 us (216 in registers that spill).
+template <typename T>
+struct WideRow {                         // four values of a row, whatever its alignment
+    const T *p;
+    __device__ __forceinline__ WideRow(const void *base, int64_t row, int width)
+        : p(base ? static_cast<const T *>(base) + row * width : nullptr)
+    {
+    }
+    __device__ __forceinline__ f32x4 at(int c, int width) const
+    {
+        return p ? in_place<kOdd>(load_four<kOdd>(p, c, width), c, width) : f32x4{};
+    }
+};
+template <typename T>
+__global__ void __launch_bounds__(512) wide_norm_kernel(NormParams p)
+{
+    __shared__ float lds[2][kMaxWaves][4];
+    __shared__ float ends[2 * kMaxWaves];
+    Reducer red = {lds, 0};
+    const int width = (int)p.width, step = (int)blockDim.x * V, c0 = (int)threadIdx.x * V;
+    const int64_t group_rows = p.gate_groups ? p.rows / p.gate_groups : 1;
+    float lo = INFINITY, hi = -INFINITY;
+    auto squares = [&](const WideRow<T> &row, float mean) {
+        float s[1] = {};
+#pragma unroll 4
+        for (int c = c0; c < width; c += step) {
+            const f32x4 v = row.at(c, width);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float d = c + i < width ? v[i] - mean : 0.0f;
+                s[0] = fmaf(d, d, s[0]);
+            }
+        }
+        red.sum(s);
+        return s[0];
+    };
+    auto mean_of = [&](const WideRow<T> &row) {
+        float s[1] = {};
+#pragma unroll 4
+        for (int c = c0; c < width; c += step) {
+            const f32x4 v = row.at(c, width);
+            s[0] += v[0] + v[1] + v[2] + v[3];
+        }
+        red.sum(s);
+        return s[0] / (float)width;
+    };
+    for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+        const WideRow<T> x(p.x, r, width), block(p.block, r, width), gate(p.gate, r / group_rows, width),
+            h(p.block ? p.h : p.x, r, width);
+        if (p.block) {
+            float mean = 0.0f, factor = 1.0f;
+            if (p.post_weight) {
+                mean = p.layer ? mean_of(block) : 0.0f;
+                factor = root(squares(block, mean), width, p.eps);
+            }
+#pragma unroll 2
+            for (int c = c0; c < width; c += step) {
+                const f32x4 v = x.at(c, width), b = block.at(c, width), post = load_vector<kOdd>(p.post_weight, p.vector_type, c, width),
+                            scale = load_vector<kOdd>(p.scale, p.vector_type, c, width);
+                const f32x4 g = p.gate ? gate.at(c, width) : f32x4{1.0f, 1.0f, 1.0f, 1.0f};
+                float t[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    t[i] = v[i] + (b[i] - mean) * factor * post[i] * g[i] * scale[i];
+                store_four<kOdd>(static_cast<T *>(p.h) + r * width, c, width, t);
+            }
+            // the row's last whole vector is read again by the thread of what is behind it
+            __threadfence_block();
+            __syncthreads();
+        }
+        const float mean = p.layer ? mean_of(h) : 0.0f, factor = root(squares(h, mean), width, p.eps);
+#pragma unroll 2
+        for (int c = c0; c < width; c += step) {
+            const f32x4 v = h.at(c, width), w = load_vector<kOdd>(p.weight, p.vector_type, c, width);
+            const f32x4 b = p.bias ? load_vector<kOdd>(p.bias, p.vector_type, c, width) : f32x4{};
+            float t[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                t[i] = (v[i] - mean) * factor * w[i] + b[i];
+                const float y = (float)(T)t[i];
+                const bool there = c + i < width;
+                lo = fminf(lo, there ? y : INFINITY);
+                hi = fmaxf(hi, there ? y : -INFINITY);
+            }
+            store_four<kOdd>(static_cast<T *>(p.y) + r * width, c, width, t);
+        }
+    }
+    report_range(p, lo, hi, ends);
 }
 
 // ---- backwards ----
@@ -424,7 +515,7 @@ NormRuns norm_runs(int64_t rows, int64_t groups)
 enum { kSumWeight, kSumBias, kSumScale, kSumPost, kSumGate, kSums };
 
 template <typename T, int NV, int W>
-__global__ void __launch_bounds__(most_threads(NV)) norm_grad_kernel(NormParams p, NormRuns runs)
+__global__ void __launch_bounds__(512) norm_grad_kernel(NormParams p, NormRuns runs)
 {
     __shared__ float lds[2][kMaxWaves][4];
     extern __shared__ f32x4 kept_lds[];
@@ -458,7 +549,6 @@ __global__ void __launch_bounds__(most_threads(NV)) norm_grad_kernel(NormParams 
         if (p.gate)
             load_row(gates, of, gr);
     };
-    constexpr bool kAhead = NV <= 2;   // the next row's loads ahead of all reductions; of wider rows once registers are free
     Row<NV> sw = {}, sb = {}, ss = {}, sp = {}, sg = {};
     if (first < last)
         load(first, group);
@@ -472,7 +562,7 @@ __global__ void __launch_bounds__(most_threads(NV)) norm_grad_kernel(NormParams 
         }
         Row<NV> n = widen<W>(hr, width), b = widen<W>(br, width), dh = widen<W>(gyr, width), gh = widen<W>(ghr, width);
         const Raw<T, NV> gate = gr;
-        if (kAhead && r + 1 < last)
+        if (r + 1 < last)              // ahead of all reductions
             load(r + 1, group);
         if constexpr (W != kEven) {
             scale_row(dh, p.grad_y ? 1.0f : 0.0f);
@@ -510,8 +600,6 @@ __global__ void __launch_bounds__(most_threads(NV)) norm_grad_kernel(NormParams 
         if (!p.grad_y)                 // (rather than 0 times what may be infinite)
             dh = gh;
         store_row(dxs, r, dh);
-        if (!kAhead && r + 1 < last)
-            load(r + 1, group);
         if (!p.block)
             continue;
         // du = dh scale gate; b is the block, normed where it is
@@ -564,6 +652,158 @@ __global__ void __launch_bounds__(most_threads(NV)) norm_grad_kernel(NormParams 
         store_row(to, at + kSumGate, sg);
 }
 
+// Wide rows backwards, in two launches: nine rows of four vectors a thread are more than its registers (spilled, rows of 16 384 took
+// 1630 us for 33.6 M values of bfloat16; 200 this way, rows of 8192 207 and 192).  The first leaves what a row's sums are, going over it from memory once for
+// every dependent reduction; with that everything is value by value, and the second takes tiles of columns by runs of rows.
+constexpr int kWideBackward = 4096;      // values that are not wide yet
+struct RowStats {
+    float mean, root, mgn, mg;           // of h: n = (h - mean) root; means of g n and of g
+    float block_mean, block_root, mtn, mt;
+};
+template <typename T>
+__global__ void __launch_bounds__(512) wide_stats_kernel(NormParams p, RowStats *__restrict__ stats)
+{
+    __shared__ float lds[2][kMaxWaves][4];
+    Reducer red = {lds, 0};
+    const int width = (int)p.width, step = (int)blockDim.x * V, c0 = (int)threadIdx.x * V;
+    const int64_t group_rows = p.gate_groups ? p.rows / p.gate_groups : 1;
+    for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+        const WideRow<T> h(p.h, r, width), gy(p.grad_y, r, width), gh(p.grad_h, r, width),
+            b(p.post_weight ? p.block : nullptr, r, width), gate(p.gate, r / group_rows, width);
+        RowStats st = {};
+        st.block_root = 1.0f;
+        if (p.layer) {
+            float s[2] = {};
+            for (int c = c0; c < width; c += step) {
+                const f32x4 x = h.at(c, width), y = b.at(c, width);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    s[0] += x[i];
+                    s[1] += y[i];
+                }
+            }
+            red.sum(s);
+            st.mean = s[0] / (float)width;
+            if (p.post_weight)
+                st.block_mean = s[1] / (float)width;
+        }
+        float s[4] = {};
+#pragma unroll 2
+        for (int c = c0; c < width; c += step) {
+            const f32x4 x = h.at(c, width), y = b.at(c, width), w = load_vector<kOdd>(p.weight, p.vector_type, c, width), g = gy.at(c, width) * w;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const bool there = c + i < width;
+                const float n = there ? x[i] - st.mean : 0.0f, m = there ? y[i] - st.block_mean : 0.0f;
+                s[0] = fmaf(n, n, s[0]);
+                s[1] = fmaf(g[i], n, s[1]);
+                s[2] += g[i];
+                s[3] = fmaf(m, m, s[3]);
+            }
+        }
+        red.sum(s);
+        st.root = root(s[0], width, p.eps);
+        st.mgn = s[1] * st.root / (float)width;
+        st.mg = p.layer ? s[2] / (float)width : 0.0f;
+        if (p.post_weight) {
+            st.block_root = root(s[3], width, p.eps);
+            float t[2] = {};
+#pragma unroll 2
+            for (int c = c0; c < width; c += step) {
+                const f32x4 x = h.at(c, width), y = b.at(c, width), w = load_vector<kOdd>(p.weight, p.vector_type, c, width),
+                            g = gy.at(c, width) * w, other = gh.at(c, width), sc = load_vector<kOdd>(p.scale, p.vector_type, c, width),
+                            post = load_vector<kOdd>(p.post_weight, p.vector_type, c, width);
+                const f32x4 ga = p.gate ? gate.at(c, width) : f32x4{1.0f, 1.0f, 1.0f, 1.0f};
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float at = (x[i] - st.mean) * st.root;
+                    const float dh = p.grad_y ? (g[i] - at * st.mgn - st.mg) * st.root + other[i] : other[i];
+                    const float du = c + i < width ? dh * sc[i] * ga[i] * post[i] : 0.0f;
+                    t[0] = fmaf(du, (y[i] - st.block_mean) * st.block_root, t[0]);
+                    t[1] += du;
+                }
+            }
+            red.sum(t);
+            st.mtn = t[0] / (float)width;
+            st.mt = p.layer ? t[1] / (float)width : 0.0f;
+        }
+        if (threadIdx.x == 0)
+            stats[r] = st;
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) wide_grad_kernel(NormParams p, NormRuns runs, const RowStats *__restrict__ stats)
+{
+    const int width = (int)p.width, c = ((int)blockIdx.x * 256 + (int)threadIdx.x) * V;
+    if (c >= width)
+        return;
+    const int64_t group_rows = p.gate_groups ? p.rows / p.gate_groups : 1, block = blockIdx.y;
+    int64_t first, last, group, left;    // as in norm_grad_kernel
+    if (runs.per_group) {
+        group = block / runs.per_group;
+        first = group * group_rows + (block - group * runs.per_group) * runs.run;
+        last = first + runs.run < (group + 1) * group_rows ? first + runs.run : (group + 1) * group_rows;
+        left = (group + 1) * group_rows - first;
+    } else {
+        first = block * runs.run;
+        last = first + runs.run < p.rows ? first + runs.run : p.rows;
+        group = first / group_rows;
+        left = group_rows;
+    }
+    const f32x4 w = load_vector<kOdd>(p.weight, p.vector_type, c, width), sc = load_vector<kOdd>(p.scale, p.vector_type, c, width),
+                post = load_vector<kOdd>(p.post_weight, p.vector_type, c, width), ones = {1.0f, 1.0f, 1.0f, 1.0f};
+    auto gate_of = [&](int64_t of) { return p.gate ? WideRow<T>(p.gate, of, width).at(c, width) : ones; };
+    f32x4 ga = gate_of(group < p.gate_groups ? group : 0), sw = {}, sb = {}, ss = {}, sp = {}, sg = {};
+    auto put = [&](void *to, int64_t row, const float (&v)[V]) { store_four<kOdd>(static_cast<T *>(to) + row * width, c, width, v); };
+#pragma unroll 2
+    for (int64_t r = first; r < last; ++r) {
+        const f32x4 x = WideRow<T>(p.h, r, width).at(c, width), gy = WideRow<T>(p.grad_y, r, width).at(c, width),
+                    gh = WideRow<T>(p.grad_h, r, width).at(c, width), y = WideRow<T>(p.block, r, width).at(c, width);
+        const RowStats st = stats[r];
+        float dh[V], du[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float at = (x[i] - st.mean) * st.root;
+            sw[i] = fmaf(gy[i], at, sw[i]);
+            sb[i] += gy[i];
+            dh[i] = p.grad_y ? (gy[i] * w[i] - at * st.mgn - st.mg) * st.root + gh[i] : gh[i];
+            const float b = (y[i] - st.block_mean) * st.block_root, hu = dh[i] * b * post[i];   // dh u
+            ss[i] = fmaf(hu, ga[i], ss[i]);
+            sg[i] = fmaf(hu, sc[i], sg[i]);
+            du[i] = dh[i] * sc[i] * ga[i];
+            sp[i] = fmaf(du[i], b, sp[i]);
+            du[i] *= post[i];
+            if (p.post_weight)
+                du[i] = (du[i] - b * st.mtn - st.mt) * st.block_root;
+        }
+        put(p.dx, r, dh);
+        if (p.block)
+            put(p.dblock, r, du);
+        if (--left == 0) {               // the group's last row
+            if (p.dgate && !runs.per_group) {
+                const float v[V] = {sg[0], sg[1], sg[2], sg[3]};
+                put(p.dgate, group, v);
+                sg = {};
+            }
+            ++group;
+            left = group_rows;
+            if (r + 1 < last)
+                ga = gate_of(group < p.gate_groups ? group : 0);
+        }
+    }
+    auto leave = [&](void *wanted, int which, const f32x4 &v) {
+        const float t[V] = {v[0], v[1], v[2], v[3]};
+        if (wanted)
+            store_four<kOdd>(p.partials + (block * kSums + which) * width, c, width, t);
+    };
+    leave(p.dweight, kSumWeight, sw);
+    leave(p.dbias, kSumBias, sb);
+    leave(p.dscale, kSumScale, ss);
+    leave(p.dpost, kSumPost, sp);
+    leave(runs.per_group ? p.dgate : nullptr, kSumGate, sg);
+}
+
 struct ColumnSums {
     void *out[kSums];
 };
@@ -610,7 +850,7 @@ bool whole_vectors(const NormParams &p)
     return true;
 }
 
-// Two vectors a thread up to 4096 values, in steps of a wavefront; then four, and eight of 1024 threads.
+// Two vectors a thread up to 4096 values, in steps of a wavefront; then four, and ("8") as many as there are.
 template <template <typename, int, int> class Launch, typename T, int W>
 hipError_t by_vectors(const NormParams &p, hipStream_t stream)
 {
@@ -646,32 +886,56 @@ struct Forward {
     static hipError_t go(const NormParams &p, int threads, hipStream_t stream)
     {
         // as many workgroups as are resident, each with its vectors in LDS, a row loaded ahead
+        if (NV == 8)
+            threads = 512;
         int64_t blocks = 256 * 2048 / threads;
         blocks = blocks < kRangePairs ? blocks : kRangePairs;   // a pair of the range each
         blocks = blocks < p.rows ? blocks : p.rows;
-        const int bytes = Kept<W, NV, 4>::bytes(threads);
-        if (hipError_t e = set_max_dynamic_lds_once(reinterpret_cast<const void *>(&norm_kernel<T, NV, W>), bytes))
-            return e;
-        hipLaunchKernelGGL((norm_kernel<T, NV, W>), dim3((unsigned)blocks), dim3(threads), bytes, stream, p);
+        if constexpr (NV == 8) {
+            hipLaunchKernelGGL(wide_norm_kernel<T>, dim3((unsigned)blocks), dim3(threads), 0, stream, p);
+        } else {
+            const int bytes = Kept<W, NV, 4>::bytes(threads);
+            if (hipError_t e = set_max_dynamic_lds_once(reinterpret_cast<const void *>(&norm_kernel<T, NV, W>), bytes))
+                return e;
+            hipLaunchKernelGGL((norm_kernel<T, NV, W>), dim3((unsigned)blocks), dim3(threads), bytes, stream, p);
+        }
         return hipGetLastError();
     }
 };
+size_t run_bytes(const NormParams &p)    // what the runs leave
+{
+    return ((size_t)norm_runs(p.rows, p.gate_groups).blocks * kSums * (size_t)p.width * sizeof(float) + 255) & ~(size_t)255;
+}
+template <typename T>
+hipError_t column_sums(const NormParams &p, const NormRuns &runs, hipStream_t stream)
+{
+    ColumnSums sums = {{p.dweight, p.dbias, p.dscale, p.dpost, runs.per_group ? p.dgate : nullptr}};
+    const unsigned ys = (unsigned)(kSumGate + (sums.out[kSumGate] ? p.gate_groups : 0));
+    hipLaunchKernelGGL(norm_column_kernel<T>, dim3((unsigned)((p.width + 63) / 64), ys), dim3(512), 0, stream, p.partials, p.width,
+                       runs, sums, p.vector_type);
+    return hipGetLastError();
+}
 template <typename T, int NV, int W>
 struct Backward {
     static hipError_t go(const NormParams &p, int threads, hipStream_t stream)
     {
         const NormRuns runs = norm_runs(p.rows, p.gate_groups);
-        const int bytes = Kept<W, NV, 3>::bytes(threads);
-        if (hipError_t e = set_max_dynamic_lds_once(reinterpret_cast<const void *>(&norm_grad_kernel<T, NV, W>), bytes))
-            return e;
-        hipLaunchKernelGGL((norm_grad_kernel<T, NV, W>), dim3((unsigned)runs.blocks), dim3(threads), bytes, stream, p, runs);
+        if constexpr (NV <= 2) {
+            const int bytes = Kept<W, NV, 3>::bytes(threads);
+            if (hipError_t e = set_max_dynamic_lds_once(reinterpret_cast<const void *>(&norm_grad_kernel<T, NV, W>), bytes))
+                return e;
+            hipLaunchKernelGGL((norm_grad_kernel<T, NV, W>), dim3((unsigned)runs.blocks), dim3(threads), bytes, stream, p, runs);
+        } else {
+            RowStats *const stats = reinterpret_cast<RowStats *>(reinterpret_cast<char *>(p.partials) + run_bytes(p));
+            hipLaunchKernelGGL(wide_stats_kernel<T>, dim3((unsigned)(p.rows < 1024 ? p.rows : 1024)), dim3(512), 0, stream, p, stats);
+            if (hipError_t e = hipGetLastError())
+                return e;
+            hipLaunchKernelGGL(wide_grad_kernel<T>, dim3((unsigned)((p.width + 1023) / 1024), (unsigned)runs.blocks), dim3(256), 0, stream,
+                               p, runs, stats);
+        }
         if (hipError_t e = hipGetLastError())
             return e;
-        ColumnSums sums = {{p.dweight, p.dbias, p.dscale, p.dpost, runs.per_group ? p.dgate : nullptr}};
-        const unsigned ys = (unsigned)(kSumGate + (sums.out[kSumGate] ? p.gate_groups : 0));
-        hipLaunchKernelGGL(norm_column_kernel<T>, dim3((unsigned)((p.width + 63) / 64), ys), dim3(512), 0, stream, p.partials,
-                           p.width, runs, sums, p.vector_type);
-        return hipGetLastError();
+        return column_sums<T>(p, runs, stream);
     }
 };
 
@@ -681,7 +945,7 @@ hipError_t launch_norm(const NormParams &p, hipStream_t stream) { return by_type
 
 size_t norm_partial_bytes(const NormParams &p)
 {
-    return (size_t)norm_runs(p.rows, p.gate_groups).blocks * kSums * (size_t)p.width * sizeof(float);
+    return run_bytes(p) + (p.width > kWideBackward ? (size_t)p.rows * sizeof(RowStats) : 0);
 }
 
 hipError_t launch_norm_gradients(const NormParams &p, hipStream_t stream) { return by_type<Backward>(p, stream); }
