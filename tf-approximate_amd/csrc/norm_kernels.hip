@@ -8,6 +8,8 @@
 // Statistics are float32, of the row as it stands in registers: the variance from the differences to the mean.
 #include "layers_internal.h"
 
+#include <algorithm>
+
 namespace axc {
 namespace {
 
@@ -267,14 +269,14 @@ __device__ __forceinline__ f32x4 load_vector(const void *p, int type, int c, int
     return in_place<W>(load_four<W>(static_cast<const f16 *>(p), c, width), c, width);
 }
 
-// The layer's vectors (weights and the like), as floats in LDS: each thread its own columns, so without a barrier.
+// The layer's vectors (weights and the like), as floats in LDS: each thread its own columns, so without a barrier.  Those that are not
+// there are ones (rather than a branch where they are used, which took a tenth longer).
 template <int W, int NV, int N>
 struct Kept {
     f32x4 *lds;
     const void *vectors[N];
     int type, width;
     static int bytes(int threads) { return N * threads * NV * V * (int)sizeof(float); }
-    // Vectors that are not there are ones.
     __device__ __forceinline__ void fill()
     {
 #pragma unroll
@@ -392,8 +394,8 @@ __global__ void __launch_bounds__(512) norm_kernel(NormParams p)
     report_range(p, lo, hi, ends);
 }
 
-// Rows of more than 8192 values do not stay in registers: every sum goes over the row again, out of the caches, and four workgroups a
-// CU take the place of loads ahead.  16 384 values of bfloat16, 33.6 M altogether, take 88 us (216 in registers that spill).
+// Rows of more than 8192 values do not stay in registers: every sum goes over the row again, out of the caches, and other workgroups of
+// the CU take the place of loads ahead.  16 384 values of bfloat16, 33.6 M altogether, take 76 us (216 in registers that spill).
 template <typename T>
 struct WideRow {                         // four values of a row, whatever its alignment
     const T *p;
@@ -885,20 +887,27 @@ template <typename T, int NV, int W>
 struct Forward {
     static hipError_t go(const NormParams &p, int threads, hipStream_t stream)
     {
-        // as many workgroups as are resident, each with its vectors in LDS, a row loaded ahead
-        if (NV == 8)
-            threads = 512;
-        int64_t blocks = 256 * 2048 / threads;
-        blocks = blocks < kRangePairs ? blocks : kRangePairs;   // a pair of the range each
-        blocks = blocks < p.rows ? blocks : p.rows;
+        int bytes = 0;
+        void (*kernel)(NormParams);
         if constexpr (NV == 8) {
-            hipLaunchKernelGGL(wide_norm_kernel<T>, dim3((unsigned)blocks), dim3(threads), 0, stream, p);
+            threads = 512;
+            kernel = wide_norm_kernel<T>;
         } else {
-            const int bytes = Kept<W, NV, 4>::bytes(threads);
-            if (hipError_t e = set_max_dynamic_lds_once(reinterpret_cast<const void *>(&norm_kernel<T, NV, W>), bytes))
+            bytes = Kept<W, NV, 4>::bytes(threads);
+            kernel = norm_kernel<T, NV, W>;
+            if (hipError_t e = set_max_dynamic_lds_once(reinterpret_cast<const void *>(kernel), bytes))
                 return e;
-            hipLaunchKernelGGL((norm_kernel<T, NV, W>), dim3((unsigned)blocks), dim3(threads), bytes, stream, p);
         }
+        // As many workgroups as are resident, each with its vectors in LDS and a row loaded ahead (rows of 8192 bfloat16, 33.6 M values:
+        // 51 us by as many as have room for their threads alone, whose last begin when the others have ended, 45 this way).
+        int64_t blocks = p.rows;
+        if (blocks > device_cus()) {
+            int a_cu = 0;
+            if (hipError_t e = hipOccupancyMaxActiveBlocksPerMultiprocessor(&a_cu, kernel, threads, bytes))
+                return e;
+            blocks = std::min<int64_t>({p.rows, kRangePairs, (int64_t)device_cus() * a_cu});   // (a pair of the range each)
+        }
+        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), bytes, stream, p);
         return hipGetLastError();
     }
 };
