@@ -516,8 +516,10 @@ NormRuns norm_runs(int64_t rows, int64_t groups)
 }
 enum { kSumWeight, kSumBias, kSumScale, kSumPost, kSumGate, kSums };
 
+// Three wavefronts a SIMD are 168 registers each: rows of 16-bit values that are no whole vectors would take 171 (1283 of
+// them, 33.6 M altogether: 177 us by two a SIMD, 133 by three); 32-bit ones would spill too many (181 us by two, 248 by three).
 template <typename T, int NV, int W>
-__global__ void __launch_bounds__(512) norm_grad_kernel(NormParams p, NormRuns runs)
+__global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 2 ? 3 : 2))) norm_grad_kernel(NormParams p, NormRuns runs)
 {
     __shared__ float lds[2][kMaxWaves][4];
     extern __shared__ f32x4 kept_lds[];
