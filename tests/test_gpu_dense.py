@@ -393,3 +393,19 @@ def test_far_offsets(pkg, tables):
     assert y.numel() > 2 ** 31
     for first, last in ((0, 40), (rows - 60, rows), (131000, 131100)):
         assert torch.equal(y[first:last], layer(x[first:last].contiguous(), k))
+
+
+def test_packed_out_of_line(pkg, tables):
+    """Refused on the host: a packed kernel and a range that do not stand where they must."""
+    import ctypes
+    lib, layer = pkg._lib.load(), pkg.FakeApproxDense(tables["noisy"][1])
+    x, packed = make((3, 16), 1), layer.pack(make((16, 8), 2))
+    y, ws = torch.empty((3, 8), device=DEV), torch.empty(1 << 20, dtype=torch.uint8, device=DEV)
+    desc = ctypes.byref(pkg._lib.DenseDesc(3, 16, 8, 0, 0, 0, 0, 0, 0.0, 0.0))
+
+    def call(seen, at):
+        return lib.axc_fake_approx_dense(layer.table.handle, desc, x.data_ptr(), seen, None, packed.data.data_ptr() + at, None, None,
+                                         y.data_ptr(), None, ws.data_ptr(), ws.numel(), None)
+
+    assert call(None, 64) == pkg._lib.INVALID_ARGUMENT and b"256" in lib.axc_last_error()
+    assert call(ws.data_ptr() + 4, 0) == pkg._lib.INVALID_ARGUMENT and b"8-byte" in lib.axc_last_error()

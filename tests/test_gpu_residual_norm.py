@@ -380,3 +380,16 @@ def test_no_rows(pkg, kind):
     assert g.x.shape == x.shape and g.block.shape == x.shape
     for sums in (g.weight, g.bias, g.scale, g.post_weight, g.gate):
         assert not sums.any()
+
+
+@pytest.mark.parametrize("rows,width", [(1, 40), (2, 8192), (5, 300), (33, 64)])
+def test_a_norm_s_range_for_a_layer(pkg, rows, width):
+    """A layer that is handed its input's range, of few rows as of many, has the results of one that looks for it."""
+    norm, layer = pkg.ResidualNorm("rms", EPS), pkg.FakeApproxDense(pkg.ops.TruthTable(pkg.synth.table_noisy(3)), "silu")
+    x, b, w, k = make((rows, width), 1, BF16), make((rows, width), 2, BF16), make((width,), 3), make((width, 50), 4, BF16)
+    h, y, seen = norm.call_in_turn(x, b, w)
+    for kernel in (k, layer.pack(k)):
+        assert torch.equal(layer(y, kernel, residual=None, input_range=seen), layer(y, kernel))
+    out, pre = layer.call_and_keep(y, k)
+    for a, c in zip(layer.gradients(out, y, k, pre, input_range=seen), layer.gradients(out, y, k, pre)):
+        assert torch.equal(a, c)

@@ -127,3 +127,11 @@ def test_no_rows_have_no_block(pkg):
     T = pkg._lib.ResidualNormTensors
     assert lib.axc_residual_norm(ctypes.byref(norm(pkg, rows=0)), ctypes.byref(T(None, None, 256, None, None, 256, 256)), None, None,
                                  None, None) == 0
+
+
+def test_ranges_out_of_line(pkg):
+    """A range is read as pairs of floats."""
+    lib, bad = pkg._lib.load(), pkg._lib.INVALID_ARGUMENT
+    desc = ctypes.byref(dense(pkg))
+    assert lib.axc_fake_approx_dense_gradients(desc, 256, 256, 260, *[256] * 6, 1 << 30, None) == bad
+    assert b"8-byte" in lib.axc_last_error()

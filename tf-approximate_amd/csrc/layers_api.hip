@@ -69,6 +69,15 @@ int check_workspace(const void *workspace, size_t have, size_t need)
     return AXC_OK;
 }
 
+int check_aligned(const void *range, const void *packed)
+{
+    if (((uintptr_t)range & 7) != 0)
+        return api_fail(AXC_INVALID_ARGUMENT, "ranges must be 8-byte aligned");
+    if (((uintptr_t)packed & 255) != 0)
+        return api_fail(AXC_INVALID_ARGUMENT, "a packed kernel must be 256-byte aligned");
+    return AXC_OK;
+}
+
 const void *element(const void *p, int64_t i, int type) { return p ? static_cast<const char *>(p) + i * type_bytes(type) : nullptr; }
 void *element(void *p, int64_t i, int type) { return p ? static_cast<char *>(p) + i * type_bytes(type) : nullptr; }
 
@@ -370,8 +379,8 @@ int axc_dense_pack(const axc_dense_desc *desc, const void *kernel, void *packed,
         return AXC_OK;
     if (!kernel || !packed)
         return api_fail(AXC_INVALID_ARGUMENT, "null tensor pointer");
-    if (((uintptr_t)packed & 255) != 0)
-        return api_fail(AXC_INVALID_ARGUMENT, "a packed kernel must be 256-byte aligned");
+    if (int rc = check_aligned(nullptr, packed))
+        return rc;
     hipStream_t stream = static_cast<hipStream_t>(stream_v);
     const Pieces pc = pieces_of(desc->depth, desc->columns, kDensePiece);
     const Packed p = packed_parts(pc, packed);
@@ -416,6 +425,8 @@ int axc_fake_approx_dense(const axc_table *table, const axc_dense_desc *desc, co
         return api_fail(AXC_INVALID_ARGUMENT, "null tensor pointer");
     if (kernel && packed)
         return api_fail(AXC_INVALID_ARGUMENT, "either a kernel or a packed one");
+    if (int rc = check_aligned(input_range, packed))
+        return rc;
     const Pieces pc = pieces_of(desc->depth, desc->columns, kDensePiece);
     DenseScratch s;
     if (int rc = carve_dense(desc, packed != nullptr, workspace, &s))
@@ -556,6 +567,8 @@ int axc_fake_approx_dense_gradients(const axc_dense_desc *desc, const void *grad
     }
     if (!grad_output || !input || !kernel)
         return api_fail(AXC_INVALID_ARGUMENT, "null tensor pointer");
+    if (int rc = check_aligned(input_range, nullptr))
+        return rc;
     if (!pre && desc->activation != AXC_ACT_NONE)
         return api_fail(AXC_INVALID_ARGUMENT, "the gradient of an activation needs what the activation was given");
     GradScratch s;
@@ -711,6 +724,8 @@ int axc_fake_approx_cross_entropy(const axc_table *table, const axc_dense_desc *
     }
     if (!input || !kernel || !targets)
         return api_fail(AXC_INVALID_ARGUMENT, "null tensor pointer");
+    if (int rc = check_aligned(input_range, nullptr))
+        return rc;
     const bool gradients = grad_input || grad_kernel || grad_bias;
     const Pieces pc = loss_pieces(desc);
     LossScratch s;
@@ -869,8 +884,8 @@ int axc_residual_norm(const axc_residual_norm_desc *desc, const axc_residual_nor
     }
     if (!p.x || !y || (p.block && !h))
         return api_fail(AXC_INVALID_ARGUMENT, "null tensor pointer");
-    if (((uintptr_t)output_range & 7) != 0)
-        return api_fail(AXC_INVALID_ARGUMENT, "a range must be 8-byte aligned");
+    if (int rc = check_aligned(output_range, nullptr))
+        return rc;
     p.h = h;
     p.y = y;
     p.range = static_cast<float *>(output_range);
