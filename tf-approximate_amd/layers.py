@@ -128,13 +128,14 @@ class FakeApproxDense:
         self._descs = {}
 
     def _desc(self, inputs, depth, columns, kernel_dtype, bias):
-        """(description, reference to it) of a call: made once for its shapes and types."""
+        """[description, reference to it, output's shape, whether a call of a packed kernel is known to need no workspace] of a call:
+        made once for its shapes and types."""
         key = (inputs.shape, inputs.dtype, depth, columns, kernel_dtype, None if bias is None else bias.dtype, self.activation,
                self.input_minmax)
         found = self._descs.get(key)
         if found is None:
             desc = _dense_desc(inputs, depth, columns, kernel_dtype, bias, self.activation, self.input_minmax)
-            found = desc, ctypes.byref(desc), inputs.shape[:-1] + (columns,)
+            found = [desc, ctypes.byref(desc), inputs.shape[:-1] + (columns,), False]
             if len(self._descs) >= 256:
                 self._descs.clear()
             self._descs[key] = found
@@ -177,17 +178,22 @@ class FakeApproxDense:
             (depth, columns), kernel_dtype = kernel.shape, kernel.dtype
         if bias is not None:
             bias = _require(bias, "bias", device, shape=(columns,))
-        _, ref, out_shape = self._desc(inputs, depth, columns, kernel_dtype, bias)
+        call = self._desc(inputs, depth, columns, kernel_dtype, bias)
+        _, ref, out_shape, bare = call
         if residual is not None:
             residual = _require(residual, "residual", device, inputs.dtype, out_shape)
-        nbytes = ctypes.c_size_t()
-        _check(lib.axc_fake_approx_dense_workspace_bytes(ref, packed, ctypes.byref(nbytes)))
-        ws = _scratch(nbytes.value, device)
+        need, ws = 0, None
+        if not (packed and bare):        # (what many rows need depends on the forms that are pinned; nothing, on the shape alone)
+            nbytes = ctypes.c_size_t()
+            _check(lib.axc_fake_approx_dense_workspace_bytes(ref, packed, ctypes.byref(nbytes)))
+            need = nbytes.value
+            ws = _scratch(need, device)
+            call[3] = packed and need == 0
         out = torch.empty(out_shape, dtype=inputs.dtype, device=device)
         pre = torch.empty(out_shape, dtype=inputs.dtype, device=device) if keep else None
         _launch(device, lib.axc_fake_approx_dense, self.table.handle, ref, inputs.data_ptr(), found,
                 None if packed else kernel.data_ptr(), kernel.data.data_ptr() if packed else None, _pointer(bias),
-                _pointer(residual), out.data_ptr(), _pointer(pre), _pointer(ws), nbytes.value, _stream(device))
+                _pointer(residual), out.data_ptr(), _pointer(pre), _pointer(ws), need, _stream(device))
         return out, pre
 
     def gradients(self, grad_output, inputs, kernel, pre=None, input_range=None, want=("inputs", "kernel", "bias")):
@@ -204,7 +210,7 @@ class FakeApproxDense:
         depth, columns = kernel.shape
         if not set(want) <= {"inputs", "kernel", "bias"}:
             raise InvalidArgumentError("want: 'inputs', 'kernel', 'bias'")
-        _, ref, out_shape = self._desc(inputs, depth, columns, kernel.dtype, None)
+        _, ref, out_shape, _ = self._desc(inputs, depth, columns, kernel.dtype, None)
         grad_output = _require(grad_output, "grad_output", device, inputs.dtype, out_shape)
         if pre is not None:
             pre = _require(pre, "pre", device, inputs.dtype, out_shape)
