@@ -308,8 +308,8 @@ int axc_fake_approx_dense(const axc_table *table, const axc_dense_desc *desc, co
 /* Gradients, straight through the grid: a quantized product counts as the exact product of the values on their grids, and the
  * grid as the identity where a value lies inside it (nudged range, both ends), as constant elsewhere; ranges count as constants.
  *   dz = grad_output activation'(pre),  grad_input = dz kernel^T,  grad_kernel = input^T dz,  grad_bias = column sums of dz
- * (the residual's gradient is grad_output itself).  pre may be null without an activation; outputs may be null, each.  Gradients
- * are rounded to bfloat16 ahead of a product only where its result is bfloat16.  rows at most 4 194 176. */
+ * (the residual's gradient is grad_output itself).  pre may be null without an activation; outputs may be null, each.  dz goes into
+ * a product with 24 bits where its result is float32, with 16 where it is bfloat16 or float16.  rows at most 4 194 176. */
 int axc_fake_approx_dense_gradients_workspace_bytes(const axc_dense_desc *desc, size_t *bytes);
 int axc_fake_approx_dense_gradients(const axc_dense_desc *desc, const void *grad_output, const void *input,
                                     const void *input_range, const void *kernel, const void *pre, void *grad_input,

@@ -1,0 +1,76 @@
+"""How exact the transformer layers' results are, beyond what their sizes alone show: bounds that leave no room for a rounding to fewer
+bits on the way than the outputs' type has."""
+import pytest
+import torch
+
+import layer_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+DEV = "cuda:0"
+
+
+def make(shape, seed, dtype=F32, std=1.0):
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(seed)
+    return (torch.randn(shape, device=DEV, generator=gen) * std).to(dtype)
+
+
+@pytest.fixture(scope="module")
+def noisy(pkg):
+    return pkg.ops.TruthTable(pkg.synth.table_noisy(3))
+
+
+def products(dz, dz_off, xg, kg, x_dtype, k_dtype):
+    """((gradient, bound) of the input, of the kernel): the gradient dz goes into the products with 16 bits or more, 24 where the
+    result is float32 (two or three terms of 8 bits, each off by at most 2^-8 of what it stands for), and is rounded once at the end.
+    Terms below 2^-126 may count as 0, as in layer_reference.dense_gradients; so may the last of two, where the value is below 2^-118."""
+    dz_off = dz_off + 4 * 2.0 ** -126
+
+    def through(a, b, off, dtype, depth):
+        terms = 2.0 ** -24 if dtype == F32 else 2.0 ** -16
+        size = a.abs() @ b.abs()
+        return a @ b, off @ b.abs() + (terms + 3 * ref.E * (depth + 300)) * size
+    gx, bx = through(dz, kg.values.t().contiguous(), dz_off, x_dtype, dz.shape[1])
+    gk, bk = through(dz.t().contiguous(), xg.values, dz_off.t().contiguous(), k_dtype, dz.shape[0])
+    gk, bk = gk.t() * kg.inside, bk.t() * kg.inside
+    gx, bx = gx * xg.inside, bx * xg.inside
+    return (gx, ref.rounded(gx, bx, x_dtype)), (gk, ref.rounded(gk, bk, k_dtype))
+
+
+TYPES = [(BF16, BF16), (F32, BF16), (BF16, F32), (F16, BF16), (BF16, F16), (F16, F16), (F32, F32)]
+
+
+@pytest.mark.parametrize("size", [(3, 5, 2), (45, 130, 127), (515, 333, 70), (1000, 300, 260)], ids=str)
+@pytest.mark.parametrize("activation", [None, "relu", "gelu", "silu"])
+@pytest.mark.parametrize("x_dtype,k_dtype", TYPES, ids=str)
+def test_products_of_gradients(pkg, noisy, size, activation, x_dtype, k_dtype):
+    rows, depth, columns = size
+    x, k = make((rows, depth), 1, x_dtype), make((depth, columns), 2, k_dtype)
+    pre, gy = make((rows, columns), 3, x_dtype, 2.0), make((rows, columns), 4, x_dtype)
+    g = pkg.FakeApproxDense(noisy, activation).gradients(gy, x, k, pre if activation else None)
+    dz, off = gy.double(), torch.zeros((rows, columns), dtype=torch.float64, device=DEV)
+    if activation:
+        dz = dz * ref.slope(pre, activation)
+        # a slope is a few operations of float32, whose exponentials' arguments z^2 / 2 or z are rounded
+        off = gy.double().abs() * ref.E * (16 + 4 * pre.double().abs() + 4 * pre.double() ** 2)
+    for name, got, (want, bound) in zip(("inputs", "kernel"), g, products(dz, off, ref.Grid(pkg, x), ref.Grid(pkg, k), x_dtype, k_dtype)):
+        ref.check(got, want, bound, name)
+
+
+@pytest.mark.parametrize("size", [(5, 64, 1000), (129, 64, 5003), (300, 48, 16390)], ids=str)
+@pytest.mark.parametrize("x_dtype,k_dtype", [(BF16, BF16), (F32, BF16), (F16, F16)], ids=str)
+def test_products_of_the_loss(pkg, noisy, size, x_dtype, k_dtype):
+    rows, depth, vocabulary = size
+    x, k = make((rows, depth), 1, x_dtype), make((depth, vocabulary), 2, k_dtype, depth ** -0.5)
+    t = torch.arange(rows, device=DEV) * 7 % vocabulary
+    _, g = pkg.FakeApproxCrossEntropy(noisy).loss_and_gradients(x, k, t)
+    xg, kg = ref.Grid(pkg, x), ref.Grid(pkg, k)
+    z, z_off = ref.product(pkg.synth.table_noisy(3), xg, kg)
+    _, _, p, p_off = ref.loss(z, z_off, t, -100)
+    dz = p.clone()
+    dz[torch.arange(rows, device=DEV), t] -= 1
+    dz, off = dz / rows, (p * p_off + 8 * ref.E * (p + dz.abs())) / rows
+    for name, got, (want, bound) in zip(("inputs", "kernel"), g, products(dz, off, xg, kg, x_dtype, k_dtype)):
+        ref.check(got, want, bound, name)

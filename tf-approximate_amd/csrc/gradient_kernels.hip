@@ -5,9 +5,9 @@
 //   dkernel[k][n] = s_in sum_m (a[m][k] - z_in) dz[m][n]      where the kernel does
 //
 // Codes minus their zero point are whole numbers of at most 8 bits: bfloat16 holds them exactly, so the matrix cores' bfloat16
-// instructions multiply them without a rounding.  The gradient is the other operand.  For a bfloat16 result it is rounded to
-// bfloat16 itself; for float16 it is the sum of two bfloat16 terms (16 bits), for float32 of three (24 bits, all that a float
-// has), and the product runs over the terms one after the other as over a longer depth.  Sums are float32 throughout.
+// instructions multiply them without a rounding.  The gradient is the other operand.  It is the sum of two bfloat16 terms (16 bits)
+// for 16-bit results, of three for float32 (24 bits, all that a float has), of fewer where those hold it (a bfloat16 gradient without an
+// activation is one), and the product runs over the terms one after the other as over a longer depth.  Sums are float32 throughout.
 //
 // Both products run over the depth that is contiguous in both operands: dz is written straight and turned, the input's codes
 // turned, the kernel's straight.  All are padded with zeros to whole tiles, so the product has no edges to look at but in its

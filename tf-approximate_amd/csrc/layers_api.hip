@@ -493,7 +493,8 @@ static int carve_gradients(const axc_dense_desc *d, void *base, GradScratch *s, 
         return api_fail(AXC_UNIMPLEMENTED, "gradients of more than 4194176 rows");
     const Pieces pc = pieces_of(d->depth, d->columns, kDensePiece);
     const int64_t M = product_pad(d->rows), N = product_pad(d->columns), K = product_pad(d->depth);
-    const int px = parts_of(d->input_type), pk = parts_of(d->kernel_type);
+    const int exact = exact_terms(d->input_type, d->activation);
+    const int px = parts_of(d->input_type, exact), pk = parts_of(d->kernel_type, exact);
     Carver c(base);
     s->o = carve_operands(c, d, pc, false, false);
     s->straight = c.take<bf16>((size_t)M * N * px);
@@ -580,7 +581,8 @@ int axc_fake_approx_dense_gradients(const axc_dense_desc *desc, const void *grad
     if (!grad_input && !grad_kernel && !grad_bias)
         return AXC_OK;
     const int64_t rows = desc->rows, K = desc->depth, N = desc->columns;
-    const int px = parts_of(desc->input_type), pk = parts_of(desc->kernel_type);
+    const int exact = exact_terms(desc->input_type, desc->activation);
+    const int px = parts_of(desc->input_type, exact), pk = parts_of(desc->kernel_type, exact);
     RangeSource ranges[2];
     if (int rc = find_ranges(desc, input, input_range, kernel, s.o.x_pairs, s.o.kernel_pairs, nullptr, 0, &ranges[0], &ranges[1],
                              stream))
@@ -625,7 +627,7 @@ struct LossPlan {
 };
 static LossPlan loss_plan(const axc_dense_desc *d, const Pieces &pc, int64_t columns)
 {
-    const int px = parts_of(d->input_type), pk = parts_of(d->kernel_type);
+    const int px = parts_of(d->input_type, 3), pk = parts_of(d->kernel_type, 3);
     const ProductShape first[2] = {{d->rows, d->depth, pc.width_of(0), px, 1}, {d->depth, pc.width_of(0), d->rows, pk, 0}};
     const ProductShape own[2] = {{d->rows, d->depth, columns, px, 1}, {d->depth, columns, d->rows, pk, 0}};
     ProductPlan a[2], b[2];
@@ -662,7 +664,7 @@ static int carve_loss(const axc_dense_desc *d, bool gradients, void *base, LossS
     s->lut = c.take<char>(s->lut_bytes);
     if (gradients) {
         const int64_t M = product_pad(d->rows), P = product_pad(pc.width), K = product_pad(d->depth);
-        const int px = parts_of(d->input_type), pk = parts_of(d->kernel_type);
+        const int px = parts_of(d->input_type, 3), pk = parts_of(d->kernel_type, 3);
         s->straight = c.take<bf16>((size_t)M * P * px);
         s->turned = c.take<bf16>((size_t)M * P * pk);
         s->x_turned = c.take<bf16>((size_t)M * K);
@@ -766,7 +768,7 @@ int axc_fake_approx_cross_entropy(const axc_table *table, const axc_dense_desc *
     if (!gradients)
         return AXC_OK;
 
-    const int px = parts_of(desc->input_type), pk = parts_of(desc->kernel_type);
+    const int px = parts_of(desc->input_type, 3), pk = parts_of(desc->kernel_type, 3);
     const int64_t M = product_pad(rows);
     const ProductOut input_out = {grad_input, desc->input_type, K, input, K, &o.grids->in, &o.grids->kernel, s.st.factor};
     // from the last piece on, whose last run's sums are still there
