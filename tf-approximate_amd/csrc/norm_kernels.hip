@@ -568,11 +568,9 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(sizeof
         const Raw<T, NV> gate = gr;
         if (r + 1 < last)              // ahead of all reductions
             load(r + 1, group);
-        if constexpr (W != kEven) {
-            scale_row(dh, p.grad_y ? 1.0f : 0.0f);
+        if constexpr (W != kEven)
             if (!p.grad_h)
                 gh = {};
-        }
         if (p.layer) {
             float s[2] = {row_sum(n), row_sum(b)};
             red.sum(s);
@@ -641,6 +639,10 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(sizeof
             store_row(dgates, of, sg);
             sg = {};
         }
+    }
+    if (!p.grad_y) {                   // what is not there was loaded for nothing, and 0 times an infinite h is no 0
+        sw = {};
+        sb = {};
     }
     const Rows<W, float> to(p.partials, width);
     const int64_t at = (int64_t)blockIdx.x * kSums;
@@ -801,7 +803,7 @@ __global__ void __launch_bounds__(256) wide_grad_kernel(NormParams p, NormRuns r
         if (wanted)
             store_four<kOdd>(p.partials + (block * kSums + which) * width, c, width, t);
     };
-    leave(p.dweight, kSumWeight, sw);
+    leave(p.dweight, kSumWeight, p.grad_y ? sw : f32x4{});   // (0 times an infinite h is no 0)
     leave(p.dbias, kSumBias, sb);
     leave(p.dscale, kSumScale, ss);
     leave(p.dpost, kSumPost, sp);
