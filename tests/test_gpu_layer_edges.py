@@ -39,3 +39,33 @@ def test_a_norm_that_nothing_reads(pkg, kind, width, dtype):
     ref.check(g.block, want, ref.rounded(want, 2 * ref.E * want.abs(), dtype))
     g = norm.gradients(gh, None, h, None, weight, bias)
     assert not g.bias.any() and not g.weight.any() and torch.equal(g.x, gh)
+
+
+GATES = [  # rows' axes, gates' axes, whether that is one gate for each of a number of runs of neighbouring rows
+    ((4, 3), (), True), ((4, 3), (1,), True), ((4, 3), (1, 1), True), ((4, 3), (4,), True), ((4, 3), (4, 1), True), ((4, 3), (4, 3), True),
+    ((4, 3), (12,), True), ((4, 3), (1, 4, 1), True), ((4, 3), (3,), False), ((4, 3), (1, 3), False), ((4, 3), (2, 1), False),
+    ((4, 3), (6,), False), ((4, 3), (3, 4), False), ((4, 3), (2, 2), False), ((4, 3), (2, 4, 1), False), ((4, 3), (0,), False),
+    ((1, 3), (3,), True), ((1, 3), (1, 3), True), ((4, 1, 3), (4, 1, 1), True), ((4, 2, 3), (4, 2), True), ((4, 2, 3), (4, 1, 3), False),
+    ((4, 2, 3), (4, 2, 1), True), ((4, 2, 3), (1, 2, 1), False), ((12,), (4,), True), ((12,), (4, 1), True), ((12,), (5,), False),
+    ((), (), True), ((), (2,), False),
+]
+
+
+@pytest.mark.parametrize("rows,gates,fits", GATES, ids=str)
+def test_gates(pkg, rows, gates, fits):
+    norm = pkg.ResidualNorm("rms")
+    x, block, weight, gate = make(rows + (20,), 1), make(rows + (20,), 2), make((20,), 3), make(gates + (20,), 4)
+    gh = make(rows + (20,), 5)
+    if not fits:
+        with pytest.raises(pkg.InvalidArgumentError):
+            norm(x, block, weight, gate=gate)
+        with pytest.raises(pkg.InvalidArgumentError):
+            norm.gradients(gh, gh, x, block, weight, gate=gate)
+        return
+    h, y = norm(x, block, weight, gate=gate)
+    each = x.numel() // gate.numel()
+    want = x.view(-1, 20).double() + block.view(-1, 20).double() * gate.view(-1, 20).double().repeat_interleave(each, 0)
+    if len(rows) > 1 and len(gates) == len(rows):            # the same as the product of both
+        assert torch.equal(want.view(h.shape), x.double() + block.double() * gate.double())
+    ref.check(h.view(-1, 20), want, ref.rounded(want, 3 * ref.E * want.abs() + 2 * ref.E * (want - x.view(-1, 20)).abs(), F32))
+    assert norm.gradients(gh, gh, h, block, weight, gate=gate).gate.shape == gate.shape

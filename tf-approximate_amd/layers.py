@@ -12,6 +12,7 @@ scratch memory of its own from torch's allocator, so calls on several streams, a
 """
 import collections
 import ctypes
+import math
 import weakref
 
 import torch
@@ -96,6 +97,25 @@ def _minmax_of(input_minmax):
     if not lo <= hi or lo in (float("inf"), float("-inf")) or hi in (float("inf"), float("-inf")):
         raise InvalidArgumentError("input_minmax must be a finite (smallest, largest)")
     return lo, hi
+
+
+def _gate_groups(rows, gates):
+    """How many gates there are, gates = the shape of their tensor and rows = that of the input, both without the width; None if they are
+    not each for a run of neighbouring rows."""
+    count, all_rows = math.prod(gates), math.prod(rows)
+    if len(rows) <= 1:                           # rows without a structure
+        return count if all_rows == 0 or count and all_rows % count == 0 else None
+    if count == 1 or (len(gates) == 1 and count == all_rows):
+        return count
+    while len(gates) > len(rows) and gates[0] == 1:
+        gates = gates[1:]
+    # leading axes of one may be left out
+    ones = next((i for i, n in enumerate(rows) if n != 1), len(rows))
+    for of in (rows, rows[ones:]):
+        same = next((i for i, (g, r) in enumerate(zip(gates, of)) if g != r), min(len(gates), len(of)))
+        if all(g == 1 for g in gates[same:]):
+            return count
+    return None
 
 
 def _rows_in(inputs):
@@ -296,8 +316,10 @@ class ResidualNorm:
 
     norm: kind "rms" (v / sqrt(mean(v^2) + eps)) or "layer" ((v - mean) / sqrt(var + eps)).  x, block, gate and the outputs are of
     one type (float32, bfloat16, float16); weight, bias, scale, post_weight [width] of one type, any of them.  gate: [..., width],
-    its other axes flattened must divide the rows: [batch, width] or [batch, 1, width] against [batch, tokens, width], or one for
-    every row.  Without a block h is x."""
+    each for a run of neighbouring rows: one for all, one for every row, or the input's leading axes, with nothing but ones behind them
+    ([batch, width] or [batch, 1, width] against [batch, tokens, width]); against an input [rows, width] any number that divides the
+    rows.  Gates that would go round faster than the rows ([tokens, width] or [1, tokens, width]) are refused: expand them.  Without
+    a block h is x."""
 
     def __init__(self, kind="rms", eps=1e-6):
         if kind not in _NORMS:
@@ -322,9 +344,10 @@ class ResidualNorm:
             gate = _require(gate, "gate", device, like.dtype)
             if gate.dim() < 1 or gate.shape[-1] != width:
                 raise InvalidArgumentError("gate must be as wide as the input")
-            groups = gate.numel() // width if width else 0
-            if rows and (groups == 0 or rows % groups):
-                raise InvalidArgumentError("the gate's groups must divide the rows")
+            groups = _gate_groups(tuple(like.shape[:-1]), tuple(gate.shape[:-1]))
+            if groups is None:
+                raise InvalidArgumentError("a gate %s is not one for each of a number of runs of rows of an input %s" %
+                                           (tuple(gate.shape), tuple(like.shape)))
         desc = _lib.ResidualNormDesc(rows, width, groups, _TYPES[like.dtype], _TYPES[weight.dtype], self.kind, self.eps)
         alive = [None, block, weight, vectors[0], gate, vectors[1], vectors[2]]
         return desc, alive
