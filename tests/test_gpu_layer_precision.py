@@ -74,3 +74,32 @@ def test_products_of_the_loss(pkg, noisy, size, x_dtype, k_dtype):
     dz, off = dz / rows, (p * p_off + 8 * ref.E * (p + dz.abs())) / rows
     for name, got, (want, bound) in zip(("inputs", "kernel"), g, products(dz, off, xg, kg, x_dtype, k_dtype)):
         ref.check(got, want, bound, name)
+
+
+@pytest.mark.parametrize("common", [0.0, 1000.0, -131072.0])
+@pytest.mark.parametrize("rows,vocabulary", [(3, 301), (45, 301), (45, 5003), (600, 5003)], ids=str)
+def test_what_all_logits_have_in_common(pkg, noisy, rows, vocabulary, common):
+    """Logits of x = 0 are the bias, exact here: multiples of 1/64 below 2^18.  The bound does not grow with their common part."""
+    gen = torch.Generator(device=DEV)
+    gen.manual_seed(vocabulary)
+    part = torch.randint(-512, 513, (vocabulary,), device=DEV, generator=gen).double() / 64
+    part[5] = 24.0                                  # rows of that target are sure of it
+    bias = (part + common).float()
+    assert torch.equal(bias.double(), part + common)
+    x, k = torch.zeros((rows, 8), device=DEV), make((8, vocabulary), 2)
+    t = torch.where(torch.arange(rows, device=DEV) % 2 == 0, 5, torch.arange(rows, device=DEV) * 11 % vocabulary)
+    loss, g = pkg.FakeApproxCrossEntropy(noisy).loss_and_gradients(x, k, t, bias, "none")
+    # a sum of exponentials in chunks, and those of differences up to 32, which are exact; then a log, and one sum
+    log_sum = torch.log(torch.exp(part - 24.0).sum())
+    want = (24.0 - part[t]) + log_sum
+    off = torch.full_like(want, float(ref.E * (vocabulary / 64 + 256 + 4 * 32)))
+    ref.check(loss, want, ref.rounded(want, off, F32), "loss")
+    p = torch.exp(part - 24.0 - log_sum).expand(rows, -1)
+    p_off = float(off[0]) + ref.E * (16 + 4 * (part - 24.0).abs())
+    dz, dz_off = p.clone(), p * p_off
+    dz[torch.arange(rows, device=DEV), t] -= 1
+    dz_off = dz_off + 2 * ref.E * (p + dz.abs())
+    sums, off = dz.sum(0), dz_off.sum(0) + (rows + 8) * ref.E * dz.abs().sum(0)
+    ref.check(g.bias, sums, ref.rounded(sums, off, F32), "bias")
+    (gx, gx_off), _ = products(dz, dz_off, ref.Grid(pkg, x), ref.Grid(pkg, k), F32, F32)
+    ref.check(g.inputs, gx, gx_off, "inputs")

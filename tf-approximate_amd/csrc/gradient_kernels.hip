@@ -45,12 +45,12 @@ struct LogitTerms {
     }
     struct Line {                        // of a row
         I term;
-        float share, lse;
+        float share, top, log_sum;
         int64_t target;
     };
     __device__ __forceinline__ Line line(int64_t r) const
     {
-        return {b.row(g.sums.row_sums[r]), g.coefficient[r], g.lse[r], g.targets[r] - g.first_column};
+        return {b.row(g.sums.row_sums[r]), g.coefficient[r], g.top[r], g.log_sum[r], g.targets[r] - g.first_column};
     }
     __device__ __forceinline__ float bias(int64_t c) const { return g.bias ? load_any(g.bias, c, g.bias_type) : 0.0f; }
     __device__ __forceinline__ I column(int64_t c) const { return b.column(g.sums.column_sums[c]); }
@@ -59,7 +59,7 @@ struct LogitTerms {
         float z = __fmul_rn(Bracket<I>::value(sum, l.term, column), scale);
         if (g.bias)
             z = __fadd_rn(z, bias);
-        const float p = __expf(z - l.lse);
+        const float p = __expf((z - l.top) - l.log_sum);
         // a row that does not count has no gradient, whatever its logits are
         return l.share == 0.0f ? 0.0f : l.share * (c == l.target ? p - 1.0f : p);
     }

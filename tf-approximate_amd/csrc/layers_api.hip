@@ -652,7 +652,7 @@ static int carve_loss(const axc_dense_desc *d, bool gradients, void *base, LossS
     const Pieces pc = loss_pieces(d);
     Carver c(base);
     s->o = carve_operands(c, d, pc, true, true);
-    float **const state[] = {&s->st.at, &s->st.lse, &s->st.rows, &s->st.coefficient};
+    float **const state[] = {&s->st.at, &s->st.top, &s->st.log_sum, &s->st.rows, &s->st.coefficient};
     for (float **p : state)
         *p = c.take<float>((size_t)d->rows);
     s->st.factor = c.take<float>(1);
@@ -782,7 +782,8 @@ int axc_fake_approx_cross_entropy(const axc_table *table, const axc_dense_desc *
             made = false;
             GradSource g = {};
             g.sums = sums;
-            g.lse = s.st.lse + r;
+            g.top = s.st.top + r;
+            g.log_sum = s.st.log_sum + r;
             g.coefficient = s.st.coefficient + r;
             g.targets = targets + r;
             g.bias = element(bias, c, desc->bias_type);

@@ -470,9 +470,9 @@ inline int exact_terms(int type, int activation)
 struct GradSource {                      // where the gradient behind the product comes from
     const void *grad, *pre;              // dense: gradient of the output, what the activation was given (or null)
     int type, activation;
-    // loss: sums of a piece, log of each row's sum of exponentials, its coefficient and target
+    // loss: sums of a piece, each row's largest logit and log of the sum of exponentials around it, its coefficient and target
     TableSums sums;
-    const float *lse, *coefficient;
+    const float *top, *log_sum, *coefficient;
     const int64_t *targets;
     const void *bias;
     int bias_type;
@@ -540,7 +540,9 @@ inline int loss_chunk(int64_t rows) { return rows >= 2048 ? 512 : rows >= 512 ? 
 struct LossState {
     float2 *parts;                       // [chunk][rows]: the largest logit and the sum of exponentials around it
     float *at;                           // per row: the target's logit
-    float *lse, *rows;                   // log of the whole sum; the row's loss
+    float *top, *log_sum;                // the largest of all, and the log of the whole sum around it: not in one, whose rounding would be that
+                                         // of what all logits have in common
+    float *rows;                         // the row's loss
     float *coefficient, *factor;         // a row's gradient is multiplied by coefficient[row] * *factor
 };
 // Of a run of rows from `first_row` on, into parts from `chunk` on; returns how many chunks in *chunks.

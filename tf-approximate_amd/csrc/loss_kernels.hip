@@ -1,9 +1,10 @@
 // Softmax cross entropy over a vocabulary whose logits are sums of table entries, a piece of the vocabulary at a time.
 //
-//   loss[m] = log sum_v exp(z[m][v]) - z[m][target[m]]
+//   loss[m] = log sum_v exp(z[m][v]) - z[m][target[m]] = (t - z[m][target[m]]) + log s
 //
 // A chunk of columns leaves its largest logit t and s = sum exp(z - t), in float32; two of them make max(t, t') and
-// s exp(t - max) + s' exp(t' - max).  Chunks whose logits are all -infinity have t = -infinity and s = 0.
+// s exp(t - max) + s' exp(t' - max).  t and log s stay apart to the end: what all of a row's logits have in common, however much, has no
+// part in the loss or in a probability exp((z - t) - log s).  Chunks whose logits are all -infinity have t = -infinity and s = 0.
 #include "layers_internal.h"
 
 namespace axc {
@@ -166,11 +167,12 @@ __global__ void __launch_bounds__(64 * kRowWaves) loss_rows_kernel(LossState st,
         return;
     for (int w = 1; w < kRowWaves; ++w)
         e.join(ends[w][lane].x, ends[w][lane].y);
-    const float lse = e.top + logf(e.sum);
+    const float log_sum = logf(e.sum);
     const int64_t t = targets[r];
-    st.lse[r] = lse;
+    st.top[r] = e.top;
+    st.log_sum[r] = log_sum;
     // a target that is no column of the vocabulary has no loss
-    st.rows[r] = t == ignore ? 0.0f : t >= 0 && t < V ? lse - st.at[r] : NAN;
+    st.rows[r] = t == ignore ? 0.0f : t >= 0 && t < V ? (e.top - st.at[r]) + log_sum : NAN;
 }
 
 // The loss out of the rows', in one order, and what each row's gradient is multiplied by.
