@@ -69,3 +69,33 @@ def test_gates(pkg, rows, gates, fits):
         assert torch.equal(want.view(h.shape), x.double() + block.double() * gate.double())
     ref.check(h.view(-1, 20), want, ref.rounded(want, 3 * ref.E * want.abs() + 2 * ref.E * (want - x.view(-1, 20)).abs(), F32))
     assert norm.gradients(gh, gh, h, block, weight, gate=gate).gate.shape == gate.shape
+
+
+@pytest.mark.parametrize("rows", [6, 45])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+def test_gradients_of_the_loss_far_apart(pkg, noisy, rows, dtype):
+    """A row's gradient is its own: what the loss' gradient is in other rows, however large, does not reach it."""
+    fn = pkg.FakeApproxCrossEntropy(noisy)
+    x, k, t = make((rows, 16), 1, dtype), make((16, 300), 2, dtype), torch.arange(rows, device=DEV)
+    t[5] = -100
+    _, plain = fn.loss_and_gradients(x, k, t, reduction="none")
+    assert torch.isfinite(plain.inputs).all()
+    some = torch.ones(rows, device=DEV)
+    some[0], some[1], some[3] = 2.0 ** 100, 2.0 ** -60, 0.0
+    _, g = fn.loss_and_gradients(x, k, t, reduction="none", grad_loss=some)
+    want = plain.inputs.double() * some.double()[:, None]        # by powers of two: nothing is rounded otherwise
+    assert torch.equal(g.inputs.double(), want)
+    for bad in (INF, NAN):
+        some[0] = bad
+        _, g = fn.loss_and_gradients(x, k, t, reduction="none", grad_loss=some)
+        assert torch.equal(g.inputs[1:].double(), want[1:])
+        assert not torch.isfinite(g.inputs[0][ref.Grid(pkg, x).inside[0]]).any()
+    for reduction in ("sum", "mean"):
+        for scale in (-4.0, INF, -INF, NAN):
+            _, one = fn.loss_and_gradients(x, k, t, reduction=reduction)
+            _, g = fn.loss_and_gradients(x, k, t, reduction=reduction, grad_loss=torch.tensor(scale, device=DEV))
+            assert not g.inputs[5].any() and one.inputs[0].any()
+            if scale == -4.0:
+                assert torch.equal(g.inputs, one.inputs * scale) and torch.equal(g.kernel, one.kernel * scale)
+            else:
+                assert not torch.isfinite(g.inputs[0][ref.Grid(pkg, x).inside[0]]).any()

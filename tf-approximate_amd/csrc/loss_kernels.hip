@@ -213,28 +213,21 @@ __global__ void __launch_bounds__(1024) loss_out_kernel(LossState st, const int6
     }
     if (!gradients)
         return;
-    // What all rows have in common goes behind the products: multiplied into softmax minus one-hot ahead of a rounding to
-    // bfloat16 it would round every row's largest part, minus the factor, off by the same amount.
+    // What all rows have in common goes behind the products: multiplied into softmax minus one-hot ahead of a rounding to terms of
+    // bfloat16 it would round every row's largest part, minus the factor, off by the same amount.  What is each row's own stays
+    // in front, and so does what is not finite: behind, rows that do not count would be 0 times infinity.
     float factor = reduction == AXC_LOSS_MEAN ? 1.0f / (float)(count > 0 ? count : 1) : 1.0f;
-    float most = 1.0f;
-    if (grad_loss) {
-        most = 0.0f;
-        if (reduction != AXC_LOSS_NONE)
-            most = fabsf(grad_loss[0]);
-        else
-            for (int64_t r = threadIdx.x; r < rows; r += 1024)
-                most = fmaxf(most, targets[r] == ignore ? 0.0f : fabsf(grad_loss[r]));
-        float least = 0.0f;
-        __shared__ float red[32];
-        block_range(least, most, red);
-        factor *= most;
+    bool own = reduction == AXC_LOSS_NONE;
+    if (grad_loss && !own) {
+        own = !(fabsf(grad_loss[0]) < INFINITY);
+        factor *= own ? 1.0f : grad_loss[0];
     }
     if (threadIdx.x == 0)
         *st.factor = factor;
     for (int64_t r = threadIdx.x; r < rows; r += 1024) {
         const float of = grad_loss ? grad_loss[reduction == AXC_LOSS_NONE ? r : 0] : 1.0f;
         const int64_t t = targets[r];
-        st.coefficient[r] = t == ignore || of == 0.0f ? 0.0f : t >= 0 && t < V ? of / most : NAN;
+        st.coefficient[r] = t == ignore || of == 0.0f ? 0.0f : t >= 0 && t < V ? (own ? of : 1.0f) : NAN;
     }
 }
 
