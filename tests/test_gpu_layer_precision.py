@@ -103,3 +103,32 @@ def test_what_all_logits_have_in_common(pkg, noisy, rows, vocabulary, common):
     ref.check(g.bias, sums, ref.rounded(sums, off, F32), "bias")
     (gx, gx_off), _ = products(dz, dz_off, ref.Grid(pkg, x), ref.Grid(pkg, k), F32, F32)
     ref.check(g.inputs, gx, gx_off, "inputs")
+
+
+@pytest.mark.parametrize("rows", [1, 3, 45])
+@pytest.mark.parametrize("activation", ["gelu", "gelu_tanh", "silu"])
+def test_activations_over_their_tails(pkg, noisy, rows, activation):
+    """What goes in is the bias, exact, as x is 0.  Bounds are relative to the result, however small: half steps of a few operations,
+    and of an exponential's argument, once for each operation that made it: 4 for z^2 / 2, 8 for the cubic, 4 for z.  Beyond exp(87) a
+    logistic function may be 0, off by 2^-125, and so may what an exponential below 2^-126 is multiplied by."""
+    z = torch.linspace(-12.0, 12.0, 4803, device=DEV)
+    layer = pkg.FakeApproxDense(noisy, activation)
+    x, k = torch.zeros((rows, 8), device=DEV), make((8, z.numel()), 2)
+    y, pre = layer.call_and_keep(x, k, z)
+    assert torch.equal(pre, z.expand(rows, -1))
+    d = z.double().requires_grad_()
+    # (1 + tanh u) / 2 is the logistic function of 2 u; as it stands in layer_reference it is 1e-16 off, which is all there is below -8
+    fn = (lambda v: v * torch.sigmoid(1.5957691216057308 * (v + 0.044715 * v ** 3))) if activation == "gelu_tanh" else \
+        ref.ACTIVATIONS[activation]
+    want = fn(d)
+    slope = torch.autograd.grad(want.sum(), d)[0]
+    want, d = want.detach(), d.detach()
+    size = {"gelu": 3 * d * d, "gelu_tanh": 8 * 1.6 * (d + 0.044715 * d ** 3).abs(), "silu": 4 * d.abs()}[activation]
+    bound = ref.E * (24 + size) * want.abs() + 2.0 ** -125 * d.abs()
+    for row in y:
+        ref.check(row, want, ref.rounded(want, bound, F32))
+    # the slope, of one row: f + z f', either of which may be the larger
+    g = layer.gradients(torch.ones_like(y[:1]), x[:1], k, pre[:1], want=("bias",)).bias
+    terms = (want / d).abs() + (slope - want / d).abs()
+    terms[d == 0] = 0.5
+    ref.check(g, slope, ref.rounded(slope, ref.E * (32 + 2 * size) * terms + 2.0 ** -125 * (1 + d.abs() ** 3), F32), "slope")
