@@ -1901,7 +1901,8 @@ int axc_table_create(const uint16_t *host_table, axc_table **out)
         return fail(AXC_INVALID_ARGUMENT, "null argument");
     // weight-code major: tableT[b][a] = T[(a << 8) | b], in squares that the first-level cache holds by row and by column, and
     // the two flipped copies by whole vectors (us a table with its upload, on one machine: entry by entry 143 for the first
-    // alone, 181 for three; 42); behind them the one for dense layers of few rows
+    // alone, 181 for three; 43); behind them the one for dense layers of few rows, by whole vectors too (entry by entry 66, 57, most of
+    // what it adds its upload)
     const size_t entries = (size_t)kTableRows * 256, used = 65536;   // row 256: the null weight's, zeros
     std::vector<uint16_t> t(4 * entries);
     uint16_t *const T = t.data(), *const F = T + entries, *const S = F + entries, *const L = S + entries;
@@ -1920,8 +1921,19 @@ int axc_table_create(const uint16_t *host_table, axc_table **out)
         uint32_t r = 0;                  // the bits of a turned round
         for (int bit = 0; bit < 8; ++bit)
             r |= (a >> bit & 1u) << (7 - bit);
-        for (uint32_t b = 0; b < 256; ++b)
-            L[r * 256 + (b ^ r)] = host_table[a * 256 + b];
+        // an entry's place in its row is b ^ r: eight together by the upper bits of r, among the eight by the lower three
+        typedef uint16_t Eight __attribute__((vector_size(16)));
+        for (uint32_t b = 0; b < 256; b += 8) {
+            Eight w;
+            memcpy(&w, host_table + a * 256 + b, 16);
+            if (r & 4)
+                w = __builtin_shufflevector(w, w, 4, 5, 6, 7, 0, 1, 2, 3);
+            if (r & 2)
+                w = __builtin_shufflevector(w, w, 2, 3, 0, 1, 6, 7, 4, 5);
+            if (r & 1)
+                w = __builtin_shufflevector(w, w, 1, 0, 3, 2, 5, 4, 7, 6);
+            memcpy(L + r * 256 + (b ^ (r & ~7u)), &w, 16);
+        }
     }
     axc_table *tab = new axc_table;
     tab->dev_tableT = nullptr;
