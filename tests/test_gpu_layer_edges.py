@@ -99,3 +99,15 @@ def test_gradients_of_the_loss_far_apart(pkg, noisy, rows, dtype):
                 assert torch.equal(g.inputs, one.inputs * scale) and torch.equal(g.kernel, one.kernel * scale)
             else:
                 assert not torch.isfinite(g.inputs[0][ref.Grid(pkg, x).inside[0]]).any()
+
+
+def test_more_rows_than_threads_of_a_launch(pkg, noisy):
+    """2^26 rows and more, a wavefront each: the last rows, against a call on those alone."""
+    rows = (1 << 26) + 37
+    x, k, bias = make((rows, 1), 1, BF16), make((1, 2), 2), make((2,), 3)
+    lo, hi = (float(v) for v in x.float().aminmax())
+    layer = pkg.FakeApproxDense(noisy, "relu", input_minmax=(lo, hi))
+    y = layer(x, k, bias)
+    for first, last in ((0, 40), ((1 << 22) - 20, (1 << 22) + 20), (rows - 60, rows)):
+        assert torch.equal(y[first:last], layer(x[first:last].contiguous(), k, bias))
+    assert torch.equal(y[-60:], layer(x, layer.pack(k), bias)[-60:])

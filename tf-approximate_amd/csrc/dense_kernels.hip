@@ -158,6 +158,7 @@ __global__ void __launch_bounds__(512) few_codes_kernel(FewInput in, int rows, i
 }
 
 constexpr int kSlab = 64;   // most of the depth that a workgroup of codes_kernel takes
+constexpr int64_t kCodesBlocks = 1 << 20;   // workgroups for the input's rows, at most
 
 // tile: not null: the codes go there too, [element of the slab][column of the workgroup].
 template <typename T>
@@ -189,7 +190,7 @@ __device__ void kernel_slab(const T *__restrict__ w, int K, int64_t N, const Pie
     }
 }
 
-// The first x_blocks workgroups take four rows of the input each, a wavefront a row (rows up to the next multiple of four are pad
+// The first x_blocks workgroups take four rows of the input at a time, a wavefront a row (rows up to the next multiple of four are pad
 // rows, of code 0).  The others take 256 columns of the kernel, four a lane, by 4 * lines of the depth, a wavefront every fourth;
 // column sums are added to what the launch before cleared, as whole numbers, so in any order.  Every workgroup makes the grid it
 // needs out of the range's pairs itself: a launch for that alone would be longer than folding 256 of them.
@@ -208,18 +209,20 @@ __global__ void __launch_bounds__(256) codes_kernel(CodesJob job, int x_blocks, 
             if (!job.kernel)
                 job.grids->kernel = *job.kernel_grid;
         }
-        const int64_t r = (int64_t)blockIdx.x * 4 + wave;
         const int Kp = job.pieces.Kp;
-        uint8_t *const codes = job.x_codes + r * Kp;
-        int32_t sum = 0;
-        if (r < job.rows)
-            sum = row_codes_any(job.x, job.x_type, r * job.K, job.K, Kp, g, codes, lane, 64);
-        else
-            for (int k = 4 * lane; k < Kp; k += 256)
-                *reinterpret_cast<uint32_t *>(codes + k) = 0u;
-        sum = wave_sum(sum);
-        if (lane == 0)
-            job.row_sums[r] = sum;
+        const int64_t padded = (job.rows + 3) / 4 * 4;
+        for (int64_t r = (int64_t)blockIdx.x * 4 + wave; r < padded; r += (int64_t)x_blocks * 4) {
+            uint8_t *const codes = job.x_codes + r * Kp;
+            int32_t sum = 0;
+            if (r < job.rows)
+                sum = row_codes_any(job.x, job.x_type, r * job.K, job.K, Kp, g, codes, lane, 64);
+            else
+                for (int k = 4 * lane; k < Kp; k += 256)
+                    *reinterpret_cast<uint32_t *>(codes + k) = 0u;
+            sum = wave_sum(sum);
+            if (lane == 0)
+                job.row_sums[r] = sum;
+        }
         return;
     }
     fold(job.kernel_range, lo, hi, ends);
@@ -837,7 +840,8 @@ hipError_t launch_few_codes(const FewInput &in, int rows, int Kb, Grids *grids, 
 
 hipError_t launch_codes(const CodesJob &job, hipStream_t stream)
 {
-    const int x_blocks = job.x ? (int)((job.rows + 3) / 4) : 0;
+    // (a launch has fewer than 2^32 threads, 2^24 of these workgroups)
+    const int x_blocks = job.x ? (int)((job.rows + 3) / 4 < kCodesBlocks ? (job.rows + 3) / 4 : kCodesBlocks) : 0;
     const int column_blocks = job.kernel ? (int)((job.pieces.Np + 255) / 256) : 1;
     // a wavefront 16 lines of the depth, fewer where that would leave CUs without work
     int lines = kSlab / 4;
