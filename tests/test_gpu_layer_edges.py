@@ -111,3 +111,18 @@ def test_more_rows_than_threads_of_a_launch(pkg, noisy):
     for first, last in ((0, 40), ((1 << 22) - 20, (1 << 22) + 20), (rows - 60, rows)):
         assert torch.equal(y[first:last], layer(x[first:last].contiguous(), k, bias))
     assert torch.equal(y[-60:], layer(x, layer.pack(k), bias)[-60:])
+
+
+@pytest.mark.parametrize("rows", [45, 4097, 5003, 16390])
+def test_a_range_handed_on_to_many_rows(pkg, noisy, rows):
+    """Rows beyond what the workgroups that read a reported range take at once."""
+    norm, layer, loss = pkg.ResidualNorm("rms"), pkg.FakeApproxDense(noisy, "silu"), pkg.FakeApproxCrossEntropy(noisy)
+    x, weight, k, gy = make((rows, 24), 1, BF16), make((24,), 2), make((24, 40), 3, BF16), make((rows, 40), 4, BF16)
+    _, y, seen = norm.call_in_turn(x, None, weight)
+    t = torch.arange(rows, device=DEV) % 40
+    for kernel in (k, layer.pack(k)):
+        assert torch.equal(layer(y, kernel, input_range=seen), layer(y, kernel))
+    _, pre = layer.call_and_keep(y, k)
+    for a, b in zip(layer.gradients(gy, y, k, pre, input_range=seen), layer.gradients(gy, y, k, pre)):
+        assert torch.equal(a, b)
+    assert torch.equal(loss(y, k, t, input_range=seen), loss(y, k, t))

@@ -50,9 +50,9 @@ __device__ void range_of_any(const void *p, int type, int64_t n, int64_t index, 
         range_of(static_cast<const f16 *>(p), n, index, stride, lo, hi);
 }
 
-// One pair per workgroup; the first x_blocks take the input, the others the kernel.  All of them clear `zeros`, into which a
-// later launch adds.
-__global__ void __launch_bounds__(1024) range_kernel(const void *x, int x_type, int64_t nx, int x_blocks, const void *kernel,
+// One pair per workgroup; the first x_blocks take the input (or one of them the pairs that a call before has reported of it: all that
+// follows then reads one), the others the kernel.  All of them clear `zeros`, into which a later launch adds.
+__global__ void __launch_bounds__(1024) range_kernel(const void *x, int x_type, int64_t nx, const float *reported, int x_blocks, const void *kernel,
                                                      int kernel_type, int64_t nk, float *x_pairs, float *kernel_pairs,
                                                      int32_t *zeros, int64_t n_zeros)
 {
@@ -63,9 +63,13 @@ __global__ void __launch_bounds__(1024) range_kernel(const void *x, int x_type, 
     for (int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x; i < n_zeros; i += (int64_t)gridDim.x * 1024)
         zeros[i] = 0;
     float lo = INFINITY, hi = -INFINITY;
-    range_of_any(second ? kernel : x, second ? kernel_type : x_type, second ? nk : nx, (int64_t)block * 1024 + threadIdx.x,
-                 (int64_t)blocks * 1024, lo, hi);
-    block_range(lo, hi, red);
+    if (!second && reported) {
+        fold({reported, kRangePairs, 0.0f, 0.0f}, lo, hi, red);
+    } else {
+        range_of_any(second ? kernel : x, second ? kernel_type : x_type, second ? nk : nx, (int64_t)block * 1024 + threadIdx.x,
+                     (int64_t)blocks * 1024, lo, hi);
+        block_range(lo, hi, red);
+    }
     if (threadIdx.x == 0) {
         float *const to = second ? kernel_pairs : x_pairs;
         to[2 * block] = lo;
@@ -193,7 +197,8 @@ __device__ void kernel_slab(const T *__restrict__ w, int K, int64_t N, const Pie
 // The first x_blocks workgroups take four rows of the input at a time, a wavefront a row (rows up to the next multiple of four are pad
 // rows, of code 0).  The others take 256 columns of the kernel, four a lane, by 4 * lines of the depth, a wavefront every fourth;
 // column sums are added to what the launch before cleared, as whole numbers, so in any order.  Every workgroup makes the grid it
-// needs out of the range's pairs itself: a launch for that alone would be longer than folding 256 of them.
+// needs out of the range's pairs itself: a launch for that alone would be longer than folding 256 of them (or, of a range that a call before
+// has reported, of an input against a packed kernel, 4096).
 __global__ void __launch_bounds__(256) codes_kernel(CodesJob job, int x_blocks, int column_blocks, int lines)
 {
     __shared__ float ends[8];
@@ -814,20 +819,20 @@ hipError_t launch_zero(void *p, int64_t bytes, hipStream_t stream)
     return hipGetLastError();
 }
 
-hipError_t launch_range(const void *x, int x_type, int64_t nx, const void *kernel, int kernel_type, int64_t nk, float *x_pairs,
-                        float *kernel_pairs, int32_t *zeros, int64_t n_zeros, int *x_count, int *kernel_count, hipStream_t stream)
+hipError_t launch_range(const void *x, int x_type, int64_t nx, const float *reported, const void *kernel, int kernel_type, int64_t nk,
+                        float *x_pairs, float *kernel_pairs, int32_t *zeros, int64_t n_zeros, int *x_count, int *kernel_count, hipStream_t stream)
 {
     auto blocks = [](int64_t n) {   // 16 values a thread and more
         const int64_t b = (n + 16383) / 16384;
         return (int)(b > kRangeBlocks ? kRangeBlocks : b);
     };
-    const int bx = x ? blocks(nx) : 0, bk = kernel ? blocks(nk) : 0;
+    const int bx = x ? blocks(nx) : reported ? 1 : 0, bk = kernel ? blocks(nk) : 0;
     *x_count = bx;
     *kernel_count = bk;
     const int total = bx + bk;
     if (total == 0)
         return hipSuccess;
-    hipLaunchKernelGGL(range_kernel, dim3(total), dim3(1024), 0, stream, x, x_type, nx, bx, kernel, kernel_type, nk, x_pairs,
+    hipLaunchKernelGGL(range_kernel, dim3(total), dim3(1024), 0, stream, x, x_type, nx, reported, bx, kernel, kernel_type, nk, x_pairs,
                        kernel_pairs, zeros, n_zeros);
     return hipGetLastError();
 }
@@ -840,8 +845,10 @@ hipError_t launch_few_codes(const FewInput &in, int rows, int Kb, Grids *grids, 
 
 hipError_t launch_codes(const CodesJob &job, hipStream_t stream)
 {
-    // (a launch has fewer than 2^32 threads, 2^24 of these workgroups)
-    const int x_blocks = job.x ? (int)((job.rows + 3) / 4 < kCodesBlocks ? (job.rows + 3) / 4 : kCodesBlocks) : 0;
+    // A launch has fewer than 2^32 threads, 2^24 of these workgroups; and where each reads a reported range, 32 KiB, four a CU go
+    // over the rows (16 384 rows, 64 -> 64, packed: 34.4 us a call, 41.1 by one for every four rows).
+    const int64_t most = job.x_range.count > kRangeBlocks ? 1024 : kCodesBlocks;
+    const int x_blocks = job.x ? (int)((job.rows + 3) / 4 < most ? (job.rows + 3) / 4 : most) : 0;
     const int column_blocks = job.kernel ? (int)((job.pieces.Np + 255) / 256) : 1;
     // a wavefront 16 lines of the depth, fewer where that would leave CUs without work
     int lines = kSlab / 4;

@@ -231,6 +231,7 @@ __device__ __forceinline__ void fold(const RangeSource &src, float &lo, float &h
     if (src.pairs) {
         lo = INFINITY;
         hi = -INFINITY;
+#pragma unroll 4
         for (int i = threadIdx.x; i < src.count; i += blockDim.x) {
             const float2 p = reinterpret_cast<const float2 *>(src.pairs)[i];
             lo = fminf(lo, p.x);
@@ -390,8 +391,10 @@ __device__ __forceinline__ i32x4 four_sums(const RawSums &s, int64_t r, int64_t 
     return t;
 }
 
-hipError_t launch_range(const void *x, int x_type, int64_t nx, const void *kernel, int kernel_type, int64_t nk, float *x_pairs,
-                        float *kernel_pairs, int32_t *zeros, int64_t n_zeros, int *x_count, int *kernel_count, hipStream_t stream);
+// reported: x is null, and this is what a call before has reported of it.
+hipError_t launch_range(const void *x, int x_type, int64_t nx, const float *reported, const void *kernel, int kernel_type, int64_t nk,
+                        float *x_pairs, float *kernel_pairs, int32_t *zeros, int64_t n_zeros, int *x_count, int *kernel_count,
+                        hipStream_t stream);
 // Codes of both operands and their sums, and the grids they are on.  x null: only the kernel's; kernel null: only the input's,
 // and the kernel's grid is that of kernel_grid.
 struct CodesJob {
