@@ -126,3 +126,20 @@ def test_a_range_handed_on_to_many_rows(pkg, noisy, rows):
     for a, b in zip(layer.gradients(gy, y, k, pre, input_range=seen), layer.gradients(gy, y, k, pre)):
         assert torch.equal(a, b)
     assert torch.equal(loss(y, k, t, input_range=seen), loss(y, k, t))
+
+
+def test_parameters(pkg, noisy):
+    """Tensors that require a gradient, where torch does not record, and in the calls that make gradients."""
+    dense, loss, norm = pkg.FakeApproxDense(noisy), pkg.FakeApproxCrossEntropy(noisy), pkg.ResidualNorm()
+    x, k, w, t = make((5, 16), 1), make((16, 30), 2), make((16,), 3), torch.arange(5, device=DEV)
+    xp, kp, wp = (torch.nn.Parameter(v) for v in (x, k, w))
+    with torch.no_grad():
+        assert torch.equal(dense(xp, kp), dense(x, k)) and torch.equal(loss(xp, kp, t), loss(x, k, t))
+        assert torch.equal(norm(xp, xp, wp)[1], norm(x, x, w)[1])
+    gy = make((5, 30), 4)
+    assert torch.equal(dense.gradients(gy, xp, kp).kernel, dense.gradients(gy, x, k).kernel)
+    assert torch.equal(loss.loss_and_gradients(xp, kp, t)[1].inputs, loss.loss_and_gradients(x, k, t)[1].inputs)
+    assert torch.equal(norm.gradients(x, x, xp, xp, wp).weight, norm.gradients(x, x, x, x, w).weight)
+    assert torch.equal(dense(x, dense.pack(kp)), dense(x, k))
+    with pytest.raises(pkg.InvalidArgumentError, match="no_grad"):
+        dense(x, kp)

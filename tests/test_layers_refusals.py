@@ -135,3 +135,20 @@ def test_ranges_out_of_line(pkg):
     desc = ctypes.byref(dense(pkg))
     assert lib.axc_fake_approx_dense_gradients(desc, 256, 256, 260, *[256] * 6, 1 << 30, None) == bad
     assert b"8-byte" in lib.axc_last_error()
+
+
+def test_tensors_that_require_a_gradient(pkg):
+    """Refused ahead of all else while torch records: the output would be a constant to it."""
+    table = object.__new__(pkg.TruthTable)
+    dense, loss, norm = pkg.FakeApproxDense(table), pkg.FakeApproxCrossEntropy(table), pkg.ResidualNorm()
+    x, k, w, t = torch.zeros(2, 4), torch.zeros(4, 3), torch.zeros(4), torch.zeros(2, dtype=torch.int64)
+    leaf = lambda t: t.clone().requires_grad_()  # noqa: E731
+    calls = [lambda: dense(leaf(x), k), lambda: dense(x, leaf(k)), lambda: dense(x, k, leaf(w[:3])), lambda: dense.call_and_keep(x, leaf(k)),
+             lambda: dense(x, k, None, leaf(x[:, :3])), lambda: loss(leaf(x), k, t), lambda: loss(x, leaf(k), t),
+             lambda: loss(x, k, t, leaf(w[:3])), lambda: norm(leaf(x), x, w), lambda: norm(x, leaf(x), w), lambda: norm(x, x, leaf(w)),
+             lambda: norm.call_in_turn(x, x, w, scale=leaf(w)), lambda: norm(x, x, w, gate=leaf(w))]
+    for call in calls:
+        with pytest.raises(pkg.InvalidArgumentError, match="no_grad"):
+            call()
+        with torch.no_grad(), pytest.raises(pkg.InvalidArgumentError, match="on the GPU"):
+            call()

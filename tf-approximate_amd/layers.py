@@ -7,7 +7,8 @@
 The reference has no table op but the convolution: its layer call (tf2/python/keras/layers/fake_approx_convolutional.py:223-261,
 min / max of both operands, fake quantization, the op, bias, activation) is made here around matrix products.  As everywhere in
 this package torch owns the memory and the stream, and all arithmetic happens in libaxconv_hip.so.  Calls take no part in
-torch.autograd: gradients are calls of their own, and can be captured into a graph as forward passes can.  Every call has
+torch.autograd: gradients are calls of their own, and can be captured into a graph as forward passes can.  A forward call on a tensor
+that requires a gradient is therefore refused while torch records (under torch.no_grad() it is not).  Every call has
 scratch memory of its own from torch's allocator, so calls on several streams, and graphs, do not meet in it.
 """
 import collections
@@ -42,6 +43,15 @@ def _require(t, what, device=None, dtype=None, shape=None):
     if shape is not None and t.shape != shape:
         raise InvalidArgumentError("%s must have the shape %s" % (what, tuple(shape)))
     return t if t.is_contiguous() else t.contiguous()
+
+
+def _unrecorded(*tensors):
+    """Torch would take the output for a constant, and what it comes from would silently have no gradient."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if torch.is_tensor(t) and t.requires_grad:
+                raise InvalidArgumentError("a gradient does not pass through this call: make it under torch.no_grad(), and take "
+                                           "gradients() for what requires one")
 
 
 def _pointer(t):
@@ -185,6 +195,7 @@ class FakeApproxDense:
     def _run(self, inputs, kernel, bias, residual, input_range, keep):
         lib = _lib.load()
         _rows_in(inputs)
+        _unrecorded(inputs, kernel, bias, residual)
         found = _range_pointer(input_range, inputs)
         inputs = _require(inputs, "input")
         device = inputs.device
@@ -261,6 +272,7 @@ class FakeApproxCrossEntropy:
 
     def __call__(self, inputs, kernel, targets, bias=None, reduction="mean", input_range=None):
         """The loss, in float32."""
+        _unrecorded(inputs, kernel, bias)
         return self._run(inputs, kernel, targets, bias, reduction, None, input_range, ())[0]
 
     def loss_and_gradients(self, inputs, kernel, targets, bias=None, reduction="mean", grad_loss=None, input_range=None,
@@ -367,6 +379,7 @@ class ResidualNorm:
     def _run(self, x, block, weight, bias, gate, scale, post_weight, want_range):
         lib = _lib.load()
         _rows_in(x)
+        _unrecorded(x, block, weight, bias, gate, scale, post_weight)
         x = _require(x, "x")
         desc, alive = self._tensors(x, block, weight, bias, gate, scale, post_weight)
         alive[0] = x
