@@ -143,3 +143,40 @@ def test_parameters(pkg, noisy):
     assert torch.equal(dense(x, dense.pack(kp)), dense(x, k))
     with pytest.raises(pkg.InvalidArgumentError, match="no_grad"):
         dense(x, kp)
+
+
+@pytest.mark.parametrize("rows,depth,columns,dtype,activation", [(270003, 8, 1001, F32, None), (270003, 8, 1001, BF16, "gelu"),
+                                                                 (360000, 700, 12, BF16, None)], ids=str)
+def test_gradients_in_runs_of_rows(pkg, noisy, rows, depth, columns, dtype, activation):
+    """More values of the gradient, or of the input, than stand in front of the products at a time."""
+    assert rows * (max(depth, columns) + 127) // 128 * 128 > 1 << 28
+    x, k, gy = make((rows, depth), 1, dtype), make((depth, columns), 2, dtype), make((rows, columns), 3, dtype)
+    pre = make((rows, columns), 4, dtype, 2.0) if activation else None
+    lo, hi = (float(v) for v in x.float().aminmax())
+    layer = pkg.FakeApproxDense(noisy, activation, input_minmax=(lo, hi))
+    g = layer.gradients(gy, x, k, pre)
+    # (a product alone may be made by another number of wavefronts a tile: summed in another order, held to the same bounds)
+    alone = [getattr(layer.gradients(gy, x, k, pre, want=(one,)), one) for one in ("inputs", "kernel", "bias")]
+    ranges = ((0, 200), (261900, 262300), (rows - 300, rows))
+    for first, last in ranges:                    # (262144: where runs of 1024 values a row end)
+        part = gy[first:last], x[first:last].contiguous(), pre[first:last].contiguous() if activation else None
+        few = layer.gradients(part[0].contiguous(), part[1], k, part[2], want=("inputs",)).inputs
+        size = gy[first:last].double().abs() @ k.double().abs().t().contiguous()
+        # the same terms, summed in another order, of columns + 300 operations, and rounded once each
+        for got in (g.inputs, alone[0]):
+            off = (got[first:last].double() - few.double()).abs()
+            assert (off <= 3 * ref.E * 1.13 * (columns + 300) * size * 1.02 + 2 * ref.half_step(dtype) * few.double().abs()).all()
+    total, size, sums, sizes = 0.0, 0.0, 0.0, 0.0
+    xg, kg = ref.Grid(pkg, x, (lo, hi)), ref.Grid(pkg, k)
+    for r in range(0, rows, 1 << 16):
+        dz = gy[r:r + (1 << 16)].double()
+        if activation:
+            dz = dz * ref.slope(pre[r:r + (1 << 16)], activation)
+        a = xg.values[r:r + (1 << 16)].t().contiguous()
+        total, size = total + a @ dz, size + a.abs() @ dz.abs()
+        sums, sizes = sums + dz.sum(0), sizes + dz.abs().sum(0)
+    # float32 sums over all rows: off by the square root of their number, in half steps of sums below the terms' sizes (600 for 360 000);
+    # terms are 16 bits or more, slopes of float32 are off by 64 half steps
+    for kernel, bias in ((g.kernel, g.bias), alone[1:]):
+        ref.check(kernel, total * kg.inside, ref.rounded(total, (2.0 ** -16 / 64 + 600 * ref.E) * size, dtype), "kernel")
+        ref.check(bias, sums, ref.rounded(sums, 600 * ref.E * sizes, dtype), "bias")

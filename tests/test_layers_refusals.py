@@ -152,3 +152,17 @@ def test_tensors_that_require_a_gradient(pkg):
             call()
         with torch.no_grad(), pytest.raises(pkg.InvalidArgumentError, match="on the GPU"):
             call()
+
+
+@pytest.mark.parametrize("types", [(0, 0, 0), (1, 1, 1), (2, 2, 2)], ids=str)
+def test_the_gradients_workspace_is_bounded(pkg, types):
+    """Whatever the rows are: copies of 2^28 values of the gradient or of the input, at most three terms of two bytes, straight and
+    turned, and what is the kernel's; a 32nd of the gradient for the bias, in float32 by 64 rows; partial sums of two products' 512 tiles
+    of 64 KiB where a depth is split."""
+    lib, n = pkg._lib.load(), ctypes.c_size_t()
+    for rows, depth, columns in ((65536, 4096, 14336), (1 << 20, 4096, 4096), (4194176, 520, 3), (1 << 20, 8192, 64), (300, 32764, 32000)):
+        for activation in (0, 2):
+            desc = dense(pkg, rows, depth, columns, types, activation)
+            assert lib.axc_fake_approx_dense_gradients_workspace_bytes(ctypes.byref(desc), ctypes.byref(n)) == 0
+            kernel = (depth + 128) * (columns + 128)
+            assert n.value <= (1 << 28) * 2 * (3 + 3 + 1) + kernel * (2 + 4 * 4) + (rows // 64 + 2) * (columns + 128) * 4 + (1 << 26)
