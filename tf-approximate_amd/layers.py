@@ -49,7 +49,7 @@ def _unrecorded(*tensors):
     """Torch would take the output for a constant, and what it comes from would silently have no gradient."""
     if torch.is_grad_enabled():
         for t in tensors:
-            if torch.is_tensor(t) and t.requires_grad:
+            if t is not None and getattr(t, "requires_grad", False):
                 raise InvalidArgumentError("a gradient does not pass through this call: make it under torch.no_grad(), and take "
                                            "gradients() for what requires one")
 
