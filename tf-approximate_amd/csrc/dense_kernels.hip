@@ -7,8 +7,8 @@
 // number and is computed as one, so a product is rounded three times: s_in s_k, the bracket, and the two multiplied.
 //
 // The sums of many rows are made by the kernels that make them for 1x1 convolutions (axc_conv2d_codes_acc_i32); those of few
-// rows, where building rows for every filter element would cost more than the lookups, by few_rows_kernel; one or two rows are all
-// token_kernel's.
+// rows, where building rows for every filter element would cost more than the lookups, by few_rows_kernel; one row of up to
+// 16 384 values, or two of up to 8192, are all token_kernel's.
 #include "layers_internal.h"
 
 namespace axc {
@@ -492,7 +492,6 @@ template <int MT>
 __global__ void __launch_bounds__(1024) token_kernel(TokenJob job)
 {
     constexpr int kDepth = kTokenCodes / MT, kRounds = kTokenCodes / 4096;   // four codes a thread and round
-    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
     extern __shared__ __align__(16) unsigned char lds[];
     unsigned char *const codes = lds + kTokenTable;                                // [row][kDepth]
     uint32_t *const red = reinterpret_cast<uint32_t *>(codes + kTokenCodes);       // [turn][wavefront][row][column]

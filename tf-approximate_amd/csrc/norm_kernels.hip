@@ -4,8 +4,9 @@
 //   norm(v) = v / sqrt(mean(v^2) + eps), or (v - mean(v)) / sqrt(var(v) + eps)
 //
 // h is rounded to the tensors' type before it is normed, so that what the backward pass reads is what was normed.  A workgroup
-// takes a row at a time and keeps it in registers: everything is read once and written once, which is what bounds these kernels.
-// Statistics are float32, of the row as it stands in registers: the variance from the differences to the mean.
+// takes a row at a time; up to 8192 values, 4096 backwards, it keeps it in registers: everything is read once and written once, which is
+// what bounds these kernels.  Wider rows are read again for every sum, by kernels of their own.
+// Statistics are float32, the variance from the differences to the mean.
 #include "layers_internal.h"
 
 #include <algorithm>
@@ -659,7 +660,7 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(sizeof
 }
 
 // Wide rows backwards, in two launches: nine rows of four vectors a thread are more than its registers (spilled, rows of 16 384 took
-// 1630 us for 33.6 M values of bfloat16; 200 this way, rows of 8192 207 and 192).  The first leaves what a row's sums are, going over it from memory once for
+// 1630 us for 33.6 M values of bfloat16; 203 this way, rows of 8192 207 and 199; a norm of the block is a further pass, 349 and 326).  The first leaves what a row's sums are, going over it from memory once for
 // every dependent reduction; with that everything is value by value, and the second takes tiles of columns by runs of rows.
 constexpr int kWideBackward = 4096;      // values that are not wide yet
 struct RowStats {
