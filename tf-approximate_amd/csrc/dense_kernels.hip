@@ -52,8 +52,8 @@ __device__ void range_of_any(const void *p, int type, int64_t n, int64_t index, 
 
 // One pair per workgroup; the first x_blocks take the input (or one of them the pairs that a call before has reported of it: all that
 // follows then reads one), the others the kernel.  All of them clear `zeros`, into which a later launch adds.
-__global__ void __launch_bounds__(1024) range_kernel(const void *x, int x_type, int64_t nx, const float *reported, int x_blocks, const void *kernel,
-                                                     int kernel_type, int64_t nk, float *x_pairs, float *kernel_pairs,
+__global__ void __launch_bounds__(1024) range_kernel(const void *x, int x_type, int64_t nx, const float *reported, int x_blocks,
+                                                     const void *kernel, int kernel_type, int64_t nk, float *x_pairs, float *kernel_pairs,
                                                      int32_t *zeros, int64_t n_zeros)
 {
     __shared__ float red[32];
@@ -197,8 +197,8 @@ __device__ void kernel_slab(const T *__restrict__ w, int K, int64_t N, const Pie
 // The first x_blocks workgroups take four rows of the input at a time, a wavefront a row (rows up to the next multiple of four are pad
 // rows, of code 0).  The others take 256 columns of the kernel, four a lane, by 4 * lines of the depth, a wavefront every fourth;
 // column sums are added to what the launch before cleared, as whole numbers, so in any order.  Every workgroup makes the grid it
-// needs out of the range's pairs itself: a launch for that alone would be longer than folding 256 of them (or, of a range that a call before
-// has reported, of an input against a packed kernel, 4096).
+// needs out of the range's pairs itself: a launch for that alone would be longer than folding 256 of them (or 4096, of a range that a
+// call before has reported, against a packed kernel).
 __global__ void __launch_bounds__(256) codes_kernel(CodesJob job, int x_blocks, int column_blocks, int lines)
 {
     __shared__ float ends[8];
@@ -819,7 +819,8 @@ hipError_t launch_zero(void *p, int64_t bytes, hipStream_t stream)
 }
 
 hipError_t launch_range(const void *x, int x_type, int64_t nx, const float *reported, const void *kernel, int kernel_type, int64_t nk,
-                        float *x_pairs, float *kernel_pairs, int32_t *zeros, int64_t n_zeros, int *x_count, int *kernel_count, hipStream_t stream)
+                        float *x_pairs, float *kernel_pairs, int32_t *zeros, int64_t n_zeros, int *x_count, int *kernel_count,
+                        hipStream_t stream)
 {
     auto blocks = [](int64_t n) {   // 16 values a thread and more
         const int64_t b = (n + 16383) / 16384;

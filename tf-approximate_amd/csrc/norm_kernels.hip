@@ -660,8 +660,9 @@ __global__ void __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(sizeof
 }
 
 // Wide rows backwards, in two launches: nine rows of four vectors a thread are more than its registers (spilled, rows of 16 384 took
-// 1630 us for 33.6 M values of bfloat16; 203 this way, rows of 8192 207 and 199; a norm of the block is a further pass, 349 and 326).  The first leaves what a row's sums are, going over it from memory once for
-// every dependent reduction; with that everything is value by value, and the second takes tiles of columns by runs of rows.
+// 1630 us for 33.6 M values of bfloat16; 203 this way, rows of 8192 207 and 199; a norm of the block is a further pass, 349 and 326).
+// The first leaves what a row's sums are, going over it from memory once for every dependent reduction; with that everything is value
+// by value, and the second takes tiles of columns by runs of rows.
 constexpr int kWideBackward = 4096;      // values that are not wide yet
 struct RowStats {
     float mean, root, mgn, mg;           // of h: n = (h - mean) root; means of g n and of g
